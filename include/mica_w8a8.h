@@ -76,6 +76,7 @@ extern "C" {
 #define MICA_DEV_TIMEOUT_SELFTEST   6
 #define MICA_DEV_TIMEOUT_STREAMK    7   /* a stream-K CTA waited too long for its neighbour's partial */
 #define MICA_DEV_BAD_LAUNCH         8   /* a kernel found its grid smaller than it needs and did nothing */
+#define MICA_DEV_BAD_PAGE           9   /* a cache step named a page, position or token list out of range */
 
 typedef struct mica_caps {
     int device;             /* CUDA ordinal queried                                     */
@@ -87,7 +88,7 @@ typedef struct mica_caps {
     int pair_clusters;      /* co-resident CTA pairs for the 256-row GEMM tiles         */
 } mica_caps;
 
-#define MICA_ABI_VERSION 5
+#define MICA_ABI_VERSION 6
 
 /* Capability query. Replaces int8_kernels.available() (v0.5/serving/lib/int8_kernels.py:146-159)
  * and the capability probe in _device_cc (:130-143). Fills *caps for `device`.         */
@@ -288,6 +289,80 @@ int mica_qk_norm_rope(void* qkv, long ld, const void* q_w, const void* k_w, cons
  * the reference's own Triton kernel is v0.5/serving/kernel_src/kernels.py:72-124).           */
 int mica_attention_prefill(const void* qkv, long ld_qkv, void* out, long ld_out, int B, int L, int H, int KV, int D,
                            float scale, void* stream);
+
+/* ---- paged K/V cache -----------------------------------------------------------------
+ * Scoring answers of several tokens over a kept context: the context's K and V stay in pages
+ * and each step runs only its new rows. No counterpart in the reference, whose engines keep
+ * nothing between requests but whole-prefix states (v0.5/serving/lib/fork.py).
+ *
+ * A layer's pages are bf16 [pages, KV, page, D] with any page stride (elements, a multiple of
+ * 8): the pool of a model is [pages, layers, 2, KV, page, D]. page is 16, 32, 64 or 128.
+ * A step of B sequences is described on the device, so a captured graph serves new steps:
+ *   table [B, P] int32 (row stride ld_table)   page numbers of each sequence
+ *   base  [B]    int32                         tokens already in the cache
+ *   cu    [B+1]  int32, increasing, cu[0] = 0  rows cu[b]..cu[b+1] of the N rows are sequence b's
+ * Row i of sequence b is cache index base[b] + i: slot index % page of page table[b][index / page].
+ * Rows behind cu[B] are padding. A base, page number or position out of range records
+ * MICA_DEV_BAD_PAGE; what it names is neither read nor written.                            */
+
+/* Per-head RMSNorm of q and k, rotary embedding and the write of k and v into their pages, in
+ * one pass over the QKV projection's output qkv [N, ld] (q: H*D | k: KV*D | v: KV*D):
+ *   y = w * x * rsqrt(mean(x^2) + eps);  out = y * cos + rotate_half(y) * sin
+ * in fp32, rounded to bf16 once (mica_qk_norm_rope reproduces HF's rounding of every step).
+ * cos, sin: bf16 [n_pos, D]; pos: int64 [N] or NULL for the cache index. q_out [N, ldq]; padding
+ * rows of q_out are zero. D in {64, 128}.                                                  */
+int mica_cache_append(const void* qkv, long ld, const void* q_w, const void* k_w, const void* cos, const void* sin,
+                      long n_pos, const int64_t* pos, void* q_out, long ldq, void* k_pages, void* v_pages,
+                      long page_stride, int pages, int page, const int* table, long ld_table, int P, const int* base,
+                      const int* cu, int B, int N, int H, int KV, int D, float eps, void* stream);
+
+/* Attention of a step's rows over the cache: q [N, ldq] (H heads of D) against K and V of
+ * indexes 0 .. base[b] + rows(b) - 1 (the step's own rows have been appended):
+ *   out[row, h] = sum_s softmax_s(scale * q[row, h] . K[s, h / (H / KV)]) V[s, h / (H / KV)]
+ * Row i sees every s < base[b], and node j of its own step when bit j % 64 of word j / 64 of
+ * mask[row] (int64 [N, ld_mask], `words` words) is set: the ancestors of a tree node and itself.
+ * mask NULL: j <= i. A row that sees nothing, and a padding row, gives zero. fp32 scores, sums
+ * and accumulation. max_new: the most rows a sequence is expected to have (a hint for the choice
+ * of tile; more are served too). H % KV == 0, H / KV <= 128, D in {64, 128}.
+ * workspace: at least mica_cache_attention_workspace_bytes(...) bytes, 16-byte aligned, used by
+ * this call alone until its kernels are done.                                              */
+size_t mica_cache_attention_workspace_bytes(int N, int max_new, int H, int KV, int D);
+int mica_cache_attention(const void* q, long ldq, const void* k_pages, const void* v_pages, long page_stride,
+                         int pages, int page, const int* table, long ld_table, int P, const int* base, const int* cu,
+                         const int64_t* mask, long ld_mask, int words, int B, int N, int max_new, int H, int KV, int D,
+                         float scale, void* out, long ldo, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Copies pages: for each i < n, page dst[i] takes the page_bytes of page src[i] (all layers of a
+ * pool at once). src and dst are HOST arrays (they travel in kernel parameters; a captured graph
+ * keeps them). No page may be written twice, or be both read and written (MICA_ERR_ARG).
+ * page_bytes and page_stride (bytes) are multiples of 16.                                  */
+int mica_cache_copy(void* pool, long page_stride, long page_bytes, int pages, const int* src, const int* dst, int n,
+                    void* stream);
+
+/* Keeps some of a step's rows: slot base[b] + j of sequence b takes K and V of slot base[b] +
+ * keep[b][j] for j < n_keep[b], in all slabs of a page (slabs = layers * 2 * KV blocks of page * D
+ * bf16, contiguous). keep int32 [B, ld_keep], increasing within a sequence and below its row
+ * count; n_keep int32 [B], at most A. new_base[b] = base[b] + n_keep[b] (a separate array). A
+ * sequence whose list is out of order or out of range is left as it was (new_base = base).
+ * page_stride in bytes.                                                                    */
+int mica_cache_keep(void* pool, long page_stride, int slabs, int pages, int page, int D, const int* table,
+                    long ld_table, int P, const int* base, const int* cu, int B, const int* keep, long ld_keep,
+                    const int* n_keep, int A, int* new_base, void* stream);
+
+/* Log probabilities of given tokens, entropy and top alternatives of logits z [N, ld] over V
+ * tokens (dtype MICA_DT_*, unit column stride, any row stride):
+ *   logprob [N, M] fp32 = z[ids] - log sum e^z; ids int64 [N, ld_ids]; a negative id gives 0, one
+ *                         past the end NaN (M may be 0)
+ *   entropy [N] fp32 in nats
+ *   top_lp [N, top] fp32, top_id [N, top] int64: the largest log probabilities, ties by the lowest
+ *                         id (0 <= top <= 32, top <= V; both NULL when top is 0)
+ * -inf logits are tokens that are not allowed; a row with nothing else gives -inf everywhere and
+ * entropy 0. A NaN or +inf logit makes the row's log probabilities and entropy NaN.
+ * workspace: mica_token_logprobs_workspace_bytes(...) bytes, 16-byte aligned.               */
+size_t mica_token_logprobs_workspace_bytes(int N, int V, int dtype, int top);
+int mica_token_logprobs(const void* z, int dtype, long ld, int N, int V, const int64_t* ids, long ld_ids, int M,
+                        int top, float* logprob, float* entropy, float* top_lp, int64_t* top_id, void* workspace,
+                        size_t workspace_bytes, void* stream);
 
 /* Failure-detection self-test: launches one block that waits on a barrier nothing
  * ever arrives on, with a wait limit of limit_us microseconds. The kernel gives up,

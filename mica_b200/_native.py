@@ -41,6 +41,7 @@ DEV_ERRORS = {
     6: 'timeout_selftest',
     7: 'timeout_streamk',
     8: 'bad_launch',
+    9: 'bad_page',
 }
 SPLIT_STREAM_K = -1
 
@@ -88,6 +89,19 @@ SIGNATURES = {
     'mica_option_logits': (_I, [_P, _I, _L, _P, _I, _F, _P, _I, _I, _P, _P, _P, _P, _I, _P]),
     'mica_qk_norm_rope': (_I, [_P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _F, _P]),
     'mica_attention_prefill': (_I, [_P, _L, _P, _L, _I, _I, _I, _I, _I, _F, _P]),
+    'mica_cache_append': (
+        _I,
+        [_P, _L, _P, _P, _P, _P, _L, _P, _P, _L, _P, _P, _L, _I, _I, _P, _L, _I, _P, _P, _I, _I, _I, _I, _I, _F, _P],
+    ),
+    'mica_cache_attention_workspace_bytes': (_Z, [_I, _I, _I, _I, _I]),
+    'mica_cache_attention': (
+        _I,
+        [_P, _L, _P, _P, _L, _I, _I, _P, _L, _I, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P, _Z, _P],
+    ),
+    'mica_cache_copy': (_I, [_P, _L, _L, _I, _P, _P, _I, _P]),
+    'mica_cache_keep': (_I, [_P, _L, _I, _I, _I, _I, _P, _L, _I, _P, _P, _I, _P, _L, _P, _I, _P, _P]),
+    'mica_token_logprobs_workspace_bytes': (_Z, [_I, _I, _I, _I]),
+    'mica_token_logprobs': (_I, [_P, _I, _L, _I, _I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _Z, _P]),
     'mica_selftest_wait_timeout': (_I, [_P, _I, _P]),
 }
 
@@ -137,6 +151,11 @@ def check(name, rc):
             detail = lib().mica_last_cuda_error().decode(errors='replace')
         raise NativeError(name, rc, detail)
     return rc
+
+
+def int_array(values):
+    """A host int32 array for the entry points that take one."""
+    return (ctypes.c_int * len(values))(*values)
 
 
 def call(name, *args):

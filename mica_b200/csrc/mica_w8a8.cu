@@ -22,6 +22,9 @@
 #include "readout.cuh"
 #include "qk_rope.cuh"
 #include "attention.cuh"
+#include "cache.cuh"
+#include "cache_attention.cuh"
+#include "logprobs.cuh"
 
 using namespace mica;
 
@@ -1044,6 +1047,176 @@ int mica_attention_prefill(const void* qkv, long ld_qkv, void* out, long ld_out,
     a.scale_log2 = scale * 1.4426950408889634f;
     attention_fwd_kernel<<<static_cast<unsigned>(ctas), ATT_THREADS, ATT_SMEM_BYTES, static_cast<cudaStream_t>(stream)>>>(
         tm, a);
+    return launch_status();
+}
+
+// ---------------------------------------------------------------------------------------
+// Paged cache. What a step's tables say is on the device, so the kernels check it there.
+static int cache_plan(CachePlan* p, const int* table, long ld_table, int P, const int* base, const int* cu, int B, int N,
+                      int pages, int page) {
+    if (B < 0 || N < 0 || P < 1 || pages < 1 || ld_table < P || (page != 16 && page != 32 && page != 64 && page != 128))
+        return MICA_ERR_SHAPE;
+    if (static_cast<long>(P) * page > (1L << 31) - 1) return MICA_ERR_RANGE;
+    *p = CachePlan{};
+    p->table = table; p->ld_table = ld_table; p->base = base; p->cu = cu; p->B = B; p->P = P; p->N = N;
+    p->pages = pages;
+    p->page_log2 = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
+    return MICA_OK;
+}
+static bool aligned_to(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int mica_cache_append(const void* qkv, long ld, const void* q_w, const void* k_w, const void* cos, const void* sin,
+                      long n_pos, const int64_t* pos, void* q_out, long ldq, void* k_pages, void* v_pages,
+                      long page_stride, int pages, int page, const int* table, long ld_table, int P, const int* base,
+                      const int* cu, int B, int N, int H, int KV, int D, float eps, void* stream) {
+    if (!qkv || !q_w || !k_w || !cos || !sin || !q_out || !k_pages || !v_pages || !table || !base || !cu)
+        return MICA_ERR_ARG;
+    AppendArgs a = {};
+    int rc = cache_plan(&a.plan, table, ld_table, P, base, cu, B, N, pages, page);
+    if (rc) return rc;
+    if (H < 1 || KV < 1 || H > 4096 || KV > 4096 || (D != 64 && D != 128) || n_pos < 1 ||
+        ld < static_cast<long>(H + 2 * KV) * D || ldq < static_cast<long>(H) * D ||
+        page_stride < static_cast<long>(KV) * page * D)
+        return MICA_ERR_SHAPE;
+    if (!aligned16(qkv) || !aligned16(q_w) || !aligned16(k_w) || !aligned16(cos) || !aligned16(sin) ||
+        !aligned16(q_out) || !aligned16(k_pages) || !aligned16(v_pages) || ld % 8 || ldq % 8 || page_stride % 8 ||
+        !aligned_to(pos, 8) || !aligned_to(table, 4) || !aligned_to(base, 4) || !aligned_to(cu, 4))
+        return MICA_ERR_ALIGN;
+    if ((rc = check_device(nullptr))) return rc;
+    if (N == 0) return MICA_OK;
+    a.qkv = static_cast<const __nv_bfloat16*>(qkv); a.ld = ld;
+    a.q_w = static_cast<const __nv_bfloat16*>(q_w); a.k_w = static_cast<const __nv_bfloat16*>(k_w);
+    a.cos = static_cast<const __nv_bfloat16*>(cos); a.sin = static_cast<const __nv_bfloat16*>(sin);
+    a.n_pos = n_pos; a.pos = reinterpret_cast<const long*>(pos);
+    a.q_out = static_cast<__nv_bfloat16*>(q_out); a.ldq = ldq;
+    a.k_pages = static_cast<__nv_bfloat16*>(k_pages); a.v_pages = static_cast<__nv_bfloat16*>(v_pages);
+    a.page_stride = page_stride; a.H = H; a.KV = KV; a.eps = eps;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const long blocks = (static_cast<long>(N) * (H + 2 * KV) + 7) / 8;
+    if (blocks > (1L << 31) - 1) return MICA_ERR_RANGE;
+    if (D == 128) cache_append_kernel<128><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+    else cache_append_kernel<64><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+    return launch_status();
+}
+
+size_t mica_cache_attention_workspace_bytes(int N, int max_new, int H, int KV, int D) { return 0; }
+
+int mica_cache_attention(const void* q, long ldq, const void* k_pages, const void* v_pages, long page_stride,
+                         int pages, int page, const int* table, long ld_table, int P, const int* base, const int* cu,
+                         const int64_t* mask, long ld_mask, int words, int B, int N, int max_new, int H, int KV, int D,
+                         float scale, void* out, long ldo, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!q || !k_pages || !v_pages || !table || !base || !cu || !out || !(scale > 0.f) || !std::isfinite(scale))
+        return MICA_ERR_ARG;
+    CacheAttnArgs a = {};
+    int rc = cache_plan(&a.plan, table, ld_table, P, base, cu, B, N, pages, page);
+    if (rc) return rc;
+    if (H < 1 || KV < 1 || H > 4096 || H % KV || H / KV > 128 || (D != 64 && D != 128) || max_new < 0 ||
+        ldq < static_cast<long>(H) * D || ldo < static_cast<long>(H) * D ||
+        page_stride < static_cast<long>(KV) * page * D || (mask && (words < 1 || ld_mask < words)))
+        return MICA_ERR_SHAPE;
+    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || ldq % 8 || ldo % 8 ||
+        page_stride % 8 || !aligned_to(mask, 8) || !aligned_to(table, 4) || !aligned_to(base, 4) || !aligned_to(cu, 4) ||
+        !aligned16(workspace))
+        return MICA_ERR_ALIGN;
+    if (workspace_bytes < mica_cache_attention_workspace_bytes(N, max_new, H, KV, D)) return MICA_ERR_WORKSPACE;
+    if ((rc = check_device(nullptr))) return rc;
+    if (N == 0) return MICA_OK;
+    a.q = static_cast<const __nv_bfloat16*>(q); a.ldq = ldq;
+    a.k_pages = static_cast<const __nv_bfloat16*>(k_pages); a.v_pages = static_cast<const __nv_bfloat16*>(v_pages);
+    a.page_stride = page_stride;
+    a.mask = reinterpret_cast<const unsigned long long*>(mask); a.ld_mask = ld_mask; a.words = words;
+    a.out = static_cast<__nv_bfloat16*>(out); a.ldo = ldo; a.H = H; a.KV = KV;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const long blocks = (static_cast<long>(N) * H + 3) / 4;
+    if (blocks > (1L << 31) - 1) return MICA_ERR_RANGE;
+    if (D == 128) cache_attention_kernel<128><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a);
+    else cache_attention_kernel<64><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a);
+    return launch_status();
+}
+
+int mica_cache_copy(void* pool, long page_stride, long page_bytes, int pages, const int* src, const int* dst, int n,
+                    void* stream) {
+    if (!pool || n < 0 || (n > 0 && (!src || !dst))) return MICA_ERR_ARG;
+    if (pages < 1 || page_bytes < 16 || page_stride < page_bytes) return MICA_ERR_SHAPE;
+    if (!aligned16(pool) || page_bytes % 16 || page_stride % 16) return MICA_ERR_ALIGN;
+    if (n > 0) {
+        // one bit per page: the pages that are written
+        const size_t bytes = (static_cast<size_t>(pages) + 7) / 8;
+        unsigned char* seen = static_cast<unsigned char*>(calloc(bytes, 1));
+        if (!seen) return MICA_ERR_ARG;
+        bool ok = true;
+        for (int i = 0; i < n && ok; ++i) {
+            ok = src[i] >= 0 && src[i] < pages && dst[i] >= 0 && dst[i] < pages && !(seen[dst[i] >> 3] >> (dst[i] & 7) & 1);
+            if (ok) seen[dst[i] >> 3] |= static_cast<unsigned char>(1 << (dst[i] & 7));
+        }
+        for (int i = 0; i < n && ok; ++i) ok = !(seen[src[i] >> 3] >> (src[i] & 7) & 1);
+        free(seen);
+        if (!ok) return MICA_ERR_ARG;
+    }
+    int rc = check_device(nullptr);
+    if (rc) return rc;
+    CopyArgs a = {};
+    a.pool = static_cast<char*>(pool); a.page_stride = page_stride; a.page_bytes = page_bytes;
+    for (int i = 0; i < n; i += COPY_PAIRS) {
+        const int m = std::min(n - i, COPY_PAIRS);
+        memcpy(a.src, src + i, m * sizeof(int));
+        memcpy(a.dst, dst + i, m * sizeof(int));
+        const long blocks = std::min((page_bytes / 16 + 255) / 256, 2048L);
+        cache_copy_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(m)), 256, 0,
+                            static_cast<cudaStream_t>(stream)>>>(a);
+        if ((rc = launch_status())) return rc;
+    }
+    return MICA_OK;
+}
+
+int mica_cache_keep(void* pool, long page_stride, int slabs, int pages, int page, int D, const int* table,
+                    long ld_table, int P, const int* base, const int* cu, int B, const int* keep, long ld_keep,
+                    const int* n_keep, int A, int* new_base, void* stream) {
+    if (!pool || !table || !base || !cu || !keep || !n_keep || !new_base || new_base == base) return MICA_ERR_ARG;
+    KeepArgs a = {};
+    int rc = cache_plan(&a.plan, table, ld_table, P, base, cu, B, 0, pages, page);
+    if (rc) return rc;
+    if (slabs < 1 || (D != 64 && D != 128) || A < 0 || ld_keep < A || B > 65535 ||
+        page_stride < static_cast<long>(slabs) * page * D * 2)
+        return MICA_ERR_SHAPE;
+    if (!aligned16(pool) || page_stride % 16 || !aligned_to(table, 4) || !aligned_to(base, 4) || !aligned_to(cu, 4) ||
+        !aligned_to(keep, 4) || !aligned_to(n_keep, 4) || !aligned_to(new_base, 4))
+        return MICA_ERR_ALIGN;
+    if ((rc = check_device(nullptr))) return rc;
+    if (B == 0) return MICA_OK;
+    a.pool = static_cast<char*>(pool); a.page_stride = page_stride; a.keep = keep; a.ld_keep = ld_keep;
+    a.n_keep = n_keep; a.A = A; a.new_base = new_base; a.heads = slabs; a.row_bytes = D * 2;
+    cache_keep_kernel<<<dim3(static_cast<unsigned>(slabs), static_cast<unsigned>(B)), 256, 0,
+                        static_cast<cudaStream_t>(stream)>>>(a);
+    return launch_status();
+}
+
+// ---------------------------------------------------------------------------------------
+size_t mica_token_logprobs_workspace_bytes(int N, int V, int dtype, int top) { return 0; }
+
+int mica_token_logprobs(const void* z, int dtype, long ld, int N, int V, const int64_t* ids, long ld_ids, int M,
+                        int top, float* logprob, float* entropy, float* top_lp, int64_t* top_id, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+    if (!z || !entropy || dtype < 0 || dtype > 2 || M < 0 || top < 0 || (M > 0 && (!ids || !logprob)) ||
+        (top > 0 && (!top_lp || !top_id)))
+        return MICA_ERR_ARG;
+    if (N < 0 || V < 1 || ld < V || ld_ids < M || top > 32 || top > V) return MICA_ERR_SHAPE;
+    if (!aligned_to(z, static_cast<unsigned>(dt_size(dtype))) || !aligned_to(ids, 8) || !aligned_to(top_id, 8) ||
+        !aligned_to(logprob, 4) || !aligned_to(entropy, 4) || !aligned_to(top_lp, 4) || !aligned16(workspace))
+        return MICA_ERR_ALIGN;
+    if (workspace_bytes < mica_token_logprobs_workspace_bytes(N, V, dtype, top)) return MICA_ERR_WORKSPACE;
+    int rc = check_device(nullptr);
+    if (rc) return rc;
+    if (N == 0) return MICA_OK;
+    LogprobArgs a = {};
+    a.z = z; a.ld = ld; a.N = N; a.V = V; a.ids = reinterpret_cast<const long*>(ids); a.ld_ids = ld_ids; a.M = M;
+    a.top = top; a.logprob = logprob; a.entropy = entropy; a.top_lp = top_lp;
+    a.top_id = reinterpret_cast<long*>(top_id);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == MICA_DT_BF16) token_logprobs_kernel<__nv_bfloat16><<<N, 512, 0, st>>>(a);
+    else if (dtype == MICA_DT_FP16) token_logprobs_kernel<__half><<<N, 512, 0, st>>>(a);
+    else token_logprobs_kernel<float><<<N, 512, 0, st>>>(a);
     return launch_status();
 }
 

@@ -1,0 +1,446 @@
+"""The paged-cache operators against their definitions in 64 bits.
+
+Tolerances, counted in half steps of bf16 (u = 2^-8, relative to the value). attention: the output is
+rounded once (u |o|) and each weight p once before the product with V, so an output element is off by at
+most u |o| + u sum_s p_s |v_s|, plus fp32 sums (2^-24 a step) and the exponential's 2^-21, far below u; the
+test allows 1.1 of that bound. append: one rounding of an fp32 value, u |y| plus fp32 noise on the products
+that may cancel (2^-20 of their sum). Copies and moves are bit-exact."""
+import pytest
+import torch
+
+from paged_reference import Case, holes, norm_rope, tree
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -8
+
+
+def run_attention(c, scale=None, **kw):
+    from mica_b200 import paged
+    return paged.attention(c.q, c.k, c.v, c.step(**kw), c.heads, scale=scale)
+
+
+def check_attention(c, o, scale=None):
+    ref = c.attention(scale)
+    was = c.keys
+    c.keys = [(k, v.abs()) for k, v in was]
+    size = c.attention(scale)                      # sum p |v|
+    c.keys = was
+    err = (o.double() - ref).abs()
+    bound = 1.1 * U * (ref.abs() + size) + 1e-6
+    assert torch.isfinite(o).all()
+    worst = float((err / bound).max()) if err.numel() else 0.0
+    assert worst <= 1.0, worst
+
+
+SHAPES = [(32, 8, 128), (4, 4, 64), (6, 2, 128), (5, 1, 64), (28, 4, 128), (16, 1, 128)]
+
+
+@pytest.mark.parametrize('heads,kv,dim', SHAPES)
+@pytest.mark.parametrize('page', [16, 32, 64, 128])
+def test_attention_next_token(heads, kv, dim, page):
+    c = Case([0, 1, 15, 16, 127, 128, 129, 700], [1] * 8, heads, kv, dim, page, seed=page + heads)
+    check_attention(c, run_attention(c, max_new=1))
+
+
+@pytest.mark.parametrize('heads,kv,dim', SHAPES)
+@pytest.mark.parametrize('mask', [None, tree, holes])
+def test_attention_of_ragged_trees(heads, kv, dim, mask):
+    c = Case([0, 300, 5, 129, 1000], [7, 1, 65, 130, 33], heads, kv, dim, 16, seed=heads + dim, mask=mask)
+    check_attention(c, run_attention(c, max_new=130))
+
+
+@pytest.mark.parametrize('new', [1, 31, 32, 33, 63, 64, 65, 128, 129, 200, 700])
+def test_attention_row_counts(new):
+    """One sequence, tree rows around the tile's edges; the hint may be wrong either way."""
+    c = Case([333], [new], 8, 2, 128, 64, seed=new, mask=tree)
+    o = run_attention(c)
+    check_attention(c, o)
+    check_attention(c, run_attention(c, max_new=1))
+    check_attention(c, run_attention(c, max_new=new))
+
+
+@pytest.mark.parametrize('ctx,new', [([20000], [1]), ([9001, 3, 0], [5, 64, 1]), ([4096] * 3, [17] * 3),
+                                     ([0], [1500]), ([777], [1025])])
+def test_attention_long_axes(ctx, new):
+    c = Case(ctx, new, 8, 2, 128, 64, seed=len(ctx))
+    check_attention(c, run_attention(c, max_new=max(new)))
+
+
+def test_attention_many_sequences():
+    ctx = [(i * 37) % 211 for i in range(500)]
+    c = Case(ctx, [1 + i % 3 for i in range(500)], 4, 2, 64, 16, seed=2)
+    check_attention(c, run_attention(c, max_new=3))
+
+
+def test_attention_sequences_without_rows_and_padding_rows():
+    """Sequences that have no rows in this step, rows behind the last sequence (zero), extra mask words."""
+    c = Case([10, 500, 0, 40], [0, 3, 0, 70], 8, 2, 128, 32, seed=4, pad_rows=9, mask=tree, extra_words=2)
+    o = run_attention(c)
+    check_attention(c, o)
+    assert float(o[-9:].float().abs().max()) == 0.0
+    empty = Case([10, 5], [0, 0], 8, 2, 128, 32, seed=4, pad_rows=3)
+    assert float(run_attention(empty).float().abs().max()) == 0.0
+
+
+def test_attention_no_rows_and_no_sequences():
+    from mica_b200 import paged
+    c = Case([10], [0], 8, 2, 128, 32)
+    assert run_attention(c).shape == (0, 8 * 128)
+    i32 = {'dtype': torch.int32, 'device': 'cuda'}
+    step = paged.Step(torch.zeros(0, 1, **i32), torch.zeros(0, **i32), torch.zeros(1, **i32))
+    q = torch.ones(2, 8 * 128, dtype=torch.bfloat16, device='cuda')
+    o = paged.attention(q, c.k, c.v, step, 8)
+    assert float(o.float().abs().max()) == 0.0
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), float('-inf')])
+@pytest.mark.parametrize('new', [20, 90])
+def test_attention_odd_values_in_masked_nodes(bad, new):
+    """A node's K and V that a row does not see change nothing in that row."""
+    c = Case([50, 130], [new, new], 8, 2, 128, 32, seed=6, mask=tree)
+    clean = run_attention(c)
+    node = new - 4
+    for b in range(2):
+        kk, vv = c.keys[b]
+        s = c.ctx[b] + node
+        p, slot = c.rows[b][s // 32], s % 32
+        vv[:, s] = bad
+        c.v[p, :, slot] = bad
+        kk[:, s] = bad
+        c.k[p, :, slot] = bad
+    o = run_attention(c)
+    blind = torch.cat([~c.seen[b][:, node] for b in range(2)])
+    assert blind.sum() > 0 and (~blind).sum() > 0
+    assert torch.equal(o[blind.cuda()], clean[blind.cuda()])
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), float('-inf')])
+def test_attention_odd_values_that_are_seen(bad):
+    """An infinite or NaN value in one element of a seen V reaches that element alone."""
+    c = Case([70], [40], 4, 2, 128, 32, seed=8, mask=tree)
+    clean = run_attention(c)
+    s = 70 + 30
+    c.v[c.rows[0][s // 32], 1, s % 32, 5] = bad
+    c.keys[0][1][1, s, 5] = bad
+    o = run_attention(c)
+    ref = c.attention()
+    assert torch.equal(torch.isnan(o), torch.isnan(ref)) and torch.equal(torch.isinf(o), torch.isinf(ref))
+    fine = torch.isfinite(ref)
+    assert (o.double() - ref)[fine].abs().max() < 0.05
+    rows = ~c.seen[0][:, 30].cuda()
+    assert torch.equal(o[rows], clean[rows])
+
+
+@pytest.mark.parametrize('scale', [1e-4, 0.3, 3.0])
+def test_attention_scales(scale):
+    """Nearly even weights, and scores whose maximum moves by hundreds between tiles."""
+    c = Case([600], [33], 8, 2, 128, 64, seed=12, mask=tree)
+    check_attention(c, run_attention(c, scale=scale), scale)
+
+
+def test_attention_growing_scores():
+    """Keys whose scores rise along the axis: the running maximum moves in every tile."""
+    c = Case([1000], [3], 4, 1, 128, 64, seed=3)
+    kk, _ = c.keys[0]
+    grow = torch.linspace(0.0, 6.0, kk.shape[1], device='cuda')[None, :, None]
+    kk.copy_((grow * torch.sign(c.q[0, :128].float())[None, None]).bfloat16())
+    for s in range(0, kk.shape[1], 64):
+        m = min(64, kk.shape[1] - s)
+        c.k[c.rows[0][s // 64], :, :m] = kk[:, s:s + m]
+    check_attention(c, run_attention(c))
+
+
+def test_attention_strided_rows_and_layer_of_a_pool():
+    """q as columns of a wider buffer, pages as one layer of a pool of three."""
+    c = Case([300, 40], [9, 70], 8, 2, 128, 64, seed=9, layers=3, layer=1, mask=tree)
+    wide = torch.randn(c.n, 12 * 128 + 24, device='cuda').bfloat16()
+    wide[:, 128:128 + 8 * 128] = c.q
+    c.q = wide[:, 128:128 + 8 * 128]
+    check_attention(c, run_attention(c))
+    odd = torch.zeros(c.n, 8 * 128 + 3, dtype=torch.bfloat16, device='cuda')     # rows not 16-byte aligned
+    odd[:, 3:] = c.q
+    assert torch.equal(run_attention(c), _with_q(c, odd[:, 3:]))
+
+
+def _with_q(c, q):
+    was, c.q = c.q, q
+    o = run_attention(c)
+    c.q = was
+    return o
+
+
+def test_attention_same_bits_again_on_other_streams_and_in_graphs():
+    """Repeated, on a side stream, two graphs replayed in turn and together with new lengths: the same bits."""
+    c = Case([3000, 20, 700], [5, 16, 1], 32, 8, 128, 64, seed=5, mask=tree)
+    o = run_attention(c)
+    for _ in range(3):
+        assert torch.equal(run_attention(c), o)
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs, outs = [], []
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            run_attention(c)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run_attention(c))
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, g in zip(side, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], o) and torch.equal(outs[1], o)
+    # the step's tensors changed in place: fewer committed tokens
+    c.base.copy_(torch.tensor([100, 20, 64], dtype=torch.int32))
+    eager = run_attention(c)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], eager) and not torch.equal(eager, o)
+
+
+def test_attention_bad_pages_are_recorded_and_not_read():
+    import ctypes
+
+    from mica_b200 import _native as N
+    st = torch.cuda.current_stream().cuda_stream
+    code = ctypes.c_int(0)
+    N.call('mica_device_error', ctypes.byref(code), st)
+    for change in ('page', 'negative', 'base', 'negative_base'):
+        c = Case([200, 30], [3, 4], 8, 2, 128, 64, seed=1)
+        good = run_attention(c)
+        if change == 'page':
+            c.table[0, 1] = c.pool.shape[0]
+        elif change == 'negative':
+            c.table[0, 0] = -1
+        elif change == 'base':
+            c.base[0] = 100000
+        else:
+            c.base[0] = -5
+        o = run_attention(c)
+        N.call('mica_device_error', ctypes.byref(code), st)
+        assert code.value == 9, change
+        assert torch.equal(o[3:], good[3:])
+        N.call('mica_device_error', ctypes.byref(code), st)
+        assert code.value == 0
+
+
+# ---- append -----------------------------------------------------------------------------
+def tables(dim, n=5000):
+    f = 1e6 ** (-torch.arange(0, dim, 2, dtype=torch.float64, device='cuda') / dim)
+    a = torch.arange(n, dtype=torch.float64, device='cuda')[:, None] * torch.cat((f, f))
+    return a.cos().bfloat16(), a.sin().bfloat16()
+
+
+@pytest.mark.parametrize('heads,kv,dim', SHAPES)
+@pytest.mark.parametrize('page', [16, 128])
+@pytest.mark.parametrize('positions', [False, True])
+def test_append(heads, kv, dim, page, positions):
+    from mica_b200 import paged
+    c = Case([0, 17, 700, 3], [1, 40, 0, 333], heads, kv, dim, page, seed=heads, layers=2, layer=1, pad_rows=2)
+    g = torch.Generator(device='cuda').manual_seed(1)
+    wide = (2 * torch.randn(c.n, (heads + 2 * kv) * dim + 8, generator=g, device='cuda')).bfloat16()
+    qkv = wide[:, :(heads + 2 * kv) * dim]
+    qkv[0, :dim] = 0
+    qw, kw = (1 + 0.1 * torch.randn(2, dim, generator=g, device='cuda')).bfloat16()
+    cos, sin = tables(dim)
+    index = torch.cat([torch.arange(a, a + t) for a, t in zip(c.ctx, c.new)]).cuda()
+    pos = torch.randint(0, 5000, (c.n,), generator=g, device='cuda') if positions else None
+    c.pool.zero_()
+    before, src = c.pool.clone(), wide.clone()
+    q = paged.append(qkv, qw, kw, cos, sin, c.k, c.v, c.step(), heads, pos=pos)
+    assert torch.equal(wide, src)
+    p = pos[:index.numel()] if positions else index
+    n = index.numel()
+    x = qkv[:n].view(n, heads + 2 * kv, dim)
+    ref = torch.cat((norm_rope(x[:, :heads], qw, cos[p], sin[p], 1e-6),
+                     norm_rope(x[:, heads:heads + kv], kw, cos[p], sin[p], 1e-6)), 1)
+    size = torch.cat((norm_rope(x[:, :heads], qw, cos[p], sin[p], 1e-6).abs().amax(-1, keepdim=True),
+                      norm_rope(x[:, heads:heads + kv], kw, cos[p], sin[p], 1e-6).abs().amax(-1, keepdim=True)), 1)
+    bound = U * ref.abs() + 2.0 ** -20 * 4 * size + 1e-12
+    assert ((q[:n].view(n, heads, dim).double() - ref[:, :heads]).abs() <= bound[:, :heads]).all()
+    assert float(q[n:].float().abs().max()) == 0.0
+    b = torch.cat([torch.full((t,), i) for i, t in enumerate(c.new)]).cuda()
+    page_of, slot = c.table.long()[b, index // page], index % page
+    got = c.k[page_of, :, slot].double()
+    assert ((got - ref[:, heads:]).abs() <= bound[:, heads:]).all()
+    assert torch.equal(c.v[page_of, :, slot], x[:, heads + kv:])
+    c.k[page_of, :, slot] = 0                      # nothing else was written
+    c.v[page_of, :, slot] = 0
+    assert torch.equal(c.pool, before)
+
+
+def test_append_bad_indexes_write_nothing():
+    import ctypes
+
+    from mica_b200 import _native as N
+    from mica_b200 import paged
+    st = torch.cuda.current_stream().cuda_stream
+    code = ctypes.c_int(0)
+    cos, sin = tables(64, 100)
+    one = torch.ones(64, dtype=torch.bfloat16, device='cuda')
+    for change in ('page', 'negative', 'base', 'pos', 'table_end'):
+        c = Case([5], [4], 4, 2, 64, 16, fill=0.0)
+        c.pool.zero_()
+        qkv = torch.ones(4, 8 * 64, dtype=torch.bfloat16, device='cuda')
+        pos = torch.zeros(4, dtype=torch.int64, device='cuda')
+        if change == 'page':
+            c.table[0, 0] = 1000
+        elif change == 'negative':
+            c.table[0, 0] = -1
+        elif change == 'base':
+            c.base[0] = -1
+        elif change == 'pos':
+            pos += 100
+        else:
+            c.base[0] = 16 * c.table.shape[1]
+        N.call('mica_device_error', ctypes.byref(code), st)
+        q = paged.append(qkv, one, one, cos, sin, c.k, c.v, c.step(), 4, pos=pos)
+        N.call('mica_device_error', ctypes.byref(code), st)
+        assert code.value == 9, change
+        assert float(c.pool.float().abs().max()) == 0.0 and float(q.float().abs().max()) == 0.0
+
+
+# ---- pages --------------------------------------------------------------------------------
+@pytest.mark.parametrize('shape', [(9, 3, 2, 2, 16, 64), (700, 1, 2, 1, 16, 64), (6, 36, 2, 8, 64, 128)])
+@pytest.mark.parametrize('pairs', [1, 3, 'all'])
+def test_copy_pages(shape, pairs):
+    from mica_b200 import paged
+    pool = torch.randn(shape, device='cuda').bfloat16()
+    pool.view(torch.int16)[0, 0, 0, 0, 0, 0] = 0x7fff          # a NaN's bits travel as they are
+    order = torch.randperm(shape[0], generator=torch.Generator().manual_seed(1)).tolist()
+    n = shape[0] // 2 if pairs == 'all' else pairs
+    src, dst = order[:n], order[n:2 * n]
+    ref = pool.clone()
+    ref[dst] = ref[src]
+    paged.copy_pages(pool, src, dst)
+    assert torch.equal(pool.view(torch.int16), ref.view(torch.int16))
+    two = order[:1] * 2, order[1:3]                             # one page into two
+    ref[two[1]] = ref[two[0]]
+    paged.copy_pages(pool, *two)
+    assert torch.equal(pool.view(torch.int16), ref.view(torch.int16))
+
+
+def test_copy_pages_of_a_wider_buffer_and_fp32():
+    from mica_b200 import paged
+    wide = torch.randn(8, 100, device='cuda')
+    pool = wide[:, :84]
+    ref = wide.clone()
+    ref[3, :84] = ref[5, :84]
+    paged.copy_pages(pool, [5], [3])
+    assert torch.equal(wide, ref)
+
+
+@pytest.mark.parametrize('layers,kv,dim,page', [(1, 1, 64, 16), (3, 2, 128, 32), (36, 8, 128, 64), (2, 5, 64, 128)])
+def test_keep_tokens(layers, kv, dim, page):
+    from mica_b200 import paged
+    ctx, new = [0, 3, 130, 40, 7, 16], [64, 16, 200, 1, 30, 0]
+    c = Case(ctx, new, kv, kv, dim, page, seed=layers, layers=layers)
+    c.pool.normal_()
+    keep = [[0, 1, 5, 9, 10, 63], [3], list(range(1, 200, 2)), [0], [], []]
+    most = max(len(k) for k in keep)
+    kt = torch.tensor([k + [-3] * (most - len(k)) for k in keep], dtype=torch.int32, device='cuda')
+    nk = torch.tensor([len(k) for k in keep], dtype=torch.int32, device='cuda')
+    ref, was = c.pool.clone(), c.pool.clone()
+    for b, rows in enumerate(keep):
+        for j, i in enumerate(rows):
+            s, d = ctx[b] + i, ctx[b] + j
+            ref[c.rows[b][d // page], :, :, :, d % page] = was[c.rows[b][s // page], :, :, :, s % page]
+    base = paged.keep_tokens(c.pool, c.step(), kt, nk)
+    assert base.tolist() == [a + len(k) for a, k in zip(ctx, keep)]
+    assert torch.equal(c.pool, ref)
+
+
+def test_keep_tokens_bad_lists_change_nothing():
+    import ctypes
+
+    from mica_b200 import _native as N
+    from mica_b200 import paged
+    st = torch.cuda.current_stream().cuda_stream
+    code = ctypes.c_int(0)
+    good = [1, 3, 4]
+    for bad, n in (([3, 1, 4], 3), ([1, 1, 2], 3), ([-1, 2, 3], 3), ([1, 2, 8], 3), ([0, 1, 2], 4), ([0, 1, 2], -1)):
+        c = Case([5, 20], [8, 8], 2, 2, 64, 16, layers=2)
+        c.pool.normal_()
+        ref = c.pool.clone()
+        for j, i in enumerate(good):
+            s, d = 20 + i, 20 + j
+            was = ref[c.rows[1][s // 16], :, :, :, s % 16].clone()
+            ref[c.rows[1][d // 16], :, :, :, d % 16] = was
+        N.call('mica_device_error', ctypes.byref(code), st)
+        base = paged.keep_tokens(c.pool, c.step(), torch.tensor([bad, good], dtype=torch.int32, device='cuda'),
+                                 torch.tensor([n, 3], dtype=torch.int32, device='cuda'))
+        N.call('mica_device_error', ctypes.byref(code), st)
+        assert code.value == 9 and base.tolist() == [5, 23]
+        assert torch.equal(c.pool, ref)
+
+
+# ---- the cache object -----------------------------------------------------------------------
+def test_cache_forks_share_pages_until_one_writes():
+    from mica_b200 import paged
+    cache = paged.PagedCache(2, 2, 64, 12, page=16)
+    a = cache.open()
+    cache.step([a], [40])
+    cache.pool.normal_()
+    cache.commit([a], [40])
+    b, c = cache.fork(a), cache.fork(a)
+    assert cache.free_pages == 9 and cache.pages_of(b) == cache.pages_of(a)
+    tail = cache.pages_of(a)[2]
+    cache.step([a, b, c], [1, 20, 1])              # two copies, the last writer keeps the page; b takes two more
+    assert cache.free_pages == 12 - 3 - 2 - 1
+    tails = [cache.pages_of(s)[2] for s in (a, b, c)]
+    assert len(set(tails)) == 3 and tail in tails
+    for t in tails:
+        assert torch.equal(cache.pool[t], cache.pool[tail])
+    cache.commit([b], [2])
+    assert len(cache.pages_of(b)) == 3
+    cache.free(a)
+    cache.free(c)
+    content = torch.cat([cache.pool[p] for p in cache.pages_of(b)])
+    assert cache.compact() == 3
+    assert sorted(cache.pages_of(b)) == [0, 1, 2]
+    assert torch.equal(torch.cat([cache.pool[p] for p in cache.pages_of(b)]), content)
+    cache.free(b)
+    assert cache.free_pages == 12
+
+
+# ---- a run of them together --------------------------------------------------------------------
+def test_a_tree_step_then_keep_equals_the_kept_tokens_appended_alone():
+    """Append a tree, attend, keep one path: the cache and the next token's attention are those of the path
+    appended without the other branches (same positions)."""
+    from mica_b200 import paged
+    heads, kv, dim = 8, 2, 128
+    g = torch.Generator(device='cuda').manual_seed(2)
+    cos, sin = tables(dim)
+    w = (1 + 0.1 * torch.randn(2, dim, generator=g, device='cuda')).bfloat16()
+    cache = paged.PagedCache(1, kv, dim, 20, page=32)
+    k, v = cache.layer(0)
+    rows = torch.randn(100 + 7 + 1, (heads + 2 * kv) * dim, generator=g, device='cuda').bfloat16()
+
+    def go(sid, x, mask=None, pos=None):
+        step = cache.step([sid], [x.shape[0]], mask=mask)
+        q = paged.append(x, w[0], w[1], cos, sin, k, v, step, heads, pos=pos)
+        return step, paged.attention(q, k, v, step, heads)
+
+    a = cache.open()
+    go(a, rows[:100])
+    cache.commit([a], [100])
+    b = cache.fork(a)
+    parents = [[-1, 0, 0, 1, 2, 4, 3]]
+    depth = [0, 1, 1, 2, 2, 3, 3]
+    pos = torch.tensor([100 + d for d in depth], device='cuda')
+    path = [0, 2, 4, 5]
+    step, o = go(a, rows[100:107], paged.tree_mask(parents, 'cuda'), pos)
+    cache.keep([a], step, [path])
+    _, ob = go(b, rows[[100 + i for i in path]])
+    cache.commit([b], [4])
+    # one summation order differs: equal to within the rounding of the weights and outputs
+    assert (o[path].float() - ob.float()).abs().max() <= 2 * U * 4
+    assert cache.length(a) == cache.length(b) == 104
+    ka, kb = (torch.cat([cache.pool[p, 0] for p in cache.pages_of(s)], 2)[:, :, :104] for s in (a, b))
+    assert torch.equal(ka, kb)
+    _, na = go(a, rows[107:])
+    _, nb = go(b, rows[107:])
+    assert torch.equal(na, nb)
