@@ -1,21 +1,47 @@
-// cache_attention.cuh -- grouped-query attention of a step's rows over a paged K/V cache.
+// cache_attention.cuh -- grouped-query attention of a step's rows over a paged K/V cache, on
+// tcgen05 (sm_100a).
 //
 //   o[i, h] = sum_s p_s V[s, h/G],  p = softmax over visible s of scale * q[i, h] . K[s, h/G]
 //
 // Row i of sequence b sees every committed token (s < base[b]) and node j of its own step
 // (s = base[b] + j) when bit j of mask[row] is set, or, without a mask, when j <= i. A row that
 // sees nothing gives zero.
+//
+// What bounds it: for a few rows the K and V bytes (each is read once: 4 D bytes a key and K/V
+// head), for T rows of G heads each above about 250 the tensor cores. So the G heads of a K/V
+// head share its tiles (row r of a 128-row tile is head r % G of node r / G, which a 3-D TMA box of
+// q lays down as it is), and the key axis is cut wherever the SMs need it:
+//
+// Work. A unit is (sequence, K/V head, block of NT * npt nodes); its key tiles of 128 follow one
+// another, units in order, in one line of tiles. Each of the CTAs (one per SM) takes an equal run of
+// that line, whatever the lengths: it starts and may end inside a unit. A unit that one CTA has whole
+// is written out; of a divided one each CTA leaves its unnormalised rows, maxima and sums in its own
+// place of the workspace (a CTA has at most two such: its first and its last), and
+// cache_attention_join adds them up in the order of the CTAs. No atomics: the same bits every time.
+// The lengths are read on the device, so a captured graph serves any.
+//
+// Warps: 0 TMA producer (Q tiles, then K and V tiles page by page: one box per page and 64 columns,
+// one lane each, the page numbers fetched a tile ahead); 1 issues the MMAs (S = Q K^T both from
+// shared memory, O += P V with P in tensor memory); the others softmax, one row a thread, as in
+// attention.cuh. NT = 1: S and P have two buffers each, so scores, softmax and P.V of three
+// consecutive tiles overlap; Q has two, so the next unit's loads run under this one's end. NT = 2:
+// two row tiles share every K and V tile (attention.cuh's schedule).
+// P is rounded to bf16 for the tensor core (V's type): off by 2^-9 of each weight, as the rounding of
+// the output is; its row sum is taken in fp32 before that.
+//
+// Keys that a row does not see get score -inf. A weight of zero still meets its V row in the MMA, and
+// 0 * NaN is not zero: in the tiles that hold nodes of the step or the end of the keys, V rows behind
+// the end are zeroed in shared memory, and an infinite or NaN element of a node's V is replaced by
+// zero and added to the accumulators of the rows that see it, no others.
 #pragma once
 
+#include "attention.cuh"
 #include "cache.cuh"
 
 namespace mica {
 
 struct CacheAttnArgs {
     CachePlan plan;
-    const __nv_bfloat16* q;     // [N, ldq] H heads of D
-    long ldq;
-    const __nv_bfloat16* k_pages;
     const __nv_bfloat16* v_pages;
     long page_stride;           // elements
     const unsigned long long* mask;   // [N, ld_mask] or nullptr (causal)
@@ -23,57 +49,735 @@ struct CacheAttnArgs {
     int words;                  // 64-bit words of a row's mask
     __nv_bfloat16* out;         // [N, ldo]
     long ldo;
-    int H, KV;
+    int KV, G;                  // K/V heads, query heads of each
+    int npt;                    // nodes of a row tile: npt * G <= 128
+    int ctas;                   // CTAs of the grid
     float scale_log2;           // scale * log2(e)
+    float* ws;                  // partials: [ctas][2] places
 };
 
-// Simplest form: one warp per (row, query head), one key at a time, running maximum and sum.
-template <int D>
-__global__ void __launch_bounds__(128) cache_attention_kernel(const CacheAttnArgs a) {
-    constexpr int E = D / 32;
-    const long w = (static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31;
-    if (w >= static_cast<long>(a.plan.N) * a.H) return;
-    const int row = static_cast<int>(w / a.H), h = static_cast<int>(w % a.H);
-    const int kvh = h / (a.H / a.KV);
-    const int b = cache_sequence_of(a.plan, row);
-    float q[E], o[E], m = -INFINITY, l = 0.f;
+// A place of the workspace: rows of O as [NT][D / 4][128] float4 (a warp's rows side by side), then
+// (max, sum) [NT][128].
+template <int D, int NT>
+__host__ __device__ constexpr long cache_attn_place_floats() { return NT * 128l * (D + 2); }
+
+// ---- the line of tiles ----------------------------------------------------------------
+struct CacheSeq {
+    int row0, T, base, keys;    // first row, rows, committed tokens, keys (0: not usable)
+};
+__device__ __forceinline__ CacheSeq cache_seq(const CachePlan& p, int b) {
+    CacheSeq s;
+    s.row0 = p.cu[b];
+    s.T = p.cu[b + 1] - s.row0;
+    s.base = p.base[b];
+    if (s.row0 < 0 || s.T < 0 || s.row0 > p.N || s.T > p.N - s.row0) s.T = 0;
+    const long keys = static_cast<long>(s.base) + s.T;
+    s.keys = s.base < 0 || keys > (static_cast<long>(p.P) << p.page_log2) ? 0 : static_cast<int>(keys);
+    return s;
+}
+// Key tiles of the row block `rb` (R nodes each): all keys under a mask, else up to its last node.
+// At least one, so that every row is written.
+__device__ __forceinline__ int cache_unit_tiles(const CacheSeq& s, int rb, int R, bool causal) {
+    int keys = s.keys;
+    if (causal && keys) keys = s.base + min(s.T, (rb + 1) * R);
+    return max(1, (keys + 127) >> 7);
+}
+__device__ __forceinline__ int cache_row_blocks(const CacheSeq& s, int R) { return (s.T + R - 1) / R; }
+__device__ __forceinline__ long cache_seq_tiles(const CacheSeq& s, int R, bool causal) {   // of one K/V head
+    const int n = cache_row_blocks(s, R);
+    if (!causal || n <= 1) return n ? static_cast<long>(n) * cache_unit_tiles(s, n - 1, R, causal) : 0;
+    long t = 0;
+    for (int rb = 0; rb < n; ++rb) t += cache_unit_tiles(s, rb, R, true);
+    return t;
+}
+
+struct CachePlace {             // a position in the line: tile `off` of sequence b
+    long total;
+    long off;
+    int b;
+};
+// Total tiles and the sequence that holds tile `first(total)`; every thread of the block calls it.
+template <typename F>
+__device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, int R, bool causal, F first) {
+    __shared__ long s_warp[32];
+    __shared__ long s_off;
+    __shared__ int s_b;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
+    const auto scan = [&](long v, long& all) {       // inclusive over the block
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        q[e] = __bfloat162float(a.q[static_cast<long>(row) * a.ldq + static_cast<long>(h) * D + lane + 32 * e]) * a.scale_log2;
-        o[e] = 0.f;
-    }
-    if (b >= 0) {
-        const int base = a.plan.base[b], first = a.plan.cu[b];
-        const int rows = min(a.plan.cu[b + 1], a.plan.N) - first;
-        bool bad = base < 0;
-        for (long s = 0; s < static_cast<long>(base) + rows && !bad; ++s) {
-            const long j = s - base;
-            if (j >= 0) {
-                const bool seen = a.mask ? j < 64l * a.words && (a.mask[row * a.ld_mask + (j >> 6)] >> (j & 63) & 1)
-                                         : j <= row - first;
-                if (!seen) continue;
-            }
-            int page, slot;
-            if (!cache_slot(a.plan, b, s, &page, &slot)) { bad = true; break; }
-            const long off = static_cast<long>(page) * a.page_stride + ((static_cast<long>(kvh) << a.plan.page_log2) + slot) * D;
-            float z = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) z += q[e] * __bfloat162float(a.k_pages[off + lane + 32 * e]);
-            z = warp_sum(z);
-            const float mn = fmaxf(m, z);
-            const float al = m == -INFINITY ? 0.f : exp2f(m - mn), p = mn == -INFINITY ? 0.f : exp2f(z - mn);
-            l = l * al + p;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = o[e] * al + p * __bfloat162float(a.v_pages[off + lane + 32 * e]);
-            m = mn;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
         }
-        if (bad && lane == 0) record_bad_page();
+        __syncthreads();
+        if (lane == 31) s_warp[warp] = v;
+        __syncthreads();
+        all = 0;
+        for (int i = 0; i < warps; ++i) {
+            if (i < warp) v += s_warp[i];
+            all += s_warp[i];
+        }
+        return v;
+    };
+    const auto tiles = [&](int b) { return b < p.B ? KV * cache_seq_tiles(cache_seq(p, b), R, causal) : 0l; };
+    const long mine = tiles(threadIdx.x);
+    long sum = mine, total = 0;
+    for (int b = threadIdx.x + blockDim.x; b < p.B; b += blockDim.x) sum += tiles(b);
+    scan(sum, total);
+    const long t = first(total);
+    if (threadIdx.x == 0) { s_b = -1; s_off = 0; }
+    long before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
+        const long n = b0 == 0 ? mine : tiles(b0 + threadIdx.x);
+        long all = 0;
+        const long end = before + scan(n, all);      // its barriers order s_b's first write
+        if (t >= end - n && t < end) {
+            s_b = b0 + threadIdx.x;
+            s_off = t - (end - n);
+        }
+        before += all;
+        if (before > t) break;
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    __syncthreads();
+    return CachePlace{total, s_off, s_b};
+}
+
+// Tiles [lo, hi) of CTA c, of `ctas` (fewer are used when there are fewer tiles).
+__device__ __forceinline__ long cache_share(long total, int ctas, int c) {
+    return ctas <= 0 ? 0 : (total * c) / ctas;
+}
+__device__ __forceinline__ int cache_used_ctas(long total, int ctas) {
+    return static_cast<int>(total < ctas ? total : ctas);
+}
+
+// The units of a CTA's run, one after another.
+struct CacheWalk {
+    CacheSeq s;
+    int b, kvh, rb;             // unit
+    int nk, j0, j1;             // its tiles, and the CTA's [j0, j1) of them
+    long left;                  // tiles of the run from j0 on
+    int R;
+    bool causal;
+
+    __device__ __forceinline__ void start(const CachePlan& p, int R_, bool causal_, int b_, long off, long n) {
+        R = R_; causal = causal_; b = b_; left = n;
+        s = cache_seq(p, b);
+        const long per = cache_seq_tiles(s, R, causal);
+        kvh = static_cast<int>(off / per);
+        off -= kvh * per;
+        rb = 0;
+        while (off >= (nk = cache_unit_tiles(s, rb, R, causal))) { off -= nk; ++rb; }
+        j0 = static_cast<int>(off);
+        j1 = static_cast<int>(min(static_cast<long>(nk), j0 + left));
+    }
+    __device__ __forceinline__ bool next(const CachePlan& p, int KV) {
+        left -= j1 - j0;
+        if (left <= 0) return false;
+        if (++rb >= cache_row_blocks(s, R)) {
+            rb = 0;
+            if (++kvh >= KV) {
+                kvh = 0;
+                do {
+                    if (++b >= p.B) return false;
+                    s = cache_seq(p, b);
+                } while (s.T == 0);
+            }
+        }
+        nk = cache_unit_tiles(s, rb, R, causal);
+        j0 = 0;
+        j1 = static_cast<int>(min(static_cast<long>(nk), left));
+        return true;
+    }
+    __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == nk; }
+    // a tile that holds nodes of the step, or the end of the keys
+    __device__ __forceinline__ bool special(int j) const { return (j + 1) * 128 > s.base || s.keys == 0; }
+};
+
+template <int D, int NT>
+struct CacheAttnShape {
+    static constexpr int HALVES = D / 64;
+    static constexpr int TILE = 128 * D * 2;
+    static constexpr int QBUF = NT == 1 ? 2 : 1;
+    static constexpr int KST = D == 128 ? 3 : 6;
+    static constexpr int VST = D == 128 ? 2 : 5;
+    static constexpr int THREADS = 64 + 128 * NT;
+    static constexpr int BARS = 512;
+    static constexpr int SMEM = 1024 + TILE * (QBUF * NT + KST + VST) + BARS;
+};
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Bits [off, off + 32) of a row's mask words, bits outside them zero.
+__device__ __forceinline__ uint32_t mask_bits(const unsigned long long* m, int words, int off) {
+    if (off <= -32) return 0u;
+    if (off < 0) return static_cast<uint32_t>(m[0] << -off);
+    const int w = off >> 6, sh = off & 63;
+    if (w >= words) return 0u;
+    unsigned long long v = m[w] >> sh;
+    if (sh > 32 && w + 1 < words) v |= m[w + 1] << (64 - sh);
+    return static_cast<uint32_t>(v);
+}
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+template <int D, int NT>
+__global__ void __launch_bounds__(CacheAttnShape<D, NT>::THREADS, 1)
+cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                       const __grid_constant__ CUtensorMap tmap_v, const CacheAttnArgs args) {
+    using S = CacheAttnShape<D, NT>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const CachePlan& plan = args.plan;
+    const bool causal = args.mask == nullptr;
+    const int R = NT * args.npt;
+
+    // padding rows
+    {
+        const int end = min(max(plan.cu[plan.B], 0), plan.N);
+        const int vecs = args.KV * args.G * D / 8;
+        for (long row = end + static_cast<long>(blockIdx.x); row < plan.N; row += gridDim.x)
+            for (int i = threadIdx.x; i < vecs; i += blockDim.x)
+                *reinterpret_cast<uint4*>(args.out + row * args.ldo + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    // this CTA's run of tiles
+    const int cta = blockIdx.x;
+    const CachePlace place = cache_locate(plan, args.KV, R, causal, [&](long total) {
+        return cache_share(total, cache_used_ctas(total, args.ctas), cta);
+    });
+    const int used = cache_used_ctas(place.total, args.ctas);
+    if (cta >= used || place.b < 0) return;
+    const long run = cache_share(place.total, used, cta + 1) - cache_share(place.total, used, cta);
+    CacheWalk wk;
+    wk.start(plan, R, causal, place.b, place.off, run);
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* sq = smem;
+    uint8_t* sk = sq + S::QBUF * NT * S::TILE;
+    uint8_t* sv = sk + S::KST * S::TILE;
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(sv + S::VST * S::TILE);   // [QBUF]
+    uint64_t* q_empty = q_full + 2;
+    uint64_t* k_full = q_empty + 2;
+    uint64_t* k_empty = k_full + S::KST;
+    uint64_t* v_full = k_empty + S::KST;
+    uint64_t* v_empty = v_full + S::VST;
+    uint64_t* s_full = v_empty + S::VST;       // [2] scores written: by buffer (NT 1) or row tile (NT 2)
+    uint64_t* s_free = s_full + 2;             // [2] scores read
+    uint64_t* p_full = s_free + 2;             // [2] P written
+    uint64_t* pv_done = p_full + 2;            // [2] P.V finished
+    uint64_t* v_fixed = pv_done + 2;           // V of a special tile made safe (all softmax warps)
+    uint64_t* drain = v_fixed + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+    uint32_t* odd_v = tmem_slot + 2;           // [2][4] keys of a special tile whose V row holds infinities or NaN
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&s_free[i], 4);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&pv_done[i], 1);
+        }
+        for (int i = 0; i < S::KST; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
+        for (int i = 0; i < S::VST; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
+        mbar_init(v_fixed, 4 * NT);
+        mbar_init(drain, 1);
+        *abort_flag = 0u;
+        fence_mbar_init();
+        tma_prefetch_desc(&tmap_q);
+        tma_prefetch_desc(&tmap_k);
+        tma_prefetch_desc(&tmap_v);
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    // tensor memory columns: NT 1: S [0,128) [128,256) P [256,320) [320,384) O [384,512);
+    //                        NT 2: S [0,128) P [128,192) [192,256) O [256,384) [384,512)
+    const auto col_s = [](int i) { return NT == 1 ? i * 128 : 0; };
+    const auto col_p = [](int i) { return (NT == 1 ? 256 : 128) + i * 64; };
+    const auto col_o = [](int x) { return NT == 1 ? 384 : 256 + x * 128; };
+
+    if (warp == 0) {
+        // ---------------------------------- producer ----------------------------------
+        const int ppt = 128 >> plan.page_log2;             // pages of a key tile
+        const int boxes = ppt * S::HALVES;                 // <= 16, lane i: page i / HALVES, columns 64 (i % HALVES)
+        const int my_page = lane / S::HALVES, my_half = lane % S::HALVES;
+        const uint32_t box_bytes = 128u << plan.page_log2;
+        const int page = 1 << plan.page_log2;
+        bool ok = true;
+        int kt = 0, vt = 0;                               // tiles loaded
+        int unit = 0;
+        // pages of key tile j of the walk's unit that hold keys; this lane's page number
+        const auto pages_in = [&](const CacheWalk& w, int j) {
+            return max(0, min(ppt, (w.s.keys - j * 128 + page - 1) >> plan.page_log2));
+        };
+        const auto fetch = [&](const CacheWalk& w, int j) {
+            return lane < boxes && my_page < pages_in(w, j)
+                       ? plan.table[static_cast<long>(w.b) * plan.ld_table + j * ppt + my_page] : 0;
+        };
+        const auto load = [&](bool is_k, int t, int n_pages, int kvh, int pg) {
+            const int st = is_k ? t % S::KST : t % S::VST;
+            const uint32_t par = ((is_k ? t / S::KST : t / S::VST) & 1u) ^ 1u;
+            uint64_t* full = is_k ? &k_full[st] : &v_full[st];
+            bool w = true;
+            if (lane == 0) {
+                w = mbar_wait(is_k ? &k_empty[st] : &v_empty[st], par, abort_flag, MICA_DEV_TIMEOUT_PRODUCER);
+                if (w) mbar_arrive_expect_tx(full, n_pages * S::HALVES * box_bytes);
+            }
+            if (!__shfl_sync(0xffffffffu, w, 0)) return false;
+            if (lane < n_pages * S::HALVES) {
+                uint8_t* d = (is_k ? sk : sv) + st * S::TILE + my_half * ATT_HALF_BYTES + my_page * box_bytes;
+                // a page outside the pool is outside the map and reads as zeros
+                if (pg < 0 || pg >= plan.pages) { pg = plan.pages; record_bad_page(); }
+                tma_load_3d(d, is_k ? &tmap_k : &tmap_v, full, my_half * 64, kvh << plan.page_log2, pg);
+            }
+            __syncwarp();
+            return true;
+        };
+        int v_pages = 0, v_kvh = 0, v_pg = 0;              // the tile whose V is still to come
+        bool more = true, pending = false;
+        const auto load_v = [&]() {
+            pending = false;
+            return load(false, vt++, v_pages, v_kvh, v_pg);
+        };
+        int pg = fetch(wk, wk.j0);
+        while (more && ok) {
+            if (wk.s.keys == 0 && lane == 0) record_bad_page();
+            // Q tiles of the unit
+            const int qb = S::QBUF == 2 ? unit & 1 : 0;
+            const uint32_t q_par = static_cast<uint32_t>(unit / S::QBUF & 1) ^ 1u;
+            // with one Q buffer the wait is for the scores of the unit's last tile, whose softmax may want V first
+            if (S::QBUF == 1 && pending && !load_v()) { ok = false; break; }
+            bool w = true;
+            if (lane == 0) {
+                w = mbar_wait(&q_empty[qb], q_par, abort_flag, MICA_DEV_TIMEOUT_PRODUCER);
+                if (w) {
+                    mbar_arrive_expect_tx(&q_full[qb], NT * S::HALVES * 128u * args.npt * args.G);
+                    for (int x = 0; x < NT; ++x)
+                        for (int h = 0; h < S::HALVES; ++h)
+                            tma_load_3d(sq + (qb * NT + x) * S::TILE + h * ATT_HALF_BYTES, &tmap_q, &q_full[qb], h * 64,
+                                        wk.kvh * args.G, wk.s.row0 + (wk.rb * NT + x) * args.npt);
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, w, 0);
+            for (int j = wk.j0; j < wk.j1 && ok; ++j) {
+                const int n_pages = pages_in(wk, j), kvh = wk.kvh, cur = pg;
+                ok = load(true, kt, n_pages, kvh, cur);
+                // the next tile's page number, a tile ahead of its use
+                if (j + 1 < wk.j1) pg = fetch(wk, j + 1);
+                else { more = wk.next(plan, args.KV); if (more) pg = fetch(wk, wk.j0); j = wk.j1; }
+                ++kt;
+                if (ok && pending) ok = load_v();
+                v_pages = n_pages; v_kvh = kvh; v_pg = cur;
+                pending = true;
+            }
+            ++unit;
+        }
+        if (ok && pending) ok = load_v();
+        // loads still in flight land before shared memory is released
+        if (lane == 0) {
+            for (int i = max(0, unit - S::QBUF); i < unit; ++i)
+                mbar_wait(&q_full[S::QBUF == 2 ? i & 1 : 0], i / S::QBUF & 1, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
+            for (int t = kt > S::KST ? kt - S::KST : 0; t < kt; ++t)
+                mbar_wait(&k_full[t % S::KST], (t / S::KST) & 1, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
+            for (int t = vt > S::VST ? vt - S::VST : 0; t < vt; ++t)
+                mbar_wait(&v_full[t % S::VST], (t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---------------------------------- MMA issuer --------------------------------
+        if (lane == 0) {
+            constexpr uint32_t idesc_qk = idesc_bf16(128, 128, false);
+            constexpr uint32_t idesc_pv = idesc_bf16(128, D, true);
+            const uint64_t q_desc0 = smem_desc_sw128(smem_u32(sq), 16, 1024);
+            const uint64_t k_desc0 = smem_desc_sw128(smem_u32(sk), 16, 1024);
+            const uint64_t v_desc0 = smem_desc_sw128(smem_u32(sv), ATT_HALF_BYTES, 1024);
+            constexpr uint64_t kStep = S::TILE >> 4;
+            bool ok = true;
+            int fills = 0;                       // score tiles issued (NT 2: of both row tiles)
+            // scores of row tile x with key tile t (counted over the run) of the unit's Q in buffer qb
+            const auto scores = [&](int x, int t, int qb) {
+                const int i = NT == 1 ? (t & 1) : x;
+                if (NT == 1) {
+                    if (t >= 2 && !mma_wait(&s_free[i], ((t >> 1) - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+                } else {
+                    if (fills > 0 && !mma_wait(&s_free[0], (fills - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+                    ++fills;
+                }
+                tc_fence_after();
+                const uint64_t qd = q_desc0 + static_cast<uint64_t>(qb * NT + x) * kStep;
+                const uint64_t kd = k_desc0 + static_cast<uint64_t>(t % S::KST) * kStep;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        a.out[static_cast<long>(row) * a.ldo + static_cast<long>(h) * D + lane + 32 * e] = __float2bfloat16_rn(o[e] * inv);
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint64_t off = static_cast<uint64_t>(((kk >> 2) * ATT_HALF_BYTES + (kk & 3) * 32) >> 4);
+                    mma_bf16_ss(tmem + col_s(i), qd + off, kd + off, idesc_qk, kk > 0 ? 1u : 0u);
+                }
+                mma_commit(&s_full[i]);
+                return true;
+            };
+            const auto values = [&](int x, int t, bool fresh) {
+                const int i = NT == 1 ? (t & 1) : x;
+                const uint32_t par = static_cast<uint32_t>(NT == 1 ? t >> 1 : t) & 1u;
+                if (!mma_wait(&p_full[i], par, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+                tc_fence_after();
+                const uint64_t vd = v_desc0 + static_cast<uint64_t>(t % S::VST) * kStep;
+                const uint32_t o = tmem + col_o(x), p = tmem + col_p(i);
+                mma_bf16_ts(o, p, vd, idesc_pv, fresh ? 0u : 1u);
+#pragma unroll
+                for (int kk = 1; kk < 8; ++kk) mma_bf16_ts(o, p + kk * 8, vd + ((kk * 16 * 128) >> 4), idesc_pv, 1u);
+                mma_commit(&pv_done[i]);
+                return true;
+            };
+            // the scores of a tile are issued before the P.V of the tile before it, across units too
+            CacheWalk pv = wk;                    // the unit of the next P.V
+            bool more = true;
+            int t = 0, unit = 0, pv_t = 0;
+            int pv_j = pv.j0;
+            const auto values_all = [&](int x) {
+                // the first tile of a unit starts the accumulator, except where the softmax has set it
+                const bool fresh = pv_j == pv.j0 && !pv.special(pv_j);
+                return values(x, pv_t, fresh);
+            };
+            const auto values_done = [&]() {
+                mma_commit(&v_empty[pv_t % S::VST]);
+                ++pv_t;
+                if (++pv_j == pv.j1 && pv.next(plan, args.KV)) pv_j = pv.j0;
+            };
+            while (more && ok) {
+                const int qb = S::QBUF == 2 ? unit & 1 : 0;
+                ok = mma_wait(&q_full[qb], unit / S::QBUF & 1, abort_flag, MICA_DEV_TIMEOUT_MMA);
+                for (int j = wk.j0; j < wk.j1 && ok; ++j, ++t) {
+                    if (!mma_wait(&k_full[t % S::KST], (t / S::KST) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA) ||
+                        !scores(0, t, qb)) { ok = false; break; }
+                    if (NT == 1) {
+                        mma_commit(&k_empty[t % S::KST]);
+                        if (j + 1 == wk.j1) mma_commit(&q_empty[qb]);
+                    }
+                    if (t > 0) {
+                        if (!mma_wait(&v_full[pv_t % S::VST], (pv_t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA) ||
+                            !values_all(0)) { ok = false; break; }
+                    }
+                    if (NT == 2) {
+                        if (!scores(1, t, qb)) { ok = false; break; }
+                        mma_commit(&k_empty[t % S::KST]);
+                        if (j + 1 == wk.j1) mma_commit(&q_empty[qb]);
+                        if (t > 0 && !values_all(1)) { ok = false; break; }
+                    }
+                    if (t > 0) values_done();
+                }
+                if (ok) { more = wk.next(plan, args.KV); ++unit; }
+            }
+            if (ok && mma_wait(&v_full[pv_t % S::VST], (pv_t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) {
+                for (int x = 0; x < NT && ok; ++x) ok = values_all(x);
+            }
+            mma_commit(drain);
+            mbar_wait(drain, 0, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------- softmax ----------------------------------
+        const int x = (warp - 2) >> 2;                     // row tile of this warpgroup
+        const int q4 = warp & 3;                           // tensor-memory lane quarter
+        const int r = q4 * 32 + lane;                      // row of the tile
+        const int node_r = r / args.G, head_r = r % args.G;
+        const uint32_t lane_off = static_cast<uint32_t>(q4 * 32) << 16;
+        const float c = args.scale_log2;
+        bool ok = true, more = true, first = true;
+        int t = 0;                                         // key tiles so far
+        int fixes = 0;                                     // special tiles so far
+        while (more && ok) {
+            const CacheSeq& s = wk.s;
+            const int node0 = (wk.rb * NT + x) * args.npt;            // first node of the tile
+            const int nodes = max(0, min(args.npt, s.T - node0));
+            const bool live = node_r < nodes;                         // this thread has a row
+            const bool warp_live = q4 * 32 < nodes * args.G;          // some thread of the warp has
+            const int node = node0 + node_r;
+            const long row = static_cast<long>(s.row0) + node;
+            const uint32_t t_o = tmem + col_o(x) + lane_off;
+            float m_use = -1e30f, l = 0.f;
+            for (int j = wk.j0; j < wk.j1; ++j, ++t) {
+                const int i2 = NT == 1 ? (t & 1) : x;
+                const int n2 = NT == 1 ? t >> 1 : t;                   // uses of that buffer before
+                const uint32_t t_s = tmem + col_s(i2) + lane_off, t_p = tmem + col_p(i2) + lane_off;
+                const bool special = wk.special(j);
+                const int k0 = j * 128;
+                // visible keys of this row, one bit each
+                uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                if (special) {
+                    const int end = causal ? min(s.keys, s.base + node + 1) : s.keys;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        vis[w] = live ? low_bits(end - k0 - 32 * w) : 0u;
+                        if (!causal && live && s.keys)
+                            vis[w] &= low_bits(s.base - k0 - 32 * w) |
+                                      mask_bits(args.mask + row * args.ld_mask, args.words, k0 + 32 * w - s.base);
+                    }
+                    // V rows behind the keys become zero; odd values of the step's own rows too, noted
+                    // (two sets of odd_v: all warps pass v_fixed of a special tile before one writes the next but one)
+                    const int st = t % S::VST;
+                    bool odd = false;
+                    if (x == 0) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
+                        if (!ok) break;
+                        const int key = k0 + r;
+                        uint4* vr = reinterpret_cast<uint4*>(sv + st * S::TILE + r * 128);
+                        if (key >= s.keys || key >= s.base) {
+#pragma unroll
+                            for (int h = 0; h < S::HALVES; ++h)
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    uint4* p = vr + h * (ATT_HALF_BYTES / 16) + (e ^ (r & 7));
+                                    if (key >= s.keys) { *p = make_uint4(0u, 0u, 0u, 0u); continue; }
+                                    uint4 v = *p;
+                                    uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+                                    bool hit = false;
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) {
+                                        if ((u[k] & 0x7f800000u) == 0x7f800000u) { u[k] &= 0x0000ffffu; hit = true; }
+                                        if ((u[k] & 0x00007f80u) == 0x00007f80u) { u[k] &= 0xffff0000u; hit = true; }
+                                    }
+                                    if (hit) { *p = v; odd = true; }
+                                }
+                        }
+                        const uint32_t bits = __ballot_sync(0xffffffffu, odd);
+                        if (lane == 0) odd_v[(fixes & 1) * 4 + q4] = bits;
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive(v_fixed);
+                }
+                bool w = true;
+                if (lane == 0) w = mma_wait(&s_full[i2], n2 & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
+                if (!__shfl_sync(0xffffffffu, w, 0)) { ok = false; break; }
+                tc_fence_after();
+                bool moved = false;                                  // the running maximum of a row
+                float alpha = 1.f;
+                uint32_t pk[64];
+                if (warp_live) {
+                    uint32_t sr[128];
+#pragma unroll
+                    for (int cc = 0; cc < 4; ++cc)
+                        tmem_ld_32x32b_x32(t_s + cc * 32, *reinterpret_cast<uint32_t (*)[32]>(&sr[cc * 32]));
+                    tmem_ld_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_free[NT == 1 ? i2 : 0]);
+                    if (special) {
+#pragma unroll
+                        for (int i = 0; i < 128; ++i)
+                            if (!(vis[i >> 5] >> (i & 31) & 1u)) sr[i] = 0xff800000u;
+                    }
+                    float mp[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        mp[e] = fmax3(__uint_as_float(sr[e]), __uint_as_float(sr[8 + e]), __uint_as_float(sr[16 + e]));
+#pragma unroll
+                    for (int i = 24; i < 128; i += 16)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            mp[e] = i + 8 + e < 128 ? fmax3(mp[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 8 + e]))
+                                                    : fmaxf(mp[e], __uint_as_float(sr[i + e]));
+                    const float mx = fmax3(fmax3(mp[0], mp[1], mp[2]), fmax3(mp[3], mp[4], mp[5]), fmaxf(mp[6], mp[7])) * c;
+                    if (mx > m_use + ATT_RESCALE_LOG2) {
+                        alpha = fast_exp2(m_use - mx);
+                        m_use = mx;
+                        moved = true;
+                    }
+                    const unsigned long long c2 = f2_pack(c, c), nm2 = f2_pack(-m_use, -m_use);
+                    unsigned long long sp[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        const unsigned long long x2 =
+                            f2_fma(f2_pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), c2, nm2);
+                        float x0, x1;
+                        f2_unpack(x2, x0, x1);
+                        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+                        sp[i & 3] = f2_add(sp[i & 3], f2_pack(p0, p1));
+                        pk[i] = pack_bf16(p0, p1);
+                    }
+                    float a0, a1, b0, b1, d0, d1, e0, e1;
+                    f2_unpack(sp[0], a0, a1);
+                    f2_unpack(sp[1], b0, b1);
+                    f2_unpack(sp[2], d0, d1);
+                    f2_unpack(sp[3], e0, e1);
+                    l = l * alpha + (((a0 + a1) + (b0 + b1)) + ((d0 + d1) + (e0 + e1)));
+                } else {
+                    if (lane == 0) mbar_arrive(&s_free[NT == 1 ? i2 : 0]);
+                }
+                // this P buffer is free once its last P.V is done; the accumulator once the tile before's is
+                bool any_odd = false;
+                const volatile uint32_t* odd4 = odd_v + (fixes & 1) * 4;
+                if (special) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(v_fixed, fixes & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
+                    if (!ok) break;
+                    any_odd = (odd4[0] | odd4[1] | odd4[2] | odd4[3]) != 0u;
+                    ++fixes;
+                }
+                const bool fresh = j == wk.j0;
+                const bool touch = warp_live && (special && fresh || any_odd ||
+                                                 (!fresh && __any_sync(0xffffffffu, moved)));
+                if (lane == 0) {
+                    w = n2 == 0 || mma_wait(&pv_done[i2], (n2 - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
+                    if (NT == 1 && w && touch && t >= 1)
+                        w = mma_wait(&pv_done[i2 ^ 1], ((t - 1) >> 1) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
+                }
+                if (!__shfl_sync(0xffffffffu, w, 0)) { ok = false; break; }
+                tc_fence_after();
+                if (touch) {
+#pragma unroll 1
+                    for (int cc = 0; cc < D / 32; ++cc) {
+                        uint32_t o[32];
+                        if (fresh) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = 0u;
+                        } else {
+                            tmem_ld_32x32b_x32(t_o + cc * 32, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        }
+                        if (any_odd) {
+                            for (int w4 = 0; w4 < 4; ++w4)
+                                for (uint32_t bits = odd4[w4]; bits; bits &= bits - 1) {
+                                    const int i = __ffs(bits) - 1;
+                                    int pgn = 0, slot = 0;
+                                    if (!(vis[w4] >> i & 1u) || !cache_slot(plan, wk.b, k0 + w4 * 32 + i, &pgn, &slot)) continue;
+                                    const uint16_t* v = reinterpret_cast<const uint16_t*>(args.v_pages) + pgn * args.page_stride +
+                                                        ((static_cast<long>(wk.kvh) << plan.page_log2) + slot) * D + cc * 32;
+#pragma unroll
+                                    for (int e = 0; e < 32; ++e) {
+                                        const uint32_t u = v[e];
+                                        if ((u & 0x7f80u) == 0x7f80u)
+                                            o[e] = __float_as_uint(__uint_as_float(o[e]) + __uint_as_float(u << 16));
+                                    }
+                                }
+                        }
+                        __syncwarp();
+                        tmem_st_32x32b_x32(t_o + cc * 32, o);
+                    }
+                }
+                if (warp_live) {
+                    tmem_st_32x32b_x32(t_p, *reinterpret_cast<uint32_t (*)[32]>(&pk[0]));
+                    tmem_st_32x32b_x32(t_p + 32, *reinterpret_cast<uint32_t (*)[32]>(&pk[32]));
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[i2]);
+            }
+            if (!ok) break;
+            // the unit's rows: out, or this CTA's place in the workspace
+            {
+                const int tl = t - 1;
+                const int i2 = NT == 1 ? (tl & 1) : x;
+                const int n2 = NT == 1 ? tl >> 1 : tl;
+                bool w = true;
+                if (lane == 0) w = mbar_wait(&pv_done[i2], n2 & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
+                if (!__shfl_sync(0xffffffffu, w, 0)) { ok = false; break; }
+                tc_fence_after();
+                if (warp_live) {
+                    const bool whole = wk.whole();
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    float4* part = reinterpret_cast<float4*>(args.ws + (cta * 2l + (first ? 0 : 1)) * cache_attn_place_floats<D, NT>()) +
+                                   x * (D / 4) * 128 + r;
+                    __nv_bfloat16* orow = args.out + row * args.ldo + (wk.kvh * args.G + head_r) * D;
+#pragma unroll
+                    for (int cc = 0; cc < D / 32; ++cc) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(t_o + cc * 32, o);
+                        tmem_ld_wait();
+                        if (live && whole) {
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) {
+                                uint4 pkt;
+                                pkt.x = pack_bf16(__uint_as_float(o[8 * v + 0]) * inv, __uint_as_float(o[8 * v + 1]) * inv);
+                                pkt.y = pack_bf16(__uint_as_float(o[8 * v + 2]) * inv, __uint_as_float(o[8 * v + 3]) * inv);
+                                pkt.z = pack_bf16(__uint_as_float(o[8 * v + 4]) * inv, __uint_as_float(o[8 * v + 5]) * inv);
+                                pkt.w = pack_bf16(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv);
+                                *reinterpret_cast<uint4*>(orow + cc * 32 + v * 8) = pkt;
+                            }
+                        } else if (live) {
+#pragma unroll
+                            for (int v = 0; v < 8; ++v)
+                                part[(cc * 8 + v) * 128] = make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]),
+                                                                       __uint_as_float(o[4 * v + 2]), __uint_as_float(o[4 * v + 3]));
+                        }
+                    }
+                    if (live && !whole) {
+                        float2* ml = reinterpret_cast<float2*>(args.ws + (cta * 2l + (first ? 0 : 1)) * cache_attn_place_floats<D, NT>() +
+                                                               NT * 128l * D);
+                        ml[x * 128 + r] = make_float2(m_use, l);
+                    }
+                    tc_fence_before();
+                }
+            }
+            first = false;
+            more = wk.next(plan, args.KV);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_free(tmem, 512);
+    }
+}
+
+// Adds up the parts of each divided unit. Block (c, y): the unit that CTA c + 1's run starts inside,
+// if c + 1 is the first to do so; its rows x columns are dealt to the blocks y.
+template <int D, int NT>
+__global__ void __launch_bounds__(128) cache_attention_join(const CacheAttnArgs args) {
+    const CachePlan& plan = args.plan;
+    const bool causal = args.mask == nullptr;
+    const int R = NT * args.npt;
+    const int c = blockIdx.x + 1;
+    const CachePlace place = cache_locate(plan, args.KV, R, causal, [&](long total) {
+        return cache_share(total, cache_used_ctas(total, args.ctas), c);
+    });
+    const int used = cache_used_ctas(place.total, args.ctas);
+    if (c >= used || place.b < 0) return;
+    const auto at = [&](int i) { return cache_share(place.total, used, i); };
+    CacheWalk wk;
+    wk.start(plan, R, causal, place.b, place.off, 1);
+    if (wk.j0 == 0) return;                                   // starts with its unit
+    const long s0 = at(c) - wk.j0, s1 = s0 + wk.nk;           // the unit's tiles
+    if (at(c - 1) > s0) return;                               // CTA c - 1 starts inside it as well
+    int n = 1;                                                // CTAs c - 1 .. c - 1 + n
+    while (c + n < used && at(c + n) < s1) ++n;
+    const int rows = min(R, wk.s.T - wk.rb * R) * args.G;
+    const long pf = cache_attn_place_floats<D, NT>();
+    const int first_place = at(c - 1) == s0 ? 0 : 1;
+    for (int idx = blockIdx.y * blockDim.x + threadIdx.x; idx < rows * (D / 4); idx += gridDim.y * blockDim.x) {
+        const int rr = idx % rows, d4 = idx / rows;
+        const int node = rr / args.G, g = rr % args.G;
+        const int x = node / args.npt, r = (node - x * args.npt) * args.G + g;
+        const auto ml = [&](int i) {
+            return *reinterpret_cast<const float2*>(args.ws + ((c - 1 + i) * 2l + (i ? 0 : first_place)) * pf + NT * 128l * D + (x * 128 + r) * 2);
+        };
+        float m = -INFINITY;
+        for (int i = 0; i <= n; ++i) m = fmaxf(m, ml(i).x);
+        float l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i <= n; ++i) {
+            const float2 v = ml(i);
+            const float w = fast_exp2(v.x - m);
+            const float4 p = *(reinterpret_cast<const float4*>(args.ws + ((c - 1 + i) * 2l + (i ? 0 : first_place)) * pf) + (x * (D / 4) + d4) * 128 + r);
+            l = fmaf(v.y, w, l);
+            o.x = fmaf(p.x, w, o.x); o.y = fmaf(p.y, w, o.y); o.z = fmaf(p.z, w, o.z); o.w = fmaf(p.w, w, o.w);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const long row = static_cast<long>(wk.s.row0) + wk.rb * R + node;
+        *reinterpret_cast<uint2*>(args.out + row * args.ldo + (wk.kvh * args.G + g) * D + d4 * 4) =
+            make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    }
 }
 
 }  // namespace mica

@@ -84,8 +84,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 static std::once_flag g_encode_once;
 
-int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t inner, uint64_t outer,
-                 uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer) {
+static int load_encode() {
     std::call_once(g_encode_once, [] {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -97,11 +96,36 @@ int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, 
         snprintf(t_err, sizeof(t_err), "cuTensorMapEncodeTiled entry point not found");
         return MICA_ERR_CUDA;
     }
+    return MICA_OK;
+}
+
+int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t inner, uint64_t outer,
+                 uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer) {
+    if (int rc = load_encode()) return rc;
     const cuuint64_t dims[2] = {inner, outer};
     const cuuint64_t strides[1] = {row_bytes};
     const cuuint32_t box[2] = {box_inner, box_outer};
     const cuuint32_t estr[2] = {1, 1};
     CUresult r = g_encode(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        snprintf(t_err, sizeof(t_err), "cuTensorMapEncodeTiled failed: CUresult %d", static_cast<int>(r));
+        return MICA_ERR_CUDA;
+    }
+    return MICA_OK;
+}
+
+// A 3-D map of bf16: dims {x, y, z} with byte strides of y and z, box {64, box_y, box_z}, 128-byte
+// swizzle, zero fill out of bounds.
+static int make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t x, uint64_t y, uint64_t z, uint64_t y_bytes,
+                             uint64_t z_bytes, uint32_t box_y, uint32_t box_z) {
+    if (int rc = load_encode()) return rc;
+    const cuuint64_t dims[3] = {x, y, z};
+    const cuuint64_t strides[2] = {y_bytes, z_bytes};
+    const cuuint32_t box[3] = {64, box_y, box_z};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
@@ -1099,7 +1123,47 @@ int mica_cache_append(const void* qkv, long ld, const void* q_w, const void* k_w
     return launch_status();
 }
 
-size_t mica_cache_attention_workspace_bytes(int N, int max_new, int H, int KV, int D) { return 0; }
+// Row tiles of the attention: NT tiles of npt nodes (npt * G rows, at most 128) share the key tiles.
+// Two as soon as one does not hold the step's rows: the K and V tiles are then read for 256.
+static void cache_attn_rows(int max_new, int G, int* nt, int* npt) {
+    const int most = 128 / G;
+    *nt = max_new <= most ? 1 : 2;
+    *npt = *nt == 1 ? std::max(1, max_new) : most;
+}
+static size_t cache_attn_bytes(int sms, int nt, int D) {
+    return static_cast<size_t>(sms) * 2 * nt * 128 * (D + 2) * sizeof(float);
+}
+size_t mica_cache_attention_workspace_bytes(int N, int max_new, int H, int KV, int D) {
+    int sms = 0, nt = 0, npt = 0;
+    if (N < 1 || max_new < 0 || H < 1 || KV < 1 || H % KV || H / KV > 128 || (D != 64 && D != 128) || check_device(&sms))
+        return 0;
+    cache_attn_rows(max_new, H / KV, &nt, &npt);
+    return cache_attn_bytes(sms, nt, D);
+}
+
+template <int D, int NT>
+static int cache_attn_prepare() {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return MICA_OK;
+    cudaError_t e = cudaFuncSetAttribute(cache_attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         CacheAttnShape<D, NT>::SMEM);
+    if (e != cudaSuccess) { set_cuda_error(e); return MICA_ERR_CUDA; }
+    done.fetch_or(bit, std::memory_order_release);
+    return MICA_OK;
+}
+
+template <int D, int NT>
+static int cache_attn_launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CacheAttnArgs& a,
+                             cudaStream_t st) {
+    if (int rc = cache_attn_prepare<D, NT>()) return rc;
+    cache_attention_kernel<D, NT><<<a.ctas, CacheAttnShape<D, NT>::THREADS, CacheAttnShape<D, NT>::SMEM, st>>>(tq, tk, tv, a);
+    if (int rc = launch_status()) return rc;
+    if (a.ctas > 1) cache_attention_join<D, NT><<<dim3(a.ctas - 1, 4), 128, 0, st>>>(a);
+    return launch_status();
+}
 
 int mica_cache_attention(const void* q, long ldq, const void* k_pages, const void* v_pages, long page_stride,
                          int pages, int page, const int* table, long ld_table, int P, const int* base, const int* cu,
@@ -1118,21 +1182,27 @@ int mica_cache_attention(const void* q, long ldq, const void* k_pages, const voi
         page_stride % 8 || !aligned_to(mask, 8) || !aligned_to(table, 4) || !aligned_to(base, 4) || !aligned_to(cu, 4) ||
         !aligned16(workspace))
         return MICA_ERR_ALIGN;
-    if (workspace_bytes < mica_cache_attention_workspace_bytes(N, max_new, H, KV, D)) return MICA_ERR_WORKSPACE;
-    if ((rc = check_device(nullptr))) return rc;
+    int sms = 0;
+    if ((rc = check_device(&sms))) return rc;
     if (N == 0) return MICA_OK;
-    a.q = static_cast<const __nv_bfloat16*>(q); a.ldq = ldq;
-    a.k_pages = static_cast<const __nv_bfloat16*>(k_pages); a.v_pages = static_cast<const __nv_bfloat16*>(v_pages);
+    int nt = 0;
+    cache_attn_rows(max_new, H / KV, &nt, &a.npt);
+    if (!workspace || workspace_bytes < cache_attn_bytes(sms, nt, D)) return MICA_ERR_WORKSPACE;
+    a.v_pages = static_cast<const __nv_bfloat16*>(v_pages);
     a.page_stride = page_stride;
     a.mask = reinterpret_cast<const unsigned long long*>(mask); a.ld_mask = ld_mask; a.words = words;
-    a.out = static_cast<__nv_bfloat16*>(out); a.ldo = ldo; a.H = H; a.KV = KV;
+    a.out = static_cast<__nv_bfloat16*>(out); a.ldo = ldo; a.KV = KV; a.G = H / KV; a.ctas = sms;
     a.scale_log2 = scale * 1.4426950408889634f;
+    a.ws = static_cast<float*>(workspace);
+    CUtensorMap tq, tk, tv;
+    const uint64_t rows = static_cast<uint64_t>(KV) * page;
+    if ((rc = make_tmap_bf16_3d(&tq, q, D, H, N, D * 2, static_cast<uint64_t>(ldq) * 2, a.G, a.npt)) ||
+        (rc = make_tmap_bf16_3d(&tk, k_pages, D, rows, pages, D * 2, static_cast<uint64_t>(page_stride) * 2, page, 1)) ||
+        (rc = make_tmap_bf16_3d(&tv, v_pages, D, rows, pages, D * 2, static_cast<uint64_t>(page_stride) * 2, page, 1)))
+        return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const long blocks = (static_cast<long>(N) * H + 3) / 4;
-    if (blocks > (1L << 31) - 1) return MICA_ERR_RANGE;
-    if (D == 128) cache_attention_kernel<128><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a);
-    else cache_attention_kernel<64><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a);
-    return launch_status();
+    if (D == 128) return nt == 1 ? cache_attn_launch<128, 1>(tq, tk, tv, a, st) : cache_attn_launch<128, 2>(tq, tk, tv, a, st);
+    return nt == 1 ? cache_attn_launch<64, 1>(tq, tk, tv, a, st) : cache_attn_launch<64, 2>(tq, tk, tv, a, st);
 }
 
 int mica_cache_copy(void* pool, long page_stride, long page_bytes, int pages, const int* src, const int* dst, int n,

@@ -299,7 +299,7 @@ def cache_append_do(qkv, q_w, k_w, cos, sin, k_pages, v_pages, table, base, cu, 
         return torch.zeros((n, heads * d), dtype=torch.bfloat16, device=qkv.device)
     q = torch.empty((n, heads * d), dtype=torch.bfloat16, device=qkv.device)
     with _on(qkv):
-        N.call('mica_cache_append', qkv.data_ptr(), qkv.stride(0), q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(),
+        N.call('mica_cache_append', qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.shape[1], q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(),
                sin.data_ptr(), cos.shape[0], _ptr(pos), q.data_ptr(), heads * d, k_pages.data_ptr(),
                v_pages.data_ptr(), k_pages.stride(0), pages, page, table.data_ptr(), table.stride(0), table.shape[1],
                base.data_ptr(), cu.data_ptr(), base.shape[0], n, heads, kv, d, eps, _stream(qkv))
@@ -315,7 +315,7 @@ def cache_attention_do(q, k_pages, v_pages, table, base, cu, mask, heads, scale,
     with _on(q):
         need = N.lib().mica_cache_attention_workspace_bytes(n, max_new, heads, kv, d)
         ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
-        N.call('mica_cache_attention', q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
+        N.call('mica_cache_attention', q.data_ptr(), q.stride(0) if n > 1 else heads * d, k_pages.data_ptr(), v_pages.data_ptr(),
                k_pages.stride(0), pages, page, table.data_ptr(), table.stride(0), table.shape[1], base.data_ptr(),
                cu.data_ptr(), _ptr(mask), mask.stride(0) if mask is not None else 0,
                mask.shape[1] if mask is not None else 0, base.shape[0], n, max_new, heads, kv, d, scale,
