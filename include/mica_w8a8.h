@@ -357,12 +357,9 @@ int mica_cache_keep(void* pool, long page_stride, int slabs, int pages, int page
  *   top_lp [N, top] fp32, top_id [N, top] int64: the largest log probabilities, ties by the lowest
  *                         id (0 <= top <= 32, top <= V; both NULL when top is 0)
  * -inf logits are tokens that are not allowed; a row with nothing else gives -inf everywhere and
- * entropy 0. A NaN or +inf logit makes the row's log probabilities and entropy NaN.
- * workspace: mica_token_logprobs_workspace_bytes(...) bytes, 16-byte aligned.               */
-size_t mica_token_logprobs_workspace_bytes(int N, int V, int dtype, int top);
+ * entropy 0. A NaN or +inf logit makes the row's log probabilities and entropy NaN.        */
 int mica_token_logprobs(const void* z, int dtype, long ld, int N, int V, const int64_t* ids, long ld_ids, int M,
-                        int top, float* logprob, float* entropy, float* top_lp, int64_t* top_id, void* workspace,
-                        size_t workspace_bytes, void* stream);
+                        int top, float* logprob, float* entropy, float* top_lp, int64_t* top_id, void* stream);
 
 /* Failure-detection self-test: launches one block that waits on a barrier nothing
  * ever arrives on, with a wait limit of limit_us microseconds. The kernel gives up,

@@ -100,8 +100,7 @@ SIGNATURES = {
     ),
     'mica_cache_copy': (_I, [_P, _L, _L, _I, _P, _P, _I, _P]),
     'mica_cache_keep': (_I, [_P, _L, _I, _I, _I, _I, _P, _L, _I, _P, _P, _I, _P, _L, _P, _I, _P, _P]),
-    'mica_token_logprobs_workspace_bytes': (_Z, [_I, _I, _I, _I]),
-    'mica_token_logprobs': (_I, [_P, _I, _L, _I, _I, _P, _L, _I, _I, _P, _P, _P, _P, _P, _Z, _P]),
+    'mica_token_logprobs': (_I, [_P, _I, _L, _I, _I, _P, _L, _I, _I, _P, _P, _P, _P, _P]),
     'mica_selftest_wait_timeout': (_I, [_P, _I, _P]),
 }
 
@@ -151,6 +150,17 @@ def check(name, rc):
             detail = lib().mica_last_cuda_error().decode(errors='replace')
         raise NativeError(name, rc, detail)
     return rc
+
+
+_ENTRIES = {}
+
+
+def entry(name):
+    """Entry point `name` itself (kept after the first look-up): the caller checks its status."""
+    f = _ENTRIES.get(name)
+    if f is None:
+        f = _ENTRIES[name] = getattr(lib(), name)
+    return f
 
 
 def int_array(values):

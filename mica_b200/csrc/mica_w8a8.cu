@@ -1263,20 +1263,54 @@ int mica_cache_keep(void* pool, long page_stride, int slabs, int pages, int page
 }
 
 // ---------------------------------------------------------------------------------------
-size_t mica_token_logprobs_workspace_bytes(int N, int V, int dtype, int top) { return 0; }
+// CTAs of a row: a cluster, so that few rows still use the chip and many rows end together. Each run
+// is to hold two full steps of its threads at least.
+static int logprob_parts(int N, int V, int dtype, int sms) {
+    const long step = static_cast<long>(LP_THREADS) * LP_UNROLL * 16 / static_cast<long>(dt_size(dtype));
+    int parts = 1;
+    while (parts < LP_CLUSTER && static_cast<long>(N) * parts < 2L * sms && V / (2L * parts) >= step) parts *= 2;
+    return parts;
+}
+
+template <typename T>
+static int logprob_launch(const LogprobArgs& a, int parts, cudaStream_t st) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = 1ull << (dev & 63);
+    cudaError_t e;
+    if (!(done.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) { set_cuda_error(e); return MICA_ERR_CUDA; }
+        done.fetch_or(bit, std::memory_order_release);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(static_cast<long>(a.N) * parts));
+    cfg.blockDim = dim3(LP_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = static_cast<unsigned>(parts);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a, parts);
+    if (e != cudaSuccess) { set_cuda_error(e); return MICA_ERR_CUDA; }
+    return launch_status();
+}
 
 int mica_token_logprobs(const void* z, int dtype, long ld, int N, int V, const int64_t* ids, long ld_ids, int M,
-                        int top, float* logprob, float* entropy, float* top_lp, int64_t* top_id, void* workspace,
-                        size_t workspace_bytes, void* stream) {
+                        int top, float* logprob, float* entropy, float* top_lp, int64_t* top_id, void* stream) {
     if (!z || !entropy || dtype < 0 || dtype > 2 || M < 0 || top < 0 || (M > 0 && (!ids || !logprob)) ||
         (top > 0 && (!top_lp || !top_id)))
         return MICA_ERR_ARG;
-    if (N < 0 || V < 1 || ld < V || ld_ids < M || top > 32 || top > V) return MICA_ERR_SHAPE;
+    if (N < 0 || V < 1 || ld < V || ld_ids < M || top > LP_TOP || top > V) return MICA_ERR_SHAPE;
+    if (static_cast<long>(N) * LP_CLUSTER > (1L << 31) - 1 || V > (1 << 30)) return MICA_ERR_RANGE;
     if (!aligned_to(z, static_cast<unsigned>(dt_size(dtype))) || !aligned_to(ids, 8) || !aligned_to(top_id, 8) ||
-        !aligned_to(logprob, 4) || !aligned_to(entropy, 4) || !aligned_to(top_lp, 4) || !aligned16(workspace))
+        !aligned_to(logprob, 4) || !aligned_to(entropy, 4) || !aligned_to(top_lp, 4))
         return MICA_ERR_ALIGN;
-    if (workspace_bytes < mica_token_logprobs_workspace_bytes(N, V, dtype, top)) return MICA_ERR_WORKSPACE;
-    int rc = check_device(nullptr);
+    int sms = 0;
+    int rc = check_device(&sms);
     if (rc) return rc;
     if (N == 0) return MICA_OK;
     LogprobArgs a = {};
@@ -1284,10 +1318,10 @@ int mica_token_logprobs(const void* z, int dtype, long ld, int N, int V, const i
     a.top = top; a.logprob = logprob; a.entropy = entropy; a.top_lp = top_lp;
     a.top_id = reinterpret_cast<long*>(top_id);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == MICA_DT_BF16) token_logprobs_kernel<__nv_bfloat16><<<N, 512, 0, st>>>(a);
-    else if (dtype == MICA_DT_FP16) token_logprobs_kernel<__half><<<N, 512, 0, st>>>(a);
-    else token_logprobs_kernel<float><<<N, 512, 0, st>>>(a);
-    return launch_status();
+    const int parts = logprob_parts(N, V, dtype, sms);
+    if (dtype == MICA_DT_BF16) return logprob_launch<__nv_bfloat16>(a, parts, st);
+    if (dtype == MICA_DT_FP16) return logprob_launch<__half>(a, parts, st);
+    return logprob_launch<float>(a, parts, st);
 }
 
 // ---------------------------------------------------------------------------------------

@@ -14,7 +14,8 @@ from __future__ import annotations
 import torch
 
 from . import ops
-from .int8_kernels import _launched, _supported
+from .int8_kernels import _launched
+from .paged import _served
 
 MAX_TOP = 32
 
@@ -38,7 +39,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0):
         raise RuntimeError(f'token_logprobs: CUDA tensors of one device only, not {logits.device} and {ids.device}')
     if logits.dtype not in ops.DTYPE_CODE:
         raise RuntimeError(f'token_logprobs: {logits.dtype} is not served (bf16, fp16 or fp32)')
-    if not _supported(logits.device):
+    if not _served(logits.device):
         raise RuntimeError('token_logprobs: not a B200 (sm_100)')
     if logits.requires_grad and torch.is_grad_enabled():
         raise RuntimeError('token_logprobs: no backward pass (call it under torch.no_grad())')

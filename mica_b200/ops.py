@@ -292,18 +292,48 @@ def _(qkv, batch, length, heads, kv_heads, scale):
 # Paged cache and token log probabilities. A step of a few tokens takes the device less time than
 # the custom-op dispatcher takes the host (about 20 us a call), so mica_b200.paged and
 # mica_b200.logprobs call the `_do` functions directly and the registered ops wrap them.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_get_device = torch._C._cuda_getDevice
+
+
+def _launch(t, entry, *args):
+    """As `with _on(t): N.call(entry, *args, _stream(t))`, without the objects those make: the entry point's
+    checks of the current device, and its launch, on t's device and that device's current stream."""
+    idx = t.get_device()
+    prev = _get_device()
+    if prev == idx:
+        rc = N.entry(entry)(*args, _raw_stream(idx))
+    else:
+        with _on(t):
+            rc = N.entry(entry)(*args, _raw_stream(idx))
+    if rc:
+        N.check(entry, rc)
+
+
 def cache_append_do(qkv, q_w, k_w, cos, sin, k_pages, v_pages, table, base, cu, heads, pos, eps):
     pages, kv, page, d = k_pages.shape
     n = qkv.shape[0]
     if n == 0 or base.shape[0] == 0:                  # nothing to do, or padding rows alone
         return torch.zeros((n, heads * d), dtype=torch.bfloat16, device=qkv.device)
     q = torch.empty((n, heads * d), dtype=torch.bfloat16, device=qkv.device)
-    with _on(qkv):
-        N.call('mica_cache_append', qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.shape[1], q_w.data_ptr(), k_w.data_ptr(), cos.data_ptr(),
-               sin.data_ptr(), cos.shape[0], _ptr(pos), q.data_ptr(), heads * d, k_pages.data_ptr(),
-               v_pages.data_ptr(), k_pages.stride(0), pages, page, table.data_ptr(), table.stride(0), table.shape[1],
-               base.data_ptr(), cu.data_ptr(), base.shape[0], n, heads, kv, d, eps, _stream(qkv))
+    _launch(qkv, 'mica_cache_append', qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.shape[1], q_w.data_ptr(),
+            k_w.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], _ptr(pos), q.data_ptr(), heads * d,
+            k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), pages, page, table.data_ptr(), table.stride(0),
+            table.shape[1], base.data_ptr(), cu.data_ptr(), base.shape[0], n, heads, kv, d, eps)
     return q
+
+
+def _cache_ws(idx, n, max_new, heads, kv, d):
+    """Workspace bytes of mica_cache_attention on device idx: they depend on the row tile alone."""
+    key = (idx, min(max_new * (heads // kv), 129), d)
+    need = _CACHE_WS.get(key)
+    if need is None:
+        with torch.cuda.device(idx):
+            need = _CACHE_WS[key] = N.lib().mica_cache_attention_workspace_bytes(n, max_new, heads, kv, d)
+    return need
+
+
+_CACHE_WS = {}
 
 
 def cache_attention_do(q, k_pages, v_pages, table, base, cu, mask, heads, scale, max_new):
@@ -312,31 +342,29 @@ def cache_attention_do(q, k_pages, v_pages, table, base, cu, mask, heads, scale,
     if n == 0 or base.shape[0] == 0:
         return torch.zeros((n, heads * d), dtype=torch.bfloat16, device=q.device)
     out = torch.empty((n, heads * d), dtype=torch.bfloat16, device=q.device)
-    with _on(q):
-        need = N.lib().mica_cache_attention_workspace_bytes(n, max_new, heads, kv, d)
-        ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
-        N.call('mica_cache_attention', q.data_ptr(), q.stride(0) if n > 1 else heads * d, k_pages.data_ptr(), v_pages.data_ptr(),
-               k_pages.stride(0), pages, page, table.data_ptr(), table.stride(0), table.shape[1], base.data_ptr(),
-               cu.data_ptr(), _ptr(mask), mask.stride(0) if mask is not None else 0,
-               mask.shape[1] if mask is not None else 0, base.shape[0], n, max_new, heads, kv, d, scale,
-               out.data_ptr(), heads * d, _ptr(ws), need, _stream(q))
+    need = _cache_ws(q.get_device(), n, max_new, heads, kv, d)
+    ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
+    words = 0 if mask is None else mask.shape[1]
+    _launch(q, 'mica_cache_attention', q.data_ptr(), q.stride(0) if n > 1 else heads * d, k_pages.data_ptr(),
+            v_pages.data_ptr(), k_pages.stride(0), pages, page, table.data_ptr(), table.stride(0), table.shape[1],
+            base.data_ptr(), cu.data_ptr(), _ptr(mask), words, words, base.shape[0], n, max_new, heads, kv, d, scale,
+            out.data_ptr(), heads * d, ws.data_ptr(), need)
     return out
 
 
 def cache_copy_do(pool, src, dst):
     a, b = N.int_array(src), N.int_array(dst)
-    with _on(pool):
-        N.call('mica_cache_copy', pool.data_ptr(), pool.stride(0) * pool.element_size(),
-               pool[0].numel() * pool.element_size(), pool.shape[0], a, b, len(src), _stream(pool))
+    _launch(pool, 'mica_cache_copy', pool.data_ptr(), pool.stride(0) * pool.element_size(),
+            pool.numel() // pool.shape[0] * pool.element_size(), pool.shape[0], a, b, len(src))
 
 
 def cache_keep_do(pool, table, base, cu, keep, n_keep):
     pages, layers, two, kv, page, d = pool.shape
     new_base = torch.empty_like(base)
-    with _on(pool):
-        N.call('mica_cache_keep', pool.data_ptr(), pool.stride(0) * 2, layers * two * kv, pages, page, d,
-               table.data_ptr(), table.stride(0), table.shape[1], base.data_ptr(), cu.data_ptr(), base.shape[0],
-               keep.data_ptr(), keep.stride(0), n_keep.data_ptr(), keep.shape[1], new_base.data_ptr(), _stream(pool))
+    most = keep.shape[1]
+    _launch(pool, 'mica_cache_keep', pool.data_ptr(), pool.stride(0) * 2, layers * two * kv, pages, page, d,
+            table.data_ptr(), table.stride(0), table.shape[1], base.data_ptr(), cu.data_ptr(), base.shape[0],
+            keep.data_ptr(), most, n_keep.data_ptr(), most, new_base.data_ptr())
     return new_base
 
 
@@ -353,12 +381,9 @@ def token_logprobs_do(logits, ids, top):
     code = DTYPE_CODE[logits.dtype]
     ld = logits.stride(0) if n > 1 else v              # a single row's stride may be anything
     ld_ids = ids.stride(0) if n > 1 else m
-    with _on(logits):
-        need = N.lib().mica_token_logprobs_workspace_bytes(n, v, code, top)
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-        N.call('mica_token_logprobs', logits.data_ptr(), code, ld, n, v, ids.data_ptr() if m else None,
-               ld_ids, m, top, lp.data_ptr() if m else None, ent.data_ptr(), top_lp.data_ptr() if top else None,
-               top_id.data_ptr() if top else None, _ptr(ws), need, _stream(logits))
+    _launch(logits, 'mica_token_logprobs', logits.data_ptr(), code, ld, n, v, ids.data_ptr() if m else None, ld_ids, m,
+            top, lp.data_ptr() if m else None, ent.data_ptr(), top_lp.data_ptr() if top else None,
+            top_id.data_ptr() if top else None)
     return lp, ent, top_lp, top_id
 
 

@@ -26,9 +26,14 @@ from typing import Optional, Sequence
 import torch
 
 from . import ops
-from .int8_kernels import _launched, _supported
+from .int8_kernels import _CAPS, _launched, _supported
 
 PAGES = (16, 32, 64, 128)      # tokens a page may hold
+
+
+def _served(dev):
+    c = _CAPS.get(dev.index)            # what _supported found the first time
+    return bool(c.supported) if c is not None else _supported(dev)
 
 
 def _cuda(name, *ts):
@@ -38,12 +43,12 @@ def _cuda(name, *ts):
     for t in ts[1:]:
         if t is not None and t.device != dev:
             raise RuntimeError(f'{name}: tensors on {dev} and {t.device}')
-    if not _supported(dev):
+    if not _served(dev):
         raise RuntimeError(f'{name}: {dev} is not a B200 (sm_100)')
 
 
 def _no_grad(name, *ts):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+    if torch.is_grad_enabled() and True in [t.requires_grad for t in ts]:
         raise RuntimeError(f'{name}: no backward pass (call it under torch.no_grad())')
 
 

@@ -83,8 +83,8 @@ def test_keep_and_logprob_refusals(lib):
     assert keep(pool=24) == 3 and keep(keep=18) == 3
 
     def lp(**kw):
-        a = dict(z=16, dtype=2, ld=100, N=2, V=100, ids=16, ld_ids=1, M=1, top=4, lp=16, ent=16, tl=16, ti=16, ws=16,
-                 ws_bytes=1 << 40, stream=None)
+        a = dict(z=16, dtype=2, ld=100, N=2, V=100, ids=16, ld_ids=1, M=1, top=4, lp=16, ent=16, tl=16, ti=16,
+                 stream=None)
         a.update(kw)
         return lib.mica_token_logprobs(*a.values())
     for bad in (dict(z=None), dict(ent=None), dict(dtype=3), dict(M=-1), dict(top=-1), dict(ids=None), dict(lp=None),
@@ -92,7 +92,7 @@ def test_keep_and_logprob_refusals(lib):
         assert lp(**bad) == 1, bad
     for bad in (dict(N=-1), dict(V=0), dict(ld=99), dict(ld_ids=0), dict(top=33), dict(V=3, top=4)):
         assert lp(**bad) == 2, bad
-    for bad in (dict(z=18), dict(ids=20), dict(ti=20), dict(lp=18), dict(ws=8)):
+    for bad in (dict(z=18), dict(ids=20), dict(ti=20), dict(lp=18)):
         assert lp(**bad) == 3, bad
 
 
