@@ -9,15 +9,16 @@
 //
 // Bound by the logits' bytes, which are read once: the maximum, S and the entropy's sum run along in
 // one pass (rescaled when the maximum grows), in base 2 and fp32. A row is one cluster of CTAs, each
-// with a run of it; the parts meet through distributed shared memory, so there is one launch and
-// no workspace.
+// with a run of it; a cluster takes row after row. In a CTA one warp keeps bulk copies of the coming
+// logits in flight through a ring in shared memory, 24 warps make the pass, and 4 warps finish the
+// row before while the pass goes on with the next. The parts of a row meet in the first CTA's
+// shared memory: one launch, no workspace.
 //
-// Alternatives without a list in the inner loop: a thread keeps only the largest logit it has seen.
-// The CTA's 32 half-warps give 32 maxima of disjoint elements, so the top-th largest of those is a
-// lower bound of the run's top-th largest logit; only threads whose maximum reaches it can hold an
-// alternative, about one in sixteen, and their elements are read again (from L2) and kept when they
-// reach the bound: about 30 candidates for 20 alternatives of random logits. They are ranked by
-// counting, in each CTA and then over the cluster.
+// Alternatives without a list in the pass: a thread keeps only the largest logit it has seen. The
+// maxima of 64 groups of threads are of disjoint elements, so the top-th largest of them is a lower
+// bound of the run's top-th largest logit; only threads whose maximum reaches it can hold an
+// alternative (about 25 of 768 for 20 alternatives of random logits), and their vectors are read
+// again, from L2, and elements that reach the bound kept. Warps sort them 32 at a time and merge.
 #pragma once
 
 #include "quant.cuh"
@@ -37,13 +38,16 @@ struct LogprobArgs {
     long* top_id;               // [N, top]
 };
 
-constexpr int LP_THREADS = 512;
+constexpr int LP_THREADS = 768;          // make the pass
 constexpr int LP_WARPS = LP_THREADS / 32;
-constexpr int LP_UNROLL = 4;             // 16-byte vectors a thread has in flight
-constexpr int LP_CAND = 1024;            // candidates a CTA can rank
+constexpr int LP_EPI = 128;              // finish a row
+constexpr int LP_BLOCK = LP_THREADS + 32 + LP_EPI;
+constexpr int LP_UNROLL = 4;             // 16-byte vectors of a thread's step
+constexpr int LP_STEP = LP_THREADS * LP_UNROLL;         // vectors of a ring stage (48 KB)
+constexpr int LP_STAGES = 3;
+constexpr int LP_CAND = 512;             // candidates a CTA can rank
 constexpr int LP_TOP = 32;
 constexpr int LP_CLUSTER = 16;
-static_assert(2 * LP_WARPS == LP_TOP, "one group maximum for each alternative");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Logits are held above this in the sums, so that a weight of zero meets no infinity; a row whose
@@ -56,6 +60,7 @@ __device__ __forceinline__ float to_f32(T v) {
     else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
     else return __bfloat162float(v);
 }
+__device__ __forceinline__ void lp_sync() { named_bar_sync(1, LP_EPI); }   // the warps that finish a row
 __device__ __forceinline__ float nan_f32() { return __uint_as_float(0x7fc00000u); }
 
 // Orders logits for the alternatives: larger value first, NaN above +inf, -0 equal to +0.
@@ -88,7 +93,7 @@ struct LpSums {
 __device__ __forceinline__ LpSums lp_join(const LpSums& a, const LpSums& b) {
     const float mc = max_nan(a.mc, b.mc);
     const float da = fmaxf(a.mc - mc, -1000.f), db = fmaxf(b.mc - mc, -1000.f);    // 2^-1000 is 0, its product too
-    const float fa = exp2f(da), fb = exp2f(db);
+    const float fa = fast_exp2(da), fb = fast_exp2(db);
     return LpSums{mc, a.s * fa + b.s * fb, fa * fmaf(da, a.s, a.w) + fb * fmaf(db, b.s, b.w)};
 }
 
@@ -150,7 +155,7 @@ __device__ __forceinline__ void lp_step(const uint4 (&q)[LP_UNROLL], LpSums& a, 
     top = max_nan(top, cm);
     const float cmc = max_nan(cm, LP_FLOOR) * kLog2e;
     if (!(cmc <= a.mc)) {
-        const float d = fmaxf(a.mc - cmc, -1000.f), f = exp2f(d);
+        const float d = fmaxf(a.mc - cmc, -1000.f), f = fast_exp2(d);
         a.w = f * fmaf(d, a.s, a.w);
         a.s *= f;
         a.mc = cmc;
@@ -182,49 +187,59 @@ __device__ __forceinline__ void lp_step(const uint4 (&q)[LP_UNROLL], LpSums& a, 
     a.w += x + y;
 }
 
-struct LpPart {                 // what a CTA tells its cluster
+struct LpPart {                 // what a CTA tells its cluster of a row
     LpSums sums;
-    int count;                  // entries of list
+    float top;                  // its largest logit as it is
+    int count;                  // entries of list, in order
+    int pad;
     unsigned long long list[LP_TOP];
 };
 
-// The whole row by one CTA, in passes, for rows beyond the sums' range (infinities, NaN, maxima
-// near the type's ends) : the definition literally.
+// The row by the LP_EPI threads, in passes, for maxima near the type's ends, infinities and NaN: the
+// definition literally.
+__device__ __forceinline__ float lp_reduce(float v, bool max, float* red) {
+    v = max ? warp_max(v) : warp_sum(v);
+    lp_sync();
+    if ((threadIdx.x & 31) == 0) red[(threadIdx.x >> 5) & 3] = v;
+    lp_sync();
+    v = red[0];
+    for (int i = 1; i < LP_EPI / 32; ++i) v = max ? fmaxf(v, red[i]) : v + red[i];
+    return v;
+}
 template <typename T>
-__device__ void lp_row_plain(const LogprobArgs& a, const T* z, float* red, float& m, float& logs, float& ent) {
+__device__ __noinline__ void lp_row_plain(const LogprobArgs& a, const T* z, int e, float* red, float& m, float& logs,
+                                          float& ent) {
     m = -INFINITY;
-    bool odd = false;
-    for (int i = threadIdx.x; i < a.V; i += LP_THREADS) {
+    float odd = 0.f;
+    for (int i = e; i < a.V; i += LP_EPI) {
         const float v = to_f32(z[i]);
-        odd |= v != v || v == INFINITY;
+        if (v != v || v == INFINITY) odd = 1.f;
         m = fmaxf(m, v);
     }
-    odd = __syncthreads_or(odd);
-    m = warp_max(m);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-    __syncthreads();
-    for (int i = 0; i < LP_WARPS; ++i) m = fmaxf(m, red[i]);
-    __syncthreads();
+    odd = lp_reduce(odd, true, red);
+    m = lp_reduce(m, true, red);
     float s = 0.f, w = 0.f;
-    for (int i = threadIdx.x; i < a.V; i += LP_THREADS) {
-        const float d = to_f32(z[i]) - m, e = m == -INFINITY ? 0.f : expf(d);
-        s += e;
-        if (e > 0.f) w -= d * e;
+    for (int i = e; i < a.V; i += LP_EPI) {
+        const float d = to_f32(z[i]) - m, x = m == -INFINITY ? 0.f : expf(d);
+        s += x;
+        if (x > 0.f) w -= d * x;
     }
-    s = block_reduce<false>(s, red);
-    w = block_reduce<false>(w, red);
+    s = lp_reduce(s, false, red);
+    w = lp_reduce(w, false, red);
     logs = m == -INFINITY ? 0.f : logf(s);
     ent = m == -INFINITY ? 0.f : logs + w / s;
-    if (odd) logs = ent = nan_f32();
+    if (odd > 0.f) logs = ent = nan_f32();
 }
 
-// Elements [i0, i1) of the row, each alternative by one pass: for runs with more ties than a list holds.
+// The largest `top` keys of elements [i0, i1), each by one pass: for runs with more large values in a
+// few threads than a list holds.
 template <typename T>
-__device__ void lp_select_plain(const T* z, int i0, int i1, int top, unsigned long long* list, unsigned long long* best) {
+__device__ __noinline__ void lp_select_plain(const T* z, int i0, int i1, int e, int top, unsigned long long* list,
+                                             unsigned long long* best) {
     unsigned long long last = ~0ull;
     for (int j = 0; j < top; ++j) {
         unsigned long long b = 0ull;
-        for (int i = i0 + threadIdx.x; i < i1; i += LP_THREADS) {
+        for (int i = i0 + e; i < i1; i += LP_EPI) {
             const unsigned long long c = rank_key(to_f32(z[i]), i);
             if (c < last && c > b) b = c;
         }
@@ -233,228 +248,430 @@ __device__ void lp_select_plain(const T* z, int i0, int i1, int top, unsigned lo
             const unsigned long long c = __shfl_xor_sync(0xffffffffu, b, o);
             b = c > b ? c : b;
         }
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = b;
-        __syncthreads();
-        for (int i = 0; i < LP_WARPS; ++i) b = best[i] > b ? best[i] : b;
+        lp_sync();
+        if ((e & 31) == 0) best[e >> 5] = b;
+        lp_sync();
+        for (int i = 0; i < LP_EPI / 32; ++i) b = best[i] > b ? best[i] : b;
         last = b;
-        if (threadIdx.x == 0) list[j] = b;
+        if (e == 0) list[j] = b;
     }
-    __syncthreads();
+    lp_sync();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS, 2) token_logprobs_kernel(const LogprobArgs a, const int parts) {
-    constexpr int N = LpVec<T>::N;
-    __shared__ float red[32];
-    __shared__ unsigned long long cand[LP_CAND];
-    __shared__ LpPart part;
-    __shared__ float s_group[LP_TOP], s_bound;
-    __shared__ int s_count;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = parts > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-    const int row = blockIdx.x / parts;
-    const T* z = static_cast<const T*>(a.z) + static_cast<long>(row) * a.ld;
-    // [0, head) single elements up to the first 16-byte boundary, nvec vectors, single elements to V
-    const int head = min(a.V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / static_cast<int>(sizeof(T)));
-    const int nvec = (a.V - head) / N;
-    const uint4* zv = reinterpret_cast<const uint4*>(z + head);
-    const int v0 = static_cast<int>(static_cast<long>(nvec) * rank / parts);
-    const int v1 = static_cast<int>(static_cast<long>(nvec) * (rank + 1) / parts);
-    // the single elements, fewer than N at either end, are the first and the last CTA's, one a thread
-    const int tail = head + nvec * N, tid = threadIdx.x;
-    const int my_loose = rank == 0 && tid < head                                       ? tid
-                         : rank == parts - 1 && tid >= 16 && tail + (tid - 16) < a.V ? tail + (tid - 16) : -1;
-
-    // ---- the pass ----
-    constexpr uint32_t kNone = std::is_same<T, float>::value ? 0xff800000u
-                               : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;    // -inf
-    LpSums sums{LP_FLOOR * kLog2e, 0.f, 0.f};
-    float top = -INFINITY;
-    int v = v0 + threadIdx.x;
-    for (; v + (LP_UNROLL - 1) * LP_THREADS < v1; v += LP_UNROLL * LP_THREADS) {
-        uint4 q[LP_UNROLL];
+// Sorts 32 keys across the lanes, largest first.
+__device__ __forceinline__ unsigned long long lp_sort32(unsigned long long k, int lane) {
 #pragma unroll
-        for (int u = 0; u < LP_UNROLL; ++u) q[u] = __ldg(zv + v + u * LP_THREADS);
-        lp_step<T>(q, sums, top);
-    }
-    if (v < v1 || my_loose >= 0) {
-        uint4 q[LP_UNROLL];
+    for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
-        for (int u = 0; u < LP_UNROLL; ++u)
-            q[u] = v + u * LP_THREADS < v1 ? __ldg(zv + v + u * LP_THREADS) : make_uint4(kNone, kNone, kNone, kNone);
-        lp_step<T>(q, sums, top);
-        if (my_loose >= 0) {
-            const float f = to_f32(z[my_loose]);
-            top = max_nan(top, f);
-            sums = lp_join(sums, LpSums{max_nan(f, LP_FLOOR) * kLog2e, 1.f, 0.f});
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
+            const bool down = (lane & size) == 0 || size == 32;      // this run: largest first
+            const bool low = (lane & o) == 0;
+            if ((k < other) == (low == down)) k = other;
         }
-    }
-
-    // ---- alternatives of the run ----
-    if (threadIdx.x == 0) s_count = 0;
-    if (a.top > 0) {
-        float g = top;
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if ((lane & 15) == 0) s_group[threadIdx.x >> 4] = g;
-        __syncthreads();
-        if (warp == 0) {
-            // the top-th largest of the 32 maxima
-            const uint32_t mine = order_key(s_group[lane]);
-            int above = 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const uint32_t o = __shfl_sync(0xffffffffu, mine, i);
-                above += o > mine || (o == mine && i < lane);
-            }
-            if (above == a.top - 1) s_bound = order_value(mine);
-        }
-        __syncthreads();
-        const float bound = s_bound;
-        const uint32_t bkey = order_key(bound);
-        const int n_mine = v1 - v0;
-        // elements that reach the bound (strict: that are above it)
-        const auto gather = [&](bool strict) {
-            const auto keep = [&](float f, int id) {
-                const uint32_t k = order_key(f);
-                if (strict ? k > bkey : k >= bkey) {
-                    const int at = atomicAdd(&s_count, 1);
-                    if (at < LP_CAND) cand[at] = rank_key(f, id);
-                }
-            };
-            uint32_t who = __ballot_sync(0xffffffffu, order_key(top) >= bkey);
-            for (; who; who &= who - 1) {
-                // the warp reads that thread's vectors, one a lane
-                const int t = warp * 32 + __ffs(who) - 1;
-                for (int i = t + lane * LP_THREADS; i < n_mine; i += 32 * LP_THREADS) {
-                    float f[N];
-                    LpVec<T>::values(__ldg(zv + v0 + i), f);
-#pragma unroll
-                    for (int e = 0; e < N; ++e) keep(f[e], head + (v0 + i) * N + e);
-                }
-            }
-            if (my_loose >= 0) keep(to_f32(z[my_loose]), my_loose);
-        };
-        gather(false);
-        __syncthreads();
-        int n = s_count;
-        const int lo = rank == 0 ? 0 : head + v0 * N, hi = rank == parts - 1 ? a.V : head + v1 * N;   // the run's elements
-        bool plain = false;
-        if (n > LP_CAND) {
-            // more ties at the bound than places (a row that allows few tokens, or equal logits): those above
-            // it, then the first ones at it in order of their ids
-            __syncthreads();
-            if (threadIdx.x == 0) s_count = 0;
-            __syncthreads();
-            gather(true);
-            __syncthreads();
-            n = s_count;
-            plain = n > LP_CAND - LP_TOP;
-            const int want = plain ? 0 : n + a.top;              // enough of them
-            for (int i0 = lo; i0 < hi && n < want; i0 += LP_THREADS) {
-                const int i = i0 + threadIdx.x;
-                const bool hit = i < hi && order_key(to_f32(z[i])) == bkey;
-                const uint32_t bits = __ballot_sync(0xffffffffu, hit);
-                __syncthreads();
-                if (lane == 0) red[warp] = __uint_as_float(__popc(bits));
-                __syncthreads();
-                int at = n;
-                for (int w = 0; w < LP_WARPS; ++w) {
-                    const int k = __float_as_uint(red[w]);
-                    if (w < warp) at += k;
-                    n += k;
-                }
-                at += __popc(bits & ((1u << lane) - 1u));
-                if (hit && at < want) cand[at] = rank_key(order_value(bkey), i);
-                n = min(n, want);
-            }
-            __syncthreads();
-        }
-        if (plain) {
-            lp_select_plain(z, lo, hi, a.top, part.list, cand);
-            if (threadIdx.x == 0) part.count = min(a.top, hi - lo);
-        } else {
-            for (int i = threadIdx.x; i < n; i += LP_THREADS) {
-                const unsigned long long k = cand[i];
-                int above = 0;
-                for (int j = 0; j < n; ++j) above += cand[j] > k;
-                if (above < a.top) part.list[above] = k;
-            }
-            if (threadIdx.x == 0) part.count = min(n, a.top);
-        }
-    }
-
-    // ---- sums of the run ----
+    return k;
+}
+// The 32 largest of two sorted sets, sorted.
+__device__ __forceinline__ unsigned long long lp_merge32(unsigned long long a, unsigned long long b, int lane) {
+    const unsigned long long r = __shfl_sync(0xffffffffu, b, 31 - lane);
+    unsigned long long k = a > r ? a : r;                            // bitonic
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const LpSums b{__shfl_xor_sync(0xffffffffu, sums.mc, o), __shfl_xor_sync(0xffffffffu, sums.s, o),
-                       __shfl_xor_sync(0xffffffffu, sums.w, o)};
-        // the same order on both sides, so both get the same bits
-        sums = lane & o ? lp_join(b, sums) : lp_join(sums, b);
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
+        if ((k < other) == ((lane & o) == 0)) k = other;
     }
-    __shared__ LpSums s_sums[LP_WARPS];
-    if (lane == 0) s_sums[warp] = sums;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < LP_WARPS; ++i) sums = lp_join(sums, s_sums[i]);
-        part.sums = sums;
-    }
+    return k;
+}
 
-    // ---- the cluster's parts ----
-    if (parts > 1) cluster_sync(); else __syncthreads();
-    if (rank == 0) {
-        const auto remote = [&](int r, const void* p) {
-            return map_to_rank(smem_u32(p), r);
-        };
-        sums = part.sums;
-        for (int r = 1; r < parts; ++r) {
-            LpSums b;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.mc) : "r"(remote(r, &part.sums.mc)) : "memory");
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.s) : "r"(remote(r, &part.sums.s)) : "memory");
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.w) : "r"(remote(r, &part.sums.w)) : "memory");
-            sums = lp_join(sums, b);
-        }
-        int n = 0;
-        if (a.top > 0) {
-            // at most 16 x 32 candidates: one a thread
-            const int r = threadIdx.x >> 5;
-            unsigned long long k = 0ull;
-            if (r < parts) {
-                int count;
-                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(count) : "r"(remote(r, &part.count)) : "memory");
-                if (lane < count)
-                    asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(k) : "r"(remote(r, &part.list[lane])) : "memory");
-            }
-            cand[threadIdx.x] = k;
-            n = parts * LP_TOP;
-            __syncthreads();
-        }
-        const float log2s = log2f(sums.s);
-        float m = 0.f, logs = 0.f, ent = kLn2 * (log2s - sums.w / sums.s);
-        // beyond the range of the sums, or NaN
-        const bool odd = !(sums.mc > 0.1f * LP_FLOOR && sums.mc < -LP_FLOOR && sums.s < INFINITY);
-        if (odd) lp_row_plain(a, z, red, m, logs, ent);
-        const auto lp = [&](float f) {
-            if (odd) return m == -INFINITY && logs == 0.f ? -INFINITY : (f - m) - logs;
-            return (fmaf(f, kLog2e, -sums.mc) - log2s) * kLn2;
-        };
-        if (threadIdx.x == 0) a.entropy[row] = ent;
-        for (int j = threadIdx.x; j < a.M; j += LP_THREADS) {
-            const long id = a.ids[static_cast<long>(row) * a.ld_ids + j];
-            a.logprob[static_cast<long>(row) * a.M + j] = id < 0 ? 0.f : id >= a.V ? nan_f32() : lp(to_f32(z[id]));
-        }
-        if (static_cast<int>(threadIdx.x) < n && cand[threadIdx.x]) {
-            const unsigned long long k = cand[threadIdx.x];
-            int above = 0;
-            for (int j = 0; j < n; ++j) above += cand[j] > k;
-            if (above < a.top) {
-                a.top_lp[static_cast<long>(row) * a.top + above] = lp(order_value(static_cast<uint32_t>(k >> 32)));
-                a.top_id[static_cast<long>(row) * a.top + above] = static_cast<long>(~static_cast<uint32_t>(k));
-            }
+// Joins the sums of `width` lanes (a power of two) in a fixed order; every lane gets the same bits.
+__device__ __forceinline__ LpSums lp_join_warp(LpSums s, int width) {
+    const int lane = threadIdx.x & 31;
+    for (int o = width >> 1; o > 0; o >>= 1) {
+        const LpSums b{__shfl_xor_sync(0xffffffffu, s.mc, o), __shfl_xor_sync(0xffffffffu, s.s, o),
+                       __shfl_xor_sync(0xffffffffu, s.w, o)};
+        s = lane & o ? lp_join(b, s) : lp_join(s, b);
+    }
+    return s;
+}
+
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, unsigned long long v) {
+    asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+// Bounded wait on a barrier that CTAs of the cluster arrive on.
+__device__ __forceinline__ bool lp_wait_cluster(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag) {
+    const unsigned long long t0 = global_ns();
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+        if (global_ns() - t0 > kWaitLimitNs) {
+            *abort_flag = 1u;
+            atomicExch(&g_dev_error, MICA_DEV_TIMEOUT_GRID);
+            return false;
         }
     }
-    if (parts > 1) cluster_sync();        // the parts' shared memory has been read
+}
+
+// A row's 16-byte vectors and the single elements before and behind them, and CTA `rank`'s part.
+template <typename T>
+struct LpRow {
+    const T* z;
+    int head, nvec, v0, v1;
+    __device__ __forceinline__ LpRow(const LogprobArgs& a, int row, int rank, int parts) {
+        z = static_cast<const T*>(a.z) + static_cast<long>(row) * a.ld;
+        head = min(a.V, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / static_cast<int>(sizeof(T)));
+        nvec = (a.V - head) / LpVec<T>::N;
+        v0 = static_cast<int>(static_cast<long>(nvec) * rank / parts);
+        v1 = static_cast<int>(static_cast<long>(nvec) * (rank + 1) / parts);
+    }
+    __device__ __forceinline__ const uint4* vectors() const { return reinterpret_cast<const uint4*>(z + head); }
+    // thread t's single element, -1 for none: fewer than 8 at either end, the first and the last CTA's
+    __device__ __forceinline__ int single(const LogprobArgs& a, int t, int rank, int parts) const {
+        const int tail = head + nvec * LpVec<T>::N;
+        return rank == 0 && t < head                                   ? t
+               : rank == parts - 1 && t >= 16 && tail + (t - 16) < a.V ? tail + (t - 16) : -1;
+    }
+};
+
+struct LpShared {
+    float4 mine[2][LP_THREADS];          // of each thread of the pass: sums and largest logit, rows in turn
+    unsigned long long cand[LP_CAND];
+    LpPart slots[2][LP_CLUSTER];         // of the first CTA: the parts of a row, rows in turn
+    unsigned long long list[4][LP_TOP];
+    int who[LP_THREADS];
+    float group[64], red[4], bound;
+    LpSums sums[4];
+    int count, n_who;
+    uint64_t full[LP_STAGES], empty[LP_STAGES], passed[2], done[2], ready[2], taken[2];
+    uint32_t abort;
+};
+constexpr int LP_SMEM = 128 + LP_STAGES * LP_STEP * 16 + static_cast<int>(sizeof(LpShared));
+static_assert(LP_SMEM <= 232448, "shared memory of a CTA");
+
+template <typename T>
+__global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const LogprobArgs a, const int parts) {
+    constexpr int N = LpVec<T>::N;
+    extern __shared__ __align__(128) uint4 ring[];
+    LpShared& sh = *reinterpret_cast<LpShared*>(ring + LP_STAGES * LP_STEP);
+    volatile uint32_t* abort_flag = &sh.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = parts > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int first_row = blockIdx.x / parts, rows_step = gridDim.x / parts;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < LP_STAGES; ++i) {
+            mbar_init(&sh.full[i], 1);
+            mbar_init(&sh.empty[i], LP_WARPS);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.passed[i], LP_WARPS);
+            mbar_init(&sh.done[i], 1);
+            mbar_init(&sh.ready[i], parts);
+            mbar_init(&sh.taken[i], 1);
+        }
+        sh.abort = 0u;
+        fence_mbar_init();
+    }
+    if (parts > 1) cluster_sync(); else __syncthreads();
+
+    // A wait that gives up lets the loops run on over whatever is there; the error word says so.
+    if (warp == LP_WARPS) {
+        // ---------------------------------- loads ----------------------------------
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int row = first_row; row < a.N && ok; row += rows_step) {
+                const LpRow<T> r(a, row, rank, parts);
+                for (int v = r.v0; v < r.v1; v += LP_STEP, ++it) {
+                    const int st = it % LP_STAGES;
+                    ok = mbar_wait(&sh.empty[st], ((it / LP_STAGES) & 1u) ^ 1u, abort_flag, MICA_DEV_TIMEOUT_PRODUCER);
+                    if (!ok) break;
+                    const uint32_t bytes = min(LP_STEP, r.v1 - v) * 16;
+                    mbar_arrive_expect_tx(&sh.full[st], bytes);
+                    asm volatile(
+                        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                        ::"r"(smem_u32(ring + st * LP_STEP)), "l"(reinterpret_cast<uint64_t>(r.vectors() + v)), "r"(bytes),
+                        "r"(smem_u32(&sh.full[st])) : "memory");
+                }
+            }
+            // copies in flight land before shared memory is released
+            for (int i = it > LP_STAGES ? it - LP_STAGES : 0; i < it; ++i)
+                mbar_wait(&sh.full[i % LP_STAGES], (i / LP_STAGES) & 1u, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
+        }
+        __syncwarp();
+    } else if (warp < LP_WARPS) {
+        // ---------------------------------- the pass ----------------------------------
+        constexpr uint32_t kNone = std::is_same<T, float>::value ? 0xff800000u
+                                   : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;    // -inf
+        int it = 0, nth = 0;
+        const int tid = threadIdx.x;
+        for (int row = first_row; row < a.N; row += rows_step, ++nth) {
+            const LpRow<T> r(a, row, rank, parts);
+            const int my_single = r.single(a, tid, rank, parts);
+            const float single = my_single >= 0 ? to_f32(r.z[my_single]) : 0.f;
+            LpSums sums{LP_FLOOR * kLog2e, 0.f, 0.f};
+            float top = -INFINITY;
+            for (int v = r.v0; v < r.v1; v += LP_STEP, ++it) {
+                const int st = it % LP_STAGES;
+                mbar_wait(&sh.full[st], (it / LP_STAGES) & 1u, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
+                uint4 q[LP_UNROLL];
+#pragma unroll
+                for (int u = 0; u < LP_UNROLL; ++u)
+                    q[u] = v + tid + u * LP_THREADS < r.v1 ? ring[st * LP_STEP + tid + u * LP_THREADS]
+                                                           : make_uint4(kNone, kNone, kNone, kNone);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.empty[st]);
+                lp_step<T>(q, sums, top);
+            }
+            if (my_single >= 0) {
+                top = max_nan(top, single);
+                sums = lp_join(sums, LpSums{max_nan(single, LP_FLOOR) * kLog2e, 1.f, 0.f});
+            }
+            const int slot = nth & 1;
+            if (nth >= 2) mbar_wait(&sh.done[slot], ((nth >> 1) - 1) & 1u, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
+            sh.mine[slot][tid] = make_float4(sums.mc, sums.s, sums.w, top);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.passed[slot]);
+        }
+    } else {
+        // ---------------------------------- finishing rows ----------------------------------
+        const int e = threadIdx.x - LP_THREADS - 32, ew = e >> 5;
+        int nth = 0;
+        for (int row = first_row; row < a.N; row += rows_step, ++nth) {
+            const LpRow<T> r(a, row, rank, parts);
+            const int slot = nth & 1;
+            const uint32_t turn = (nth >> 1) & 1u;
+            if (e == 0) sh.count = sh.n_who = 0;
+            mbar_wait(&sh.passed[slot], turn, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
+            // six threads' sums and maxima each; two of these are a group
+            LpSums sums;
+            float top;
+            {
+                float4 f = sh.mine[slot][e];
+                sums = LpSums{f.x, f.y, f.z};
+                top = f.w;
+#pragma unroll
+                for (int i = 1; i < LP_THREADS / LP_EPI; ++i) {
+                    f = sh.mine[slot][e + i * LP_EPI];
+                    sums = lp_join(sums, LpSums{f.x, f.y, f.z});
+                    top = max_nan(top, f.w);
+                }
+            }
+            const float g = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            if ((e & 1) == 0) sh.group[e >> 1] = g;
+            sums = lp_join_warp(sums, 32);
+            if (lane == 0) sh.sums[ew] = sums;
+            lp_sync();
+            float top_all = -INFINITY;
+            for (int i = 0; i < 64; i += 32) top_all = max_nan(top_all, sh.group[i + lane]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top_all = max_nan(top_all, __shfl_xor_sync(0xffffffffu, top_all, o));
+            unsigned long long best = 0ull;          // of warp 0: the run's alternatives in order
+            int n = 0;
+            if (a.top > 0) {
+                if (e < 64) {
+                    // the top-th largest of the 64 maxima
+                    const uint32_t me = order_key(sh.group[e]);
+                    int above = 0;
+#pragma unroll 16
+                    for (int i = 0; i < 64; ++i) {
+                        const uint32_t o = order_key(sh.group[i]);
+                        above += o > me || (o == me && i < e);
+                    }
+                    if (above == a.top - 1) sh.bound = sh.group[e];
+                }
+                lp_sync();
+                const uint32_t bkey = order_key(sh.bound);
+                const int n_mine = r.v1 - r.v0, per = (n_mine + LP_THREADS - 1) / LP_THREADS;
+                // threads of the pass whose maximum reaches the bound, then their vectors' elements that do
+                // (strict: are above it)
+#pragma unroll
+                for (int i = 0; i < LP_THREADS / LP_EPI; ++i)
+                    if (order_key(sh.mine[slot][e + i * LP_EPI].w) >= bkey) sh.who[atomicAdd(&sh.n_who, 1)] = e + i * LP_EPI;
+                const auto gather = [&](bool strict) {
+                    const auto keep = [&](float f, int id) {
+                        const uint32_t k = order_key(f);
+                        if (strict ? k > bkey : k >= bkey) {
+                            const int at = atomicAdd(&sh.count, 1);
+                            if (at < LP_CAND) sh.cand[at] = rank_key(f, id);
+                        }
+                    };
+                    const int total = sh.n_who * per;
+                    for (int w0 = e; w0 < total; w0 += 4 * LP_EPI) {
+                        uint4 q[4];
+                        int at[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const int w = w0 + u * LP_EPI;
+                            at[u] = w < total ? sh.who[w / per] + (w % per) * LP_THREADS : n_mine;
+                            if (at[u] < n_mine) q[u] = __ldg(r.vectors() + r.v0 + at[u]);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            if (at[u] >= n_mine) continue;
+                            float f[N];
+                            LpVec<T>::values(q[u], f);
+                            float m = f[0];
+#pragma unroll
+                            for (int i = 1; i < N; ++i) m = max_nan(m, f[i]);
+                            if (order_key(m) < bkey) continue;
+#pragma unroll
+                            for (int i = 0; i < N; ++i) keep(f[i], r.head + (r.v0 + at[u]) * N + i);
+                        }
+                    }
+                    const int my_single = r.single(a, e, rank, parts);
+                    if (my_single >= 0) keep(to_f32(r.z[my_single]), my_single);
+                };
+                lp_sync();
+                gather(false);
+                lp_sync();
+                n = sh.count;
+                // the run's elements
+                const int lo = rank == 0 ? 0 : r.head + r.v0 * N, hi = rank == parts - 1 ? a.V : r.head + r.v1 * N;
+                bool plain = false;
+                if (n > LP_CAND) {
+                    // more ties at the bound than places (a row that allows few tokens, or equal logits): those
+                    // above it, then the first ones at it in order of their ids
+                    lp_sync();
+                    if (e == 0) sh.count = 0;
+                    lp_sync();
+                    gather(true);
+                    lp_sync();
+                    n = sh.count;
+                    plain = n > LP_CAND - LP_TOP;
+                    const int want = plain ? 0 : n + a.top;              // enough of them
+                    for (int i0 = lo; i0 < hi && n < want; i0 += LP_EPI) {
+                        const int i = i0 + e;
+                        const bool hit = i < hi && order_key(to_f32(r.z[i])) == bkey;
+                        const uint32_t bits = __ballot_sync(0xffffffffu, hit);
+                        lp_sync();
+                        if (lane == 0) sh.red[ew] = __int_as_float(__popc(bits));
+                        lp_sync();
+                        int at = n;
+                        for (int w = 0; w < LP_EPI / 32; ++w) {
+                            const int k = __float_as_int(sh.red[w]);
+                            if (w < ew) at += k;
+                            n += k;
+                        }
+                        at += __popc(bits & ((1u << lane) - 1u));
+                        if (hit && at < want) sh.cand[at] = rank_key(order_value(bkey), i);
+                        n = min(n, want);
+                    }
+                    lp_sync();
+                }
+                if (plain) {
+                    lp_select_plain(r.z, lo, hi, e, a.top, sh.list[0], sh.cand);
+                    n = min(a.top, hi - lo);
+                    best = lane < n ? sh.list[0][lane] : 0ull;
+                } else {
+                    // each warp sorts 32 at a time and keeps the 32 largest
+                    for (int i = ew * 32; i < n; i += LP_EPI) {
+                        const unsigned long long k = lp_sort32(i + lane < n ? sh.cand[i + lane] : 0ull, lane);
+                        best = i == ew * 32 ? k : lp_merge32(best, k, lane);
+                    }
+                    if (n > 32) {
+                        sh.list[ew][lane] = best;
+                        lp_sync();
+                        if (ew == 0)
+                            for (int w = 1; w < LP_EPI / 32; ++w) best = lp_merge32(best, sh.list[w][lane], lane);
+                    }
+                    n = min(n, a.top);
+                }
+            }
+
+            // ---- to the first CTA ----
+            if (ew == 0) {
+                if (lane == 0) mbar_arrive(&sh.done[slot]);
+                sums = lp_join_warp(sh.sums[lane & 3], 4);
+                // the slot's last row has been taken
+                if (parts > 1 && nth >= 2) lp_wait_cluster(&sh.taken[slot], turn ^ 1u, abort_flag);
+                const uint32_t here = smem_u32(&sh.slots[slot][rank]), to = parts > 1 ? map_to_rank(here, 0) : here;
+                if (lane < n) st_cluster(to + offsetof(LpPart, list) + lane * 8, best);
+                if (lane == 0) {
+                    st_cluster(to, sums.mc);
+                    st_cluster(to + 4, sums.s);
+                    st_cluster(to + 8, sums.w);
+                    st_cluster(to + offsetof(LpPart, top), top_all);
+                    st_cluster(to + offsetof(LpPart, count), __int_as_float(n));
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    if (parts > 1) {
+                        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                        mbar_arrive_cluster(map_to_rank(smem_u32(&sh.ready[slot]), 0));
+                    } else {
+                        mbar_arrive(&sh.ready[slot]);
+                    }
+                }
+            }
+            if (rank != 0) { lp_sync(); continue; }
+
+            // ---- the row ----
+            // given tokens' logits are fetched before the wait
+            float given = 0.f;
+            long id = -1;
+            if (e < a.M) {
+                id = a.ids[static_cast<long>(row) * a.ld_ids + e];
+                if (id >= 0 && id < a.V) given = to_f32(r.z[id]);
+            }
+            lp_wait_cluster(&sh.ready[slot], turn, abort_flag);
+            const LpPart* p = sh.slots[slot];
+            sums = lp_join_warp(lane < parts ? p[lane].sums : LpSums{LP_FLOOR * kLog2e, 0.f, 0.f}, LP_CLUSTER);
+            sums = LpSums{__shfl_sync(0xffffffffu, sums.mc, 0), __shfl_sync(0xffffffffu, sums.s, 0),
+                          __shfl_sync(0xffffffffu, sums.w, 0)};
+            top_all = lane < parts ? p[lane].top : -INFINITY;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top_all = max_nan(top_all, __shfl_xor_sync(0xffffffffu, top_all, o));
+            if (a.top > 0) {
+                // warp w merges the lists of parts w, w + 4, ..., warp 0 the four results
+                best = 0ull;
+                for (int i = ew; i < parts; i += LP_EPI / 32) {
+                    const unsigned long long k = lane < p[i].count ? p[i].list[lane] : 0ull;
+                    best = i == ew ? k : lp_merge32(best, k, lane);
+                }
+                if (parts > 1) {
+                    sh.list[ew][lane] = best;
+                    lp_sync();
+                    if (ew == 0)
+                        for (int w = 1; w < min(parts, LP_EPI / 32); ++w) best = lp_merge32(best, sh.list[w][lane], lane);
+                }
+            }
+            const float log2s = log2f(sums.s);
+            float m = -INFINITY, logs = 0.f, ent = kLn2 * (log2s - sums.w / sums.s);
+            // nothing allowed; or beyond the range of the sums, or NaN
+            const bool none = top_all == -INFINITY;
+            const bool odd = !none && !(sums.mc > 0.1f * LP_FLOOR && sums.mc < -LP_FLOOR && sums.s < INFINITY);
+            if (none) ent = 0.f;
+            if (odd) lp_row_plain(a, r.z, e, sh.red, m, logs, ent);
+            const auto lp = [&](float f) {
+                if (none) return -INFINITY;
+                if (odd) return (f - m) - logs;
+                return (fmaf(f, kLog2e, -sums.mc) - log2s) * kLn2;
+            };
+            if (e == 0) a.entropy[row] = ent;
+            for (int j = e; j < a.M; j += LP_EPI) {
+                if (j != e) {
+                    id = a.ids[static_cast<long>(row) * a.ld_ids + j];
+                    given = id >= 0 && id < a.V ? to_f32(r.z[id]) : 0.f;
+                }
+                a.logprob[static_cast<long>(row) * a.M + j] = id < 0 ? 0.f : id >= a.V ? nan_f32() : lp(given);
+            }
+            if (ew == 0 && lane < a.top) {
+                a.top_lp[static_cast<long>(row) * a.top + lane] = lp(order_value(static_cast<uint32_t>(best >> 32)));
+                a.top_id[static_cast<long>(row) * a.top + lane] = static_cast<long>(~static_cast<uint32_t>(best));
+            }
+            lp_sync();                            // the slot has been read
+            if (parts > 1 && e < parts) mbar_arrive_cluster(map_to_rank(smem_u32(&sh.taken[slot]), e));
+        }
+    }
+    if (parts > 1) cluster_sync();        // no CTA ends while another may still write to it
 }
 
 }  // namespace mica

@@ -8,6 +8,7 @@
 #include <cudaTypedefs.h>
 
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -1263,30 +1264,41 @@ int mica_cache_keep(void* pool, long page_stride, int slabs, int pages, int page
 }
 
 // ---------------------------------------------------------------------------------------
-// CTAs of a row: a cluster, so that few rows still use the chip and many rows end together. Each run
-// is to hold two full steps of its threads at least.
+// CTAs of a row. One CTA an SM makes sms / parts clusters that take the rows in turn: the time is the
+// rows of the busiest cluster, each costing its part's bytes and, between rows, about as much as
+// LP_ROW_COST bytes. A part of fewer than LP_PART_BYTES is not worth a CTA.
+constexpr long LP_ROW_COST = 16 << 10, LP_PART_BYTES = 12 << 10;
 static int logprob_parts(int N, int V, int dtype, int sms) {
-    const long step = static_cast<long>(LP_THREADS) * LP_UNROLL * 16 / static_cast<long>(dt_size(dtype));
-    int parts = 1;
-    while (parts < LP_CLUSTER && static_cast<long>(N) * parts < 2L * sms && V / (2L * parts) >= step) parts *= 2;
-    return parts;
+    int best = 1;
+    long least = LONG_MAX;
+    for (int parts = 1; parts <= LP_CLUSTER; parts *= 2) {
+        const long clusters = std::max(1, sms / parts), bytes = static_cast<long>(V) * static_cast<long>(dt_size(dtype)) / parts;
+        if (parts > 1 && bytes < LP_PART_BYTES) break;
+        const long cost = ((N + clusters - 1) / clusters) * (bytes + LP_ROW_COST);
+        if (cost < least) { least = cost; best = parts; }
+    }
+    return best;
 }
 
 template <typename T>
-static int logprob_launch(const LogprobArgs& a, int parts, cudaStream_t st) {
+static int logprob_launch(const LogprobArgs& a, int parts, int sms, cudaStream_t st) {
     int dev = 0;
     cudaGetDevice(&dev);
     static std::atomic<uint64_t> done{0};
     const uint64_t bit = 1ull << (dev & 63);
     cudaError_t e;
     if (!(done.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) { set_cuda_error(e); return MICA_ERR_CUDA; }
+        if ((e = cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess ||
+            (e = cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, LP_SMEM)) != cudaSuccess) {
+            set_cuda_error(e);
+            return MICA_ERR_CUDA;
+        }
         done.fetch_or(bit, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(static_cast<long>(a.N) * parts));
-    cfg.blockDim = dim3(LP_THREADS);
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min(a.N, std::max(1, sms / parts)) * parts));
+    cfg.blockDim = dim3(LP_BLOCK);
+    cfg.dynamicSmemBytes = LP_SMEM;
     cfg.stream = st;
     cudaLaunchAttribute at[1] = {};
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1305,7 +1317,7 @@ int mica_token_logprobs(const void* z, int dtype, long ld, int N, int V, const i
         (top > 0 && (!top_lp || !top_id)))
         return MICA_ERR_ARG;
     if (N < 0 || V < 1 || ld < V || ld_ids < M || top > LP_TOP || top > V) return MICA_ERR_SHAPE;
-    if (static_cast<long>(N) * LP_CLUSTER > (1L << 31) - 1 || V > (1 << 30)) return MICA_ERR_RANGE;
+    if (V > (1 << 30) || N > (1 << 30)) return MICA_ERR_RANGE;
     if (!aligned_to(z, static_cast<unsigned>(dt_size(dtype))) || !aligned_to(ids, 8) || !aligned_to(top_id, 8) ||
         !aligned_to(logprob, 4) || !aligned_to(entropy, 4) || !aligned_to(top_lp, 4))
         return MICA_ERR_ALIGN;
@@ -1319,9 +1331,9 @@ int mica_token_logprobs(const void* z, int dtype, long ld, int N, int V, const i
     a.top_id = reinterpret_cast<long*>(top_id);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int parts = logprob_parts(N, V, dtype, sms);
-    if (dtype == MICA_DT_BF16) return logprob_launch<__nv_bfloat16>(a, parts, st);
-    if (dtype == MICA_DT_FP16) return logprob_launch<__half>(a, parts, st);
-    return logprob_launch<float>(a, parts, st);
+    if (dtype == MICA_DT_BF16) return logprob_launch<__nv_bfloat16>(a, parts, sms, st);
+    if (dtype == MICA_DT_FP16) return logprob_launch<__half>(a, parts, sms, st);
+    return logprob_launch<float>(a, parts, sms, st);
 }
 
 // ---------------------------------------------------------------------------------------
