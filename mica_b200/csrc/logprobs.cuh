@@ -38,15 +38,16 @@ struct LogprobArgs {
     long* top_id;               // [N, top]
 };
 
-constexpr int LP_THREADS = 768;          // make the pass
+constexpr int LP_THREADS = 640;          // make the pass
 constexpr int LP_WARPS = LP_THREADS / 32;
-constexpr int LP_EPI = 128;              // finish a row
-constexpr int LP_BLOCK = LP_THREADS + 32 + LP_EPI;
+constexpr int LP_EPI = 128;              // finish a row; two groups of them take rows in turn
+constexpr int LP_BLOCK = LP_THREADS + 32 + 2 * LP_EPI;
 constexpr int LP_UNROLL = 4;             // 16-byte vectors of a thread's step
-constexpr int LP_STEP = LP_THREADS * LP_UNROLL;         // vectors of a ring stage (48 KB)
+constexpr int LP_STEP = LP_THREADS * LP_UNROLL;         // vectors of a ring stage (40 KB)
 constexpr int LP_STAGES = 3;
 constexpr int LP_CAND = 512;             // candidates a CTA can rank
 constexpr int LP_TOP = 32;
+constexpr int LP_BACK = 768;             // vectors read again at once
 constexpr int LP_CLUSTER = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -60,7 +61,7 @@ __device__ __forceinline__ float to_f32(T v) {
     else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
     else return __bfloat162float(v);
 }
-__device__ __forceinline__ void lp_sync() { named_bar_sync(1, LP_EPI); }   // the warps that finish a row
+__device__ __forceinline__ void lp_sync(int g) { named_bar_sync(1 + g, LP_EPI); }   // a group that finishes a row
 __device__ __forceinline__ float nan_f32() { return __uint_as_float(0x7fc00000u); }
 
 // Orders logits for the alternatives: larger value first, NaN above +inf, -0 equal to +0.
@@ -119,17 +120,17 @@ struct LpVec {
     }
 };
 
-// One thread's step: its sums and largest logit take in LP_UNROLL vectors.
-template <typename T>
-__device__ __forceinline__ void lp_step(const uint4 (&q)[LP_UNROLL], LpSums& a, float& top) {
+// One thread's step: its sums and largest logit take in U vectors.
+template <typename T, int U>
+__device__ __forceinline__ void lp_step(const uint4 (&q)[U], LpSums& a, float& top) {
     constexpr int N = LpVec<T>::N;
     float cm;
-    uint4 c[LP_UNROLL];
+    uint4 c[U];
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {       // maxima of pairs
         __nv_bfloat162 m2 = *reinterpret_cast<const __nv_bfloat162*>(&q[0].x);
         const __nv_bfloat162 lo2 = __float2bfloat162_rn(LP_FLOOR);
 #pragma unroll
-        for (int u = 0; u < LP_UNROLL; ++u) {
+        for (int u = 0; u < U; ++u) {
             const uint32_t* w = reinterpret_cast<const uint32_t*>(&q[u]);
             uint32_t* o = reinterpret_cast<uint32_t*>(&c[u]);
 #pragma unroll
@@ -145,7 +146,7 @@ __device__ __forceinline__ void lp_step(const uint4 (&q)[LP_UNROLL], LpSums& a, 
         float f[N];
         cm = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < LP_UNROLL; ++u) {
+        for (int u = 0; u < U; ++u) {
             LpVec<T>::values(q[u], f);
 #pragma unroll
             for (int i = 0; i < N; ++i) cm = max_nan(cm, f[i]);
@@ -163,7 +164,7 @@ __device__ __forceinline__ void lp_step(const uint4 (&q)[LP_UNROLL], LpSums& a, 
     const unsigned long long c2 = f2_pack(kLog2e, kLog2e), n2 = f2_pack(-a.mc, -a.mc);
     unsigned long long s2 = 0ull, w2 = 0ull;
 #pragma unroll
-    for (int u = 0; u < LP_UNROLL; ++u) {
+    for (int u = 0; u < U; ++u) {
         float f[N];
         LpVec<T>::values(c[u], f);
 #pragma unroll
@@ -197,18 +198,18 @@ struct LpPart {                 // what a CTA tells its cluster of a row
 
 // The row by the LP_EPI threads, in passes, for maxima near the type's ends, infinities and NaN: the
 // definition literally.
-__device__ __forceinline__ float lp_reduce(float v, bool max, float* red) {
+__device__ __forceinline__ float lp_reduce(float v, bool max, float* red, int g) {
     v = max ? warp_max(v) : warp_sum(v);
-    lp_sync();
-    if ((threadIdx.x & 31) == 0) red[(threadIdx.x >> 5) & 3] = v;
-    lp_sync();
+    lp_sync(g);
+    if ((threadIdx.x & 31) == 0) red[((threadIdx.x - LP_THREADS - 32) >> 5) & 3] = v;
+    lp_sync(g);
     v = red[0];
     for (int i = 1; i < LP_EPI / 32; ++i) v = max ? fmaxf(v, red[i]) : v + red[i];
     return v;
 }
 template <typename T>
-__device__ __noinline__ void lp_row_plain(const LogprobArgs& a, const T* z, int e, float* red, float& m, float& logs,
-                                          float& ent) {
+__device__ __noinline__ void lp_row_plain(const LogprobArgs& a, const T* z, int e, int g, float* red, float& m,
+                                          float& logs, float& ent) {
     m = -INFINITY;
     float odd = 0.f;
     for (int i = e; i < a.V; i += LP_EPI) {
@@ -216,16 +217,16 @@ __device__ __noinline__ void lp_row_plain(const LogprobArgs& a, const T* z, int 
         if (v != v || v == INFINITY) odd = 1.f;
         m = fmaxf(m, v);
     }
-    odd = lp_reduce(odd, true, red);
-    m = lp_reduce(m, true, red);
+    odd = lp_reduce(odd, true, red, g);
+    m = lp_reduce(m, true, red, g);
     float s = 0.f, w = 0.f;
     for (int i = e; i < a.V; i += LP_EPI) {
         const float d = to_f32(z[i]) - m, x = m == -INFINITY ? 0.f : expf(d);
         s += x;
         if (x > 0.f) w -= d * x;
     }
-    s = lp_reduce(s, false, red);
-    w = lp_reduce(w, false, red);
+    s = lp_reduce(s, false, red, g);
+    w = lp_reduce(w, false, red, g);
     logs = m == -INFINITY ? 0.f : logf(s);
     ent = m == -INFINITY ? 0.f : logs + w / s;
     if (odd > 0.f) logs = ent = nan_f32();
@@ -234,7 +235,7 @@ __device__ __noinline__ void lp_row_plain(const LogprobArgs& a, const T* z, int 
 // The largest `top` keys of elements [i0, i1), each by one pass: for runs with more large values in a
 // few threads than a list holds.
 template <typename T>
-__device__ __noinline__ void lp_select_plain(const T* z, int i0, int i1, int e, int top, unsigned long long* list,
+__device__ __noinline__ void lp_select_plain(const T* z, int i0, int i1, int e, int g, int top, unsigned long long* list,
                                              unsigned long long* best) {
     unsigned long long last = ~0ull;
     for (int j = 0; j < top; ++j) {
@@ -248,18 +249,18 @@ __device__ __noinline__ void lp_select_plain(const T* z, int i0, int i1, int e, 
             const unsigned long long c = __shfl_xor_sync(0xffffffffu, b, o);
             b = c > b ? c : b;
         }
-        lp_sync();
+        lp_sync(g);
         if ((e & 31) == 0) best[e >> 5] = b;
-        lp_sync();
+        lp_sync(g);
         for (int i = 0; i < LP_EPI / 32; ++i) b = best[i] > b ? best[i] : b;
         last = b;
         if (e == 0) list[j] = b;
     }
-    lp_sync();
+    lp_sync(g);
 }
 
 // Sorts 32 keys across the lanes, largest first.
-__device__ __forceinline__ unsigned long long lp_sort32(unsigned long long k, int lane) {
+__device__ __noinline__ unsigned long long lp_sort32(unsigned long long k, int lane) {
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -272,7 +273,7 @@ __device__ __forceinline__ unsigned long long lp_sort32(unsigned long long k, in
     return k;
 }
 // The 32 largest of two sorted sets, sorted.
-__device__ __forceinline__ unsigned long long lp_merge32(unsigned long long a, unsigned long long b, int lane) {
+__device__ __noinline__ unsigned long long lp_merge32(unsigned long long a, unsigned long long b, int lane) {
     const unsigned long long r = __shfl_sync(0xffffffffu, b, 31 - lane);
     unsigned long long k = a > r ? a : r;                            // bitonic
 #pragma unroll
@@ -283,15 +284,22 @@ __device__ __forceinline__ unsigned long long lp_merge32(unsigned long long a, u
     return k;
 }
 
-// Joins the sums of `width` lanes (a power of two) in a fixed order; every lane gets the same bits.
-__device__ __forceinline__ LpSums lp_join_warp(LpSums s, int width) {
-    const int lane = threadIdx.x & 31;
-    for (int o = width >> 1; o > 0; o >>= 1) {
-        const LpSums b{__shfl_xor_sync(0xffffffffu, s.mc, o), __shfl_xor_sync(0xffffffffu, s.s, o),
-                       __shfl_xor_sync(0xffffffffu, s.w, o)};
-        s = lane & o ? lp_join(b, s) : lp_join(s, b);
+// Joins the lanes' sums: the maximum first, then each is rescaled to it once and added, in a fixed
+// order; every lane gets the same bits. (Not inlined, as the sort and the merge: a row is finished once
+// in thousands of instructions of the pass, so its code is fetched anew, and that took longer than
+// running it.)
+__device__ __noinline__ LpSums lp_join_warp(LpSums a) {
+    float mc = a.mc;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mc = max_nan(mc, __shfl_xor_sync(0xffffffffu, mc, o));
+    const float d = fmaxf(a.mc - mc, -1000.f), f = fast_exp2(d);
+    float s = a.s * f, w = f * fmaf(d, a.s, a.w);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        w += __shfl_xor_sync(0xffffffffu, w, o);
     }
-    return s;
+    return LpSums{mc, s, w};
 }
 
 __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
@@ -341,15 +349,21 @@ struct LpRow {
     }
 };
 
+struct LpGroup {                // what finishing a row works on
+    unsigned long long cand[LP_CAND];
+    unsigned long long list[4][LP_TOP];
+    uint4 back[LP_BACK];                 // vectors read again
+    int back_at[LP_BACK], hit[LP_BACK];
+    int who[LP_THREADS];
+    uint32_t group[64], bound;           // order keys
+    float red[4], top[4];
+    LpSums sums[4];
+    int count, n_who, n_hit;
+};
 struct LpShared {
     float4 mine[2][LP_THREADS];          // of each thread of the pass: sums and largest logit, rows in turn
-    unsigned long long cand[LP_CAND];
     LpPart slots[2][LP_CLUSTER];         // of the first CTA: the parts of a row, rows in turn
-    unsigned long long list[4][LP_TOP];
-    int who[LP_THREADS];
-    float group[64], red[4], bound;
-    LpSums sums[4];
-    int count, n_who;
+    LpGroup work[2];
     uint64_t full[LP_STAGES], empty[LP_STAGES], passed[2], done[2], ready[2], taken[2];
     uint32_t abort;
 };
@@ -420,15 +434,24 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
             float top = -INFINITY;
             for (int v = r.v0; v < r.v1; v += LP_STEP, ++it) {
                 const int st = it % LP_STAGES;
+                const uint4* in = ring + st * LP_STEP + tid;
                 mbar_wait(&sh.full[st], (it / LP_STAGES) & 1u, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
-                uint4 q[LP_UNROLL];
+                if (v + LP_STEP <= r.v1) {
+                    uint4 q[LP_UNROLL];
 #pragma unroll
-                for (int u = 0; u < LP_UNROLL; ++u)
-                    q[u] = v + tid + u * LP_THREADS < r.v1 ? ring[st * LP_STEP + tid + u * LP_THREADS]
-                                                           : make_uint4(kNone, kNone, kNone, kNone);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.empty[st]);
-                lp_step<T>(q, sums, top);
+                    for (int u = 0; u < LP_UNROLL; ++u) q[u] = in[u * LP_THREADS];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.empty[st]);
+                    lp_step<T>(q, sums, top);
+                } else {
+                    // the row's last stage: a vector at a time
+                    for (int u = v + warp * 32; u < r.v1; u += LP_THREADS, in += LP_THREADS) {
+                        uint4 q[1] = {u + lane < r.v1 ? *in : make_uint4(kNone, kNone, kNone, kNone)};
+                        lp_step<T>(q, sums, top);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.empty[st]);
+                }
             }
             if (my_single >= 0) {
                 top = max_nan(top, single);
@@ -442,154 +465,183 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
         }
     } else {
         // ---------------------------------- finishing rows ----------------------------------
-        const int e = threadIdx.x - LP_THREADS - 32, ew = e >> 5;
-        int nth = 0;
-        for (int row = first_row; row < a.N; row += rows_step, ++nth) {
+        const int g = (warp - LP_WARPS - 1) / (LP_EPI / 32);
+        const int e = (threadIdx.x - LP_THREADS - 32) % LP_EPI, ew = e >> 5, slot = g;
+        LpGroup& wk = sh.work[g];
+        int nth = g;
+        for (long next = first_row + static_cast<long>(g) * rows_step; next < a.N; next += 2l * rows_step, nth += 2) {
+            const int row = static_cast<int>(next);
             const LpRow<T> r(a, row, rank, parts);
-            const int slot = nth & 1;
             const uint32_t turn = (nth >> 1) & 1u;
-            if (e == 0) sh.count = sh.n_who = 0;
+            if (e == 0) wk.count = wk.n_who = 0;
+            // the given tokens are on their way during the pass
+            long id = -1;
+            if (rank == 0 && e < a.M) id = a.ids[static_cast<long>(row) * a.ld_ids + e];
             mbar_wait(&sh.passed[slot], turn, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
             // six threads' sums and maxima each; two of these are a group
+            constexpr int kEach = LP_THREADS / LP_EPI;
             LpSums sums;
-            float top;
-            {
-                float4 f = sh.mine[slot][e];
-                sums = LpSums{f.x, f.y, f.z};
-                top = f.w;
+            float4 six[kEach];
+            float top = -INFINITY, mc = -INFINITY;
 #pragma unroll
-                for (int i = 1; i < LP_THREADS / LP_EPI; ++i) {
-                    f = sh.mine[slot][e + i * LP_EPI];
-                    sums = lp_join(sums, LpSums{f.x, f.y, f.z});
-                    top = max_nan(top, f.w);
-                }
+            for (int i = 0; i < kEach; ++i) {
+                six[i] = sh.mine[slot][e + i * LP_EPI];
+                top = max_nan(top, six[i].w);
+                mc = max_nan(mc, six[i].x);
             }
-            const float g = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            if ((e & 1) == 0) sh.group[e >> 1] = g;
-            sums = lp_join_warp(sums, 32);
-            if (lane == 0) sh.sums[ew] = sums;
-            lp_sync();
-            float top_all = -INFINITY;
-            for (int i = 0; i < 64; i += 32) top_all = max_nan(top_all, sh.group[i + lane]);
+            sums = LpSums{mc, 0.f, 0.f};
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top_all = max_nan(top_all, __shfl_xor_sync(0xffffffffu, top_all, o));
+            for (int i = 0; i < kEach; ++i) {
+                const float d = fmaxf(six[i].x - mc, -1000.f), f = fast_exp2(d);
+                sums.s = fmaf(six[i].y, f, sums.s);
+                sums.w = fmaf(f, fmaf(d, six[i].y, six[i].z), sums.w);
+            }
+            sums = lp_join_warp(sums);
+            if (lane == 0) wk.sums[ew] = sums;
+            const float pair = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            if ((e & 1) == 0) wk.group[e >> 1] = order_key(pair);
+#pragma unroll
+            for (int o = 16; o > 1; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            if (lane == 0) wk.top[ew] = top;
+            lp_sync(g);
             unsigned long long best = 0ull;          // of warp 0: the run's alternatives in order
             int n = 0;
             if (a.top > 0) {
-                if (e < 64) {
-                    // the top-th largest of the 64 maxima
-                    const uint32_t me = order_key(sh.group[e]);
+                {
+                    // the top-th largest of the 64 maxima; two threads count for each
+                    const int i0 = e >> 1;
+                    const uint32_t me = wk.group[i0];
                     int above = 0;
-#pragma unroll 16
-                    for (int i = 0; i < 64; ++i) {
-                        const uint32_t o = order_key(sh.group[i]);
-                        above += o > me || (o == me && i < e);
+                    const uint4* g4 = reinterpret_cast<const uint4*>(wk.group) + (e & 1) * 8;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint4 k = g4[i];
+                        const int at = (e & 1) * 32 + i * 4;
+                        above += (k.x > me || (k.x == me && at < i0)) + (k.y > me || (k.y == me && at + 1 < i0)) +
+                                 (k.z > me || (k.z == me && at + 2 < i0)) + (k.w > me || (k.w == me && at + 3 < i0));
                     }
-                    if (above == a.top - 1) sh.bound = sh.group[e];
+                    above += __shfl_xor_sync(0xffffffffu, above, 1);
+                    if (above == a.top - 1 && (e & 1) == 0) wk.bound = me;
                 }
-                lp_sync();
-                const uint32_t bkey = order_key(sh.bound);
+                lp_sync(g);
+                const uint32_t bkey = wk.bound;
                 const int n_mine = r.v1 - r.v0, per = (n_mine + LP_THREADS - 1) / LP_THREADS;
                 // threads of the pass whose maximum reaches the bound, then their vectors' elements that do
                 // (strict: are above it)
 #pragma unroll
-                for (int i = 0; i < LP_THREADS / LP_EPI; ++i)
-                    if (order_key(sh.mine[slot][e + i * LP_EPI].w) >= bkey) sh.who[atomicAdd(&sh.n_who, 1)] = e + i * LP_EPI;
+                for (int i = 0; i < kEach; ++i)
+                    if (order_key(six[i].w) >= bkey) wk.who[atomicAdd(&wk.n_who, 1)] = e + i * LP_EPI;
                 const auto gather = [&](bool strict) {
                     const auto keep = [&](float f, int id) {
                         const uint32_t k = order_key(f);
                         if (strict ? k > bkey : k >= bkey) {
-                            const int at = atomicAdd(&sh.count, 1);
-                            if (at < LP_CAND) sh.cand[at] = rank_key(f, id);
+                            const int at = atomicAdd(&wk.count, 1);
+                            if (at < LP_CAND) wk.cand[at] = rank_key(f, id);
                         }
                     };
-                    const int total = sh.n_who * per;
-                    for (int w0 = e; w0 < total; w0 += 4 * LP_EPI) {
-                        uint4 q[4];
-                        int at[4];
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const int w = w0 + u * LP_EPI;
-                            at[u] = w < total ? sh.who[w / per] + (w % per) * LP_THREADS : n_mine;
-                            if (at[u] < n_mine) q[u] = __ldg(r.vectors() + r.v0 + at[u]);
+                    // their vectors come into shared memory, LP_BACK at a time; of those with an element that
+                    // passes, each element is a thread's
+                    const int items = wk.n_who * per;
+                    for (int b0 = 0; b0 < items; b0 += LP_BACK) {
+                        const int nb = min(LP_BACK, items - b0);
+#pragma unroll 1
+                        for (int i = e; i < nb; i += LP_EPI) {
+                            const int w = (b0 + i) / per, at = wk.who[w] + (b0 + i - w * per) * LP_THREADS;
+                            wk.back_at[i] = at;
+                            if (at < n_mine)
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&wk.back[i])),
+                                             "l"(reinterpret_cast<uint64_t>(r.vectors() + r.v0 + at)) : "memory");
                         }
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            if (at[u] >= n_mine) continue;
+                        if (e == 0) wk.n_hit = 0;
+                        asm volatile("cp.async.wait_all;" ::: "memory");
+                        lp_sync(g);
+#pragma unroll 1
+                        for (int i = e; i < nb; i += LP_EPI) {
+                            if (wk.back_at[i] >= n_mine) continue;
                             float f[N];
-                            LpVec<T>::values(q[u], f);
-                            float m = f[0];
+                            LpVec<T>::values(wk.back[i], f);
 #pragma unroll
-                            for (int i = 1; i < N; ++i) m = max_nan(m, f[i]);
-                            if (order_key(m) < bkey) continue;
-#pragma unroll
-                            for (int i = 0; i < N; ++i) keep(f[i], r.head + (r.v0 + at[u]) * N + i);
+                            for (int k = 1; k < N; ++k) f[0] = max_nan(f[0], f[k]);
+                            if (order_key(f[0]) >= bkey) wk.hit[atomicAdd(&wk.n_hit, 1)] = i;
                         }
+                        lp_sync(g);
+                        const int nh = wk.n_hit * N;
+#pragma unroll 1
+                        for (int i = e; i < nh; i += LP_EPI) {
+                            const int b = wk.hit[i / N];
+                            keep(to_f32(reinterpret_cast<const T*>(&wk.back[b])[i % N]),
+                                 r.head + (r.v0 + wk.back_at[b]) * N + i % N);
+                        }
+                        if (b0 + LP_BACK < items) lp_sync(g);
                     }
                     const int my_single = r.single(a, e, rank, parts);
                     if (my_single >= 0) keep(to_f32(r.z[my_single]), my_single);
                 };
-                lp_sync();
+                lp_sync(g);
                 gather(false);
-                lp_sync();
-                n = sh.count;
+                lp_sync(g);
+                n = wk.count;
                 // the run's elements
                 const int lo = rank == 0 ? 0 : r.head + r.v0 * N, hi = rank == parts - 1 ? a.V : r.head + r.v1 * N;
                 bool plain = false;
                 if (n > LP_CAND) {
                     // more ties at the bound than places (a row that allows few tokens, or equal logits): those
                     // above it, then the first ones at it in order of their ids
-                    lp_sync();
-                    if (e == 0) sh.count = 0;
-                    lp_sync();
+                    lp_sync(g);
+                    if (e == 0) wk.count = 0;
+                    lp_sync(g);
                     gather(true);
-                    lp_sync();
-                    n = sh.count;
+                    lp_sync(g);
+                    n = wk.count;
                     plain = n > LP_CAND - LP_TOP;
                     const int want = plain ? 0 : n + a.top;              // enough of them
                     for (int i0 = lo; i0 < hi && n < want; i0 += LP_EPI) {
                         const int i = i0 + e;
                         const bool hit = i < hi && order_key(to_f32(r.z[i])) == bkey;
                         const uint32_t bits = __ballot_sync(0xffffffffu, hit);
-                        lp_sync();
-                        if (lane == 0) sh.red[ew] = __int_as_float(__popc(bits));
-                        lp_sync();
+                        lp_sync(g);
+                        if (lane == 0) wk.red[ew] = __int_as_float(__popc(bits));
+                        lp_sync(g);
                         int at = n;
                         for (int w = 0; w < LP_EPI / 32; ++w) {
-                            const int k = __float_as_int(sh.red[w]);
+                            const int k = __float_as_int(wk.red[w]);
                             if (w < ew) at += k;
                             n += k;
                         }
                         at += __popc(bits & ((1u << lane) - 1u));
-                        if (hit && at < want) sh.cand[at] = rank_key(order_value(bkey), i);
+                        if (hit && at < want) wk.cand[at] = rank_key(order_value(bkey), i);
                         n = min(n, want);
                     }
-                    lp_sync();
+                    lp_sync(g);
                 }
                 if (plain) {
-                    lp_select_plain(r.z, lo, hi, e, a.top, sh.list[0], sh.cand);
+                    lp_select_plain(r.z, lo, hi, e, g, a.top, wk.list[0], wk.cand);
                     n = min(a.top, hi - lo);
-                    best = lane < n ? sh.list[0][lane] : 0ull;
+                    best = lane < n ? wk.list[0][lane] : 0ull;
                 } else {
                     // each warp sorts 32 at a time and keeps the 32 largest
                     for (int i = ew * 32; i < n; i += LP_EPI) {
-                        const unsigned long long k = lp_sort32(i + lane < n ? sh.cand[i + lane] : 0ull, lane);
+                        const unsigned long long k = lp_sort32(i + lane < n ? wk.cand[i + lane] : 0ull, lane);
                         best = i == ew * 32 ? k : lp_merge32(best, k, lane);
                     }
                     if (n > 32) {
-                        sh.list[ew][lane] = best;
-                        lp_sync();
+                        wk.list[ew][lane] = best;
+                        lp_sync(g);
                         if (ew == 0)
-                            for (int w = 1; w < LP_EPI / 32; ++w) best = lp_merge32(best, sh.list[w][lane], lane);
+                            for (int w = 1; w < LP_EPI / 32; ++w) best = lp_merge32(best, wk.list[w][lane], lane);
                     }
                     n = min(n, a.top);
                 }
             }
 
+            float given = rank == 0 && id >= 0 && id < a.V ? to_f32(r.z[id]) : 0.f;
+
             // ---- to the first CTA ----
             if (ew == 0) {
                 if (lane == 0) mbar_arrive(&sh.done[slot]);
-                sums = lp_join_warp(sh.sums[lane & 3], 4);
+                float top_all = max_nan(max_nan(wk.top[0], wk.top[1]), max_nan(wk.top[2], wk.top[3]));
+                sums = lp_join_warp(lane < 4 ? wk.sums[lane] : LpSums{LP_FLOOR * kLog2e, 0.f, 0.f});
                 // the slot's last row has been taken
                 if (parts > 1 && nth >= 2) lp_wait_cluster(&sh.taken[slot], turn ^ 1u, abort_flag);
                 const uint32_t here = smem_u32(&sh.slots[slot][rank]), to = parts > 1 ? map_to_rank(here, 0) : here;
@@ -611,24 +663,17 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
                     }
                 }
             }
-            if (rank != 0) { lp_sync(); continue; }
+            if (rank != 0) { lp_sync(g); continue; }
 
             // ---- the row ----
-            // given tokens' logits are fetched before the wait
-            float given = 0.f;
-            long id = -1;
-            if (e < a.M) {
-                id = a.ids[static_cast<long>(row) * a.ld_ids + e];
-                if (id >= 0 && id < a.V) given = to_f32(r.z[id]);
-            }
             lp_wait_cluster(&sh.ready[slot], turn, abort_flag);
             const LpPart* p = sh.slots[slot];
-            sums = lp_join_warp(lane < parts ? p[lane].sums : LpSums{LP_FLOOR * kLog2e, 0.f, 0.f}, LP_CLUSTER);
-            sums = LpSums{__shfl_sync(0xffffffffu, sums.mc, 0), __shfl_sync(0xffffffffu, sums.s, 0),
-                          __shfl_sync(0xffffffffu, sums.w, 0)};
-            top_all = lane < parts ? p[lane].top : -INFINITY;
+            sums = p[0].sums;
+            if (parts > 1) sums = lp_join_warp(lane < parts ? p[lane].sums : LpSums{LP_FLOOR * kLog2e, 0.f, 0.f});
+            float top_all = lane < parts ? p[lane].top : -INFINITY;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top_all = max_nan(top_all, __shfl_xor_sync(0xffffffffu, top_all, o));
+            for (int o = 8; o > 0; o >>= 1) top_all = max_nan(top_all, __shfl_xor_sync(0xffffffffu, top_all, o));
+            top_all = __shfl_sync(0xffffffffu, top_all, 0);
             if (a.top > 0) {
                 // warp w merges the lists of parts w, w + 4, ..., warp 0 the four results
                 best = 0ull;
@@ -637,10 +682,10 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
                     best = i == ew ? k : lp_merge32(best, k, lane);
                 }
                 if (parts > 1) {
-                    sh.list[ew][lane] = best;
-                    lp_sync();
+                    wk.list[ew][lane] = best;
+                    lp_sync(g);
                     if (ew == 0)
-                        for (int w = 1; w < min(parts, LP_EPI / 32); ++w) best = lp_merge32(best, sh.list[w][lane], lane);
+                        for (int w = 1; w < min(parts, LP_EPI / 32); ++w) best = lp_merge32(best, wk.list[w][lane], lane);
                 }
             }
             const float log2s = log2f(sums.s);
@@ -649,7 +694,7 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
             const bool none = top_all == -INFINITY;
             const bool odd = !none && !(sums.mc > 0.1f * LP_FLOOR && sums.mc < -LP_FLOOR && sums.s < INFINITY);
             if (none) ent = 0.f;
-            if (odd) lp_row_plain(a, r.z, e, sh.red, m, logs, ent);
+            if (odd) lp_row_plain(a, r.z, e, g, wk.red, m, logs, ent);
             const auto lp = [&](float f) {
                 if (none) return -INFINITY;
                 if (odd) return (f - m) - logs;
@@ -667,7 +712,7 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
                 a.top_lp[static_cast<long>(row) * a.top + lane] = lp(order_value(static_cast<uint32_t>(best >> 32)));
                 a.top_id[static_cast<long>(row) * a.top + lane] = static_cast<long>(~static_cast<uint32_t>(best));
             }
-            lp_sync();                            // the slot has been read
+            lp_sync(g);                            // the slot has been read
             if (parts > 1 && e < parts) mbar_arrive_cluster(map_to_rank(smem_u32(&sh.taken[slot]), e));
         }
     }
