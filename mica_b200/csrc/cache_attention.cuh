@@ -54,6 +54,7 @@ struct CacheAttnArgs {
     int ctas;                   // CTAs of the grid
     float scale_log2;           // scale * log2(e)
     float* ws;                  // partials: [ctas][2] places
+    int4* cuts;                 // [ctas][2] the unit a CTA starts inside, for the CTA that is the first to
 };
 
 // A place of the workspace: rows of O as [NT][D / 4][128] float4 (a warp's rows side by side), then
@@ -121,11 +122,21 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
     };
     const auto tiles = [&](int b) { return b < p.B ? KV * cache_seq_tiles(cache_seq(p, b), R, causal) : 0l; };
     const long mine = tiles(threadIdx.x);
-    long sum = mine, total = 0;
+    long total = 0;
+    if (threadIdx.x == 0) { s_b = -1; s_off = 0; }
+    if (p.B <= static_cast<int>(blockDim.x)) {
+        const long end = scan(mine, total), t = first(total);
+        if (t >= end - mine && t < end) {
+            s_b = threadIdx.x;
+            s_off = t - (end - mine);
+        }
+        __syncthreads();
+        return CachePlace{total, s_off, s_b};
+    }
+    long sum = mine;
     for (int b = threadIdx.x + blockDim.x; b < p.B; b += blockDim.x) sum += tiles(b);
     scan(sum, total);
     const long t = first(total);
-    if (threadIdx.x == 0) { s_b = -1; s_off = 0; }
     long before = 0;
     for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
         const long n = b0 == 0 ? mine : tiles(b0 + threadIdx.x);
@@ -142,13 +153,24 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
     return CachePlace{total, s_off, s_b};
 }
 
-// Tiles [lo, hi) of CTA c, of `ctas` (fewer are used when there are fewer tiles).
-__device__ __forceinline__ long cache_share(long total, int ctas, int c) {
-    return ctas <= 0 ? 0 : (total * c) / ctas;
-}
-__device__ __forceinline__ int cache_used_ctas(long total, int ctas) {
-    return static_cast<int>(total < ctas ? total : ctas);
-}
+// The runs of the CTAs: total / used tiles each, the first total % used one more. Fewer CTAs are used
+// when there are fewer tiles.
+struct CacheShare {
+    long each;
+    int rest, used;
+    __device__ __forceinline__ CacheShare(long total, int ctas) {
+        used = static_cast<int>(total < ctas ? total : ctas);
+        if (total <= 0x7fffffffl) {
+            const unsigned n = static_cast<unsigned>(total), d = max(used, 1);
+            each = n / d;
+            rest = static_cast<int>(n - static_cast<unsigned>(each) * d);
+        } else {
+            each = total / used;
+            rest = static_cast<int>(total - each * used);
+        }
+    }
+    __device__ __forceinline__ long at(int c) const { return each * c + min(c, rest); }
+};
 
 // The units of a CTA's run, one after another.
 struct CacheWalk {
@@ -163,7 +185,8 @@ struct CacheWalk {
         R = R_; causal = causal_; b = b_; left = n;
         s = cache_seq(p, b);
         const long per = cache_seq_tiles(s, R, causal);
-        kvh = static_cast<int>(off / per);
+        kvh = off <= 0x7fffffffl && per <= 0x7fffffffl ? static_cast<int>(static_cast<unsigned>(off) / static_cast<unsigned>(per))
+                                                       : static_cast<int>(off / per);
         off -= kvh * per;
         rb = 0;
         while (off >= (nk = cache_unit_tiles(s, rb, R, causal))) { off -= nk; ++rb; }
@@ -212,17 +235,29 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
         : "memory");
 }
 
-// Bits [off, off + 32) of a row's mask words, bits outside them zero.
-__device__ __forceinline__ uint32_t mask_bits(const unsigned long long* m, int words, int off) {
-    if (off <= -32) return 0u;
-    if (off < 0) return static_cast<uint32_t>(m[0] << -off);
-    const int w = off >> 6, sh = off & 63;
-    if (w >= words) return 0u;
-    unsigned long long v = m[w] >> sh;
-    if (sh > 32 && w + 1 < words) v |= m[w + 1] << (64 - sh);
-    return static_cast<uint32_t>(v);
+// 128 bits of a row's mask words from bit `off` (which may be negative) on, bits outside them zero.
+__device__ __forceinline__ void mask_bits(const unsigned long long* m, int words, int off, uint32_t (&out)[4]) {
+    const int w = off >> 6, sh = off & 63;                     // floor
+    unsigned long long v[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) v[i] = w + i >= 0 && w + i < words ? m[w + i] : 0ull;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const unsigned long long x = sh ? v[i] >> sh | v[i + 1] << (64 - sh) : v[i];
+        out[2 * i] = static_cast<uint32_t>(x);
+        out[2 * i + 1] = static_cast<uint32_t>(x >> 32);
+    }
 }
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// Rows behind the last sequence become zero; the whole block calls it.
+__device__ __forceinline__ void cache_zero_padding(const CacheAttnArgs& args, int D) {
+    const int end = min(max(args.plan.cu[args.plan.B], 0), args.plan.N);
+    const int vecs = args.KV * args.G * D / 8;
+    for (long row = end + static_cast<long>(blockIdx.x); row < args.plan.N; row += gridDim.x)
+        for (int i = threadIdx.x; i < vecs; i += blockDim.x)
+            *reinterpret_cast<uint4*>(args.out + row * args.ldo + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+}
 
 template <int D, int NT>
 __global__ void __launch_bounds__(CacheAttnShape<D, NT>::THREADS, 1)
@@ -234,24 +269,23 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     const bool causal = args.mask == nullptr;
     const int R = NT * args.npt;
 
-    // padding rows
-    {
-        const int end = min(max(plan.cu[plan.B], 0), plan.N);
-        const int vecs = args.KV * args.G * D / 8;
-        for (long row = end + static_cast<long>(blockIdx.x); row < plan.N; row += gridDim.x)
-            for (int i = threadIdx.x; i < vecs; i += blockDim.x)
-                *reinterpret_cast<uint4*>(args.out + row * args.ldo + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");    // the join kernel may take its place
+    const int cta = blockIdx.x;
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmap_q);
+        tma_prefetch_desc(&tmap_k);
+        tma_prefetch_desc(&tmap_v);
     }
     // this CTA's run of tiles
-    const int cta = blockIdx.x;
-    const CachePlace place = cache_locate(plan, args.KV, R, causal, [&](long total) {
-        return cache_share(total, cache_used_ctas(total, args.ctas), cta);
-    });
-    const int used = cache_used_ctas(place.total, args.ctas);
-    if (cta >= used || place.b < 0) return;
-    const long run = cache_share(place.total, used, cta + 1) - cache_share(place.total, used, cta);
+    const CachePlace place = cache_locate(plan, args.KV, R, causal, [&](long total) { return CacheShare(total, args.ctas).at(cta); });
+    const CacheShare share(place.total, args.ctas);
+    if (cta >= share.used || place.b < 0) {
+        if (threadIdx.x == 0) args.cuts[2 * cta] = make_int4(0, 0, 0, 0);
+        cache_zero_padding(args, D);
+        return;
+    }
     CacheWalk wk;
-    wk.start(plan, R, causal, place.b, place.off, run);
+    wk.start(plan, R, causal, place.b, place.off, share.at(cta + 1) - share.at(cta));
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -272,7 +306,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     uint64_t* drain = v_fixed + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile uint32_t* abort_flag = tmem_slot + 1;
-    uint32_t* odd_v = tmem_slot + 2;           // [2][4] keys of a special tile whose V row holds infinities or NaN
+    uint32_t* odd_v = tmem_slot + 2;           // [2][NT][4] keys of a special tile whose V row holds infinities or NaN
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -289,9 +323,6 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         mbar_init(drain, 1);
         *abort_flag = 0u;
         fence_mbar_init();
-        tma_prefetch_desc(&tmap_q);
-        tma_prefetch_desc(&tmap_k);
-        tma_prefetch_desc(&tmap_v);
     }
     if (warp == 1) tmem_alloc(tmem_slot, 512);
     tc_fence_before();
@@ -435,9 +466,10 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 mma_commit(&pv_done[i]);
                 return true;
             };
-            // the scores of a tile are issued before the P.V of the tile before it, across units too
+            // the scores of a tile are issued before the P.V of the tile before it, inside a unit: at its end
+            // the rows are waited for, and the next unit's Q and K may be a while coming
             CacheWalk pv = wk;                    // the unit of the next P.V
-            bool more = true;
+            bool more = true, pending = false;    // a tile's P.V is still to be issued
             int t = 0, unit = 0, pv_t = 0;
             int pv_j = pv.j0;
             const auto values_all = [&](int x) {
@@ -448,10 +480,19 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             const auto values_done = [&]() {
                 mma_commit(&v_empty[pv_t % S::VST]);
                 ++pv_t;
+                pending = false;
                 if (++pv_j == pv.j1 && pv.next(plan, args.KV)) pv_j = pv.j0;
+            };
+            const auto flush = [&]() {
+                if (!mma_wait(&v_full[pv_t % S::VST], (pv_t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+                for (int x = 0; x < NT; ++x)
+                    if (!values_all(x)) return false;
+                values_done();
+                return true;
             };
             while (more && ok) {
                 const int qb = S::QBUF == 2 ? unit & 1 : 0;
+                if (pending && !flush()) { ok = false; break; }
                 ok = mma_wait(&q_full[qb], unit / S::QBUF & 1, abort_flag, MICA_DEV_TIMEOUT_MMA);
                 for (int j = wk.j0; j < wk.j1 && ok; ++j, ++t) {
                     if (!mma_wait(&k_full[t % S::KST], (t / S::KST) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA) ||
@@ -460,7 +501,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                         mma_commit(&k_empty[t % S::KST]);
                         if (j + 1 == wk.j1) mma_commit(&q_empty[qb]);
                     }
-                    if (t > 0) {
+                    if (pending) {
                         if (!mma_wait(&v_full[pv_t % S::VST], (pv_t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA) ||
                             !values_all(0)) { ok = false; break; }
                     }
@@ -468,21 +509,34 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                         if (!scores(1, t, qb)) { ok = false; break; }
                         mma_commit(&k_empty[t % S::KST]);
                         if (j + 1 == wk.j1) mma_commit(&q_empty[qb]);
-                        if (t > 0 && !values_all(1)) { ok = false; break; }
+                        if (pending && !values_all(1)) { ok = false; break; }
                     }
-                    if (t > 0) values_done();
+                    if (pending) values_done();
+                    pending = true;
                 }
                 if (ok) { more = wk.next(plan, args.KV); ++unit; }
             }
-            if (ok && mma_wait(&v_full[pv_t % S::VST], (pv_t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) {
-                for (int x = 0; x < NT && ok; ++x) ok = values_all(x);
-            }
+            if (ok && pending) flush();
             mma_commit(drain);
             mbar_wait(drain, 0, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
         }
         __syncwarp();
     } else {
         // ---------------------------------- softmax ----------------------------------
+        if (threadIdx.x == 64) {
+            // the unit this CTA starts inside, for the join: its first row, node rows, K/V head, and the CTAs
+            // that hold parts of it, the one before and `n` from this one on
+            const long s0 = share.at(cta) - wk.j0;
+            int4 cut = make_int4(0, 0, 0, 0), more = cut;
+            if (wk.j0 > 0 && share.at(cta - 1) <= s0) {
+                int n = 1;
+                while (cta + n < share.used && share.at(cta + n) < s0 + wk.nk) ++n;
+                cut = make_int4(min(R, wk.s.T - wk.rb * R) * args.G, wk.s.row0 + wk.rb * R, wk.kvh, n);
+                more.x = share.at(cta - 1) == s0 ? 0 : 1;         // the place of the first part
+            }
+            args.cuts[2 * cta] = cut;
+            args.cuts[2 * cta + 1] = more;
+        }
         const int x = (warp - 2) >> 2;                     // row tile of this warpgroup
         const int q4 = warp & 3;                           // tensor-memory lane quarter
         const int r = q4 * 32 + lane;                      // row of the tile
@@ -512,45 +566,57 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
                 if (special) {
                     const int end = causal ? min(s.keys, s.base + node + 1) : s.keys;
+                    uint32_t bits[4];
+                    if (!causal && live && s.keys)
+                        mask_bits(args.mask + row * args.ld_mask, args.words, k0 - s.base, bits);
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         vis[w] = live ? low_bits(end - k0 - 32 * w) : 0u;
-                        if (!causal && live && s.keys)
-                            vis[w] &= low_bits(s.base - k0 - 32 * w) |
-                                      mask_bits(args.mask + row * args.ld_mask, args.words, k0 + 32 * w - s.base);
+                        if (!causal) vis[w] &= low_bits(s.base - k0 - 32 * w) | (s.keys ? bits[w] : 0u);
                     }
                     // V rows behind the keys become zero; odd values of the step's own rows too, noted
                     // (two sets of odd_v: all warps pass v_fixed of a special tile before one writes the next but one)
                     const int st = t % S::VST;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
+                    if (!ok) break;
+                    const int key = k0 + r;
                     bool odd = false;
-                    if (x == 0) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
-                        if (!ok) break;
-                        const int key = k0 + r;
-                        uint4* vr = reinterpret_cast<uint4*>(sv + st * S::TILE + r * 128);
-                        if (key >= s.keys || key >= s.base) {
+                    if (key >= s.base || key >= s.keys) {
+                        // with two row tiles, half of the row's columns each
+                        const int h0 = NT == 2 ? x : 0, h1 = NT == 2 ? min(x + 1, S::HALVES) : S::HALVES;
+                        for (int h = h0; h < h1; ++h) {
+                            uint4* vr = reinterpret_cast<uint4*>(sv + st * S::TILE + h * ATT_HALF_BYTES + r * 128);
+                            if (key >= s.keys) {
 #pragma unroll
-                            for (int h = 0; h < S::HALVES; ++h)
+                                for (int e = 0; e < 8; ++e) vr[e ^ (r & 7)] = make_uint4(0u, 0u, 0u, 0u);
+                                continue;
+                            }
+                            // 0 * v is zero for finite v only
+                            __nv_bfloat162 any = bf2(0u);
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    uint4* p = vr + h * (ATT_HALF_BYTES / 16) + (e ^ (r & 7));
-                                    if (key >= s.keys) { *p = make_uint4(0u, 0u, 0u, 0u); continue; }
-                                    uint4 v = *p;
-                                    uint32_t* u = reinterpret_cast<uint32_t*>(&v);
-                                    bool hit = false;
-#pragma unroll
-                                    for (int k = 0; k < 4; ++k) {
-                                        if ((u[k] & 0x7f800000u) == 0x7f800000u) { u[k] &= 0x0000ffffu; hit = true; }
-                                        if ((u[k] & 0x00007f80u) == 0x00007f80u) { u[k] &= 0xffff0000u; hit = true; }
-                                    }
-                                    if (hit) { *p = v; odd = true; }
+                            for (int e = 0; e < 8; ++e) {
+                                const uint4 v = vr[e ^ (r & 7)];
+                                any = __hfma2(bf2(v.x), bf2(0u), any);
+                                any = __hfma2(bf2(v.y), bf2(0u), any);
+                                any = __hfma2(bf2(v.z), bf2(0u), any);
+                                any = __hfma2(bf2(v.w), bf2(0u), any);
+                            }
+                            if (bits2(any) & 0x7fff7fffu) {
+                                odd = true;
+                                uint32_t* u = reinterpret_cast<uint32_t*>(vr);
+                                for (int e = 0; e < 32; ++e) {
+                                    if ((u[e] & 0x7f800000u) == 0x7f800000u) u[e] &= 0x0000ffffu;
+                                    if ((u[e] & 0x00007f80u) == 0x00007f80u) u[e] &= 0xffff0000u;
                                 }
+                            }
                         }
-                        const uint32_t bits = __ballot_sync(0xffffffffu, odd);
-                        if (lane == 0) odd_v[(fixes & 1) * 4 + q4] = bits;
-                        fence_proxy_async_smem();
-                        __syncwarp();
                     }
+                    {
+                        const uint32_t found = __ballot_sync(0xffffffffu, odd);
+                        if (lane == 0) odd_v[((fixes & 1) * NT + x) * 4 + q4] = found;
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
                     if (lane == 0) mbar_arrive(v_fixed);
                 }
                 bool w = true;
@@ -613,11 +679,13 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 }
                 // this P buffer is free once its last P.V is done; the accumulator once the tile before's is
                 bool any_odd = false;
-                const volatile uint32_t* odd4 = odd_v + (fixes & 1) * 4;
+                const volatile uint32_t* odd4 = odd_v + (fixes & 1) * 4 * NT;
                 if (special) {
                     ok = __all_sync(0xffffffffu, mbar_wait(v_fixed, fixes & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
                     if (!ok) break;
-                    any_odd = (odd4[0] | odd4[1] | odd4[2] | odd4[3]) != 0u;
+                    uint32_t some = 0u;
+                    for (int i = 0; i < 4 * NT; ++i) some |= odd4[i];
+                    any_odd = some != 0u;
                     ++fixes;
                 }
                 const bool fresh = j == wk.j0;
@@ -645,7 +713,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                         }
                         if (any_odd) {
                             for (int w4 = 0; w4 < 4; ++w4)
-                                for (uint32_t bits = odd4[w4]; bits; bits &= bits - 1) {
+                                for (uint32_t bits = odd4[w4] | odd4[(NT - 1) * 4 + w4]; bits; bits &= bits - 1) {
                                     const int i = __ffs(bits) - 1;
                                     int pgn = 0, slot = 0;
                                     if (!(vis[w4] >> i & 1u) || !cache_slot(plan, wk.b, k0 + w4 * 32 + i, &pgn, &slot)) continue;
@@ -729,55 +797,49 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         tc_fence_after();
         tmem_free(tmem, 512);
     }
+    cache_zero_padding(args, D);
 }
 
-// Adds up the parts of each divided unit. Block (c, y): the unit that CTA c + 1's run starts inside,
-// if c + 1 is the first to do so; its rows x columns are dealt to the blocks y.
+// Adds up the parts of each divided unit, in the order of the CTAs. Block (c, y): the unit that CTA
+// c + 1 is the first to start inside, if it is; a thread takes four columns of a row.
 template <int D, int NT>
-__global__ void __launch_bounds__(128) cache_attention_join(const CacheAttnArgs args) {
-    const CachePlan& plan = args.plan;
-    const bool causal = args.mask == nullptr;
-    const int R = NT * args.npt;
+__global__ void __launch_bounds__(256) cache_attention_join(const CacheAttnArgs args) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int c = blockIdx.x + 1;
-    const CachePlace place = cache_locate(plan, args.KV, R, causal, [&](long total) {
-        return cache_share(total, cache_used_ctas(total, args.ctas), c);
-    });
-    const int used = cache_used_ctas(place.total, args.ctas);
-    if (c >= used || place.b < 0) return;
-    const auto at = [&](int i) { return cache_share(place.total, used, i); };
-    CacheWalk wk;
-    wk.start(plan, R, causal, place.b, place.off, 1);
-    if (wk.j0 == 0) return;                                   // starts with its unit
-    const long s0 = at(c) - wk.j0, s1 = s0 + wk.nk;           // the unit's tiles
-    if (at(c - 1) > s0) return;                               // CTA c - 1 starts inside it as well
-    int n = 1;                                                // CTAs c - 1 .. c - 1 + n
-    while (c + n < used && at(c + n) < s1) ++n;
-    const int rows = min(R, wk.s.T - wk.rb * R) * args.G;
+    const int4 cut = args.cuts[2 * c];
+    const int rows = cut.x, n = cut.w;
+    const int idx = blockIdx.y * blockDim.x + threadIdx.x;
+    if (idx >= rows * (D / 4)) return;
+    const int first_place = args.cuts[2 * c + 1].x;
     const long pf = cache_attn_place_floats<D, NT>();
-    const int first_place = at(c - 1) == s0 ? 0 : 1;
-    for (int idx = blockIdx.y * blockDim.x + threadIdx.x; idx < rows * (D / 4); idx += gridDim.y * blockDim.x) {
-        const int rr = idx % rows, d4 = idx / rows;
-        const int node = rr / args.G, g = rr % args.G;
-        const int x = node / args.npt, r = (node - x * args.npt) * args.G + g;
-        const auto ml = [&](int i) {
-            return *reinterpret_cast<const float2*>(args.ws + ((c - 1 + i) * 2l + (i ? 0 : first_place)) * pf + NT * 128l * D + (x * 128 + r) * 2);
-        };
-        float m = -INFINITY;
-        for (int i = 0; i <= n; ++i) m = fmaxf(m, ml(i).x);
-        float l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = 0; i <= n; ++i) {
-            const float2 v = ml(i);
-            const float w = fast_exp2(v.x - m);
-            const float4 p = *(reinterpret_cast<const float4*>(args.ws + ((c - 1 + i) * 2l + (i ? 0 : first_place)) * pf) + (x * (D / 4) + d4) * 128 + r);
-            l = fmaf(v.y, w, l);
-            o.x = fmaf(p.x, w, o.x); o.y = fmaf(p.y, w, o.y); o.z = fmaf(p.z, w, o.z); o.w = fmaf(p.w, w, o.w);
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const long row = static_cast<long>(wk.s.row0) + wk.rb * R + node;
-        *reinterpret_cast<uint2*>(args.out + row * args.ldo + (wk.kvh * args.G + g) * D + d4 * 4) =
-            make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    const int rr = idx % rows, d4 = idx / rows;
+    const int node = rr / args.G, g = rr % args.G;
+    const int x = NT == 1 ? 0 : node / args.npt, r = (node - x * args.npt) * args.G + g;
+    const float* part0 = args.ws + ((c - 1) * 2l + first_place) * pf;
+    const float* parts = args.ws + c * 2l * pf;
+    const auto at = [&](int i) { return i == 0 ? part0 : parts + (i - 1) * 2l * pf; };
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    // two parts at a time: loads first
+    for (int i = 0; i <= n; i += 2) {
+        const bool two = i < n;
+        const float* a0 = at(i);
+        const float* a1 = at(two ? i + 1 : i);
+        const float2 m0 = __ldcg(reinterpret_cast<const float2*>(a0 + NT * 128l * D) + x * 128 + r);
+        const float2 m1 = __ldcg(reinterpret_cast<const float2*>(a1 + NT * 128l * D) + x * 128 + r);
+        const float4 p0 = __ldcg(reinterpret_cast<const float4*>(a0) + (x * (D / 4) + d4) * 128 + r);
+        const float4 p1 = __ldcg(reinterpret_cast<const float4*>(a1) + (x * (D / 4) + d4) * 128 + r);
+        const float mn = fmaxf(m, fmaxf(m0.x, m1.x));
+        const float wo = fast_exp2(m - mn), w0 = fast_exp2(m0.x - mn), w1 = two ? fast_exp2(m1.x - mn) : 0.f;
+        m = mn;
+        const auto add = [&](float a, float b, float e) { return two ? fmaf(e, w1, fmaf(b, w0, a * wo)) : fmaf(b, w0, a * wo); };
+        l = add(l, m0.y, m1.y);
+        o.x = add(o.x, p0.x, p1.x); o.y = add(o.y, p0.y, p1.y); o.z = add(o.z, p0.z, p1.z); o.w = add(o.w, p0.w, p1.w);
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const long row = static_cast<long>(cut.y) + node;
+    *reinterpret_cast<uint2*>(args.out + row * args.ldo + (cut.z * args.G + g) * D + d4 * 4) =
+        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
 
 }  // namespace mica

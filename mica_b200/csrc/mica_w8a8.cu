@@ -1107,7 +1107,8 @@ int mica_cache_append(const void* qkv, long ld, const void* q_w, const void* k_w
         !aligned16(q_out) || !aligned16(k_pages) || !aligned16(v_pages) || ld % 8 || ldq % 8 || page_stride % 8 ||
         !aligned_to(pos, 8) || !aligned_to(table, 4) || !aligned_to(base, 4) || !aligned_to(cu, 4))
         return MICA_ERR_ALIGN;
-    if ((rc = check_device(nullptr))) return rc;
+    int sms = 0;
+    if ((rc = check_device(&sms))) return rc;
     if (N == 0) return MICA_OK;
     a.qkv = static_cast<const __nv_bfloat16*>(qkv); a.ld = ld;
     a.q_w = static_cast<const __nv_bfloat16*>(q_w); a.k_w = static_cast<const __nv_bfloat16*>(k_w);
@@ -1117,10 +1118,13 @@ int mica_cache_append(const void* qkv, long ld, const void* q_w, const void* k_w
     a.k_pages = static_cast<__nv_bfloat16*>(k_pages); a.v_pages = static_cast<__nv_bfloat16*>(v_pages);
     a.page_stride = page_stride; a.H = H; a.KV = KV; a.eps = eps;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const long blocks = (static_cast<long>(N) * (H + 2 * KV) + 7) / 8;
+    // few rows are split over warps until the chip has about 16 warps an SM
+    const int sets = (H + 2 * KV + 256 / D - 1) / (256 / D);
+    const int split = static_cast<int>(std::min<long>(sets, std::max(1L, 16L * sms / N)));
+    const long blocks = (static_cast<long>(N) * split + 7) / 8;
     if (blocks > (1L << 31) - 1) return MICA_ERR_RANGE;
-    if (D == 128) cache_append_kernel<128><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
-    else cache_append_kernel<64><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+    if (D == 128) cache_append_kernel<128><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, split);
+    else cache_append_kernel<64><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, split);
     return launch_status();
 }
 
@@ -1132,7 +1136,7 @@ static void cache_attn_rows(int max_new, int G, int* nt, int* npt) {
     *npt = *nt == 1 ? std::max(1, max_new) : most;
 }
 static size_t cache_attn_bytes(int sms, int nt, int D) {
-    return static_cast<size_t>(sms) * 2 * nt * 128 * (D + 2) * sizeof(float);
+    return static_cast<size_t>(sms) * 2 * (nt * 128 * (D + 2) * sizeof(float) + sizeof(int4));
 }
 size_t mica_cache_attention_workspace_bytes(int N, int max_new, int H, int KV, int D) {
     int sms = 0, nt = 0, npt = 0;
@@ -1162,7 +1166,19 @@ static int cache_attn_launch(const CUtensorMap& tq, const CUtensorMap& tk, const
     if (int rc = cache_attn_prepare<D, NT>()) return rc;
     cache_attention_kernel<D, NT><<<a.ctas, CacheAttnShape<D, NT>::THREADS, CacheAttnShape<D, NT>::SMEM, st>>>(tq, tk, tv, a);
     if (int rc = launch_status()) return rc;
-    if (a.ctas > 1) cache_attention_join<D, NT><<<dim3(a.ctas - 1, 4), 128, 0, st>>>(a);
+    if (a.ctas < 2) return MICA_OK;
+    // the join is launched under the attention kernel's end (it waits for all of it before it reads)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.ctas - 1, (NT * a.npt * a.G * (D / 4) + 255) / 256);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1] = {};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, cache_attention_join<D, NT>, a);
+    if (e != cudaSuccess) { set_cuda_error(e); return MICA_ERR_CUDA; }
     return launch_status();
 }
 
@@ -1195,6 +1211,7 @@ int mica_cache_attention(const void* q, long ldq, const void* k_pages, const voi
     a.out = static_cast<__nv_bfloat16*>(out); a.ldo = ldo; a.KV = KV; a.G = H / KV; a.ctas = sms;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.ws = static_cast<float*>(workspace);
+    a.cuts = reinterpret_cast<int4*>(a.ws + static_cast<size_t>(sms) * 2 * nt * 128 * (D + 2));
     CUtensorMap tq, tk, tv;
     const uint64_t rows = static_cast<uint64_t>(KV) * page;
     if ((rc = make_tmap_bf16_3d(&tq, q, D, H, N, D * 2, static_cast<uint64_t>(ldq) * 2, a.G, a.npt)) ||
