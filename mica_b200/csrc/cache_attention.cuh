@@ -13,15 +13,17 @@
 // q lays down as it is), and the key axis is cut wherever the SMs need it:
 //
 // Work. A unit is (sequence, K/V head, block of NT * npt nodes); its key tiles of 128 follow one
-// another, units in order, in one line of tiles. Each of the CTAs (one per SM) takes an equal run of
-// that line, whatever the lengths: it starts and may end inside a unit. A unit that one CTA has whole
+// another, units in order, in one line (where each unit has some places more for what it costs by
+// itself). Each of the CTAs (one per SM) takes an equal run of that line, whatever the lengths: it
+// starts and may end inside a unit. A unit that one CTA has whole
 // is written out; of a divided one each CTA leaves its unnormalised rows, maxima and sums in its own
 // place of the workspace (a CTA has at most two such: its first and its last), and
 // cache_attention_join adds them up in the order of the CTAs. No atomics: the same bits every time.
 // The lengths are read on the device, so a captured graph serves any.
 //
-// Warps: 0 TMA producer (Q tiles, then K and V tiles page by page: one box per page and 64 columns,
-// one lane each, the page numbers fetched a tile ahead); 1 issues the MMAs (S = Q K^T both from
+// Warps: 0 loads Q and K tiles, 2 V tiles, by TMA page by page: one box per page and 64 columns, one
+// lane each, the page numbers fetched a tile ahead (a box takes the warp about 90 cycles, so that with
+// pages of 16 one warp for both was as slow as memory); 1 issues the MMAs (S = Q K^T both from
 // shared memory, O += P V with P in tensor memory); the others softmax, one row a thread, as in
 // attention.cuh. NT = 1: S and P have two buffers each, so scores, softmax and P.V of three
 // consecutive tiles overlap; Q has two, so the next unit's loads run under this one's end. NT = 2:
@@ -84,22 +86,22 @@ __device__ __forceinline__ int cache_unit_tiles(const CacheSeq& s, int rb, int R
     return max(1, (keys + 127) >> 7);
 }
 __device__ __forceinline__ int cache_row_blocks(const CacheSeq& s, int R) { return (s.T + R - 1) / R; }
-__device__ __forceinline__ long cache_seq_tiles(const CacheSeq& s, int R, bool causal) {   // of one K/V head
+__device__ __forceinline__ long cache_seq_places(const CacheSeq& s, int R, int E, bool causal) {   // of one K/V head
     const int n = cache_row_blocks(s, R);
-    if (!causal || n <= 1) return n ? static_cast<long>(n) * cache_unit_tiles(s, n - 1, R, causal) : 0;
+    if (!causal || n <= 1) return n ? static_cast<long>(n) * (cache_unit_tiles(s, n - 1, R, causal) + E) : 0;
     long t = 0;
-    for (int rb = 0; rb < n; ++rb) t += cache_unit_tiles(s, rb, R, true);
+    for (int rb = 0; rb < n; ++rb) t += cache_unit_tiles(s, rb, R, true) + E;
     return t;
 }
 
-struct CachePlace {             // a position in the line: tile `off` of sequence b
+struct CachePlace {             // a place of the line: the off-th of sequence b
     long total;
     long off;
     int b;
 };
-// Total tiles and the sequence that holds tile `first(total)`; every thread of the block calls it.
+// The line's length and the sequence that holds place `first(total)`; every thread of the block calls it.
 template <typename F>
-__device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, int R, bool causal, F first) {
+__device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, int R, int E, bool causal, F first) {
     __shared__ long s_warp[32];
     __shared__ long s_off;
     __shared__ int s_b;
@@ -120,7 +122,7 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
         }
         return v;
     };
-    const auto tiles = [&](int b) { return b < p.B ? KV * cache_seq_tiles(cache_seq(p, b), R, causal) : 0l; };
+    const auto tiles = [&](int b) { return b < p.B ? KV * cache_seq_places(cache_seq(p, b), R, E, causal) : 0l; };
     const long mine = tiles(threadIdx.x);
     long total = 0;
     if (threadIdx.x == 0) { s_b = -1; s_off = 0; }
@@ -153,8 +155,8 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
     return CachePlace{total, s_off, s_b};
 }
 
-// The runs of the CTAs: total / used tiles each, the first total % used one more. Fewer CTAs are used
-// when there are fewer tiles.
+// The runs of the CTAs: total / used places each, the first total % used one more. Fewer CTAs are used
+// when there are fewer places.
 struct CacheShare {
     long each;
     int rest, used;
@@ -172,30 +174,33 @@ struct CacheShare {
     __device__ __forceinline__ long at(int c) const { return each * c + min(c, rest); }
 };
 
-// The units of a CTA's run, one after another.
+// The units of a CTA's run, one after another: those of which it has tiles.
 struct CacheWalk {
     CacheSeq s;
     int b, kvh, rb;             // unit
     int nk, j0, j1;             // its tiles, and the CTA's [j0, j1) of them
-    long left;                  // tiles of the run from j0 on
-    int R;
+    long left;                  // places of the run from the unit's first on
+    int R, E;
     bool causal;
 
-    __device__ __forceinline__ void start(const CachePlan& p, int R_, bool causal_, int b_, long off, long n) {
-        R = R_; causal = causal_; b = b_; left = n;
+    // false: the run lies in front of a unit's first tile
+    __device__ __forceinline__ bool start(const CachePlan& p, int R_, int E_, bool causal_, int b_, long off, long n) {
+        R = R_; E = E_; causal = causal_; b = b_;
         s = cache_seq(p, b);
-        const long per = cache_seq_tiles(s, R, causal);
+        const long per = cache_seq_places(s, R, E, causal);
         kvh = off <= 0x7fffffffl && per <= 0x7fffffffl ? static_cast<int>(static_cast<unsigned>(off) / static_cast<unsigned>(per))
                                                        : static_cast<int>(off / per);
         off -= kvh * per;
         rb = 0;
-        while (off >= (nk = cache_unit_tiles(s, rb, R, causal))) { off -= nk; ++rb; }
-        j0 = static_cast<int>(off);
-        j1 = static_cast<int>(min(static_cast<long>(nk), j0 + left));
+        while (off >= (nk = cache_unit_tiles(s, rb, R, causal)) + E) { off -= nk + E; ++rb; }
+        left = n + off;
+        j0 = max(0, static_cast<int>(off) - E);
+        j1 = static_cast<int>(min(static_cast<long>(nk), left - E));
+        return j1 > j0;
     }
     __device__ __forceinline__ bool next(const CachePlan& p, int KV) {
-        left -= j1 - j0;
-        if (left <= 0) return false;
+        left -= nk + E;
+        if (left <= E) return false;
         if (++rb >= cache_row_blocks(s, R)) {
             rb = 0;
             if (++kvh >= KV) {
@@ -208,7 +213,7 @@ struct CacheWalk {
         }
         nk = cache_unit_tiles(s, rb, R, causal);
         j0 = 0;
-        j1 = static_cast<int>(min(static_cast<long>(nk), left));
+        j1 = static_cast<int>(min(static_cast<long>(nk), left - E));
         return true;
     }
     __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == nk; }
@@ -223,7 +228,10 @@ struct CacheAttnShape {
     static constexpr int QBUF = NT == 1 ? 2 : 1;
     static constexpr int KST = D == 128 ? 3 : 6;
     static constexpr int VST = D == 128 ? 2 : 5;
-    static constexpr int THREADS = 64 + 128 * NT;
+    static constexpr int THREADS = 96 + 128 * NT;
+    // What a unit costs beside its tiles (its rows' way out, nothing in flight), in tiles: it stands in the
+    // line for that many places more.
+    static constexpr int UNIT = NT == 1 ? 1 : 2;
     static constexpr int BARS = 512;
     static constexpr int SMEM = 1024 + TILE * (QBUF * NT + KST + VST) + BARS;
 };
@@ -277,15 +285,16 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         tma_prefetch_desc(&tmap_v);
     }
     // this CTA's run of tiles
-    const CachePlace place = cache_locate(plan, args.KV, R, causal, [&](long total) { return CacheShare(total, args.ctas).at(cta); });
+    const CachePlace place = cache_locate(plan, args.KV, R, S::UNIT, causal,
+                                          [&](long total) { return CacheShare(total, args.ctas).at(cta); });
     const CacheShare share(place.total, args.ctas);
-    if (cta >= share.used || place.b < 0) {
+    CacheWalk wk;
+    if (cta >= share.used || place.b < 0 ||
+        !wk.start(plan, R, S::UNIT, causal, place.b, place.off, share.at(cta + 1) - share.at(cta))) {
         if (threadIdx.x == 0) args.cuts[2 * cta] = make_int4(0, 0, 0, 0);
         cache_zero_padding(args, D);
         return;
     }
-    CacheWalk wk;
-    wk.start(plan, R, causal, place.b, place.off, share.at(cta + 1) - share.at(cta));
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -335,91 +344,79 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     const auto col_p = [](int i) { return (NT == 1 ? 256 : 128) + i * 64; };
     const auto col_o = [](int x) { return NT == 1 ? 384 : 256 + x * 128; };
 
-    if (warp == 0) {
-        // ---------------------------------- producer ----------------------------------
+    if (warp == 0 || warp == 2) {
+        // ---------------------------------- producers ---------------------------------
+        const bool is_k = warp == 0;
+        const int stages = is_k ? S::KST : S::VST;
+        uint64_t* const full = is_k ? k_full : v_full;
+        uint64_t* const empty = is_k ? k_empty : v_empty;
+        uint8_t* const ring = is_k ? sk : sv;
+        const CUtensorMap* const map = is_k ? &tmap_k : &tmap_v;
         const int ppt = 128 >> plan.page_log2;             // pages of a key tile
         const int boxes = ppt * S::HALVES;                 // <= 16, lane i: page i / HALVES, columns 64 (i % HALVES)
         const int my_page = lane / S::HALVES, my_half = lane % S::HALVES;
         const uint32_t box_bytes = 128u << plan.page_log2;
         const int page = 1 << plan.page_log2;
-        bool ok = true;
-        int kt = 0, vt = 0;                               // tiles loaded
-        int unit = 0;
+        bool ok = true, more = true;
+        int unit = 0, t = 0, st = 0;                       // units, tiles, ring stage
+        uint32_t par = 1u;                                 // of the stage's `empty`
         // pages of key tile j of the walk's unit that hold keys; this lane's page number
-        const auto pages_in = [&](const CacheWalk& w, int j) {
-            return max(0, min(ppt, (w.s.keys - j * 128 + page - 1) >> plan.page_log2));
+        const auto pages_in = [&](int j) { return max(0, min(ppt, (wk.s.keys - j * 128 + page - 1) >> plan.page_log2)); };
+        const auto fetch = [&](int j) {
+            return lane < boxes && my_page < pages_in(j)
+                       ? plan.table[static_cast<long>(wk.b) * plan.ld_table + j * ppt + my_page] : 0;
         };
-        const auto fetch = [&](const CacheWalk& w, int j) {
-            return lane < boxes && my_page < pages_in(w, j)
-                       ? plan.table[static_cast<long>(w.b) * plan.ld_table + j * ppt + my_page] : 0;
-        };
-        const auto load = [&](bool is_k, int t, int n_pages, int kvh, int pg) {
-            const int st = is_k ? t % S::KST : t % S::VST;
-            const uint32_t par = ((is_k ? t / S::KST : t / S::VST) & 1u) ^ 1u;
-            uint64_t* full = is_k ? &k_full[st] : &v_full[st];
-            bool w = true;
-            if (lane == 0) {
-                w = mbar_wait(is_k ? &k_empty[st] : &v_empty[st], par, abort_flag, MICA_DEV_TIMEOUT_PRODUCER);
-                if (w) mbar_arrive_expect_tx(full, n_pages * S::HALVES * box_bytes);
-            }
-            if (!__shfl_sync(0xffffffffu, w, 0)) return false;
-            if (lane < n_pages * S::HALVES) {
-                uint8_t* d = (is_k ? sk : sv) + st * S::TILE + my_half * ATT_HALF_BYTES + my_page * box_bytes;
-                // a page outside the pool is outside the map and reads as zeros
-                if (pg < 0 || pg >= plan.pages) { pg = plan.pages; record_bad_page(); }
-                tma_load_3d(d, is_k ? &tmap_k : &tmap_v, full, my_half * 64, kvh << plan.page_log2, pg);
-            }
-            __syncwarp();
-            return true;
-        };
-        int v_pages = 0, v_kvh = 0, v_pg = 0;              // the tile whose V is still to come
-        bool more = true, pending = false;
-        const auto load_v = [&]() {
-            pending = false;
-            return load(false, vt++, v_pages, v_kvh, v_pg);
-        };
-        int pg = fetch(wk, wk.j0);
+        int pg = fetch(wk.j0);
         while (more && ok) {
-            if (wk.s.keys == 0 && lane == 0) record_bad_page();
-            // Q tiles of the unit
-            const int qb = S::QBUF == 2 ? unit & 1 : 0;
-            const uint32_t q_par = static_cast<uint32_t>(unit / S::QBUF & 1) ^ 1u;
-            // with one Q buffer the wait is for the scores of the unit's last tile, whose softmax may want V first
-            if (S::QBUF == 1 && pending && !load_v()) { ok = false; break; }
-            bool w = true;
-            if (lane == 0) {
-                w = mbar_wait(&q_empty[qb], q_par, abort_flag, MICA_DEV_TIMEOUT_PRODUCER);
-                if (w) {
-                    mbar_arrive_expect_tx(&q_full[qb], NT * S::HALVES * 128u * args.npt * args.G);
-                    for (int x = 0; x < NT; ++x)
-                        for (int h = 0; h < S::HALVES; ++h)
-                            tma_load_3d(sq + (qb * NT + x) * S::TILE + h * ATT_HALF_BYTES, &tmap_q, &q_full[qb], h * 64,
-                                        wk.kvh * args.G, wk.s.row0 + (wk.rb * NT + x) * args.npt);
+            if (is_k) {
+                if (wk.s.keys == 0 && lane == 0) record_bad_page();
+                // Q tiles of the unit
+                const int qb = S::QBUF == 2 ? unit & 1 : 0;
+                bool w = true;
+                if (lane == 0) {
+                    w = mbar_wait(&q_empty[qb], static_cast<uint32_t>(unit / S::QBUF & 1) ^ 1u, abort_flag,
+                                  MICA_DEV_TIMEOUT_PRODUCER);
+                    if (w) {
+                        mbar_arrive_expect_tx(&q_full[qb], NT * S::HALVES * 128u * args.npt * args.G);
+                        for (int x = 0; x < NT; ++x)
+                            for (int h = 0; h < S::HALVES; ++h)
+                                tma_load_3d(sq + (qb * NT + x) * S::TILE + h * ATT_HALF_BYTES, &tmap_q, &q_full[qb], h * 64,
+                                            wk.kvh * args.G, wk.s.row0 + (wk.rb * NT + x) * args.npt);
+                    }
                 }
-            }
-            ok = __shfl_sync(0xffffffffu, w, 0);
-            for (int j = wk.j0; j < wk.j1 && ok; ++j) {
-                const int n_pages = pages_in(wk, j), kvh = wk.kvh, cur = pg;
-                ok = load(true, kt, n_pages, kvh, cur);
-                // the next tile's page number, a tile ahead of its use
-                if (j + 1 < wk.j1) pg = fetch(wk, j + 1);
-                else { more = wk.next(plan, args.KV); if (more) pg = fetch(wk, wk.j0); j = wk.j1; }
-                ++kt;
-                if (ok && pending) ok = load_v();
-                v_pages = n_pages; v_kvh = kvh; v_pg = cur;
-                pending = true;
+                ok = __shfl_sync(0xffffffffu, w, 0);
             }
             ++unit;
+            const int end = wk.j1;
+            for (int j = wk.j0; j < end && ok; ++j, ++t) {
+                const int n = pages_in(j) * S::HALVES, kvh = wk.kvh;
+                int cur = pg;
+                // the next tile's page number, a tile ahead of its use
+                if (j + 1 < end) pg = fetch(j + 1);
+                else if ((more = wk.next(plan, args.KV))) pg = fetch(wk.j0);
+                bool w = true;
+                if (lane == 0) {
+                    w = mbar_wait(&empty[st], par, abort_flag, MICA_DEV_TIMEOUT_PRODUCER);
+                    if (w) mbar_arrive_expect_tx(&full[st], n * box_bytes);
+                }
+                ok = __shfl_sync(0xffffffffu, w, 0);
+                if (ok && lane < n) {
+                    // a page outside the pool is outside the map and reads as zeros
+                    if (cur < 0 || cur >= plan.pages) { cur = plan.pages; record_bad_page(); }
+                    tma_load_3d(ring + st * S::TILE + my_half * ATT_HALF_BYTES + my_page * box_bytes, map, &full[st], my_half * 64,
+                                kvh << plan.page_log2, cur);
+                }
+                __syncwarp();
+                if (++st == stages) { st = 0; par ^= 1u; }
+            }
         }
-        if (ok && pending) ok = load_v();
         // loads still in flight land before shared memory is released
         if (lane == 0) {
-            for (int i = max(0, unit - S::QBUF); i < unit; ++i)
-                mbar_wait(&q_full[S::QBUF == 2 ? i & 1 : 0], i / S::QBUF & 1, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
-            for (int t = kt > S::KST ? kt - S::KST : 0; t < kt; ++t)
-                mbar_wait(&k_full[t % S::KST], (t / S::KST) & 1, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
-            for (int t = vt > S::VST ? vt - S::VST : 0; t < vt; ++t)
-                mbar_wait(&v_full[t % S::VST], (t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
+            if (is_k)
+                for (int i = max(0, unit - S::QBUF); i < unit; ++i)
+                    mbar_wait(&q_full[S::QBUF == 2 ? i & 1 : 0], i / S::QBUF & 1, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
+            for (int i = max(0, t - stages); i < t; ++i)
+                mbar_wait(&full[i % stages], (i / stages) & 1, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -523,21 +520,21 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         __syncwarp();
     } else {
         // ---------------------------------- softmax ----------------------------------
-        if (threadIdx.x == 64) {
+        if (threadIdx.x == 96) {
             // the unit this CTA starts inside, for the join: its first row, node rows, K/V head, and the CTAs
             // that hold parts of it, the one before and `n` from this one on
-            const long s0 = share.at(cta) - wk.j0;
+            const long s0 = share.at(cta) - wk.j0;                // the unit's first tile in the line
             int4 cut = make_int4(0, 0, 0, 0), more = cut;
             if (wk.j0 > 0 && share.at(cta - 1) <= s0) {
                 int n = 1;
                 while (cta + n < share.used && share.at(cta + n) < s0 + wk.nk) ++n;
                 cut = make_int4(min(R, wk.s.T - wk.rb * R) * args.G, wk.s.row0 + wk.rb * R, wk.kvh, n);
-                more.x = share.at(cta - 1) == s0 ? 0 : 1;         // the place of the first part
+                more.x = share.at(cta - 1) >= s0 - S::UNIT ? 0 : 1;   // the first part's place: it may be its CTA's first unit
             }
             args.cuts[2 * cta] = cut;
             args.cuts[2 * cta + 1] = more;
         }
-        const int x = (warp - 2) >> 2;                     // row tile of this warpgroup
+        const int x = (warp - 3) >> 2;                     // row tile of this warpgroup
         const int q4 = warp & 3;                           // tensor-memory lane quarter
         const int r = q4 * 32 + lane;                      // row of the tile
         const int node_r = r / args.G, head_r = r % args.G;
@@ -801,45 +798,51 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 }
 
 // Adds up the parts of each divided unit, in the order of the CTAs. Block (c, y): the unit that CTA
-// c + 1 is the first to start inside, if it is; a thread takes four columns of a row.
+// c + 1 is the first to start inside, if it is; a thread takes 16 columns of a row, four vectors of
+// each part in flight.
 template <int D, int NT>
-__global__ void __launch_bounds__(256) cache_attention_join(const CacheAttnArgs args) {
+__global__ void __launch_bounds__(128) cache_attention_join(const CacheAttnArgs args) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int c = blockIdx.x + 1;
     const int4 cut = args.cuts[2 * c];
     const int rows = cut.x, n = cut.w;
     const int idx = blockIdx.y * blockDim.x + threadIdx.x;
-    if (idx >= rows * (D / 4)) return;
+    if (idx >= rows * (D / 16)) return;
     const int first_place = args.cuts[2 * c + 1].x;
     const long pf = cache_attn_place_floats<D, NT>();
-    const int rr = idx % rows, d4 = idx / rows;
-    const int node = rr / args.G, g = rr % args.G;
+    const int rr = idx % rows, d16 = idx / rows;
+    const int node = rr / args.G, g = rr - node * args.G;
     const int x = NT == 1 ? 0 : node / args.npt, r = (node - x * args.npt) * args.G + g;
     const float* part0 = args.ws + ((c - 1) * 2l + first_place) * pf;
     const float* parts = args.ws + c * 2l * pf;
-    const auto at = [&](int i) { return i == 0 ? part0 : parts + (i - 1) * 2l * pf; };
     float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    // two parts at a time: loads first
-    for (int i = 0; i <= n; i += 2) {
-        const bool two = i < n;
-        const float* a0 = at(i);
-        const float* a1 = at(two ? i + 1 : i);
-        const float2 m0 = __ldcg(reinterpret_cast<const float2*>(a0 + NT * 128l * D) + x * 128 + r);
-        const float2 m1 = __ldcg(reinterpret_cast<const float2*>(a1 + NT * 128l * D) + x * 128 + r);
-        const float4 p0 = __ldcg(reinterpret_cast<const float4*>(a0) + (x * (D / 4) + d4) * 128 + r);
-        const float4 p1 = __ldcg(reinterpret_cast<const float4*>(a1) + (x * (D / 4) + d4) * 128 + r);
-        const float mn = fmaxf(m, fmaxf(m0.x, m1.x));
-        const float wo = fast_exp2(m - mn), w0 = fast_exp2(m0.x - mn), w1 = two ? fast_exp2(m1.x - mn) : 0.f;
+    float4 o[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i <= n; ++i) {
+        const float* a = i == 0 ? part0 : parts + (i - 1) * 2l * pf;
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(a + NT * 128l * D) + x * 128 + r);
+        float4 p[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) p[v] = __ldcg(reinterpret_cast<const float4*>(a) + (x * (D / 4) + d16 * 4 + v) * 128 + r);
+        const float mn = fmaxf(m, ml.x), wo = fast_exp2(m - mn), w = fast_exp2(ml.x - mn);
         m = mn;
-        const auto add = [&](float a, float b, float e) { return two ? fmaf(e, w1, fmaf(b, w0, a * wo)) : fmaf(b, w0, a * wo); };
-        l = add(l, m0.y, m1.y);
-        o.x = add(o.x, p0.x, p1.x); o.y = add(o.y, p0.y, p1.y); o.z = add(o.z, p0.z, p1.z); o.w = add(o.w, p0.w, p1.w);
+        l = fmaf(ml.y, w, l * wo);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            o[v].x = fmaf(p[v].x, w, o[v].x * wo);
+            o[v].y = fmaf(p[v].y, w, o[v].y * wo);
+            o[v].z = fmaf(p[v].z, w, o[v].z * wo);
+            o[v].w = fmaf(p[v].w, w, o[v].w * wo);
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const long row = static_cast<long>(cut.y) + node;
-    *reinterpret_cast<uint2*>(args.out + row * args.ldo + (cut.z * args.G + g) * D + d4 * 4) =
-        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    uint4* to = reinterpret_cast<uint4*>(args.out + row * args.ldo + (cut.z * args.G + g) * D + d16 * 16);
+#pragma unroll
+    for (int v = 0; v < 4; v += 2)
+        to[v / 2] = make_uint4(pack_bf16(o[v].x * inv, o[v].y * inv), pack_bf16(o[v].z * inv, o[v].w * inv),
+                               pack_bf16(o[v + 1].x * inv, o[v + 1].y * inv), pack_bf16(o[v + 1].z * inv, o[v + 1].w * inv));
 }
 
 }  // namespace mica

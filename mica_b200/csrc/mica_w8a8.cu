@@ -1169,8 +1169,8 @@ static int cache_attn_launch(const CUtensorMap& tq, const CUtensorMap& tk, const
     if (a.ctas < 2) return MICA_OK;
     // the join is launched under the attention kernel's end (it waits for all of it before it reads)
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.ctas - 1, (NT * a.npt * a.G * (D / 4) + 255) / 256);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(a.ctas - 1, (NT * a.npt * a.G * (D / 16) + 127) / 128);
+    cfg.blockDim = dim3(128);
     cfg.stream = st;
     cudaLaunchAttribute at[1] = {};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
