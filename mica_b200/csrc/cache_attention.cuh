@@ -217,9 +217,15 @@ struct CacheWalk {
         return true;
     }
     __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == nk; }
-    // a tile that holds nodes of the step, or the end of the keys
-    __device__ __forceinline__ bool special(int j) const { return (j + 1) * 128 > s.base || s.keys == 0; }
 };
+
+// What a role needs of the unit it is at: the K warp walks the run and leaves it here, four units deep.
+struct CacheUnit {
+    int b, kvh, row0, node0, nodes;     // row0: global row of its first node (node0 of its sequence)
+    int base, keys, j0, j1;
+    int flags;                          // 1: the run's last unit, 2: all of the unit's tiles, 4: the run's first unit
+};
+constexpr int CACHE_UNITS = 4;
 
 template <int D, int NT>
 struct CacheAttnShape {
@@ -228,11 +234,11 @@ struct CacheAttnShape {
     static constexpr int QBUF = NT == 1 ? 2 : 1;
     static constexpr int KST = D == 128 ? 3 : 6;
     static constexpr int VST = D == 128 ? 2 : 5;
-    static constexpr int THREADS = 96 + 128 * NT;
+    static constexpr int THREADS = 128 + 128 * NT;
     // What a unit costs beside its tiles (its rows' way out, nothing in flight), in tiles: it stands in the
     // line for that many places more.
     static constexpr int UNIT = NT == 1 ? 1 : 2;
-    static constexpr int BARS = 512;
+    static constexpr int BARS = 768;
     static constexpr int SMEM = 1024 + TILE * (QBUF * NT + KST + VST) + BARS;
 };
 
@@ -312,10 +318,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     uint64_t* p_full = s_free + 2;             // [2] P written
     uint64_t* pv_done = p_full + 2;            // [2] P.V finished
     uint64_t* v_fixed = pv_done + 2;           // V of a special tile made safe (all softmax warps)
-    uint64_t* drain = v_fixed + 1;
+    uint64_t* unit_full = v_fixed + 1;         // [CACHE_UNITS]
+    uint64_t* drain = unit_full + CACHE_UNITS;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     uint32_t* odd_v = tmem_slot + 2;           // [2][NT][4] keys of a special tile whose V row holds infinities or NaN
+    volatile CacheUnit* units = reinterpret_cast<volatile CacheUnit*>(odd_v + 16);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -329,6 +337,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         for (int i = 0; i < S::KST; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
         for (int i = 0; i < S::VST; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
         mbar_init(v_fixed, 4 * NT);
+        for (int i = 0; i < CACHE_UNITS; ++i) mbar_init(&unit_full[i], 1);
         mbar_init(drain, 1);
         *abort_flag = 0u;
         fence_mbar_init();
@@ -357,54 +366,66 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         const int my_page = lane / S::HALVES, my_half = lane % S::HALVES;
         const uint32_t box_bytes = 128u << plan.page_log2;
         const int page = 1 << plan.page_log2;
-        bool ok = true, more = true;
-        int unit = 0, t = 0, st = 0;                       // units, tiles, ring stage
+        bool ok = true, last = false;
+        int t = 0, st = 0, unit = 0;                       // tiles, ring stage, units
         uint32_t par = 1u;                                 // of the stage's `empty`
-        // pages of key tile j of the walk's unit that hold keys; this lane's page number
-        const auto pages_in = [&](int j) { return max(0, min(ppt, (wk.s.keys - j * 128 + page - 1) >> plan.page_log2)); };
-        const auto fetch = [&](int j) {
-            return lane < boxes && my_page < pages_in(j)
-                       ? plan.table[static_cast<long>(wk.b) * plan.ld_table + j * ppt + my_page] : 0;
-        };
-        int pg = fetch(wk.j0);
-        while (more && ok) {
+        for (; !last && ok; ++unit) {
+            const int slot = unit % CACHE_UNITS;
             if (is_k) {
-                if (wk.s.keys == 0 && lane == 0) record_bad_page();
-                // Q tiles of the unit
+                // A unit's place is taken again when the one two back (NT 2: one back) has all its scores: those
+                // were issued after the unit before it had its weights, so its rows, and all before, are out.
                 const int qb = S::QBUF == 2 ? unit & 1 : 0;
                 bool w = true;
                 if (lane == 0) {
                     w = mbar_wait(&q_empty[qb], static_cast<uint32_t>(unit / S::QBUF & 1) ^ 1u, abort_flag,
                                   MICA_DEV_TIMEOUT_PRODUCER);
                     if (w) {
+                        if (wk.s.keys == 0) record_bad_page();
+                        const int node0 = wk.rb * R;
                         mbar_arrive_expect_tx(&q_full[qb], NT * S::HALVES * 128u * args.npt * args.G);
                         for (int x = 0; x < NT; ++x)
                             for (int h = 0; h < S::HALVES; ++h)
                                 tma_load_3d(sq + (qb * NT + x) * S::TILE + h * ATT_HALF_BYTES, &tmap_q, &q_full[qb], h * 64,
-                                            wk.kvh * args.G, wk.s.row0 + (wk.rb * NT + x) * args.npt);
+                                            wk.kvh * args.G, wk.s.row0 + node0 + x * args.npt);
+                        volatile CacheUnit& u = units[slot];
+                        u.b = wk.b; u.kvh = wk.kvh; u.row0 = wk.s.row0 + node0; u.node0 = node0; u.nodes = min(R, wk.s.T - node0);
+                        u.base = wk.s.base; u.keys = wk.s.keys; u.j0 = wk.j0; u.j1 = wk.j1;
+                        const int all = wk.whole() ? 2 : 0;
+                        u.flags = (wk.next(plan, args.KV) ? 0 : 1) | all | (unit == 0 ? 4 : 0);
+                        mbar_arrive(&unit_full[slot]);
                     }
                 }
                 ok = __shfl_sync(0xffffffffu, w, 0);
+                __syncwarp();
+            } else {
+                ok = __all_sync(0xffffffffu, mbar_wait(&unit_full[slot], unit / CACHE_UNITS & 1, abort_flag,
+                                                       MICA_DEV_TIMEOUT_PRODUCER));
             }
-            ++unit;
-            const int end = wk.j1;
-            for (int j = wk.j0; j < end && ok; ++j, ++t) {
-                const int n = pages_in(j) * S::HALVES, kvh = wk.kvh;
+            if (!ok) break;
+            const volatile CacheUnit& u = units[slot];
+            const int b = u.b, keys = u.keys, end = u.j1, y = u.kvh << plan.page_log2;
+            last = u.flags & 1;
+            // pages of key tile j that hold keys; this lane's page number, a tile ahead of its use
+            const auto pages_in = [&](int j) { return max(0, min(ppt, (keys - j * 128 + page - 1) >> plan.page_log2)); };
+            const int* row = plan.table + static_cast<long>(b) * plan.ld_table + my_page;
+            const auto fetch = [&](int j) { return lane < boxes && my_page < pages_in(j) ? row[j * ppt] : 0; };
+            int pg = fetch(u.j0);
+            for (int j = u.j0; j < end; ++j, ++t) {
+                const int n = pages_in(j) * S::HALVES;
                 int cur = pg;
-                // the next tile's page number, a tile ahead of its use
                 if (j + 1 < end) pg = fetch(j + 1);
-                else if ((more = wk.next(plan, args.KV))) pg = fetch(wk.j0);
                 bool w = true;
                 if (lane == 0) {
                     w = mbar_wait(&empty[st], par, abort_flag, MICA_DEV_TIMEOUT_PRODUCER);
                     if (w) mbar_arrive_expect_tx(&full[st], n * box_bytes);
                 }
                 ok = __shfl_sync(0xffffffffu, w, 0);
-                if (ok && lane < n) {
+                if (!ok) break;
+                if (lane < n) {
                     // a page outside the pool is outside the map and reads as zeros
                     if (cur < 0 || cur >= plan.pages) { cur = plan.pages; record_bad_page(); }
                     tma_load_3d(ring + st * S::TILE + my_half * ATT_HALF_BYTES + my_page * box_bytes, map, &full[st], my_half * 64,
-                                kvh << plan.page_log2, cur);
+                                y, cur);
                 }
                 __syncwarp();
                 if (++st == stages) { st = 0; par ^= 1u; }
@@ -428,20 +449,22 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             const uint64_t k_desc0 = smem_desc_sw128(smem_u32(sk), 16, 1024);
             const uint64_t v_desc0 = smem_desc_sw128(smem_u32(sv), ATT_HALF_BYTES, 1024);
             constexpr uint64_t kStep = S::TILE >> 4;
-            bool ok = true;
-            int fills = 0;                       // score tiles issued (NT 2: of both row tiles)
-            // scores of row tile x with key tile t (counted over the run) of the unit's Q in buffer qb
-            const auto scores = [&](int x, int t, int qb) {
+            bool ok = true, last = false;
+            int t = 0, unit = 0;                  // tiles with scores issued, units
+            int kst = 0, vst = 0, pv = 0;         // ring stages, tiles with P.V issued
+            uint32_t kpar = 0u, vpar = 0u;
+            // scores of row tile x with the tile in kst, Q in buffer qb
+            const auto scores = [&](int x, int qb) {
                 const int i = NT == 1 ? (t & 1) : x;
                 if (NT == 1) {
                     if (t >= 2 && !mma_wait(&s_free[i], ((t >> 1) - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
                 } else {
-                    if (fills > 0 && !mma_wait(&s_free[0], (fills - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
-                    ++fills;
+                    // the one buffer's last fill: tile t - 1 of row tile 1, or t of row tile 0
+                    if (2 * t + x > 0 && !mma_wait(&s_free[0], (x ^ 1) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
                 }
                 tc_fence_after();
                 const uint64_t qd = q_desc0 + static_cast<uint64_t>(qb * NT + x) * kStep;
-                const uint64_t kd = k_desc0 + static_cast<uint64_t>(t % S::KST) * kStep;
+                const uint64_t kd = k_desc0 + static_cast<uint64_t>(kst) * kStep;
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     const uint64_t off = static_cast<uint64_t>(((kk >> 2) * ATT_HALF_BYTES + (kk & 3) * 32) >> 4);
@@ -450,12 +473,11 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 mma_commit(&s_full[i]);
                 return true;
             };
-            const auto values = [&](int x, int t, bool fresh) {
-                const int i = NT == 1 ? (t & 1) : x;
-                const uint32_t par = static_cast<uint32_t>(NT == 1 ? t >> 1 : t) & 1u;
-                if (!mma_wait(&p_full[i], par, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+            const auto values = [&](int x, bool fresh) {
+                const int i = NT == 1 ? (pv & 1) : x;
+                if (!mma_wait(&p_full[i], (NT == 1 ? pv >> 1 : pv) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
                 tc_fence_after();
-                const uint64_t vd = v_desc0 + static_cast<uint64_t>(t % S::VST) * kStep;
+                const uint64_t vd = v_desc0 + static_cast<uint64_t>(vst) * kStep;
                 const uint32_t o = tmem + col_o(x), p = tmem + col_p(i);
                 mma_bf16_ts(o, p, vd, idesc_pv, fresh ? 0u : 1u);
 #pragma unroll
@@ -463,64 +485,50 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 mma_commit(&pv_done[i]);
                 return true;
             };
-            // the scores of a tile are issued before the P.V of the tile before it, inside a unit: at its end
-            // the rows are waited for, and the next unit's Q and K may be a while coming
-            CacheWalk pv = wk;                    // the unit of the next P.V
-            bool more = true, pending = false;    // a tile's P.V is still to be issued
-            int t = 0, unit = 0, pv_t = 0;
-            int pv_j = pv.j0;
-            const auto values_all = [&](int x) {
-                // the first tile of a unit starts the accumulator, except where the softmax has set it
-                const bool fresh = pv_j == pv.j0 && !pv.special(pv_j);
-                return values(x, pv_t, fresh);
+            const auto v_ready = [&]() { return mma_wait(&v_full[vst], vpar, abort_flag, MICA_DEV_TIMEOUT_MMA); };
+            const auto v_release = [&]() {
+                mma_commit(&v_empty[vst]);
+                if (++vst == S::VST) { vst = 0; vpar ^= 1u; }
+                ++pv;
             };
-            const auto values_done = [&]() {
-                mma_commit(&v_empty[pv_t % S::VST]);
-                ++pv_t;
-                pending = false;
-                if (++pv_j == pv.j1 && pv.next(plan, args.KV)) pv_j = pv.j0;
-            };
-            const auto flush = [&]() {
-                if (!mma_wait(&v_full[pv_t % S::VST], (pv_t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
-                for (int x = 0; x < NT; ++x)
-                    if (!values_all(x)) return false;
-                values_done();
-                return true;
-            };
-            while (more && ok) {
+            // Inside a unit the scores of a tile are issued before the P.V of the tile before it. At its end the
+            // rows are waited for, and the next unit's Q and K may be a while coming.
+            for (; !last; ++unit) {
                 const int qb = S::QBUF == 2 ? unit & 1 : 0;
-                if (pending && !flush()) { ok = false; break; }
-                ok = mma_wait(&q_full[qb], unit / S::QBUF & 1, abort_flag, MICA_DEV_TIMEOUT_MMA);
-                for (int j = wk.j0; j < wk.j1 && ok; ++j, ++t) {
-                    if (!mma_wait(&k_full[t % S::KST], (t / S::KST) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA) ||
-                        !scores(0, t, qb)) { ok = false; break; }
-                    if (NT == 1) {
-                        mma_commit(&k_empty[t % S::KST]);
-                        if (j + 1 == wk.j1) mma_commit(&q_empty[qb]);
-                    }
-                    if (pending) {
-                        if (!mma_wait(&v_full[pv_t % S::VST], (pv_t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA) ||
-                            !values_all(0)) { ok = false; break; }
-                    }
+                if (!mma_wait(&unit_full[unit % CACHE_UNITS], unit / CACHE_UNITS & 1, abort_flag, MICA_DEV_TIMEOUT_MMA) ||
+                    !mma_wait(&q_full[qb], unit / S::QBUF & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) break;
+                const volatile CacheUnit& u = units[unit % CACHE_UNITS];
+                const int n = u.j1 - u.j0;
+                // the first tile starts the accumulator, except where the softmax has set it
+                bool fresh = !((u.j0 + 1) * 128 > u.base || u.keys == 0);
+                last = u.flags & 1;
+                for (int j = 0; j < n; ++j, ++t) {
+                    ok = mma_wait(&k_full[kst], kpar, abort_flag, MICA_DEV_TIMEOUT_MMA) && scores(0, qb);
+                    if (!ok) break;
+                    if (NT == 1) mma_commit(&k_empty[kst]);
+                    if (j > 0 && !(v_ready() && values(0, fresh))) { ok = false; break; }
                     if (NT == 2) {
-                        if (!scores(1, t, qb)) { ok = false; break; }
-                        mma_commit(&k_empty[t % S::KST]);
-                        if (j + 1 == wk.j1) mma_commit(&q_empty[qb]);
-                        if (pending && !values_all(1)) { ok = false; break; }
+                        if (!scores(1, qb)) { ok = false; break; }
+                        mma_commit(&k_empty[kst]);
+                        if (j > 0 && !values(1, fresh)) { ok = false; break; }
                     }
-                    if (pending) values_done();
-                    pending = true;
+                    if (++kst == S::KST) { kst = 0; kpar ^= 1u; }
+                    if (j > 0) {
+                        v_release();
+                        fresh = false;
+                    }
                 }
-                if (ok) { more = wk.next(plan, args.KV); ++unit; }
+                if (!ok) break;
+                mma_commit(&q_empty[qb]);
+                if (!v_ready() || !values(0, fresh) || (NT == 2 && !values(1, fresh))) break;
+                v_release();
             }
-            if (ok && pending) flush();
             mma_commit(drain);
             mbar_wait(drain, 0, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
         }
         __syncwarp();
-    } else {
-        // ---------------------------------- softmax ----------------------------------
-        if (threadIdx.x == 96) {
+    } else if (warp == 3) {
+        if (lane == 0) {
             // the unit this CTA starts inside, for the join: its first row, node rows, K/V head, and the CTAs
             // that hold parts of it, the one before and `n` from this one on
             const long s0 = share.at(cta) - wk.j0;                // the unit's first tile in the line
@@ -534,42 +542,48 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             args.cuts[2 * cta] = cut;
             args.cuts[2 * cta + 1] = more;
         }
-        const int x = (warp - 3) >> 2;                     // row tile of this warpgroup
+    } else {
+        // ---------------------------------- softmax ----------------------------------
+        const int x = (warp - 4) >> 2;                     // row tile of this warpgroup
         const int q4 = warp & 3;                           // tensor-memory lane quarter
         const int r = q4 * 32 + lane;                      // row of the tile
         const int node_r = r / args.G, head_r = r % args.G;
         const uint32_t lane_off = static_cast<uint32_t>(q4 * 32) << 16;
         const float c = args.scale_log2;
-        bool ok = true, more = true, first = true;
-        int t = 0;                                         // key tiles so far
+        bool ok = true, last = false;
+        int t = 0, unit = 0;                               // key tiles so far, units
         int fixes = 0;                                     // special tiles so far
-        while (more && ok) {
-            const CacheSeq& s = wk.s;
-            const int node0 = (wk.rb * NT + x) * args.npt;            // first node of the tile
-            const int nodes = max(0, min(args.npt, s.T - node0));
+        for (; !last && ok; ++unit) {
+            ok = __all_sync(0xffffffffu, mma_wait(&unit_full[unit % CACHE_UNITS], unit / CACHE_UNITS & 1, abort_flag,
+                                                  MICA_DEV_TIMEOUT_EPILOGUE));
+            if (!ok) break;
+            const volatile CacheUnit& u = units[unit % CACHE_UNITS];
+            last = u.flags & 1;
+            const int nodes = max(0, min(args.npt, u.nodes - x * args.npt));
             const bool live = node_r < nodes;                         // this thread has a row
             const bool warp_live = q4 * 32 < nodes * args.G;          // some thread of the warp has
-            const int node = node0 + node_r;
-            const long row = static_cast<long>(s.row0) + node;
+            const int j0 = u.j0, j1 = u.j1, base = u.base, keys = u.keys;
             const uint32_t t_o = tmem + col_o(x) + lane_off;
             float m_use = -1e30f, l = 0.f;
-            for (int j = wk.j0; j < wk.j1; ++j, ++t) {
+            for (int j = j0; j < j1; ++j, ++t) {
                 const int i2 = NT == 1 ? (t & 1) : x;
                 const int n2 = NT == 1 ? t >> 1 : t;                   // uses of that buffer before
                 const uint32_t t_s = tmem + col_s(i2) + lane_off, t_p = tmem + col_p(i2) + lane_off;
-                const bool special = wk.special(j);
+                const bool special = (j + 1) * 128 > base || keys == 0;
                 const int k0 = j * 128;
                 // visible keys of this row, one bit each
                 uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
                 if (special) {
-                    const int end = causal ? min(s.keys, s.base + node + 1) : s.keys;
+                    const int node = u.node0 + x * args.npt + node_r;
+                    const int end = causal ? min(keys, base + node + 1) : keys;
                     uint32_t bits[4];
-                    if (!causal && live && s.keys)
-                        mask_bits(args.mask + row * args.ld_mask, args.words, k0 - s.base, bits);
+                    if (!causal && live && keys)
+                        mask_bits(args.mask + static_cast<long>(u.row0 + x * args.npt + node_r) * args.ld_mask, args.words,
+                                  k0 - base, bits);
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         vis[w] = live ? low_bits(end - k0 - 32 * w) : 0u;
-                        if (!causal) vis[w] &= low_bits(s.base - k0 - 32 * w) | (s.keys ? bits[w] : 0u);
+                        if (!causal) vis[w] &= low_bits(base - k0 - 32 * w) | (keys ? bits[w] : 0u);
                     }
                     // V rows behind the keys become zero; odd values of the step's own rows too, noted
                     // (two sets of odd_v: all warps pass v_fixed of a special tile before one writes the next but one)
@@ -578,12 +592,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     if (!ok) break;
                     const int key = k0 + r;
                     bool odd = false;
-                    if (key >= s.base || key >= s.keys) {
+                    if (key >= base || key >= keys) {
                         // with two row tiles, half of the row's columns each
                         const int h0 = NT == 2 ? x : 0, h1 = NT == 2 ? min(x + 1, S::HALVES) : S::HALVES;
                         for (int h = h0; h < h1; ++h) {
                             uint4* vr = reinterpret_cast<uint4*>(sv + st * S::TILE + h * ATT_HALF_BYTES + r * 128);
-                            if (key >= s.keys) {
+                            if (key >= keys) {
 #pragma unroll
                                 for (int e = 0; e < 8; ++e) vr[e ^ (r & 7)] = make_uint4(0u, 0u, 0u, 0u);
                                 continue;
@@ -685,7 +699,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     any_odd = some != 0u;
                     ++fixes;
                 }
-                const bool fresh = j == wk.j0;
+                const bool fresh = j == j0;
                 const bool touch = warp_live && (special && fresh || any_odd ||
                                                  (!fresh && __any_sync(0xffffffffu, moved)));
                 if (lane == 0) {
@@ -713,9 +727,9 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                                 for (uint32_t bits = odd4[w4] | odd4[(NT - 1) * 4 + w4]; bits; bits &= bits - 1) {
                                     const int i = __ffs(bits) - 1;
                                     int pgn = 0, slot = 0;
-                                    if (!(vis[w4] >> i & 1u) || !cache_slot(plan, wk.b, k0 + w4 * 32 + i, &pgn, &slot)) continue;
+                                    if (!(vis[w4] >> i & 1u) || !cache_slot(plan, u.b, k0 + w4 * 32 + i, &pgn, &slot)) continue;
                                     const uint16_t* v = reinterpret_cast<const uint16_t*>(args.v_pages) + pgn * args.page_stride +
-                                                        ((static_cast<long>(wk.kvh) << plan.page_log2) + slot) * D + cc * 32;
+                                                        ((static_cast<long>(u.kvh) << plan.page_log2) + slot) * D + cc * 32;
 #pragma unroll
                                     for (int e = 0; e < 32; ++e) {
                                         const uint32_t u = v[e];
@@ -748,11 +762,13 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 if (!__shfl_sync(0xffffffffu, w, 0)) { ok = false; break; }
                 tc_fence_after();
                 if (warp_live) {
-                    const bool whole = wk.whole();
+                    const bool whole = u.flags & 2;
+                    const int kvh = u.kvh, place = u.flags & 4 ? 0 : 1;
+                    const long row = static_cast<long>(u.row0) + x * args.npt + node_r;
                     const float inv = l == 0.f ? 0.f : 1.f / l;
-                    float4* part = reinterpret_cast<float4*>(args.ws + (cta * 2l + (first ? 0 : 1)) * cache_attn_place_floats<D, NT>()) +
+                    float4* part = reinterpret_cast<float4*>(args.ws + (cta * 2l + place) * cache_attn_place_floats<D, NT>()) +
                                    x * (D / 4) * 128 + r;
-                    __nv_bfloat16* orow = args.out + row * args.ldo + (wk.kvh * args.G + head_r) * D;
+                    __nv_bfloat16* orow = args.out + row * args.ldo + (kvh * args.G + head_r) * D;
 #pragma unroll
                     for (int cc = 0; cc < D / 32; ++cc) {
                         uint32_t o[32];
@@ -776,15 +792,13 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                         }
                     }
                     if (live && !whole) {
-                        float2* ml = reinterpret_cast<float2*>(args.ws + (cta * 2l + (first ? 0 : 1)) * cache_attn_place_floats<D, NT>() +
+                        float2* ml = reinterpret_cast<float2*>(args.ws + (cta * 2l + place) * cache_attn_place_floats<D, NT>() +
                                                                NT * 128l * D);
                         ml[x * 128 + r] = make_float2(m_use, l);
                     }
                     tc_fence_before();
                 }
             }
-            first = false;
-            more = wk.next(plan, args.KV);
         }
     }
 
