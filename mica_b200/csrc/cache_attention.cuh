@@ -223,7 +223,8 @@ struct CacheWalk {
 struct CacheUnit {
     int b, kvh, row0, node0, nodes;     // row0: global row of its first node (node0 of its sequence)
     int base, keys, j0, j1;
-    int flags;                          // 1: the run's last unit, 2: all of the unit's tiles, 4: the run's first unit
+    int flags;                          // 1: the run's last unit, 2: all of the unit's tiles, 4: the run's first unit,
+                                        // 8: its nodes fill one row tile at most
 };
 constexpr int CACHE_UNITS = 4;
 
@@ -271,6 +272,54 @@ __device__ __forceinline__ void cache_zero_padding(const CacheAttnArgs& args, in
     for (long row = end + static_cast<long>(blockIdx.x); row < args.plan.N; row += gridDim.x)
         for (int i = threadIdx.x; i < vecs; i += blockDim.x)
             *reinterpret_cast<uint4*>(args.out + row * args.ldo + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// The keys k0 .. k0 + 127 that node `node` of unit u's sequence sees (row: its row of the step), one bit
+// each; in the tiles that hold nodes of the step or the end of the keys.
+__device__ __forceinline__ void cache_visible(const CacheAttnArgs& args, const volatile CacheUnit& u, int x, int node_r,
+                                              int k0, uint32_t (&vis)[4]) {
+    const int base = u.base, keys = u.keys, node = x * args.npt + node_r;
+    const bool live = node_r < args.npt && node < u.nodes && keys > 0;
+    const bool causal = args.mask == nullptr;
+    const int end = causal ? min(keys, base + u.node0 + node + 1) : keys;
+    uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+    if (!causal && live)
+        mask_bits(args.mask + static_cast<long>(u.row0 + node) * args.ld_mask, args.words, k0 - base, bits);
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        vis[w] = live ? low_bits(end - k0 - 32 * w) & (low_bits(base - k0 - 32 * w) | bits[w]) : 0u;
+}
+// Row r (key k0 + r) of columns 64 h0 .. of a V tile in shared memory, made safe for weights of zero: rows
+// behind the keys become zero, infinities and NaN of the step's own rows too. Returns whether there were any.
+__device__ __noinline__ bool cache_fix_v(uint8_t* tile, int r, int h0, int h1, bool behind) {
+    bool odd = false;
+    for (int h = h0; h < h1; ++h) {
+        uint4* vr = reinterpret_cast<uint4*>(tile + h * ATT_HALF_BYTES + r * 128);
+        if (behind) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) vr[e ^ (r & 7)] = make_uint4(0u, 0u, 0u, 0u);
+            continue;
+        }
+        // 0 * v is zero for finite v only
+        __nv_bfloat162 any = bf2(0u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint4 v = vr[e ^ (r & 7)];
+            any = __hfma2(bf2(v.x), bf2(0u), any);
+            any = __hfma2(bf2(v.y), bf2(0u), any);
+            any = __hfma2(bf2(v.z), bf2(0u), any);
+            any = __hfma2(bf2(v.w), bf2(0u), any);
+        }
+        if (bits2(any) & 0x7fff7fffu) {
+            odd = true;
+            uint32_t* u = reinterpret_cast<uint32_t*>(vr);
+            for (int e = 0; e < 32; ++e) {
+                if ((u[e] & 0x7f800000u) == 0x7f800000u) u[e] &= 0x0000ffffu;
+                if ((u[e] & 0x00007f80u) == 0x00007f80u) u[e] &= 0xffff0000u;
+            }
+        }
+    }
+    return odd;
 }
 
 template <int D, int NT>
@@ -391,7 +440,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                         u.b = wk.b; u.kvh = wk.kvh; u.row0 = wk.s.row0 + node0; u.node0 = node0; u.nodes = min(R, wk.s.T - node0);
                         u.base = wk.s.base; u.keys = wk.s.keys; u.j0 = wk.j0; u.j1 = wk.j1;
                         const int all = wk.whole() ? 2 : 0;
-                        u.flags = (wk.next(plan, args.KV) ? 0 : 1) | all | (unit == 0 ? 4 : 0);
+                        u.flags = (wk.next(plan, args.KV) ? 0 : 1) | all | (unit == 0 ? 4 : 0) | (u.nodes <= args.npt ? 8 : 0);
                         mbar_arrive(&unit_full[slot]);
                     }
                 }
@@ -452,6 +501,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             bool ok = true, last = false;
             int t = 0, unit = 0;                  // tiles with scores issued, units
             int kst = 0, vst = 0, pv = 0;         // ring stages, tiles with P.V issued
+            int fills = 0, pv1 = 0;               // NT 2: score tiles issued, P.V of row tile 1
             uint32_t kpar = 0u, vpar = 0u;
             // scores of row tile x with the tile in kst, Q in buffer qb
             const auto scores = [&](int x, int qb) {
@@ -459,8 +509,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 if (NT == 1) {
                     if (t >= 2 && !mma_wait(&s_free[i], ((t >> 1) - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
                 } else {
-                    // the one buffer's last fill: tile t - 1 of row tile 1, or t of row tile 0
-                    if (2 * t + x > 0 && !mma_wait(&s_free[0], (x ^ 1) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+                    if (fills > 0 && !mma_wait(&s_free[0], (fills - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+                    ++fills;
                 }
                 tc_fence_after();
                 const uint64_t qd = q_desc0 + static_cast<uint64_t>(qb * NT + x) * kStep;
@@ -475,7 +525,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             };
             const auto values = [&](int x, bool fresh) {
                 const int i = NT == 1 ? (pv & 1) : x;
-                if (!mma_wait(&p_full[i], (NT == 1 ? pv >> 1 : pv) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+                if (!mma_wait(&p_full[i], (NT == 1 ? pv >> 1 : x ? pv1 : pv) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+                if (NT == 2) pv1 += x;
                 tc_fence_after();
                 const uint64_t vd = v_desc0 + static_cast<uint64_t>(vst) * kStep;
                 const uint32_t o = tmem + col_o(x), p = tmem + col_p(i);
@@ -502,26 +553,31 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 // the first tile starts the accumulator, except where the softmax has set it
                 bool fresh = !((u.j0 + 1) * 128 > u.base || u.keys == 0);
                 last = u.flags & 1;
-                for (int j = 0; j < n; ++j, ++t) {
-                    ok = mma_wait(&k_full[kst], kpar, abort_flag, MICA_DEV_TIMEOUT_MMA) && scores(0, qb);
-                    if (!ok) break;
-                    if (NT == 1) mma_commit(&k_empty[kst]);
-                    if (j > 0 && !(v_ready() && values(0, fresh))) { ok = false; break; }
-                    if (NT == 2) {
-                        if (!scores(1, qb)) { ok = false; break; }
-                        mma_commit(&k_empty[kst]);
-                        if (j > 0 && !values(1, fresh)) { ok = false; break; }
+                const auto tiles = [&](auto two) {
+                    constexpr bool both = decltype(two)::value;
+                    for (int j = 0; j < n; ++j, ++t) {
+                        if (!mma_wait(&k_full[kst], kpar, abort_flag, MICA_DEV_TIMEOUT_MMA) || !scores(0, qb)) return false;
+                        if (!both) mma_commit(&k_empty[kst]);
+                        if (j > 0 && !(v_ready() && values(0, fresh))) return false;
+                        if (both) {
+                            if (!scores(1, qb)) return false;
+                            mma_commit(&k_empty[kst]);
+                            if (j > 0 && !values(1, fresh)) return false;
+                        }
+                        if (++kst == S::KST) { kst = 0; kpar ^= 1u; }
+                        if (j > 0) {
+                            v_release();
+                            fresh = false;
+                        }
                     }
-                    if (++kst == S::KST) { kst = 0; kpar ^= 1u; }
-                    if (j > 0) {
-                        v_release();
-                        fresh = false;
-                    }
-                }
+                    mma_commit(&q_empty[qb]);
+                    if (!v_ready() || !values(0, fresh) || (both && !values(1, fresh))) return false;
+                    v_release();
+                    return true;
+                };
+                if (NT == 2 && !(u.flags & 8)) ok = tiles(std::true_type());
+                else ok = tiles(std::false_type());
                 if (!ok) break;
-                mma_commit(&q_empty[qb]);
-                if (!v_ready() || !values(0, fresh) || (NT == 2 && !values(1, fresh))) break;
-                v_release();
             }
             mma_commit(drain);
             mbar_wait(drain, 0, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
@@ -546,12 +602,11 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         // ---------------------------------- softmax ----------------------------------
         const int x = (warp - 4) >> 2;                     // row tile of this warpgroup
         const int q4 = warp & 3;                           // tensor-memory lane quarter
-        const int r = q4 * 32 + lane;                      // row of the tile
-        const int node_r = r / args.G, head_r = r % args.G;
         const uint32_t lane_off = static_cast<uint32_t>(q4 * 32) << 16;
         const float c = args.scale_log2;
         bool ok = true, last = false;
-        int t = 0, unit = 0;                               // key tiles so far, units
+        int t = 0, unit = 0;                               // this row tile's key tiles so far, units
+        int skipped = 0;                                   // and those of units it had no rows in
         int fixes = 0;                                     // special tiles so far
         for (; !last && ok; ++unit) {
             ok = __all_sync(0xffffffffu, mma_wait(&unit_full[unit % CACHE_UNITS], unit / CACHE_UNITS & 1, abort_flag,
@@ -559,76 +614,44 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             if (!ok) break;
             const volatile CacheUnit& u = units[unit % CACHE_UNITS];
             last = u.flags & 1;
-            const int nodes = max(0, min(args.npt, u.nodes - x * args.npt));
-            const bool live = node_r < nodes;                         // this thread has a row
-            const bool warp_live = q4 * 32 < nodes * args.G;          // some thread of the warp has
-            const int j0 = u.j0, j1 = u.j1, base = u.base, keys = u.keys;
+            const bool warp_live = q4 * 32 < (u.nodes - x * args.npt) * args.G;   // some thread of the warp has a row
+            // tiles from `t_special` on hold nodes of the step, or the end of the keys
+            const int t_first = t, t_end = t + u.j1 - u.j0;
+            const int t_special = u.keys ? max(t, t + (u.base >> 7) - u.j0) : t;
+            if (NT == 2 && x == 1 && (u.flags & 8)) {                 // no rows: row tile 0 goes on alone
+                skipped += t_end - t_first;
+                fixes += max(0, t_end - t_special);
+                continue;
+            }
             const uint32_t t_o = tmem + col_o(x) + lane_off;
             float m_use = -1e30f, l = 0.f;
-            for (int j = j0; j < j1; ++j, ++t) {
+            for (; t < t_end; ++t) {
                 const int i2 = NT == 1 ? (t & 1) : x;
                 const int n2 = NT == 1 ? t >> 1 : t;                   // uses of that buffer before
                 const uint32_t t_s = tmem + col_s(i2) + lane_off, t_p = tmem + col_p(i2) + lane_off;
-                const bool special = (j + 1) * 128 > base || keys == 0;
-                const int k0 = j * 128;
-                // visible keys of this row, one bit each
-                uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                const bool special = t >= t_special;
                 if (special) {
-                    const int node = u.node0 + x * args.npt + node_r;
-                    const int end = causal ? min(keys, base + node + 1) : keys;
-                    uint32_t bits[4];
-                    if (!causal && live && keys)
-                        mask_bits(args.mask + static_cast<long>(u.row0 + x * args.npt + node_r) * args.ld_mask, args.words,
-                                  k0 - base, bits);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        vis[w] = live ? low_bits(end - k0 - 32 * w) : 0u;
-                        if (!causal) vis[w] &= low_bits(base - k0 - 32 * w) | (keys ? bits[w] : 0u);
-                    }
-                    // V rows behind the keys become zero; odd values of the step's own rows too, noted
                     // (two sets of odd_v: all warps pass v_fixed of a special tile before one writes the next but one)
-                    const int st = t % S::VST;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (t / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
+                    const int vt = t + skipped, st = vt % S::VST;     // V's ring
+                    ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (vt / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
                     if (!ok) break;
-                    const int key = k0 + r;
+                    const int r = q4 * 32 + lane, key = (u.j0 + t - t_first) * 128 + r;
+                    const bool alone = NT == 1 || (u.flags & 8);       // two row tiles take half of the columns each
                     bool odd = false;
-                    if (key >= base || key >= keys) {
-                        // with two row tiles, half of the row's columns each
-                        const int h0 = NT == 2 ? x : 0, h1 = NT == 2 ? min(x + 1, S::HALVES) : S::HALVES;
-                        for (int h = h0; h < h1; ++h) {
-                            uint4* vr = reinterpret_cast<uint4*>(sv + st * S::TILE + h * ATT_HALF_BYTES + r * 128);
-                            if (key >= keys) {
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) vr[e ^ (r & 7)] = make_uint4(0u, 0u, 0u, 0u);
-                                continue;
-                            }
-                            // 0 * v is zero for finite v only
-                            __nv_bfloat162 any = bf2(0u);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const uint4 v = vr[e ^ (r & 7)];
-                                any = __hfma2(bf2(v.x), bf2(0u), any);
-                                any = __hfma2(bf2(v.y), bf2(0u), any);
-                                any = __hfma2(bf2(v.z), bf2(0u), any);
-                                any = __hfma2(bf2(v.w), bf2(0u), any);
-                            }
-                            if (bits2(any) & 0x7fff7fffu) {
-                                odd = true;
-                                uint32_t* u = reinterpret_cast<uint32_t*>(vr);
-                                for (int e = 0; e < 32; ++e) {
-                                    if ((u[e] & 0x7f800000u) == 0x7f800000u) u[e] &= 0x0000ffffu;
-                                    if ((u[e] & 0x00007f80u) == 0x00007f80u) u[e] &= 0xffff0000u;
-                                }
-                            }
-                        }
-                    }
-                    {
-                        const uint32_t found = __ballot_sync(0xffffffffu, odd);
-                        if (lane == 0) odd_v[((fixes & 1) * NT + x) * 4 + q4] = found;
-                    }
+                    if (key >= u.base || key >= u.keys)
+                        odd = cache_fix_v(sv + st * S::TILE, r, alone ? 0 : x, alone ? S::HALVES : min(x + 1, S::HALVES),
+                                          key >= u.keys);
+                    const uint32_t found = __ballot_sync(0xffffffffu, odd);
                     fence_proxy_async_smem();
+                    if (lane == 0) {
+                        odd_v[((fixes & 1) * NT + x) * 4 + q4] = found;
+                        if (NT == 2 && alone) odd_v[((fixes & 1) * NT + 1) * 4 + q4] = 0u;
+                    }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(v_fixed);
+                    if (lane == 0) {
+                        mbar_arrive(v_fixed);
+                        if (NT == 2 && alone) mbar_arrive(v_fixed);      // for row tile 1's warp
+                    }
                 }
                 bool w = true;
                 if (lane == 0) w = mma_wait(&s_full[i2], n2 & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
@@ -647,6 +670,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s_free[NT == 1 ? i2 : 0]);
                     if (special) {
+                        uint32_t vis[4];
+                        cache_visible(args, u, x, (q4 * 32 + lane) / args.G, (u.j0 + t - t_first) * 128, vis);
 #pragma unroll
                         for (int i = 0; i < 128; ++i)
                             if (!(vis[i >> 5] >> (i & 31) & 1u)) sr[i] = 0xff800000u;
@@ -690,8 +715,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 }
                 // this P buffer is free once its last P.V is done; the accumulator once the tile before's is
                 bool any_odd = false;
-                const volatile uint32_t* odd4 = odd_v + (fixes & 1) * 4 * NT;
                 if (special) {
+                    const volatile uint32_t* odd4 = odd_v + (fixes & 1) * 4 * NT;
                     ok = __all_sync(0xffffffffu, mbar_wait(v_fixed, fixes & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
                     if (!ok) break;
                     uint32_t some = 0u;
@@ -699,7 +724,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     any_odd = some != 0u;
                     ++fixes;
                 }
-                const bool fresh = j == j0;
+                const bool fresh = t == t_first;
                 const bool touch = warp_live && (special && fresh || any_odd ||
                                                  (!fresh && __any_sync(0xffffffffu, moved)));
                 if (lane == 0) {
@@ -723,20 +748,26 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
                         }
                         if (any_odd) {
-                            for (int w4 = 0; w4 < 4; ++w4)
-                                for (uint32_t bits = odd4[w4] | odd4[(NT - 1) * 4 + w4]; bits; bits &= bits - 1) {
-                                    const int i = __ffs(bits) - 1;
-                                    int pgn = 0, slot = 0;
-                                    if (!(vis[w4] >> i & 1u) || !cache_slot(plan, u.b, k0 + w4 * 32 + i, &pgn, &slot)) continue;
-                                    const uint16_t* v = reinterpret_cast<const uint16_t*>(args.v_pages) + pgn * args.page_stride +
-                                                        ((static_cast<long>(u.kvh) << plan.page_log2) + slot) * D + cc * 32;
+                            const volatile uint32_t* odd4 = odd_v + (~fixes & 1) * 4 * NT;      // counted already
+                            const int k0 = (u.j0 + t - t_first) * 128;
+                            uint32_t vis[4];
+                            cache_visible(args, u, x, (q4 * 32 + lane) / args.G, k0, vis);
+#pragma unroll 1
+                            for (int i = 0; i < 128; ++i) {
+                                const uint32_t bit = 1u << (i & 31);
+                                const uint32_t seen = i < 64 ? (i < 32 ? vis[0] : vis[1]) : (i < 96 ? vis[2] : vis[3]);
+                                int pgn = 0, slot = 0;
+                                if (!((odd4[i >> 5] | odd4[(NT - 1) * 4 + (i >> 5)]) & bit) || !(seen & bit) ||
+                                    !cache_slot(plan, u.b, k0 + i, &pgn, &slot)) continue;
+                                const uint16_t* v = reinterpret_cast<const uint16_t*>(args.v_pages) + pgn * args.page_stride +
+                                                    ((static_cast<long>(u.kvh) << plan.page_log2) + slot) * D + cc * 32;
 #pragma unroll
-                                    for (int e = 0; e < 32; ++e) {
-                                        const uint32_t u = v[e];
-                                        if ((u & 0x7f80u) == 0x7f80u)
-                                            o[e] = __float_as_uint(__uint_as_float(o[e]) + __uint_as_float(u << 16));
-                                    }
+                                for (int e = 0; e < 32; ++e) {
+                                    const uint32_t bits = v[e];
+                                    if ((bits & 0x7f80u) == 0x7f80u)
+                                        o[e] = __float_as_uint(__uint_as_float(o[e]) + __uint_as_float(bits << 16));
                                 }
+                            }
                         }
                         __syncwarp();
                         tmem_st_32x32b_x32(t_o + cc * 32, o);
@@ -764,6 +795,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 if (warp_live) {
                     const bool whole = u.flags & 2;
                     const int kvh = u.kvh, place = u.flags & 4 ? 0 : 1;
+                    const int r = q4 * 32 + lane, node_r = r / args.G, head_r = r - node_r * args.G;   // row of the tile
+                    const bool live = node_r < min(args.npt, u.nodes - x * args.npt);                // it is one
                     const long row = static_cast<long>(u.row0) + x * args.npt + node_r;
                     const float inv = l == 0.f ? 0.f : 1.f / l;
                     float4* part = reinterpret_cast<float4*>(args.ws + (cta * 2l + place) * cache_attn_place_floats<D, NT>()) +
