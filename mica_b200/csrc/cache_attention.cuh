@@ -845,11 +845,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 }
 
 // Adds up the parts of each divided unit, in the order of the CTAs. Block (c, y): the unit that CTA
-// c + 1 is the first to start inside, if it is; a thread takes 16 columns of a row, four vectors of
-// each part in flight.
+// c + 1 is the first to start inside, if it is; a thread takes 16 columns of a row, three parts in
+// flight (a long sequence's unit is in ten and more).
 template <int D, int NT>
 __global__ void __launch_bounds__(128) cache_attention_join(const CacheAttnArgs args) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int AHEAD = 3;
     const int c = blockIdx.x + 1;
     const int4 cut = args.cuts[2 * c];
     const int rows = cut.x, n = cut.w;
@@ -866,21 +867,31 @@ __global__ void __launch_bounds__(128) cache_attention_join(const CacheAttnArgs 
     float4 o[4];
 #pragma unroll
     for (int v = 0; v < 4; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i <= n; ++i) {
-        const float* a = i == 0 ? part0 : parts + (i - 1) * 2l * pf;
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(a + NT * 128l * D) + x * 128 + r);
-        float4 p[4];
+    for (int i0 = 0; i0 <= n; i0 += AHEAD) {
+        float2 ml[AHEAD];
+        float4 p[AHEAD][4];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) p[v] = __ldcg(reinterpret_cast<const float4*>(a) + (x * (D / 4) + d16 * 4 + v) * 128 + r);
-        const float mn = fmaxf(m, ml.x), wo = fast_exp2(m - mn), w = fast_exp2(ml.x - mn);
-        m = mn;
-        l = fmaf(ml.y, w, l * wo);
+        for (int u = 0; u < AHEAD; ++u) {
+            const int i = i0 + u;
+            if (i > n) continue;
+            const float* a = i == 0 ? part0 : parts + (i - 1) * 2l * pf;
+            ml[u] = __ldcg(reinterpret_cast<const float2*>(a + NT * 128l * D) + x * 128 + r);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            o[v].x = fmaf(p[v].x, w, o[v].x * wo);
-            o[v].y = fmaf(p[v].y, w, o[v].y * wo);
-            o[v].z = fmaf(p[v].z, w, o[v].z * wo);
-            o[v].w = fmaf(p[v].w, w, o[v].w * wo);
+            for (int v = 0; v < 4; ++v) p[u][v] = __ldcg(reinterpret_cast<const float4*>(a) + (x * (D / 4) + d16 * 4 + v) * 128 + r);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (i0 + u > n) continue;
+            const float mn = fmaxf(m, ml[u].x), wo = fast_exp2(m - mn), w = fast_exp2(ml[u].x - mn);
+            m = mn;
+            l = fmaf(ml[u].y, w, l * wo);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                o[v].x = fmaf(p[u][v].x, w, o[v].x * wo);
+                o[v].y = fmaf(p[u][v].y, w, o[v].y * wo);
+                o[v].z = fmaf(p[u][v].z, w, o[v].z * wo);
+                o[v].w = fmaf(p[u][v].w, w, o[v].w * wo);
+            }
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;

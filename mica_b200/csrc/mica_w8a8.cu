@@ -1228,6 +1228,7 @@ int mica_cache_copy(void* pool, long page_stride, long page_bytes, int pages, co
     if (!pool || n < 0 || (n > 0 && (!src || !dst))) return MICA_ERR_ARG;
     if (pages < 1 || page_bytes < 16 || page_stride < page_bytes) return MICA_ERR_SHAPE;
     if (!aligned16(pool) || page_bytes % 16 || page_stride % 16) return MICA_ERR_ALIGN;
+    if (page_bytes > (1L << 44)) return MICA_ERR_RANGE;
     if (n > 0) {
         // one bit per page: the pages that are written
         const size_t bytes = (static_cast<size_t>(pages) + 7) / 8;
@@ -1250,7 +1251,7 @@ int mica_cache_copy(void* pool, long page_stride, long page_bytes, int pages, co
         const int m = std::min(n - i, COPY_PAIRS);
         memcpy(a.src, src + i, m * sizeof(int));
         memcpy(a.dst, dst + i, m * sizeof(int));
-        const long blocks = std::min((page_bytes / 16 + 255) / 256, 2048L);
+        const long blocks = (page_bytes / 16 + 256 * COPY_AHEAD - 1) / (256 * COPY_AHEAD);
         cache_copy_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(m)), 256, 0,
                             static_cast<cudaStream_t>(stream)>>>(a);
         if ((rc = launch_status())) return rc;
@@ -1271,11 +1272,15 @@ int mica_cache_keep(void* pool, long page_stride, int slabs, int pages, int page
     if (!aligned16(pool) || page_stride % 16 || !aligned_to(table, 4) || !aligned_to(base, 4) || !aligned_to(cu, 4) ||
         !aligned_to(keep, 4) || !aligned_to(n_keep, 4) || !aligned_to(new_base, 4))
         return MICA_ERR_ALIGN;
-    if ((rc = check_device(nullptr))) return rc;
+    int sms = 0;
+    if ((rc = check_device(&sms))) return rc;
     if (B == 0) return MICA_OK;
     a.pool = static_cast<char*>(pool); a.page_stride = page_stride; a.keep = keep; a.ld_keep = ld_keep;
-    a.n_keep = n_keep; a.A = A; a.new_base = new_base; a.heads = slabs; a.row_bytes = D * 2;
-    cache_keep_kernel<<<dim3(static_cast<unsigned>(slabs), static_cast<unsigned>(B)), 256, 0,
+    a.n_keep = n_keep; a.A = A; a.new_base = new_base; a.slabs = slabs; a.row_bytes = D * 2;
+    // about eight blocks an SM, each with whole batches of slabs
+    const long want = static_cast<long>(slabs) * B / (8L * sms);
+    a.per_block = static_cast<int>(std::max<long>(1, std::min<long>((want + KEEP_AHEAD - 1) / KEEP_AHEAD, (slabs + KEEP_AHEAD - 1) / KEEP_AHEAD))) * KEEP_AHEAD;
+    cache_keep_kernel<<<dim3(static_cast<unsigned>((slabs + a.per_block - 1) / a.per_block), static_cast<unsigned>(B)), 256, 0,
                         static_cast<cudaStream_t>(stream)>>>(a);
     return launch_status();
 }
