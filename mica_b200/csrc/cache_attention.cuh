@@ -630,8 +630,14 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 const int n2 = NT == 1 ? t >> 1 : t;                   // uses of that buffer before
                 const uint32_t t_s = tmem + col_s(i2) + lane_off, t_p = tmem + col_p(i2) + lane_off;
                 const bool special = t >= t_special;
+                bool w = true;
+                if (lane == 0) w = mma_wait(&s_full[i2], n2 & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
+                if (!__shfl_sync(0xffffffffu, w, 0)) { ok = false; break; }
+                tc_fence_after();
                 if (special) {
-                    // (two sets of odd_v: all warps pass v_fixed of a special tile before one writes the next but one)
+                    // Only now, with the tile's scores: they were issued after the P.V of the tile two before, so the
+                    // ring stage's last turn is over and its barrier's parity says whether this one's is. (Two sets
+                    // of odd_v: all warps pass v_fixed of a special tile before one writes the next but one.)
                     const int vt = t + skipped, st = vt % S::VST;     // V's ring
                     ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (vt / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
                     if (!ok) break;
@@ -653,10 +659,6 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                         if (NT == 2 && alone) mbar_arrive(v_fixed);      // for row tile 1's warp
                     }
                 }
-                bool w = true;
-                if (lane == 0) w = mma_wait(&s_full[i2], n2 & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
-                if (!__shfl_sync(0xffffffffu, w, 0)) { ok = false; break; }
-                tc_fence_after();
                 bool moved = false;                                  // the running maximum of a row
                 float alpha = 1.f;
                 uint32_t pk[64];

@@ -93,6 +93,29 @@ def test_attention_no_rows_and_no_sequences():
     assert float(o.float().abs().max()) == 0.0
 
 
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('ctx,new', [([70761, 30001], [13, 15]), ([40000], [60]), ([5000, 9000, 130], [33, 64, 40])])
+def test_attention_adds_up_every_key_once(dim, ctx, new):
+    """V says where its key stands: one column for each place of 16 keys in the tile (of the first 8 columns),
+    one for each tile modulo the rest. Scores near zero make all weights alike, so a column is the share of its
+    keys, off by the roundings of the weights (u each, at most) and of the output: a tile lost, read twice or
+    changed under way, in one step of 16 keys even, is a change of a 60th of its column's own share or more."""
+    c = Case(ctx, new, 8, 2, dim, 64, seed=dim, mask=tree)
+    for b in range(len(ctx)):
+        kk, vv = c.keys[b]
+        s = torch.arange(vv.shape[1], device='cuda')
+        vv.zero_()
+        vv[:, s, s % 128 // 16] = 1
+        vv[:, s, 8 + s // 128 % (dim - 8)] = 1
+        for i in range(0, vv.shape[1], 64):
+            m = min(64, vv.shape[1] - i)
+            c.v[c.rows[b][i // 64], :, :m] = vv[:, i:i + m]
+    ref = c.attention(1e-3)
+    for _ in range(20):
+        o = run_attention(c, scale=1e-3).double()
+        assert ((o - ref).abs() <= 2.2 * U * ref + 1e-9).all(), float(((o - ref).abs() / (ref + 1e-9)).max())
+
+
 @pytest.mark.parametrize('bad', [float('nan'), float('inf'), float('-inf')])
 @pytest.mark.parametrize('new', [20, 90])
 def test_attention_odd_values_in_masked_nodes(bad, new):
