@@ -152,20 +152,27 @@ def check(name, rc):
     return rc
 
 
-_ENTRIES = {}
+_CALLS = None
 
 
-def entry(name):
-    """Entry point `name` itself (kept after the first look-up): the caller checks its status."""
-    f = _ENTRIES.get(name)
-    if f is None:
-        f = _ENTRIES[name] = getattr(lib(), name)
-    return f
-
-
-def int_array(values):
-    """A host int32 array for the entry points that take one."""
-    return (ctypes.c_int * len(values))(*values)
+def calls():
+    """The compiled calls (csrc/calls.cpp) on the loaded library; raises OSError when they are not built."""
+    global _CALLS
+    if _CALLS is None:
+        handle = lib()
+        import torch  # noqa: F401  (its libraries first)
+        try:
+            from . import _calls
+        except ImportError as e:
+            raise OSError(f'{Path(__file__).resolve().parent / "_calls.so"}: {e} (build it with '
+                          '`python -c "import mica_b200.build as b; b.build()"`)') from None
+        from .int8_kernels import _supported
+        with _LOCK:
+            if _CALLS is None:
+                at = {name: ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in SIGNATURES}
+                _calls.bind(at, check, lambda i: _supported(torch.device('cuda', i)))
+                _CALLS = _calls
+    return _CALLS
 
 
 def call(name, *args):

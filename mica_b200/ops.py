@@ -22,8 +22,6 @@ shapes without running anything.
     torch.ops.mica.cache_copy(pool, src, dst)                           (in place)
     torch.ops.mica.cache_keep(pool, table, base, cu, keep, n_keep)      -> new base  (in place)
     torch.ops.mica.token_logprobs(logits, ids, top)                     -> (logprob, entropy, top_lp, top_id)
-The cache and log-probability ops take arguments that mica_b200.paged and mica_b200.logprobs have
-checked; call those.
 """
 from __future__ import annotations
 
@@ -289,109 +287,14 @@ def _(qkv, batch, length, heads, kv_heads, scale):
 
 
 # ---------------------------------------------------------------------------------------
-# Paged cache and token log probabilities. A step of a few tokens takes the device less time than
-# the custom-op dispatcher takes the host (about 20 us a call), so mica_b200.paged and
-# mica_b200.logprobs call the `_do` functions directly and the registered ops wrap them.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_get_device = torch._C._cuda_getDevice
-
-
-def _launch(t, entry, *args):
-    """As `with _on(t): N.call(entry, *args, _stream(t))`, without the objects those make: the entry point's
-    checks of the current device, and its launch, on t's device and that device's current stream."""
-    idx = t.get_device()
-    prev = _get_device()
-    if prev == idx:
-        rc = N.entry(entry)(*args, _raw_stream(idx))
-    else:
-        with _on(t):
-            rc = N.entry(entry)(*args, _raw_stream(idx))
-    if rc:
-        N.check(entry, rc)
-
-
-def cache_append_do(qkv, q_w, k_w, cos, sin, k_pages, v_pages, table, base, cu, heads, pos, eps):
-    pages, kv, page, d = k_pages.shape
-    n = qkv.shape[0]
-    if n == 0 or base.shape[0] == 0:                  # nothing to do, or padding rows alone
-        return torch.zeros((n, heads * d), dtype=torch.bfloat16, device=qkv.device)
-    q = torch.empty((n, heads * d), dtype=torch.bfloat16, device=qkv.device)
-    _launch(qkv, 'mica_cache_append', qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.shape[1], q_w.data_ptr(),
-            k_w.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], _ptr(pos), q.data_ptr(), heads * d,
-            k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), pages, page, table.data_ptr(), table.stride(0),
-            table.shape[1], base.data_ptr(), cu.data_ptr(), base.shape[0], n, heads, kv, d, eps)
-    return q
-
-
-def _cache_ws(idx, n, max_new, heads, kv, d):
-    """Workspace bytes of mica_cache_attention on device idx: they depend on the row tile alone."""
-    key = (idx, min(max_new * (heads // kv), 129), d)
-    need = _CACHE_WS.get(key)
-    if need is None:
-        with torch.cuda.device(idx):
-            need = _CACHE_WS[key] = N.lib().mica_cache_attention_workspace_bytes(n, max_new, heads, kv, d)
-    return need
-
-
-_CACHE_WS = {}
-
-
-def cache_attention_do(q, k_pages, v_pages, table, base, cu, mask, heads, scale, max_new):
-    pages, kv, page, d = k_pages.shape
-    n = q.shape[0]
-    if n == 0 or base.shape[0] == 0:
-        return torch.zeros((n, heads * d), dtype=torch.bfloat16, device=q.device)
-    out = torch.empty((n, heads * d), dtype=torch.bfloat16, device=q.device)
-    need = _cache_ws(q.get_device(), n, max_new, heads, kv, d)
-    ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
-    words = 0 if mask is None else mask.shape[1]
-    _launch(q, 'mica_cache_attention', q.data_ptr(), q.stride(0) if n > 1 else heads * d, k_pages.data_ptr(),
-            v_pages.data_ptr(), k_pages.stride(0), pages, page, table.data_ptr(), table.stride(0), table.shape[1],
-            base.data_ptr(), cu.data_ptr(), _ptr(mask), words, words, base.shape[0], n, max_new, heads, kv, d, scale,
-            out.data_ptr(), heads * d, ws.data_ptr(), need)
-    return out
-
-
-def cache_copy_do(pool, src, dst):
-    a, b = N.int_array(src), N.int_array(dst)
-    _launch(pool, 'mica_cache_copy', pool.data_ptr(), pool.stride(0) * pool.element_size(),
-            pool.numel() // pool.shape[0] * pool.element_size(), pool.shape[0], a, b, len(src))
-
-
-def cache_keep_do(pool, table, base, cu, keep, n_keep):
-    pages, layers, two, kv, page, d = pool.shape
-    new_base = torch.empty_like(base)
-    most = keep.shape[1]
-    _launch(pool, 'mica_cache_keep', pool.data_ptr(), pool.stride(0) * 2, layers * two * kv, pages, page, d,
-            table.data_ptr(), table.stride(0), table.shape[1], base.data_ptr(), cu.data_ptr(), base.shape[0],
-            keep.data_ptr(), most, n_keep.data_ptr(), most, new_base.data_ptr())
-    return new_base
-
-
-def token_logprobs_do(logits, ids, top):
-    n, v = logits.shape
-    m = ids.shape[1]
-    dev = logits.device
-    lp = torch.empty((n, m), dtype=torch.float32, device=dev)
-    ent = torch.empty((n,), dtype=torch.float32, device=dev)
-    top_lp = torch.empty((n, top), dtype=torch.float32, device=dev)
-    top_id = torch.empty((n, top), dtype=torch.int64, device=dev)
-    if n == 0:
-        return lp, ent, top_lp, top_id
-    code = DTYPE_CODE[logits.dtype]
-    ld = logits.stride(0) if n > 1 else v              # a single row's stride may be anything
-    ld_ids = ids.stride(0) if n > 1 else m
-    _launch(logits, 'mica_token_logprobs', logits.data_ptr(), code, ld, n, v, ids.data_ptr() if m else None, ld_ids, m,
-            top, lp.data_ptr() if m else None, ent.data_ptr(), top_lp.data_ptr() if top else None,
-            top_id.data_ptr() if top else None)
-    return lp, ent, top_lp, top_id
-
-
+# Paged cache and token log probabilities: the compiled calls (csrc/calls.cpp) check, allocate and
+# launch. mica_b200.paged and mica_b200.logprobs call those directly (a step of a few tokens takes the
+# device less time than this dispatcher takes the host, about 20 us a call); these are for graph tooling.
 @torch.library.custom_op('mica::cache_append', mutates_args=('k_pages', 'v_pages'))
 def cache_append(qkv: torch.Tensor, q_w: torch.Tensor, k_w: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                  k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, base: torch.Tensor,
                  cu: torch.Tensor, heads: int, pos: Optional[torch.Tensor], eps: float) -> torch.Tensor:
-    return cache_append_do(qkv, q_w, k_w, cos, sin, k_pages, v_pages, table, base, cu, heads, pos, eps)
+    return N.calls().append(qkv, q_w, k_w, cos, sin, k_pages, v_pages, table, base, cu, heads, pos, eps)
 
 
 @cache_append.register_fake
@@ -401,9 +304,9 @@ def _(qkv, q_w, k_w, cos, sin, k_pages, v_pages, table, base, cu, heads, pos, ep
 
 @torch.library.custom_op('mica::cache_attention', mutates_args=())
 def cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
-                    base: torch.Tensor, cu: torch.Tensor, mask: Optional[torch.Tensor], heads: int, scale: float,
-                    max_new: int) -> torch.Tensor:
-    return cache_attention_do(q, k_pages, v_pages, table, base, cu, mask, heads, scale, max_new)
+                    base: torch.Tensor, cu: torch.Tensor, mask: Optional[torch.Tensor], heads: int,
+                    scale: Optional[float], max_new: Optional[int]) -> torch.Tensor:
+    return N.calls().attention(q, k_pages, v_pages, table, base, cu, mask, heads, scale, max_new)
 
 
 @cache_attention.register_fake
@@ -413,7 +316,7 @@ def _(q, k_pages, v_pages, table, base, cu, mask, heads, scale, max_new):
 
 @torch.library.custom_op('mica::cache_copy', mutates_args=('pool',))
 def cache_copy(pool: torch.Tensor, src: list[int], dst: list[int]) -> None:
-    cache_copy_do(pool, src, dst)
+    N.calls().copy_pages(pool, src, dst)
 
 
 @cache_copy.register_fake
@@ -424,7 +327,7 @@ def _(pool, src, dst):
 @torch.library.custom_op('mica::cache_keep', mutates_args=('pool',))
 def cache_keep(pool: torch.Tensor, table: torch.Tensor, base: torch.Tensor, cu: torch.Tensor, keep: torch.Tensor,
                n_keep: torch.Tensor) -> torch.Tensor:
-    return cache_keep_do(pool, table, base, cu, keep, n_keep)
+    return N.calls().keep_tokens(pool, table, base, cu, keep, n_keep)
 
 
 @cache_keep.register_fake
@@ -435,12 +338,12 @@ def _(pool, table, base, cu, keep, n_keep):
 @torch.library.custom_op('mica::token_logprobs', mutates_args=())
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int
                    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return token_logprobs_do(logits, ids, top)
+    return N.calls().token_logprobs(logits, ids, top)
 
 
 @token_logprobs.register_fake
 def _(logits, ids, top):
     n = logits.shape[0]
     f32 = {'dtype': torch.float32}
-    return (logits.new_empty((n, ids.shape[1]), **f32), logits.new_empty((n,), **f32),
+    return (logits.new_empty(ids.shape, **f32), logits.new_empty((n,), **f32),
             logits.new_empty((n, top), **f32), logits.new_empty((n, top), dtype=torch.int64))

@@ -25,31 +25,11 @@ from typing import Optional, Sequence
 
 import torch
 
-from . import ops
-from .int8_kernels import _CAPS, _launched, _supported
+from . import _native as N
+from . import ops  # noqa: F401  (registers torch.ops.mica.*)
+from .int8_kernels import _launched
 
 PAGES = (16, 32, 64, 128)      # tokens a page may hold
-
-
-def _served(dev):
-    c = _CAPS.get(dev.index)            # what _supported found the first time
-    return bool(c.supported) if c is not None else _supported(dev)
-
-
-def _cuda(name, *ts):
-    dev = ts[0].device
-    if dev.type != 'cuda':
-        raise RuntimeError(f'{name}: CUDA tensors only (this library has no CPU path)')
-    for t in ts[1:]:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f'{name}: tensors on {dev} and {t.device}')
-    if not _served(dev):
-        raise RuntimeError(f'{name}: {dev} is not a B200 (sm_100)')
-
-
-def _no_grad(name, *ts):
-    if torch.is_grad_enabled() and True in [t.requires_grad for t in ts]:
-        raise RuntimeError(f'{name}: no backward pass (call it under torch.no_grad())')
 
 
 class Step:
@@ -88,45 +68,12 @@ class Step:
         self.table, self.base, self.cu, self.mask, self.max_new = table, base, cu, mask, max_new
 
 
-def _pages_ok(name, k, v):
-    if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride():
-        raise ValueError(f'{name}: K pages {tuple(k.shape)} and V pages {tuple(v.shape)}')
-    pages, kv, page, d = k.shape
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
-        raise RuntimeError(f'{name}: pages of {k.dtype} are not served (bf16)')
-    if page not in PAGES or d not in (64, 128) or k.stride()[1:] != (page * d, d, 1) or kv < 1 or pages < 1 or (
-            k.stride(0) < kv * page * d):
-        raise ValueError(f'{name}: pages {tuple(k.shape)} with strides {k.stride()} (a page is [KV, page, D] '
-                         f'contiguous, page in {PAGES}, D 64 or 128)')
-    return kv, d
-
-
 def append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, step: Step, heads: int, pos=None, eps: float = 1e-6):
     """Per-head RMSNorm of q and k, rotation by `pos` (int64 [N]; None: the cache index) and the write of K
     and V into the step's slots, in one pass over the QKV projection's output [N, (H + 2 KV) D] (q | k | v,
     unit column stride). Returns q [N, H D]; qkv is not changed. fp32, rounded to bf16 once
     (ops.qk_norm_rope keeps HF's rounding of every step). cos, sin bf16 [positions, D]."""
-    kv, d = _pages_ok('append', k_pages, v_pages)
-    n = qkv.shape[0]
-    if qkv.dim() != 2 or heads < 1 or qkv.shape[1] != (heads + 2 * kv) * d or qkv.stride(1) != 1:
-        raise ValueError(f'append: qkv {tuple(qkv.shape)} for {heads} + 2 x {kv} heads of {d}')
-    if q_norm.shape != (d,) or k_norm.shape != (d,) or cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != d:
-        raise ValueError(f'append: norms {tuple(q_norm.shape)}, {tuple(k_norm.shape)}, tables {tuple(cos.shape)}, '
-                         f'{tuple(sin.shape)} for heads of {d}')
-    if not (qkv.dtype == q_norm.dtype == k_norm.dtype == cos.dtype == sin.dtype == torch.bfloat16):
-        raise RuntimeError('append: bf16 tensors only')
-    if pos is not None and (pos.dtype != torch.int64 or pos.shape != (n,)):
-        raise ValueError(f'append: pos is int64 [{n}], not {pos.dtype} {tuple(pos.shape)}')
-    if not cos.is_contiguous() or not sin.is_contiguous() or cos.shape[0] < 1:
-        raise ValueError('append: cos and sin are contiguous [positions, D]')
-    _cuda('append', qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, step.table, step.base, step.cu, pos)
-    _no_grad('append', qkv, q_norm, k_norm)
-    if n > 1 and (qkv.stride(0) < qkv.shape[1] or qkv.stride(0) % 8) or qkv.data_ptr() % 16:
-        qkv = qkv.clone(memory_format=torch.contiguous_format)
-    if pos is not None and not pos.is_contiguous():
-        pos = pos.contiguous()
-    q = ops.cache_append_do(qkv, q_norm.contiguous(), k_norm.contiguous(), cos, sin, k_pages, v_pages, step.table,
-                            step.base, step.cu, heads, pos, float(eps))
+    q = N.calls().append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, step.table, step.base, step.cu, heads, pos, eps)
     _launched()
     return q
 
@@ -135,50 +82,16 @@ def attention(q, k_pages, v_pages, step: Step, heads: int, scale: Optional[float
     """Grouped-query attention of the step's rows (appended before) over the cache: q [N, H D] (unit column
     stride, any row stride) -> [N, H D] bf16. Every row sees its sequence's committed tokens and, of its own
     step, what step.mask says. A row that sees nothing, and a padding row, is zero."""
-    kv, d = _pages_ok('attention', k_pages, v_pages)
-    n = q.shape[0]
-    if q.dim() != 2 or heads < 1 or heads % kv or heads // kv > 128 or q.shape[1] != heads * d or q.stride(1) != 1:
-        raise ValueError(f'attention: q {tuple(q.shape)} for {heads} heads of {d} over {kv} K/V heads')
-    if q.dtype != torch.bfloat16:
-        raise RuntimeError(f'attention: {q.dtype} is not served (bf16)')
-    mask = step.mask
-    if mask is not None and mask.shape[0] != n:
-        raise ValueError(f'attention: mask of {mask.shape[0]} rows for {n}')
-    scale = d ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float('inf'):
-        raise ValueError(f'attention: scale {scale}')
-    _cuda('attention', q, k_pages, v_pages, step.table, step.base, step.cu, mask)
-    _no_grad('attention', q, k_pages, v_pages)
-    if n > 1 and (q.stride(0) < q.shape[1] or q.stride(0) % 8) or q.data_ptr() % 16:
-        q = q.clone(memory_format=torch.contiguous_format)
-    out = ops.cache_attention_do(q, k_pages, v_pages, step.table, step.base, step.cu, mask, heads, scale,
-                                 n if step.max_new is None else min(step.max_new, n))
-    _launched()
+    out = N.calls().attention(q, k_pages, v_pages, step.table, step.base, step.cu, step.mask, heads, scale, step.max_new)
+    _launched(2)
     return out
-
-
-def _pool_ok(name, pool):
-    if pool.dim() < 2 or pool.shape[0] < 1 or not pool[0].is_contiguous() or pool.stride(0) < pool[0].numel() or (
-            pool.data_ptr() % 16 or pool.stride(0) * pool.element_size() % 16
-            or pool[0].numel() * pool.element_size() % 16 or pool[0].numel() == 0):
-        raise ValueError(f'{name}: pool {tuple(pool.shape)} with strides {pool.stride()} (each page contiguous, whole '
-                         '16-byte pieces)')
 
 
 def copy_pages(pool, src: Sequence[int], dst: Sequence[int]) -> None:
     """pool[dst[i]] = pool[src[i]] for lists of page numbers, every layer of a page at once. No page may be
     written twice, or be both read and written. A captured graph keeps the lists."""
-    _pool_ok('copy_pages', pool)
-    if len(src) != len(dst):
-        raise ValueError(f'copy_pages: {len(src)} pages onto {len(dst)}')
-    both = set(dst)
-    if len(both) != len(dst) or not both.isdisjoint(src):
-        raise ValueError('copy_pages: a page is written twice, or read and written')
-    if len(src) and not (0 <= min(src) and max(src) < pool.shape[0] and 0 <= min(dst) and max(dst) < pool.shape[0]):
-        raise ValueError(f'copy_pages: a page outside the pool of {pool.shape[0]}')
-    _cuda('copy_pages', pool)
+    N.calls().copy_pages(pool, src, dst)
     if len(src):
-        ops.cache_copy_do(pool, src, dst)
         _launched()
 
 
@@ -186,18 +99,7 @@ def keep_tokens(pool, step: Step, keep, n_keep):
     """Of the step's rows, sequence b keeps keep[b, :n_keep[b]] (int32 [B, A], increasing; int32 [B]): their K
     and V move to the slots behind its committed tokens, in all layers of the pool [pages, layers, 2, KV, page,
     D]. Returns the new base int32 [B]. A sequence whose list is out of order or range is left as it was."""
-    if pool.dim() != 6 or pool.shape[2] != 2 or pool.dtype != torch.bfloat16 or pool.shape[4] not in PAGES or (
-            pool.shape[5] not in (64, 128)):
-        raise ValueError(f'keep_tokens: pool {pool.dtype} {tuple(pool.shape)}')
-    _pool_ok('keep_tokens', pool)
-    b = step.base.shape[0]
-    if keep.dim() != 2 or keep.shape[0] != b or n_keep.shape != (b,) or not keep.dtype == n_keep.dtype == torch.int32:
-        raise ValueError(f'keep_tokens: keep {keep.dtype} {tuple(keep.shape)}, n_keep {n_keep.dtype} '
-                         f'{tuple(n_keep.shape)} for {b} sequences')
-    _cuda('keep_tokens', pool, step.table, step.base, step.cu, keep, n_keep)
-    if b == 0 or keep.shape[1] == 0:
-        return step.base.clone()
-    new_base = ops.cache_keep_do(pool, step.table, step.base, step.cu, keep.contiguous(), n_keep.contiguous())
+    new_base = N.calls().keep_tokens(pool, step.table, step.base, step.cu, keep, n_keep)
     _launched()
     return new_base
 

@@ -467,3 +467,49 @@ def test_a_tree_step_then_keep_equals_the_kept_tokens_appended_alone():
     _, na = go(a, rows[107:])
     _, nb = go(b, rows[107:])
     assert torch.equal(na, nb)
+
+
+def test_registered_ops_are_the_same_calls():
+    from mica_b200 import logprobs
+    c = Case([100, 7], [5, 9], 8, 2, 128, 32, seed=1, mask=tree)
+    o = torch.ops.mica.cache_attention(c.q, c.k, c.v, c.table, c.base, c.cu, c.mask, 8, None, None)
+    assert torch.equal(o, run_attention(c))
+    z, ids = torch.randn(4, 999, device='cuda'), torch.zeros(4, 2, dtype=torch.int64, device='cuda')
+    for a, b in zip(torch.ops.mica.token_logprobs(z, ids, 3), logprobs.token_logprobs(z, ids, 3)):
+        assert torch.equal(a, b)
+    pool = torch.randn(4, 8, device='cuda')
+    ref = pool.clone()
+    ref[1] = ref[3]
+    torch.ops.mica.cache_copy(pool, [3], [1])
+    assert torch.equal(pool, ref)
+
+
+def test_gradients_are_refused():
+    from mica_b200 import logprobs, paged
+    c = Case([10], [2], 8, 2, 128, 32)
+    c.q.requires_grad_(True)
+    with pytest.raises(RuntimeError, match='no backward'):
+        run_attention(c)
+    with torch.no_grad():
+        run_attention(c)
+    z = torch.randn(2, 50, device='cuda', requires_grad=True)
+    with pytest.raises(RuntimeError, match='no backward'):
+        logprobs.token_logprobs(z, torch.zeros(2, dtype=torch.int64, device='cuda'))
+    with pytest.raises(RuntimeError, match='tensors on'):
+        paged.attention(c.q.detach(), c.k.cpu(), c.v.cpu(), c.step(), 8)
+
+
+def test_two_steps_of_one_cache_at_once():
+    """Two attentions on two streams over the same pages: each has its own workspace."""
+    c = Case([9000, 40], [3, 64], 32, 8, 128, 64, seed=7, mask=tree)
+    d = Case([9000, 40], [3, 64], 32, 8, 128, 64, seed=7, mask=tree)
+    d.k, d.v, d.q = c.k, c.v, c.q.flip(0).contiguous()
+    ref = run_attention(c), run_attention(d)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        a = run_attention(c)
+        with torch.cuda.stream(side):
+            b = run_attention(d)
+        torch.cuda.synchronize()
+        assert torch.equal(a, ref[0]) and torch.equal(b, ref[1])
