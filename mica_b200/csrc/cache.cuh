@@ -200,6 +200,196 @@ __global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a
     }
 }
 
+// The same for many rows: a CTA takes every grid-th row through a ring in shared memory. One warp looks
+// up the places of 32 coming rows at once (a lane each) and keeps bulk copies of rows, cos and sin in
+// flight; eight warps norm and turn q and k where they lie; one thread sends q, and each head's k and v,
+// out by bulk copies. Nothing waits for a look-up or a load of its own row.
+constexpr int APPEND_WARPS = 8, APPEND_STAGES = 8;
+struct AppendStage {
+    long off;                   // of the row's slot in a K or V page (elements, head 0)
+    int row, ok;
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                 ::"l"(reinterpret_cast<uint64_t>(dst)), "r"(smem_u32(src)), "r"(bytes) : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(APPEND_WARPS * 32 + 64, 2) cache_append_ring_kernel(const AppendArgs a, const int stages) {
+    constexpr int LPH = D / 8, HP = 32 / LPH;
+    extern __shared__ __align__(128) uint8_t append_ring[];
+    __shared__ uint64_t full[APPEND_STAGES], done[APPEND_STAGES], empty[APPEND_STAGES];
+    __shared__ AppendStage info[APPEND_STAGES];
+    __shared__ uint32_t s_abort;
+    volatile uint32_t* abort_flag = &s_abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t row_bytes = static_cast<uint32_t>(a.H + 2 * a.KV) * D * 2, stage_bytes = row_bytes + 4 * D;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < stages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&done[i], APPEND_WARPS);
+            mbar_init(&empty[i], 1);
+        }
+        s_abort = 0u;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    const int rows = blockIdx.x < a.plan.N ? (a.plan.N - 1 - static_cast<int>(blockIdx.x)) / static_cast<int>(gridDim.x) + 1 : 0;
+    if (warp == APPEND_WARPS) {
+        // ---------------------------------- places and loads ----------------------------------
+        int st = 0;
+        uint32_t par = 1u;
+        bool go = true;
+        for (int i0 = 0; i0 < rows && go; i0 += 32) {
+            // this lane's row of the next 32
+            const int row = static_cast<int>(blockIdx.x) + (i0 + lane) * static_cast<int>(gridDim.x);
+            long off = 0, p = 0;
+            bool ok = false;
+            if (i0 + lane < rows) {
+                int lo = 0, n = a.plan.B;                       // ends cu[1..B] that are <= row
+                while (n > 0) {
+                    const int half = n >> 1;
+                    if (a.plan.cu[lo + half + 1] <= row) { lo += half + 1; n -= half + 1; }
+                    else n = half;
+                }
+                if (lo < a.plan.B && row >= a.plan.cu[lo]) {
+                    const int base = a.plan.base[lo];
+                    const long index = static_cast<long>(base) + (row - a.plan.cu[lo]);
+                    int page = 0, slot = 0;
+                    ok = base >= 0 && cache_slot(a.plan, lo, index, &page, &slot);
+                    p = a.pos ? a.pos[row] : index;
+                    ok = ok && p >= 0 && p < a.n_pos;
+                    off = static_cast<long>(page) * a.page_stride + static_cast<long>(slot) * D;
+                    if (!ok) record_bad_page();
+                }
+            }
+            const int n = min(32, rows - i0);
+            for (int i = 0; i < n; ++i) {
+                const long off_i = __shfl_sync(0xffffffffu, off, i), p_i = __shfl_sync(0xffffffffu, p, i);
+                const int row_i = __shfl_sync(0xffffffffu, row, i);
+                const bool ok_i = __shfl_sync(0xffffffffu, ok, i);
+                bool w = true;
+                if (lane == 0) {
+                    w = mbar_wait(&empty[st], par, abort_flag, MICA_DEV_TIMEOUT_PRODUCER);
+                    if (w) {
+                        info[st].off = off_i;
+                        info[st].row = row_i;
+                        info[st].ok = ok_i;
+                        uint8_t* to = append_ring + st * stage_bytes;
+                        mbar_arrive_expect_tx(&full[st], ok_i ? stage_bytes : 0u);
+                        if (ok_i) {
+                            bulk_load(to, a.qkv + static_cast<long>(row_i) * a.ld, row_bytes, &full[st]);
+                            bulk_load(to + row_bytes, a.cos + p_i * D, 2 * D, &full[st]);
+                            bulk_load(to + row_bytes + 2 * D, a.sin + p_i * D, 2 * D, &full[st]);
+                        }
+                    }
+                }
+                go = __shfl_sync(0xffffffffu, w, 0);
+                if (!go) break;
+                if (++st == stages) { st = 0; par ^= 1u; }
+            }
+        }
+        // copies in flight land before shared memory is released
+        if (lane == 0)
+            for (int i = max(0, rows - stages); i < rows; ++i)
+                mbar_wait(&full[i % stages], (i / stages) & 1u, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
+        __syncwarp();
+    } else if (warp == APPEND_WARPS + 1) {
+        // ---------------------------------- stores ----------------------------------
+        if (lane == 0) {
+            int st = 0, before = -1;
+            uint32_t par = 0u;
+            for (int i = 0; i < rows; ++i) {
+                if (!mbar_wait(&done[st], par, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE)) break;
+                const uint8_t* from = append_ring + st * stage_bytes;
+                bulk_store(a.q_out + static_cast<long>(info[st].row) * a.ldq, from, a.H * D * 2);
+                if (info[st].ok) {
+                    from += a.H * D * 2;
+                    const long off = info[st].off;
+                    for (int h = 0; h < a.KV; ++h) {
+                        const long at = off + (static_cast<long>(h) << a.plan.page_log2) * D;
+                        bulk_store(a.k_pages + at, from + h * D * 2, D * 2);
+                        bulk_store(a.v_pages + at, from + (a.KV + h) * D * 2, D * 2);
+                    }
+                }
+                tma_store_commit();
+                // the stage before has been read when all but this group are
+                tma_store_wait_read<1>();
+                if (before >= 0) mbar_arrive(&empty[before]);
+                before = st;
+                if (++st == stages) { st = 0; par ^= 1u; }
+            }
+            tma_store_wait_all<0>();
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------- norm and rotation ----------------------------------
+        const int heads = a.H + a.KV, sub = lane / LPH, d = 4 * (lane % LPH);
+        const auto pair = [&](const __nv_bfloat16* t, uint2& l, uint2& h) {
+            l = *reinterpret_cast<const uint2*>(t + d);
+            h = *reinterpret_cast<const uint2*>(t + d + D / 2);
+        };
+        uint2 ql, qh, kl, kh;
+        pair(a.q_w, ql, qh);
+        pair(a.k_w, kl, kh);
+        int st = 0;
+        uint32_t par = 0u;
+        for (int i = 0; i < rows; ++i) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&full[st], par, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE))) break;
+            __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(append_ring + st * stage_bytes);
+            if (info[st].ok) {
+                uint2 c0, c1, n0, n1;
+                pair(x + row_bytes / 2, c0, c1);
+                pair(x + row_bytes / 2 + D, n0, n1);
+                float cl[4], ch[4], sl[4], sh[4];
+                unpack4_bf16(c0, cl);
+                unpack4_bf16(c1, ch);
+                unpack4_bf16(n0, sl);
+                unpack4_bf16(n1, sh);
+                for (int h0 = warp * HP; h0 < heads; h0 += APPEND_WARPS * HP) {
+                    const int h = h0 + sub;
+                    __nv_bfloat16* at = x + min(h, heads - 1) * D;
+                    uint2 l, u;
+                    pair(at, l, u);
+                    float fl[4], fh[4], wl[4], wh[4], ss = 0.f;
+                    unpack4_bf16(l, fl);
+                    unpack4_bf16(u, fh);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ss = fmaf(fl[e], fl[e], fmaf(fh[e], fh[e], ss));
+#pragma unroll
+                    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    const float r = rsqrtf(ss * (1.f / D) + a.eps);
+                    unpack4_bf16(h < a.H ? ql : kl, wl);
+                    unpack4_bf16(h < a.H ? qh : kh, wh);
+                    float o0[4], o1[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float y0 = fl[e] * r * wl[e], y1 = fh[e] * r * wh[e];
+                        o0[e] = y0 * cl[e] - y1 * sl[e];
+                        o1[e] = y1 * ch[e] + y0 * sh[e];
+                    }
+                    if (h < heads) {
+                        *reinterpret_cast<uint2*>(at + d) = make_uint2(pack_bf16(o0[0], o0[1]), pack_bf16(o0[2], o0[3]));
+                        *reinterpret_cast<uint2*>(at + d + D / 2) = make_uint2(pack_bf16(o1[0], o1[1]), pack_bf16(o1[2], o1[3]));
+                    }
+                }
+            } else {
+                for (int e = threadIdx.x; e < a.H * D / 8; e += APPEND_WARPS * 32) reinterpret_cast<uint4*>(x)[e] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();                       // the bulk stores read what was written here
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&done[st]);
+            if (++st == stages) { st = 0; par ^= 1u; }
+        }
+    }
+    __syncthreads();
+}
+
 // ---------------------------------------------------------------------------------------
 // Page copies: pool[dst[i]] = pool[src[i]], the pairs in the kernel's parameters (the host has
 // checked them: in range, no page written twice or both read and written). Bound by memory: a block

@@ -295,6 +295,45 @@ def test_append(heads, kv, dim, page, positions):
     assert torch.equal(c.pool, before)
 
 
+@pytest.mark.parametrize('heads,kv,dim', [(32, 8, 128), (5, 1, 64), (16, 1, 128)])
+def test_append_many_rows(heads, kv, dim):
+    """A prompt of thousands of rows (the ring): ragged sequences, padding rows, one sequence without room."""
+    from mica_b200 import paged
+    ctx, new = [0, 300, 5, 64], [2000, 1, 900, 3000]
+    c = Case(ctx, new, heads, kv, dim, 64, seed=heads, layers=2, layer=1, pad_rows=5)
+    g = torch.Generator(device='cuda').manual_seed(1)
+    qkv = (2 * torch.randn(c.n, (heads + 2 * kv) * dim, generator=g, device='cuda')).bfloat16()
+    qw, kw = (1 + 0.1 * torch.randn(2, dim, generator=g, device='cuda')).bfloat16()
+    cos, sin = tables(dim)
+    c.pool.zero_()
+    pos = torch.randint(0, 5000, (c.n,), generator=g, device='cuda')
+    c.base[1] = 64 * c.table.shape[1]                     # its row has no slot
+    q = paged.append(qkv, qw, kw, cos, sin, c.k, c.v, c.step(), heads, pos=pos)
+    n = sum(new)
+    x = qkv[:n].view(n, heads + 2 * kv, dim)
+    ref = torch.cat((norm_rope(x[:, :heads], qw, cos[pos[:n]], sin[pos[:n]], 1e-6),
+                     norm_rope(x[:, heads:heads + kv], kw, cos[pos[:n]], sin[pos[:n]], 1e-6)), 1)
+    bound = U * ref.abs() + 2.0 ** -20 * 4 * ref.abs().amax(-1, keepdim=True) + 1e-12
+    good = torch.ones(n, dtype=torch.bool, device='cuda')
+    good[2000] = False
+    assert ((q[:n].view(n, heads, dim).double() - ref[:, :heads]).abs() <= bound[:, :heads])[good].all()
+    assert float(q[n:].float().abs().max()) == 0.0 and float(q[2000].float().abs().max()) == 0.0
+    b = torch.cat([torch.full((t,), i) for i, t in enumerate(new)]).cuda()[good]
+    index = torch.cat([torch.arange(a, a + t) for a, t in zip(ctx, new)]).cuda()[good]
+    page_of, slot = c.table.long()[b, index // 64], index % 64
+    assert ((c.k[page_of, :, slot].double() - ref[good][:, heads:]).abs() <= bound[good][:, heads:]).all()
+    assert torch.equal(c.v[page_of, :, slot], x[good][:, heads + kv:])
+    c.k[page_of, :, slot] = 0
+    c.v[page_of, :, slot] = 0
+    assert float(c.pool.float().abs().max()) == 0.0
+    import ctypes
+
+    from mica_b200 import _native as N
+    code = ctypes.c_int(0)
+    N.call('mica_device_error', ctypes.byref(code), torch.cuda.current_stream().cuda_stream)
+    assert code.value == 9
+
+
 def test_append_bad_indexes_write_nothing():
     import ctypes
 
