@@ -84,8 +84,9 @@ struct AppendArgs {
 // A row is one or more warps' (`split`: few rows are spread over the chip), each with every
 // split-th set of HP heads; cos, sin and both norm weights stay in registers across them. The first
 // loads of x are on their way while the row's place in the cache is looked up, and four sets are in
-// flight: with one warp a (row, head) and scalar loads the 8000-row prompt took 153 us
-// APPEND_US.
+// flight. 8000 rows of 48 heads of 128 took 153 us with one warp a (row, head) and scalar loads, and take
+// 55 us so, whatever the split (on fp32 pairs 65 to 88, with 16-byte loads 54 to 93: registers); rows in
+// such numbers go through the ring below. Eight rows take 6 to 8 us, a launch.
 // Keeps the words as they are in registers (their unpacked values, hoisted out of the loop, would take
 // twice as many). Emits nothing.
 __device__ __forceinline__ void keep_packed(uint2& q) { asm volatile("" : "+r"(q.x), "+r"(q.y)); }
@@ -204,7 +205,8 @@ __global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a
 // up the places of 32 coming rows at once (a lane each) and keeps bulk copies of rows, cos and sin in
 // flight; eight warps norm and turn q and k where they lie; one thread sends q, and each head's k and v,
 // out by bulk copies. Nothing waits for a look-up or a load of its own row.
-constexpr int APPEND_WARPS = 8, APPEND_STAGES = 8;
+constexpr int APPEND_WARPS = 8, APPEND_STAGES = 8, APPEND_CTAS = 3;
+constexpr long APPEND_SMEM = 70 << 10;      // of a CTA's ring
 struct AppendStage {
     long off;                   // of the row's slot in a K or V page (elements, head 0)
     int row, ok;
@@ -220,7 +222,7 @@ __device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t 
 }
 
 template <int D>
-__global__ void __launch_bounds__(APPEND_WARPS * 32 + 64, 2) cache_append_ring_kernel(const AppendArgs a, const int stages) {
+__global__ void __launch_bounds__(APPEND_WARPS * 32 + 64, APPEND_CTAS) cache_append_ring_kernel(const AppendArgs a, const int stages) {
     constexpr int LPH = D / 8, HP = 32 / LPH;
     extern __shared__ __align__(128) uint8_t append_ring[];
     __shared__ uint64_t full[APPEND_STAGES], done[APPEND_STAGES], empty[APPEND_STAGES];

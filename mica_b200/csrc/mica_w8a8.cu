@@ -1118,10 +1118,11 @@ int mica_cache_append(const void* qkv, long ld, const void* q_w, const void* k_w
     a.k_pages = static_cast<__nv_bfloat16*>(k_pages); a.v_pages = static_cast<__nv_bfloat16*>(v_pages);
     a.page_stride = page_stride; a.H = H; a.KV = KV; a.eps = eps;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // Many rows go through the ring, two CTAs an SM, eight rows and more each (8000 rows of 48 heads of 128: 55 us
-    // a warp a row, RING_US by it; 8 rows: 8.2 us against 9 and more, its places and loads one behind the other).
+    // Many rows go through the ring, three CTAs an SM, five rows and more each: 8000 rows of 48 heads of 128 take
+    // 42 us (one CTA an SM 57, two 46, four 44), a warp a row 55. Few rows take one look-up and one load either way,
+    // which the ring has one behind the other, with its barriers.
     const long stage = static_cast<long>(H + 2 * KV) * D * 2 + 4 * D;
-    const int stages = static_cast<int>(std::min<long>(APPEND_STAGES, (110 << 10) / stage));
+    const int stages = static_cast<int>(std::min<long>(APPEND_STAGES, APPEND_SMEM / stage));
     if (N >= 16L * sms && stages >= 3) {
         const auto kernel = D == 128 ? cache_append_ring_kernel<128> : cache_append_ring_kernel<64>;
         static std::atomic<uint64_t> done{0};
@@ -1129,13 +1130,13 @@ int mica_cache_append(const void* qkv, long ld, const void* q_w, const void* k_w
         cudaGetDevice(&dev);
         const uint64_t bit = 1ull << (dev & 63);
         if (!(done.load(std::memory_order_acquire) & bit)) {
-            cudaError_t e = cudaFuncSetAttribute(cache_append_ring_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, 110 << 10);
+            cudaError_t e = cudaFuncSetAttribute(cache_append_ring_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, APPEND_SMEM);
             if (e == cudaSuccess)
-                e = cudaFuncSetAttribute(cache_append_ring_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, 110 << 10);
+                e = cudaFuncSetAttribute(cache_append_ring_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, APPEND_SMEM);
             if (e != cudaSuccess) { set_cuda_error(e); return MICA_ERR_CUDA; }
             done.fetch_or(bit, std::memory_order_release);
         }
-        kernel<<<2 * sms, APPEND_WARPS * 32 + 64, static_cast<size_t>(stages) * stage, st>>>(a, stages);
+        kernel<<<APPEND_CTAS * sms, APPEND_WARPS * 32 + 64, static_cast<size_t>(stages) * stage, st>>>(a, stages);
         return launch_status();
     }
     // few rows are split over warps until the chip has about 16 warps an SM
