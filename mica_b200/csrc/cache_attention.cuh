@@ -14,8 +14,8 @@
 //
 // Work. A unit is (sequence, K/V head, block of NT * npt nodes); its key tiles of 128 follow one
 // another, units in order, in one line (where each unit has some places more for what it costs by
-// itself). Each of the CTAs (one per SM) takes an equal run of that line, whatever the lengths: it
-// starts and may end inside a unit. A unit that one CTA has whole
+// itself, and tiles that are shared by two row tiles count for more). Each of the CTAs (one per SM)
+// takes an equal run of that line, whatever the lengths: it starts and may end inside a unit. A unit that one CTA has whole
 // is written out; of a divided one each CTA leaves its unnormalised rows, maxima and sums in its own
 // place of the workspace (a CTA has at most two such: its first and its last), and
 // cache_attention_join adds them up in the order of the CTAs. No atomics: the same bits every time.
@@ -86,13 +86,24 @@ __device__ __forceinline__ int cache_unit_tiles(const CacheSeq& s, int rb, int R
     return max(1, (keys + 127) >> 7);
 }
 __device__ __forceinline__ int cache_row_blocks(const CacheSeq& s, int R) { return (s.T + R - 1) / R; }
-__device__ __forceinline__ long cache_seq_places(const CacheSeq& s, int R, int E, bool causal) {   // of one K/V head
-    const int n = cache_row_blocks(s, R);
-    if (!causal || n <= 1) return n ? static_cast<long>(n) * (cache_unit_tiles(s, n - 1, R, causal) + E) : 0;
-    long t = 0;
-    for (int rb = 0; rb < n; ++rb) t += cache_unit_tiles(s, rb, R, true) + E;
-    return t;
-}
+// What a unit counts in the line: its tiles and UNIT more (its rows' way out, nothing in flight), times a
+// weight for a tile, 4 with two row tiles and 3 where its nodes fill only one of the two.
+template <int NT>
+struct CacheCost {
+    static constexpr int UNIT = NT == 1 ? 1 : 2;
+    static constexpr int TILE = NT == 1 ? 1 : 4;
+    __device__ __forceinline__ static int weight(const CacheSeq& s, int rb, int R) {
+        return NT == 1 ? 1 : s.T - rb * R <= R / 2 ? 3 : 4;
+    }
+    __device__ __forceinline__ static long seq(const CacheSeq& s, int R, bool causal) {      // of one K/V head
+        const int n = cache_row_blocks(s, R);
+        if (n == 0) return 0;
+        long t = static_cast<long>(cache_unit_tiles(s, n - 1, R, causal) + UNIT) * weight(s, n - 1, R);
+        if (!causal) return t + static_cast<long>(n - 1) * (cache_unit_tiles(s, 0, R, false) + UNIT) * TILE;
+        for (int rb = 0; rb + 1 < n; ++rb) t += static_cast<long>(cache_unit_tiles(s, rb, R, true) + UNIT) * TILE;
+        return t;
+    }
+};
 
 struct CachePlace {             // a place of the line: the off-th of sequence b
     long total;
@@ -100,8 +111,8 @@ struct CachePlace {             // a place of the line: the off-th of sequence b
     int b;
 };
 // The line's length and the sequence that holds place `first(total)`; every thread of the block calls it.
-template <typename F>
-__device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, int R, int E, bool causal, F first) {
+template <int NT, typename F>
+__device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, int R, bool causal, F first) {
     __shared__ long s_warp[32];
     __shared__ long s_off;
     __shared__ int s_b;
@@ -122,7 +133,7 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
         }
         return v;
     };
-    const auto tiles = [&](int b) { return b < p.B ? KV * cache_seq_places(cache_seq(p, b), R, E, causal) : 0l; };
+    const auto tiles = [&](int b) { return b < p.B ? KV * CacheCost<NT>::seq(cache_seq(p, b), R, causal) : 0l; };
     const long mine = tiles(threadIdx.x);
     long total = 0;
     if (threadIdx.x == 0) { s_b = -1; s_off = 0; }
@@ -156,51 +167,66 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
 }
 
 // The runs of the CTAs: total / used places each, the first total % used one more. Fewer CTAs are used
-// when there are fewer places.
+// when there are fewer tiles, so that a run has a tile's places at least.
 struct CacheShare {
     long each;
     int rest, used;
-    __device__ __forceinline__ CacheShare(long total, int ctas) {
-        used = static_cast<int>(total < ctas ? total : ctas);
+    __device__ __forceinline__ CacheShare(long total, int ctas, int tile) {
+        const long most = total / tile;
+        used = static_cast<int>(most < ctas ? most : ctas);
         if (total <= 0x7fffffffl) {
             const unsigned n = static_cast<unsigned>(total), d = max(used, 1);
             each = n / d;
             rest = static_cast<int>(n - static_cast<unsigned>(each) * d);
         } else {
-            each = total / used;
+            each = total / max(used, 1);
             rest = static_cast<int>(total - each * used);
         }
     }
     __device__ __forceinline__ long at(int c) const { return each * c + min(c, rest); }
 };
 
-// The units of a CTA's run, one after another: those of which it has tiles.
+// The units of a CTA's run, one after another: those of which it has tiles. A tile is the run's that holds
+// the first of its places; a unit's first UNIT tiles' places are nobody's.
+template <int NT>
 struct CacheWalk {
+    using Cost = CacheCost<NT>;
     CacheSeq s;
     int b, kvh, rb;             // unit
     int nk, j0, j1;             // its tiles, and the CTA's [j0, j1) of them
+    int w;                      // places of a tile
     long left;                  // places of the run from the unit's first on
-    int R, E;
+    int R;
     bool causal;
 
-    // false: the run lies in front of a unit's first tile
-    __device__ __forceinline__ bool start(const CachePlan& p, int R_, int E_, bool causal_, int b_, long off, long n) {
-        R = R_; E = E_; causal = causal_; b = b_;
+    __device__ __forceinline__ long unit_places() const { return static_cast<long>(nk + Cost::UNIT) * w; }
+    __device__ __forceinline__ int tiles_before(long places) const {       // of those places of the unit
+        if (places >= unit_places()) return nk;
+        return max(0, static_cast<int>((static_cast<unsigned>(places) + w - 1) / static_cast<unsigned>(w)) - Cost::UNIT);
+    }
+    __device__ __forceinline__ void unit() {
+        nk = cache_unit_tiles(s, rb, R, causal);
+        w = Cost::weight(s, rb, R);
+    }
+    // off: the run's first place in sequence b_; false: it has no tile
+    __device__ __forceinline__ bool start(const CachePlan& p, int KV, int R_, bool causal_, int b_, long off, long n) {
+        R = R_; causal = causal_; b = b_;
         s = cache_seq(p, b);
-        const long per = cache_seq_places(s, R, E, causal);
+        const long per = Cost::seq(s, R, causal);
         kvh = off <= 0x7fffffffl && per <= 0x7fffffffl ? static_cast<int>(static_cast<unsigned>(off) / static_cast<unsigned>(per))
                                                        : static_cast<int>(off / per);
         off -= kvh * per;
         rb = 0;
-        while (off >= (nk = cache_unit_tiles(s, rb, R, causal)) + E) { off -= nk + E; ++rb; }
+        for (unit(); off >= unit_places(); unit()) { off -= unit_places(); ++rb; }
         left = n + off;
-        j0 = max(0, static_cast<int>(off) - E);
-        j1 = static_cast<int>(min(static_cast<long>(nk), left - E));
+        j0 = tiles_before(off);
+        if (j0 == nk) return next(p, KV);                   // behind the first place of its last tile
+        j1 = tiles_before(left);
         return j1 > j0;
     }
     __device__ __forceinline__ bool next(const CachePlan& p, int KV) {
-        left -= nk + E;
-        if (left <= E) return false;
+        left -= unit_places();
+        if (left <= 0) return false;
         if (++rb >= cache_row_blocks(s, R)) {
             rb = 0;
             if (++kvh >= KV) {
@@ -211,10 +237,10 @@ struct CacheWalk {
                 } while (s.T == 0);
             }
         }
-        nk = cache_unit_tiles(s, rb, R, causal);
+        unit();
         j0 = 0;
-        j1 = static_cast<int>(min(static_cast<long>(nk), left - E));
-        return true;
+        j1 = tiles_before(left);
+        return j1 > 0;
     }
     __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == nk; }
 };
@@ -236,9 +262,6 @@ struct CacheAttnShape {
     static constexpr int KST = D == 128 ? 3 : 6;
     static constexpr int VST = D == 128 ? 2 : 5;
     static constexpr int THREADS = 128 + 128 * NT;
-    // What a unit costs beside its tiles (its rows' way out, nothing in flight), in tiles: it stands in the
-    // line for that many places more.
-    static constexpr int UNIT = NT == 1 ? 1 : 2;
     static constexpr int BARS = 768;
     static constexpr int SMEM = 1024 + TILE * (QBUF * NT + KST + VST) + BARS;
 };
@@ -340,12 +363,13 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         tma_prefetch_desc(&tmap_v);
     }
     // this CTA's run of tiles
-    const CachePlace place = cache_locate(plan, args.KV, R, S::UNIT, causal,
-                                          [&](long total) { return CacheShare(total, args.ctas).at(cta); });
-    const CacheShare share(place.total, args.ctas);
-    CacheWalk wk;
+    using Cost = CacheCost<NT>;
+    const CachePlace place = cache_locate<NT>(plan, args.KV, R, causal,
+                                              [&](long total) { return CacheShare(total, args.ctas, Cost::TILE).at(cta); });
+    const CacheShare share(place.total, args.ctas, Cost::TILE);
+    CacheWalk<NT> wk;
     if (cta >= share.used || place.b < 0 ||
-        !wk.start(plan, R, S::UNIT, causal, place.b, place.off, share.at(cta + 1) - share.at(cta))) {
+        !wk.start(plan, args.KV, R, causal, place.b, place.off, share.at(cta + 1) - share.at(cta))) {
         if (threadIdx.x == 0) args.cuts[2 * cta] = make_int4(0, 0, 0, 0);
         cache_zero_padding(args, D);
         return;
@@ -480,6 +504,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 if (++st == stages) { st = 0; par ^= 1u; }
             }
         }
+        // the place of this CTA's last unit, for the join
+        if (is_k && lane == 0) args.cuts[2 * cta + 1] = make_int4(unit > 1 ? 1 : 0, 0, 0, 0);
         // loads still in flight land before shared memory is released
         if (lane == 0) {
             if (is_k)
@@ -587,16 +613,18 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         if (lane == 0) {
             // the unit this CTA starts inside, for the join: its first row, node rows, K/V head, and the CTAs
             // that hold parts of it, the one before and `n` from this one on
-            const long s0 = share.at(cta) - wk.j0;                // the unit's first tile in the line
-            int4 cut = make_int4(0, 0, 0, 0), more = cut;
-            if (wk.j0 > 0 && share.at(cta - 1) <= s0) {
-                int n = 1;
-                while (cta + n < share.used && share.at(cta + n) < s0 + wk.nk) ++n;
-                cut = make_int4(min(R, wk.s.T - wk.rb * R) * args.G, wk.s.row0 + wk.rb * R, wk.kvh, n);
-                more.x = share.at(cta - 1) >= s0 - S::UNIT ? 0 : 1;   // the first part's place: it may be its CTA's first unit
+            int4 cut = make_int4(0, 0, 0, 0);
+            if (wk.j0 > 0) {
+                // places of the unit before each CTA's run: up to its first tile, up to its last
+                const long first = static_cast<long>(Cost::UNIT) * wk.w, last = static_cast<long>(wk.nk - 1 + Cost::UNIT) * wk.w;
+                const long unit0 = share.at(cta + 1) - wk.left;
+                if (share.at(cta - 1) - unit0 <= first) {
+                    int n = 1;
+                    while (cta + n < share.used && share.at(cta + n) - unit0 <= last) ++n;
+                    cut = make_int4(min(R, wk.s.T - wk.rb * R) * args.G, wk.s.row0 + wk.rb * R, wk.kvh, n);
+                }
             }
             args.cuts[2 * cta] = cut;
-            args.cuts[2 * cta + 1] = more;
         }
     } else {
         // ---------------------------------- softmax ----------------------------------
@@ -858,7 +886,7 @@ __global__ void __launch_bounds__(128) cache_attention_join(const CacheAttnArgs 
     const int rows = cut.x, n = cut.w;
     const int idx = blockIdx.y * blockDim.x + threadIdx.x;
     if (idx >= rows * (D / 16)) return;
-    const int first_place = args.cuts[2 * c + 1].x;
+    const int first_place = args.cuts[2 * (c - 1) + 1].x;            // of the part that the CTA before left last
     const long pf = cache_attn_place_floats<D, NT>();
     const int rr = idx % rows, d16 = idx / rows;
     const int node = rr / args.G, g = rr - node * args.G;
