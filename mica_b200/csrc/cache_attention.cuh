@@ -134,6 +134,19 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
         return v;
     };
     const auto tiles = [&](int b) { return b < p.B ? KV * CacheCost<NT>::seq(cache_seq(p, b), R, causal) : 0l; };
+    if (p.B <= 32) {                                 // every warp by itself
+        const long n = tiles(lane);
+        long end = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long u = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += u;
+        }
+        const long total = __shfl_sync(0xffffffffu, end, 31), t = first(total);
+        const uint32_t here = __ballot_sync(0xffffffffu, t >= end - n && t < end);
+        const int b = __ffs(here) - 1;
+        return CachePlace{total, t - __shfl_sync(0xffffffffu, end - n, max(b, 0)), b};
+    }
     const long mine = tiles(threadIdx.x);
     long total = 0;
     if (threadIdx.x == 0) { s_b = -1; s_off = 0; }
