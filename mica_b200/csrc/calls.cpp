@@ -148,7 +148,7 @@ Tensor append(const Tensor& qkv_, const Tensor& q_w, const Tensor& k_w, const Te
     no_grad(name, {&qkv_, &q_w, &k_w});
     const c10::cuda::CUDAGuard guard(qkv_.device());
     if (n == 0 || st.B == 0) return at::zeros({n, heads * pg.d}, qkv_.options());      // padding rows alone
-    const Tensor qkv = rows16(qkv_), qw = rows16(q_w.unsqueeze(0)), kw = rows16(k_w.unsqueeze(0));
+    const Tensor qkv = rows16(qkv_), qw = rows16(q_w.contiguous().unsqueeze(0)), kw = rows16(k_w.contiguous().unsqueeze(0));
     const Tensor pos = pos_ ? pos_->contiguous() : Tensor();
     Tensor q = at::empty({n, heads * pg.d}, qkv_.options());
     status("mica_cache_append",

@@ -533,6 +533,8 @@ int mica_query(int device, mica_caps* caps) {
     return MICA_OK;
 }
 
+static int cache_prepare(int* n);     // the paged cache's and the log probabilities' kernels
+
 int mica_preload(int* n_kernels) {
     int rc = check_device(nullptr);
     if (rc) return rc;
@@ -583,6 +585,7 @@ int mica_preload(int* n_kernels) {
     PREP_SK(128, float)
     PREP_SK(256, float)
 #undef PREP_SK
+    if ((rc = cache_prepare(&n))) return rc;
     if (n_kernels) *n_kernels = n;
     return MICA_OK;
 }
@@ -1088,6 +1091,24 @@ static int cache_plan(CachePlan* p, const int* table, long ld_table, int P, cons
     p->page_log2 = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
     return MICA_OK;
 }
+// Sets a kernel's shared-memory limit, once a device.
+template <typename K>
+static int smem_limit(K kernel, int bytes, std::atomic<uint64_t>& done, bool wide_clusters = false) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return MICA_OK;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && wide_clusters) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) { set_cuda_error(e); return MICA_ERR_CUDA; }
+    done.fetch_or(bit, std::memory_order_release);
+    return MICA_OK;
+}
+static int append_ring_prepare() {
+    static std::atomic<uint64_t> wide{0}, narrow{0};
+    if (int rc = smem_limit(cache_append_ring_kernel<128>, APPEND_SMEM, wide)) return rc;
+    return smem_limit(cache_append_ring_kernel<64>, APPEND_SMEM, narrow);
+}
 static bool aligned_to(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 int mica_cache_append(const void* qkv, long ld, const void* q_w, const void* k_w, const void* cos, const void* sin,
@@ -1125,17 +1146,7 @@ int mica_cache_append(const void* qkv, long ld, const void* q_w, const void* k_w
     const int stages = static_cast<int>(std::min<long>(APPEND_STAGES, APPEND_SMEM / stage));
     if (N >= 16L * sms && stages >= 3) {
         const auto kernel = D == 128 ? cache_append_ring_kernel<128> : cache_append_ring_kernel<64>;
-        static std::atomic<uint64_t> done{0};
-        int dev = 0;
-        cudaGetDevice(&dev);
-        const uint64_t bit = 1ull << (dev & 63);
-        if (!(done.load(std::memory_order_acquire) & bit)) {
-            cudaError_t e = cudaFuncSetAttribute(cache_append_ring_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, APPEND_SMEM);
-            if (e == cudaSuccess)
-                e = cudaFuncSetAttribute(cache_append_ring_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, APPEND_SMEM);
-            if (e != cudaSuccess) { set_cuda_error(e); return MICA_ERR_CUDA; }
-            done.fetch_or(bit, std::memory_order_release);
-        }
+        if ((rc = append_ring_prepare())) return rc;
         kernel<<<APPEND_CTAS * sms, APPEND_WARPS * 32 + 64, static_cast<size_t>(stages) * stage, st>>>(a, stages);
         return launch_status();
     }
@@ -1169,16 +1180,8 @@ size_t mica_cache_attention_workspace_bytes(int N, int max_new, int H, int KV, i
 
 template <int D, int NT>
 static int cache_attn_prepare() {
-    int dev = 0;
-    cudaGetDevice(&dev);
     static std::atomic<uint64_t> done{0};
-    const uint64_t bit = 1ull << (dev & 63);
-    if (done.load(std::memory_order_acquire) & bit) return MICA_OK;
-    cudaError_t e = cudaFuncSetAttribute(cache_attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         CacheAttnShape<D, NT>::SMEM);
-    if (e != cudaSuccess) { set_cuda_error(e); return MICA_ERR_CUDA; }
-    done.fetch_or(bit, std::memory_order_release);
-    return MICA_OK;
+    return smem_limit(cache_attention_kernel<D, NT>, CacheAttnShape<D, NT>::SMEM, done);
 }
 
 template <int D, int NT>
@@ -1324,20 +1327,14 @@ static int logprob_parts(int N, int V, int dtype, int sms) {
 }
 
 template <typename T>
-static int logprob_launch(const LogprobArgs& a, int parts, int sms, cudaStream_t st) {
-    int dev = 0;
-    cudaGetDevice(&dev);
+static int logprob_prepare() {
     static std::atomic<uint64_t> done{0};
-    const uint64_t bit = 1ull << (dev & 63);
-    cudaError_t e;
-    if (!(done.load(std::memory_order_acquire) & bit)) {
-        if ((e = cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess ||
-            (e = cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, LP_SMEM)) != cudaSuccess) {
-            set_cuda_error(e);
-            return MICA_ERR_CUDA;
-        }
-        done.fetch_or(bit, std::memory_order_release);
-    }
+    return smem_limit(token_logprobs_kernel<T>, LP_SMEM, done, true);
+}
+
+template <typename T>
+static int logprob_launch(const LogprobArgs& a, int parts, int sms, cudaStream_t st) {
+    if (int rc = logprob_prepare<T>()) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(std::min(a.N, std::max(1, sms / parts)) * parts));
     cfg.blockDim = dim3(LP_BLOCK);
@@ -1349,7 +1346,7 @@ static int logprob_launch(const LogprobArgs& a, int parts, int sms, cudaStream_t
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a, parts);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a, parts);
     if (e != cudaSuccess) { set_cuda_error(e); return MICA_ERR_CUDA; }
     return launch_status();
 }
@@ -1377,6 +1374,26 @@ int mica_token_logprobs(const void* z, int dtype, long ld, int N, int V, const i
     if (dtype == MICA_DT_BF16) return logprob_launch<__nv_bfloat16>(a, parts, sms, st);
     if (dtype == MICA_DT_FP16) return logprob_launch<__half>(a, parts, sms, st);
     return logprob_launch<float>(a, parts, sms, st);
+}
+
+static int cache_prepare(int* n) {
+    int rc = MICA_OK;
+    if ((rc = append_ring_prepare()) || (rc = cache_attn_prepare<128, 1>()) || (rc = cache_attn_prepare<128, 2>()) ||
+        (rc = cache_attn_prepare<64, 1>()) || (rc = cache_attn_prepare<64, 2>()) || (rc = logprob_prepare<__nv_bfloat16>()) ||
+        (rc = logprob_prepare<__half>()) || (rc = logprob_prepare<float>()))
+        return rc;
+    // loads the kernels that need no attribute
+    const void* others[] = {reinterpret_cast<const void*>(cache_append_kernel<128>), reinterpret_cast<const void*>(cache_append_kernel<64>),
+                            reinterpret_cast<const void*>(cache_attention_join<128, 1>), reinterpret_cast<const void*>(cache_attention_join<128, 2>),
+                            reinterpret_cast<const void*>(cache_attention_join<64, 1>), reinterpret_cast<const void*>(cache_attention_join<64, 2>),
+                            reinterpret_cast<const void*>(cache_copy_kernel), reinterpret_cast<const void*>(cache_keep_kernel)};
+    for (const void* k : others) {
+        cudaFuncAttributes at;
+        cudaError_t e = cudaFuncGetAttributes(&at, k);
+        if (e != cudaSuccess) { set_cuda_error(e); return MICA_ERR_CUDA; }
+    }
+    *n += 9 + static_cast<int>(sizeof(others) / sizeof(others[0]));
+    return MICA_OK;
 }
 
 // ---------------------------------------------------------------------------------------

@@ -46,7 +46,7 @@ class Step:
 
     Row i of sequence b sits at cache index base[b] + i and sees all of the committed tokens."""
 
-    __slots__ = ('table', 'base', 'cu', 'mask', 'max_new')
+    __slots__ = ('table', 'base', 'cu', 'mask', 'max_new', 'rows')
 
     def __init__(self, table, base, cu, max_new: Optional[int] = None, mask=None):
         if table.dim() != 2 or base.dim() != 1 or cu.dim() != 1 or not (
@@ -66,13 +66,15 @@ class Step:
         if max_new is not None and max_new < 0:
             raise ValueError(f'Step: max_new {max_new}')
         self.table, self.base, self.cu, self.mask, self.max_new = table, base, cu, mask, max_new
+        self.rows = None               # rows of each sequence, where the host knows them (PagedCache.step)
 
 
 def append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, step: Step, heads: int, pos=None, eps: float = 1e-6):
     """Per-head RMSNorm of q and k, rotation by `pos` (int64 [N]; None: the cache index) and the write of K
     and V into the step's slots, in one pass over the QKV projection's output [N, (H + 2 KV) D] (q | k | v,
     unit column stride). Returns q [N, H D]; qkv is not changed. fp32, rounded to bf16 once
-    (ops.qk_norm_rope keeps HF's rounding of every step). cos, sin bf16 [positions, D]."""
+    (ops.qk_norm_rope keeps HF's rounding of every step). cos, sin bf16 [positions, D]. Sequences of a step
+    have slots of their own: a page that two of them write is the caller's mistake (PagedCache copies it first)."""
     q = N.calls().append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, step.table, step.base, step.cu, heads, pos, eps)
     _launched()
     return q
@@ -238,7 +240,9 @@ class PagedCache:
         meta = torch.tensor(flat + [self._seqs[s][1] for s in sids] + cu, dtype=torch.int32)
         meta = meta.pin_memory().to(self.pool.device, non_blocking=True)
         w = b * width
-        return Step(meta[:w].view(b, width), meta[w:w + b], meta[w + b:], max_new=max(new, default=0), mask=mask)
+        s = Step(meta[:w].view(b, width), meta[w:w + b], meta[w + b:], max_new=max(new, default=0), mask=mask)
+        s.rows = list(new)
+        return s
 
     def commit(self, sids: Sequence[int], new: Sequence[int]) -> None:
         """The first new[b] appended rows of each sequence become committed tokens."""
@@ -252,13 +256,13 @@ class PagedCache:
 
     def keep(self, sids: Sequence[int], step: Step, keep: Sequence[Sequence[int]]) -> None:
         """Commits the rows keep[b] (increasing) of the step's tree: the accepted tokens of each sequence."""
-        if len(sids) != len(keep) or len(sids) != step.base.shape[0]:
-            raise ValueError(f'keep: {len(keep)} lists for {len(sids)} sequences')
-        for sid, rows in zip(sids, keep):
+        if len(sids) != len(keep) or step.rows is None or len(sids) != len(step.rows):
+            raise ValueError(f'keep: {len(keep)} lists for {len(sids)} sequences of a step of this cache')
+        for sid, rows, n in zip(sids, keep, step.rows):
             pages, length = self._seqs[sid]
-            if any(a >= b for a, b in zip(rows, rows[1:])) or (rows and (
-                    rows[0] < 0 or length + rows[-1] >= len(pages) * self.page)):
-                raise ValueError(f'keep: rows {list(rows)} of sequence {sid}')
+            if any(a >= b for a, b in zip(rows, rows[1:])) or (rows and (rows[0] < 0 or rows[-1] >= n)) or (
+                    length + n > len(pages) * self.page):
+                raise ValueError(f'keep: rows {list(rows)} of {n} of sequence {sid}')
         most = max((len(r) for r in keep), default=0)
         if any(list(r) != list(range(len(r))) for r in keep):
             flat = [list(r) + [0] * (most - len(r)) for r in keep]

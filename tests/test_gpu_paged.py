@@ -552,3 +552,22 @@ def test_two_steps_of_one_cache_at_once():
             b = run_attention(d)
         torch.cuda.synchronize()
         assert torch.equal(a, ref[0]) and torch.equal(b, ref[1])
+
+
+def test_strided_norm_weights_and_positions():
+    from mica_b200 import paged
+    c = Case([3], [5], 4, 2, 64, 16)
+    qkv = torch.randn(5, 8 * 64, device='cuda').bfloat16()
+    w = torch.randn(128, device='cuda').bfloat16()
+    cos, sin = tables(64)
+    pos = torch.arange(10, device='cuda')
+    a = paged.append(qkv, w[::2], w[1::2], cos, sin, c.k, c.v, c.step(), 4, pos=pos[::2])
+    k = c.k.clone()
+    b = paged.append(qkv, w[::2].clone(), w[1::2].clone(), cos, sin, c.k, c.v, c.step(), 4, pos=pos[::2].clone())
+    assert torch.equal(a, b) and torch.equal(k.view(torch.int16), c.k.view(torch.int16))
+
+
+def test_long_causal_extension_of_many_row_blocks():
+    """Thousands of new rows over a context: row blocks of different lengths, cut anywhere in the line."""
+    c = Case([100, 900], [1300, 700], 4, 1, 64, 128, seed=31)
+    check_attention(c, run_attention(c, max_new=1300))

@@ -199,6 +199,13 @@ def test_cache_host_state(monkeypatch):
     assert len(copies) == 1 and c.pages_of(kids[2]) == [0, 1]
     with pytest.raises(ValueError):
         c.commit([kids[2]], [13])
+    step = paged.Step(*(torch.zeros(n, dtype=torch.int32) for n in ((1, 2), (1,), (2,))))
+    with pytest.raises(ValueError):
+        c.keep([kids[2]], step, [[0]])                 # not a step of the cache
+    step.rows = [2]
+    for rows in ([2], [1, 0], [0, 0], [-1]):
+        with pytest.raises(ValueError):
+            c.keep([kids[2]], step, [rows])
     with pytest.raises(ValueError):
         c.reserve([kids[2], kids[2]], [1, 1])
     for s in kids:
