@@ -28,8 +28,9 @@
 // attention.cuh. NT = 1: S and P have two buffers each, so scores, softmax and P.V of three
 // consecutive tiles overlap; Q has two, so the next unit's loads run under this one's end. NT = 2:
 // two row tiles share every K and V tile (attention.cuh's schedule).
-// P is rounded to bf16 for the tensor core (V's type): off by 2^-9 of each weight, as the rounding of
-// the output is; its row sum is taken in fp32 before that.
+// P is rounded to bf16 for the tensor core (V's type): each weight is off by a half step, 2^-8 of it at
+// most, and these errors are independent, so the result is off by about as much as its own rounding to
+// bf16; the row sum is taken in fp32 before that.
 //
 // Keys that a row does not see get score -inf. A weight of zero still meets its V row in the MMA, and
 // 0 * NaN is not zero: in the tiles that hold nodes of the step or the end of the keys, V rows behind
@@ -327,7 +328,7 @@ __device__ __forceinline__ void cache_visible(const CacheAttnArgs& args, const v
 }
 // Row r (key k0 + r) of columns 64 h0 .. of a V tile in shared memory, made safe for weights of zero: rows
 // behind the keys become zero, infinities and NaN of the step's own rows too. Returns whether there were any.
-__device__ __noinline__ bool cache_fix_v(uint8_t* tile, int r, int h0, int h1, bool behind) {
+__device__ __forceinline__ bool cache_fix_v(uint8_t* tile, int r, int h0, int h1, bool behind) {
     bool odd = false;
     for (int h = h0; h < h1; ++h) {
         uint4* vr = reinterpret_cast<uint4*>(tile + h * ATT_HALF_BYTES + r * 128);
@@ -356,6 +357,34 @@ __device__ __noinline__ bool cache_fix_v(uint8_t* tile, int r, int h0, int h1, b
         }
     }
     return odd;
+}
+
+// A tile of V that holds nodes of the step or the end of the keys, made safe by the softmax warps: each waits
+// for it, takes its rows (two row tiles half of the columns each), leaves in `odd` which had odd values, and
+// arrives on v_fixed. (`odd` is one of two sets: all warps pass v_fixed of a special tile before one writes the
+// next but one.)
+template <int D, int NT>
+__device__ __noinline__ bool cache_safe_v(uint8_t* tile, uint64_t* full, uint32_t parity, uint64_t* v_fixed, uint32_t* odd,
+                                          const volatile CacheUnit& u, int k0, int x, volatile uint32_t* abort_flag) {
+    if (!__all_sync(0xffffffffu, mbar_wait(full, parity, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE))) return false;
+    constexpr int HALVES = D / 64;
+    const int lane = threadIdx.x & 31, q4 = (threadIdx.x >> 5) & 3, r = q4 * 32 + lane, key = k0 + r;
+    const bool alone = NT == 1 || (u.flags & 8);
+    bool any = false;
+    if (key >= u.base || key >= u.keys)
+        any = cache_fix_v(tile, r, alone ? 0 : x, alone ? HALVES : min(x + 1, HALVES), key >= u.keys);
+    const uint32_t found = __ballot_sync(0xffffffffu, any);
+    fence_proxy_async_smem();
+    if (lane == 0) {
+        odd[x * 4 + q4] = found;
+        if (NT == 2 && alone) odd[4 + q4] = 0u;
+    }
+    __syncwarp();
+    if (lane == 0) {
+        mbar_arrive(v_fixed);
+        if (NT == 2 && alone) mbar_arrive(v_fixed);          // for row tile 1's warp
+    }
+    return true;
 }
 
 template <int D, int NT>
@@ -675,30 +704,13 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 if (lane == 0) w = mma_wait(&s_full[i2], n2 & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
                 if (!__shfl_sync(0xffffffffu, w, 0)) { ok = false; break; }
                 tc_fence_after();
+                // Only now, with the tile's scores: they were issued after the P.V of the tile two before, so V's
+                // ring stage has had its last turn and its barrier's parity says whether this one's is over.
                 if (special) {
-                    // Only now, with the tile's scores: they were issued after the P.V of the tile two before, so the
-                    // ring stage's last turn is over and its barrier's parity says whether this one's is. (Two sets
-                    // of odd_v: all warps pass v_fixed of a special tile before one writes the next but one.)
-                    const int vt = t + skipped, st = vt % S::VST;     // V's ring
-                    ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (vt / S::VST) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
+                    const int vt = t + skipped;
+                    ok = cache_safe_v<D, NT>(sv + vt % S::VST * S::TILE, &v_full[vt % S::VST], (vt / S::VST) & 1, v_fixed,
+                                             odd_v + (fixes & 1) * NT * 4, u, (u.j0 + t - t_first) * 128, x, abort_flag);
                     if (!ok) break;
-                    const int r = q4 * 32 + lane, key = (u.j0 + t - t_first) * 128 + r;
-                    const bool alone = NT == 1 || (u.flags & 8);       // two row tiles take half of the columns each
-                    bool odd = false;
-                    if (key >= u.base || key >= u.keys)
-                        odd = cache_fix_v(sv + st * S::TILE, r, alone ? 0 : x, alone ? S::HALVES : min(x + 1, S::HALVES),
-                                          key >= u.keys);
-                    const uint32_t found = __ballot_sync(0xffffffffu, odd);
-                    fence_proxy_async_smem();
-                    if (lane == 0) {
-                        odd_v[((fixes & 1) * NT + x) * 4 + q4] = found;
-                        if (NT == 2 && alone) odd_v[((fixes & 1) * NT + 1) * 4 + q4] = 0u;
-                    }
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(v_fixed);
-                        if (NT == 2 && alone) mbar_arrive(v_fixed);      // for row tile 1's warp
-                    }
                 }
                 bool moved = false;                                  // the running maximum of a row
                 float alpha = 1.f;
