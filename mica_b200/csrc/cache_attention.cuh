@@ -15,9 +15,9 @@
 // Work. A unit is (sequence, K/V head, block of NT * npt nodes); its key tiles of 128 follow one
 // another, units in order, in one line (where each unit has some places more for what it costs by
 // itself, and tiles that are shared by two row tiles count for more). Each of the CTAs (one per SM)
-// takes an equal run of that line, whatever the lengths: it starts and may end inside a unit. A unit that one CTA has whole
-// is written out; of a divided one each CTA leaves its unnormalised rows, maxima and sums in its own
-// place of the workspace (a CTA has at most two such: its first and its last), and
+// takes an equal run of that line, whatever the lengths: it starts and may end inside a unit. A unit
+// that one CTA has whole is written out; of a divided one each CTA leaves its unnormalised rows, maxima
+// and sums in its own place of the workspace (a CTA has at most two such: its first and its last), and
 // cache_attention_join adds them up in the order of the CTAs. No atomics: the same bits every time.
 // The lengths are read on the device, so a captured graph serves any.
 //
@@ -36,6 +36,12 @@
 // 0 * NaN is not zero: in the tiles that hold nodes of the step or the end of the keys, V rows behind
 // the end are zeroed in shared memory, and an infinite or NaN element of a node's V is replaced by
 // zero and added to the accumulators of the rows that see it, no others.
+//
+// Measured (32 heads over 8, D = 128, cold L2): 13 and 15 tokens over 70761 and 87495 keys 129 us, the key
+// tiles among them at the memory's 6.5 TB/s (1.5 us a tile and SM); 16 trees of up to 64 nodes over up
+// to 9000 keys 93 us, 2.1 us a tile of two row tiles (softmax and the one score buffer, as in
+// attention.cuh); 700 nodes over 20000 keys 220 us, 1.05 PFLOP/s; one token over up to 700 keys 10 us from
+// the first CTA's start to the join's end.
 #pragma once
 
 #include "attention.cuh"

@@ -10,15 +10,19 @@
 // Bound by the logits' bytes, which are read once: the maximum, S and the entropy's sum run along in
 // one pass (rescaled when the maximum grows), in base 2 and fp32. A row is one cluster of CTAs, each
 // with a run of it; a cluster takes row after row. In a CTA one warp keeps bulk copies of the coming
-// logits in flight through a ring in shared memory, 24 warps make the pass, and 4 warps finish the
-// row before while the pass goes on with the next. The parts of a row meet in the first CTA's
+// logits in flight through a ring in shared memory, 20 warps make the pass, and two groups of 4
+// warps finish rows in turn while the pass goes on with the next. The parts of a row meet in the first CTA's
 // shared memory: one launch, no workspace.
 //
 // Alternatives without a list in the pass: a thread keeps only the largest logit it has seen. The
 // maxima of 64 groups of threads are of disjoint elements, so the top-th largest of them is a lower
 // bound of the run's top-th largest logit; only threads whose maximum reaches it can hold an
-// alternative (about 25 of 768 for 20 alternatives of random logits), and their vectors are read
+// alternative (about 25 of 640 for 20 alternatives of random logits), and their vectors are read
 // again, from L2, and elements that reach the bound kept. Warps sort them 32 at a time and merge.
+//
+// Measured (cold L2): 1025 rows of 151936 bf16, top 20, 76 us, 65 of them with warm instruction and data
+// caches (4.8 TB/s; without alternatives 69, fp32 112 us = 5.6 TB/s); 6 rows of 151936 fp32, top 8, 16 us
+// of which 8 are a launch. One CTA a row with a pass for each alternative took 6269 us.
 #pragma once
 
 #include "quant.cuh"
