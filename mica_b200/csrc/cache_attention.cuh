@@ -33,9 +33,10 @@
 // bf16; the row sum is taken in fp32 before that.
 //
 // Keys that a row does not see get score -inf. A weight of zero still meets its V row in the MMA, and
-// 0 * NaN is not zero: in the tiles that hold nodes of the step or the end of the keys, V rows behind
-// the end are zeroed in shared memory, and an infinite or NaN element of a node's V is replaced by
-// zero and added to the accumulators of the rows that see it, no others.
+// 0 * NaN is not zero: in the tiles that some row of the unit does not see all of (they hold nodes of
+// the step, or the end of the keys), V rows behind the end are zeroed in shared memory, and an infinite
+// or NaN element of a node's V is replaced by zero and added to the accumulators of the rows that see
+// it, no others.
 //
 // Measured (32 heads over 8, D = 128, cold L2): 13 and 15 tokens over 70761 and 87495 keys 129 us, the key
 // tiles among them at the memory's 6.5 TB/s (1.5 us a tile and SM); 16 trees of up to 64 nodes over up
@@ -269,6 +270,7 @@ struct CacheWalk {
 struct CacheUnit {
     int b, kvh, row0, node0, nodes;     // row0: global row of its first node (node0 of its sequence)
     int base, keys, j0, j1;
+    int special;                        // the first tile that some row does not see all of, or that ends the keys
     int flags;                          // 1: the run's last unit, 2: all of the unit's tiles, 4: the run's first unit,
                                         // 8: its nodes fill one row tile at most
 };
@@ -511,6 +513,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                         volatile CacheUnit& u = units[slot];
                         u.b = wk.b; u.kvh = wk.kvh; u.row0 = wk.s.row0 + node0; u.node0 = node0; u.nodes = min(R, wk.s.T - node0);
                         u.base = wk.s.base; u.keys = wk.s.keys; u.j0 = wk.j0; u.j1 = wk.j1;
+                        // every row sees the committed tokens, and without a mask what the first row sees
+                        u.special = wk.s.keys ? min(wk.s.keys, wk.s.base + (causal ? node0 + 1 : 0)) >> 7 : 0;
                         const int all = wk.whole() ? 2 : 0;
                         u.flags = (wk.next(plan, args.KV) ? 0 : 1) | all | (unit == 0 ? 4 : 0) | (u.nodes <= args.npt ? 8 : 0);
                         mbar_arrive(&unit_full[slot]);
@@ -625,7 +629,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 const volatile CacheUnit& u = units[unit % CACHE_UNITS];
                 const int n = u.j1 - u.j0;
                 // the first tile starts the accumulator, except where the softmax has set it
-                bool fresh = !((u.j0 + 1) * 128 > u.base || u.keys == 0);
+                bool fresh = u.j0 < u.special;
                 last = u.flags & 1;
                 const auto tiles = [&](auto two) {
                     constexpr bool both = decltype(two)::value;
@@ -691,9 +695,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             const volatile CacheUnit& u = units[unit % CACHE_UNITS];
             last = u.flags & 1;
             const bool warp_live = q4 * 32 < (u.nodes - x * args.npt) * args.G;   // some thread of the warp has a row
-            // tiles from `t_special` on hold nodes of the step, or the end of the keys
-            const int t_first = t, t_end = t + u.j1 - u.j0;
-            const int t_special = u.keys ? max(t, t + (u.base >> 7) - u.j0) : t;
+            const int t_first = t, t_end = t + u.j1 - u.j0, t_special = max(t, t + u.special - u.j0);
             if (NT == 2 && x == 1 && (u.flags & 8)) {                 // no rows: row tile 0 goes on alone
                 skipped += t_end - t_first;
                 fixes += max(0, t_end - t_special);
@@ -905,63 +907,82 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     cache_zero_padding(args, D);
 }
 
-// Adds up the parts of each divided unit, in the order of the CTAs. Block (c, y): the unit that CTA
-// c + 1 is the first to start inside, if it is; a thread takes 16 columns of a row, three parts in
-// flight (a long sequence's unit is in ten and more).
+// Adds up the parts of each divided unit, always in the same order. Blocks (c, y): the unit that CTA c + 1 is
+// the first to start inside, if it is. A thread takes 16 columns of a row, three parts in flight; where a
+// long sequence's unit is in many parts, `lanes` neighbouring threads take every lanes-th part each and add
+// theirs up (one sequence of 100000 keys and one K/V head is in 148: 35 us one part after the other).
 template <int D, int NT>
 __global__ void __launch_bounds__(128) cache_attention_join(const CacheAttnArgs args) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int AHEAD = 3;
     const int c = blockIdx.x + 1;
     const int4 cut = args.cuts[2 * c];
-    const int rows = cut.x, n = cut.w;
-    const int idx = blockIdx.y * blockDim.x + threadIdx.x;
-    if (idx >= rows * (D / 16)) return;
+    const int rows = cut.x, n = cut.w, items = rows * (D / 16);
+    if (items == 0) return;
+    const int lanes = n < 2 * AHEAD ? 1 : n < 8 * AHEAD ? 4 : 16;
     const int first_place = args.cuts[2 * (c - 1) + 1].x;            // of the part that the CTA before left last
     const long pf = cache_attn_place_floats<D, NT>();
-    const int rr = idx % rows, d16 = idx / rows;
-    const int node = rr / args.G, g = rr - node * args.G;
-    const int x = NT == 1 ? 0 : node / args.npt, r = (node - x * args.npt) * args.G + g;
     const float* part0 = args.ws + ((c - 1) * 2l + first_place) * pf;
     const float* parts = args.ws + c * 2l * pf;
-    float m = -INFINITY, l = 0.f;
-    float4 o[4];
+    const int mine = threadIdx.x % lanes, groups = gridDim.y * blockDim.x / lanes;
+    // whole warps go round together: an item behind the last is the last once more, not written
+    for (int i0 = (blockIdx.y * blockDim.x + (threadIdx.x & ~31)) / lanes; i0 < items; i0 += groups) {
+        const int item = i0 + (threadIdx.x & 31) / lanes, idx = min(item, items - 1);
+        const int rr = idx % rows, d16 = idx / rows;
+        const int node = rr / args.G, g = rr - node * args.G;
+        const int x = NT == 1 ? 0 : node / args.npt, r = (node - x * args.npt) * args.G + g;
+        float m = -INFINITY, l = 0.f;
+        float4 o[4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 <= n; i0 += AHEAD) {
-        float2 ml[AHEAD];
-        float4 p[AHEAD][4];
+        for (int v = 0; v < 4; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p0 = mine; p0 <= n; p0 += AHEAD * lanes) {
+            float2 ml[AHEAD];
+            float4 p[AHEAD][4];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int i = i0 + u;
-            if (i > n) continue;
-            const float* a = i == 0 ? part0 : parts + (i - 1) * 2l * pf;
-            ml[u] = __ldcg(reinterpret_cast<const float2*>(a + NT * 128l * D) + x * 128 + r);
+            for (int u = 0; u < AHEAD; ++u) {
+                const int i = p0 + u * lanes;
+                if (i > n) continue;
+                const float* a = i == 0 ? part0 : parts + (i - 1) * 2l * pf;
+                ml[u] = __ldcg(reinterpret_cast<const float2*>(a + NT * 128l * D) + x * 128 + r);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) p[u][v] = __ldcg(reinterpret_cast<const float4*>(a) + (x * (D / 4) + d16 * 4 + v) * 128 + r);
-        }
+                for (int v = 0; v < 4; ++v) p[u][v] = __ldcg(reinterpret_cast<const float4*>(a) + (x * (D / 4) + d16 * 4 + v) * 128 + r);
+            }
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            if (i0 + u > n) continue;
-            const float mn = fmaxf(m, ml[u].x), wo = fast_exp2(m - mn), w = fast_exp2(ml[u].x - mn);
-            m = mn;
-            l = fmaf(ml[u].y, w, l * wo);
+            for (int u = 0; u < AHEAD; ++u) {
+                if (p0 + u * lanes > n) continue;
+                const float mn = fmaxf(m, ml[u].x), wo = fast_exp2(m - mn), w = fast_exp2(ml[u].x - mn);
+                m = mn;
+                l = fmaf(ml[u].y, w, l * wo);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                o[v].x = fmaf(p[u][v].x, w, o[v].x * wo);
-                o[v].y = fmaf(p[u][v].y, w, o[v].y * wo);
-                o[v].z = fmaf(p[u][v].z, w, o[v].z * wo);
-                o[v].w = fmaf(p[u][v].w, w, o[v].w * wo);
+                for (int v = 0; v < 4; ++v) {
+                    o[v].x = fmaf(p[u][v].x, w, o[v].x * wo);
+                    o[v].y = fmaf(p[u][v].y, w, o[v].y * wo);
+                    o[v].z = fmaf(p[u][v].z, w, o[v].z * wo);
+                    o[v].w = fmaf(p[u][v].w, w, o[v].w * wo);
+                }
             }
         }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const long row = static_cast<long>(cut.y) + node;
-    uint4* to = reinterpret_cast<uint4*>(args.out + row * args.ldo + (cut.z * args.G + g) * D + d16 * 16);
+        for (int s = 1; s < lanes; s <<= 1) {
+            const float mo = __shfl_xor_sync(0xffffffffu, m, s), mn = fmaxf(m, mo);
+            const float w = m == -INFINITY ? 0.f : fast_exp2(m - mn);                  // -inf: no part
+            const auto add = [&](float f) {
+                f = m == -INFINITY ? 0.f : f * w;
+                return f + __shfl_xor_sync(0xffffffffu, f, s);
+            };
+            l = add(l);
 #pragma unroll
-    for (int v = 0; v < 4; v += 2)
-        to[v / 2] = make_uint4(pack_bf16(o[v].x * inv, o[v].y * inv), pack_bf16(o[v].z * inv, o[v].w * inv),
-                               pack_bf16(o[v + 1].x * inv, o[v + 1].y * inv), pack_bf16(o[v + 1].z * inv, o[v + 1].w * inv));
+            for (int v = 0; v < 4; ++v) o[v] = make_float4(add(o[v].x), add(o[v].y), add(o[v].z), add(o[v].w));
+            m = mn;
+        }
+        if (mine || item >= items) continue;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const long row = static_cast<long>(cut.y) + node;
+        uint4* to = reinterpret_cast<uint4*>(args.out + row * args.ldo + (cut.z * args.G + g) * D + d16 * 16);
+#pragma unroll
+        for (int v = 0; v < 4; v += 2)
+            to[v / 2] = make_uint4(pack_bf16(o[v].x * inv, o[v].y * inv), pack_bf16(o[v].z * inv, o[v].w * inv),
+                                   pack_bf16(o[v + 1].x * inv, o[v + 1].y * inv), pack_bf16(o[v + 1].z * inv, o[v + 1].w * inv));
+    }
 }
 
 }  // namespace mica

@@ -66,6 +66,31 @@ def test_attention_long_axes(ctx, new):
     check_attention(c, run_attention(c, max_new=max(new)))
 
 
+@pytest.mark.parametrize('heads,new', [(1, 1), (5, 1), (5, 60), (4, 7)])
+def test_attention_of_one_unit_in_many_parts(heads, new):
+    """One K/V head and a long context: its one unit is cut into a part for each SM (and with few keys into
+    some), which several threads join."""
+    for ctx in (128 * 148 * 2 + 17, 128 * 20, 128 * 9, 128 * 5, 128 * 3 + 1):
+        c = Case([ctx], [new], heads, 1, 128, 128, seed=ctx + new, mask=tree)
+        o = run_attention(c, max_new=new)
+        check_attention(c, o)
+        assert torch.equal(o, run_attention(c, max_new=new))
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+def test_odd_values_in_a_causal_extension(bad):
+    """Without a mask, rows do not see later rows' K and V: an odd value there changes nothing before its row."""
+    c = Case([90, 0], [300, 200], 8, 2, 128, 32, seed=11)
+    clean = run_attention(c)
+    for b, at in ((0, 170), (1, 30)):
+        s = c.ctx[b] + at
+        c.v[c.rows[b][s // 32], :, s % 32] = bad
+        c.k[c.rows[b][s // 32], :, s % 32] = bad
+    o = run_attention(c)
+    assert torch.equal(o[:170], clean[:170]) and torch.equal(o[300:330], clean[300:330])
+    assert not torch.isfinite(o[170:300]).any(1).all() and not torch.isfinite(o[330:]).any(1).all()
+
+
 def test_attention_many_sequences():
     ctx = [(i * 37) % 211 for i in range(500)]
     c = Case(ctx, [1 + i % 3 for i in range(500)], 4, 2, 64, 16, seed=2)
