@@ -61,6 +61,7 @@ struct CacheAttnArgs {
     long ldo;
     int KV, G;                  // K/V heads, query heads of each
     int npt;                    // nodes of a row tile: npt * G <= 128
+    int copies;                 // of the rows in a row tile: 4, 2 or 1 (npt * G <= 128 / copies; NT 1)
     int ctas;                   // CTAs of the grid
     float scale_log2;           // scale * log2(e)
     float* ws;                  // partials: [ctas][2] places
@@ -284,8 +285,10 @@ struct CacheAttnShape {
     static constexpr int KST = D == 128 ? 3 : 6;
     static constexpr int VST = D == 128 ? 2 : 5;
     static constexpr int THREADS = 128 + 128 * NT;
-    static constexpr int BARS = 768;
-    static constexpr int SMEM = 1024 + TILE * (QBUF * NT + KST + VST) + BARS;
+    static constexpr int BARS = D == 128 ? 576 : 672;                     // barriers and units
+    static constexpr int STATS = NT == 1 ? 128 * 8 : 0;                  // the copies' (max, sum)
+    static constexpr int SMEM = 1024 + TILE * (QBUF * NT + KST + VST) + BARS + STATS;
+    static_assert((4 + 2 * KST + 2 * VST + 8 + 1 + CACHE_UNITS + 2) * 8 + 8 + 64 + CACHE_UNITS * sizeof(CacheUnit) <= BARS, "BARS");
 };
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
@@ -395,10 +398,45 @@ __device__ __noinline__ bool cache_safe_v(uint8_t* tile, uint64_t* full, uint32_
     return true;
 }
 
+// Copies of the rows meet the keys of one another with weights of zero, and 0 * infinity is NaN: a sum that is
+// not finite is set to what the infinities and NaN among the V that its row sees in this CTA's tiles make of it.
+// Three bits for each of 8 columns from `col`: NaN, infinity, -infinity. The whole warp calls it; mend: this
+// thread's row is asked for.
+template <int D>
+__device__ __noinline__ uint32_t cache_odd_kinds(const CacheAttnArgs& args, const volatile CacheUnit& u, int node_r, int col,
+                                                 bool mend) {
+    const CachePlan& plan = args.plan;
+    const int lane = threadIdx.x & 31, b = u.b, special = u.special;
+    const auto kinds = [&](int key) {
+        int page = 0, slot = 0;
+        if (!cache_slot(plan, b, key, &page, &slot)) return 0u;
+        const uint16_t* v = reinterpret_cast<const uint16_t*>(args.v_pages) + page * args.page_stride +
+                            ((static_cast<long>(u.kvh) << plan.page_log2) + slot) * D + col;
+        uint32_t k = 0u;
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t bits = v[e];
+            if ((bits & 0x7f80u) == 0x7f80u) k |= (bits & 0x7fu ? 1u : bits & 0x8000u ? 4u : 2u) << (3 * e);
+        }
+        return k;
+    };
+    uint32_t k = 0u;
+    for (int key = u.j0 * 128 + lane; key < min(u.j1, special) * 128; key += 32) k |= kinds(key);    // all rows see these
+    k = __reduce_or_sync(0xffffffffu, k);
+    for (int j = max(u.j0, special); mend && j < u.j1; ++j) {
+        uint32_t vis[4];
+        cache_visible(args, u, 0, node_r, j * 128, vis);
+        for (int i = 0; i < 128; ++i) {
+            const uint32_t seen = i < 64 ? (i < 32 ? vis[0] : vis[1]) : (i < 96 ? vis[2] : vis[3]);
+            if (seen >> (i & 31) & 1u) k |= kinds(j * 128 + i);
+        }
+    }
+    return mend ? k : 0u;
+}
+
 template <int D, int NT>
 __global__ void __launch_bounds__(CacheAttnShape<D, NT>::THREADS, 1)
 cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                       const __grid_constant__ CUtensorMap tmap_v, const CacheAttnArgs args) {
+                       const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CacheAttnArgs args) {
     using S = CacheAttnShape<D, NT>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const CachePlan& plan = args.plan;
@@ -443,15 +481,18 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     uint64_t* v_fixed = pv_done + 2;           // V of a special tile made safe (all softmax warps)
     uint64_t* unit_full = v_fixed + 1;         // [CACHE_UNITS]
     uint64_t* drain = unit_full + CACHE_UNITS;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* exchange = drain + 1;            // between the softmax warps at a unit's end (copies)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(exchange + 1);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     uint32_t* odd_v = tmem_slot + 2;           // [2][NT][4] keys of a special tile whose V row holds infinities or NaN
     volatile CacheUnit* units = reinterpret_cast<volatile CacheUnit*>(odd_v + 16);
+    float2* stats = reinterpret_cast<float2*>(sv + S::VST * S::TILE + S::BARS);
+    const int copies = NT == 1 ? args.copies : 1;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 1);
-            mbar_init(&q_empty[i], 1);
+            mbar_init(&q_empty[i], copies > 1 ? 5 : 1);       // the softmax warps add the copies up in it
             mbar_init(&s_full[i], 1);
             mbar_init(&s_free[i], 4);
             mbar_init(&p_full[i], 4);
@@ -462,6 +503,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         mbar_init(v_fixed, 4 * NT);
         for (int i = 0; i < CACHE_UNITS; ++i) mbar_init(&unit_full[i], 1);
         mbar_init(drain, 1);
+        mbar_init(exchange, 4);
         *abort_flag = 0u;
         fence_mbar_init();
     }
@@ -505,11 +547,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     if (w) {
                         if (wk.s.keys == 0) record_bad_page();
                         const int node0 = wk.rb * R;
-                        mbar_arrive_expect_tx(&q_full[qb], NT * S::HALVES * 128u * args.npt * args.G);
-                        for (int x = 0; x < NT; ++x)
+                        mbar_arrive_expect_tx(&q_full[qb], NT * copies * S::HALVES * 128u * args.npt * args.G);
+                        for (int x = 0; x < NT * copies; ++x)        // one of the two is 1
                             for (int h = 0; h < S::HALVES; ++h)
-                                tma_load_3d(sq + (qb * NT + x) * S::TILE + h * ATT_HALF_BYTES, &tmap_q, &q_full[qb], h * 64,
-                                            wk.kvh * args.G, wk.s.row0 + node0 + x * args.npt);
+                                tma_load_3d(NT == 1 ? sq + qb * S::TILE + h * ATT_HALF_BYTES + x * (ATT_HALF_BYTES / copies)
+                                                    : sq + x * S::TILE + h * ATT_HALF_BYTES, &tmap_q, &q_full[qb], h * 64,
+                                            wk.kvh * args.G, wk.s.row0 + node0 + (NT == 1 ? 0 : x) * args.npt);
                         volatile CacheUnit& u = units[slot];
                         u.b = wk.b; u.kvh = wk.kvh; u.row0 = wk.s.row0 + node0; u.node0 = node0; u.nodes = min(R, wk.s.T - node0);
                         u.base = wk.s.base; u.keys = wk.s.keys; u.j0 = wk.j0; u.j1 = wk.j1;
@@ -684,7 +727,19 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         const int q4 = warp & 3;                           // tensor-memory lane quarter
         const uint32_t lane_off = static_cast<uint32_t>(q4 * 32) << 16;
         const float c = args.scale_log2;
+        // with copies, copy `cp` of the rows has a part of each tile's keys: this warp's row and its first key
+        const int cp = copies == 4 ? q4 : copies == 2 ? q4 >> 1 : 0, keys_each = 128 / copies;
+        const int r = q4 * 32 + lane - cp * keys_each, key0 = cp * keys_each;
+        if (NT == 1 && copies > 1) {                       // the weights of the other parts stay zero
+            uint32_t zero[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) zero[i] = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tmem_st_32x32b_x32(tmem + col_p(0) + i * 32 + lane_off, zero);
+            tmem_st_wait();
+        }
         bool ok = true, last = false;
+        int phases = 0;                                    // of `exchange`
         int t = 0, unit = 0;                               // this row tile's key tiles so far, units
         int skipped = 0;                                   // and those of units it had no rows in
         int fixes = 0;                                     // special tiles so far
@@ -694,13 +749,15 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             if (!ok) break;
             const volatile CacheUnit& u = units[unit % CACHE_UNITS];
             last = u.flags & 1;
-            const bool warp_live = q4 * 32 < (u.nodes - x * args.npt) * args.G;   // some thread of the warp has a row
+            const bool warp_live = r - lane < (u.nodes - x * args.npt) * args.G;   // some thread of the warp has a row
             const int t_first = t, t_end = t + u.j1 - u.j0, t_special = max(t, t + u.special - u.j0);
             if (NT == 2 && x == 1 && (u.flags & 8)) {                 // no rows: row tile 0 goes on alone
                 skipped += t_end - t_first;
                 fixes += max(0, t_end - t_special);
                 continue;
             }
+            const int node_r = r / args.G, head_r = r - node_r * args.G;
+            const bool live = node_r < min(args.npt, u.nodes - x * args.npt);             // this thread has a row
             const uint32_t t_o = tmem + col_o(x) + lane_off;
             float m_use = -1e30f, l = 0.f;
             for (; t < t_end; ++t) {
@@ -708,9 +765,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 const int n2 = NT == 1 ? t >> 1 : t;                   // uses of that buffer before
                 const uint32_t t_s = tmem + col_s(i2) + lane_off, t_p = tmem + col_p(i2) + lane_off;
                 const bool special = t >= t_special;
-                bool w = true;
-                if (lane == 0) w = mma_wait(&s_full[i2], n2 & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
-                if (!__shfl_sync(0xffffffffu, w, 0)) { ok = false; break; }
+                ok = __all_sync(0xffffffffu, mma_wait(&s_full[i2], n2 & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
+                if (!ok) break;
                 tc_fence_after();
                 // Only now, with the tile's scores: they were issued after the P.V of the tile two before, so V's
                 // ring stage has had its last turn and its barrier's parity says whether this one's is over.
@@ -723,20 +779,22 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 bool moved = false;                                  // the running maximum of a row
                 float alpha = 1.f;
                 uint32_t pk[64];
-                if (warp_live) {
-                    uint32_t sr[128];
+                // keys key0 .. of the tile, 32 W of them: weights into pk, row maximum and sum
+                const auto weights = [&](auto part) {
+                    constexpr int W = decltype(part)::value;
+                    uint32_t sr[32 * W];
 #pragma unroll
-                    for (int cc = 0; cc < 4; ++cc)
-                        tmem_ld_32x32b_x32(t_s + cc * 32, *reinterpret_cast<uint32_t (*)[32]>(&sr[cc * 32]));
+                    for (int cc = 0; cc < W; ++cc)
+                        tmem_ld_32x32b_x32(t_s + key0 + cc * 32, *reinterpret_cast<uint32_t (*)[32]>(&sr[cc * 32]));
                     tmem_ld_wait();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s_free[NT == 1 ? i2 : 0]);
                     if (special) {
                         uint32_t vis[4];
-                        cache_visible(args, u, x, (q4 * 32 + lane) / args.G, (u.j0 + t - t_first) * 128, vis);
+                        cache_visible(args, u, x, node_r, (u.j0 + t - t_first) * 128 + key0, vis);
 #pragma unroll
-                        for (int i = 0; i < 128; ++i)
+                        for (int i = 0; i < 32 * W; ++i)
                             if (!(vis[i >> 5] >> (i & 31) & 1u)) sr[i] = 0xff800000u;
                     }
                     float mp[8];
@@ -744,21 +802,21 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     for (int e = 0; e < 8; ++e)
                         mp[e] = fmax3(__uint_as_float(sr[e]), __uint_as_float(sr[8 + e]), __uint_as_float(sr[16 + e]));
 #pragma unroll
-                    for (int i = 24; i < 128; i += 16)
+                    for (int i = 24; i < 32 * W; i += 16)
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            mp[e] = i + 8 + e < 128 ? fmax3(mp[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 8 + e]))
-                                                    : fmaxf(mp[e], __uint_as_float(sr[i + e]));
+                            mp[e] = i + 8 + e < 32 * W ? fmax3(mp[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 8 + e]))
+                                                       : fmaxf(mp[e], __uint_as_float(sr[i + e]));
                     const float mx = fmax3(fmax3(mp[0], mp[1], mp[2]), fmax3(mp[3], mp[4], mp[5]), fmaxf(mp[6], mp[7])) * c;
                     if (mx > m_use + ATT_RESCALE_LOG2) {
                         alpha = fast_exp2(m_use - mx);
                         m_use = mx;
-                        moved = true;
+                        moved = live;                // what a thread without a row reads and adds up is nobody's
                     }
                     const unsigned long long c2 = f2_pack(c, c), nm2 = f2_pack(-m_use, -m_use);
                     unsigned long long sp[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) {
+                    for (int i = 0; i < 16 * W; ++i) {
                         const unsigned long long x2 =
                             f2_fma(f2_pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), c2, nm2);
                         float x0, x1;
@@ -773,6 +831,11 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     f2_unpack(sp[2], d0, d1);
                     f2_unpack(sp[3], e0, e1);
                     l = l * alpha + (((a0 + a1) + (b0 + b1)) + ((d0 + d1) + (e0 + e1)));
+                };
+                if (warp_live) {
+                    if (NT == 2 || copies == 1) weights(std::integral_constant<int, 4>());
+                    else if (copies == 2) weights(std::integral_constant<int, 2>());
+                    else weights(std::integral_constant<int, 1>());
                 } else {
                     if (lane == 0) mbar_arrive(&s_free[NT == 1 ? i2 : 0]);
                 }
@@ -790,13 +853,13 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 const bool fresh = t == t_first;
                 const bool touch = warp_live && (special && fresh || any_odd ||
                                                  (!fresh && __any_sync(0xffffffffu, moved)));
-                if (lane == 0) {
-                    w = n2 == 0 || mma_wait(&pv_done[i2], (n2 - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
-                    if (NT == 1 && w && touch && t >= 1)
-                        w = mma_wait(&pv_done[i2 ^ 1], ((t - 1) >> 1) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
-                }
-                if (!__shfl_sync(0xffffffffu, w, 0)) { ok = false; break; }
-                tc_fence_after();
+                // NT 1: the scores were issued after the P.V of the tile two before, and are there
+                if (NT == 2 && n2 > 0)
+                    ok = __all_sync(0xffffffffu, mma_wait(&pv_done[i2], (n2 - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
+                if (NT == 1 && touch && t >= 1)
+                    ok = __all_sync(0xffffffffu, mma_wait(&pv_done[i2 ^ 1], ((t - 1) >> 1) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
+                if (!ok) break;
+                if (NT == 2 || touch) tc_fence_after();
                 if (touch) {
 #pragma unroll 1
                     for (int cc = 0; cc < D / 32; ++cc) {
@@ -814,9 +877,9 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                             const volatile uint32_t* odd4 = odd_v + (~fixes & 1) * 4 * NT;      // counted already
                             const int k0 = (u.j0 + t - t_first) * 128;
                             uint32_t vis[4];
-                            cache_visible(args, u, x, (q4 * 32 + lane) / args.G, k0, vis);
+                            cache_visible(args, u, x, node_r, k0, vis);
 #pragma unroll 1
-                            for (int i = 0; i < 128; ++i) {
+                            for (int i = key0; i < key0 + keys_each; ++i) {
                                 const uint32_t bit = 1u << (i & 31);
                                 const uint32_t seen = i < 64 ? (i < 32 ? vis[0] : vis[1]) : (i < 96 ? vis[2] : vis[3]);
                                 int pgn = 0, slot = 0;
@@ -837,8 +900,13 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     }
                 }
                 if (warp_live) {
-                    tmem_st_32x32b_x32(t_p, *reinterpret_cast<uint32_t (*)[32]>(&pk[0]));
-                    tmem_st_32x32b_x32(t_p + 32, *reinterpret_cast<uint32_t (*)[32]>(&pk[32]));
+                    if (NT == 1 && copies == 4) {
+                        tmem_st_32x32b_x16(t_p + key0 / 2, *reinterpret_cast<uint32_t (*)[16]>(&pk[0]));
+                    } else {
+                        tmem_st_32x32b_x32(t_p + key0 / 2, *reinterpret_cast<uint32_t (*)[32]>(&pk[0]));
+                        if (NT == 2 || copies == 1)
+                            tmem_st_32x32b_x32(t_p + 32, *reinterpret_cast<uint32_t (*)[32]>(&pk[32]));
+                    }
                     tmem_st_wait();
                 }
                 tc_fence_before();
@@ -855,16 +923,87 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 if (lane == 0) w = mbar_wait(&pv_done[i2], n2 & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
                 if (!__shfl_sync(0xffffffffu, w, 0)) { ok = false; break; }
                 tc_fence_after();
-                if (warp_live) {
-                    const bool whole = u.flags & 2;
-                    const int kvh = u.kvh, place = u.flags & 4 ? 0 : 1;
-                    const int r = q4 * 32 + lane, node_r = r / args.G, head_r = r - node_r * args.G;   // row of the tile
-                    const bool live = node_r < min(args.npt, u.nodes - x * args.npt);                // it is one
-                    const long row = static_cast<long>(u.row0) + x * args.npt + node_r;
+                const bool whole = u.flags & 2;
+                const long row = static_cast<long>(u.row0) + x * args.npt + node_r;
+                float* place = args.ws + (cta * 2l + (u.flags & 4 ? 0 : 1)) * cache_attn_place_floats<D, NT>();
+                float4* part = reinterpret_cast<float4*>(place) + x * (D / 4) * 128 + r;
+                float2* part_ml = reinterpret_cast<float2*>(place + NT * 128l * D) + x * 128 + r;
+                __nv_bfloat16* orow = args.out + row * args.ldo + (u.kvh * args.G + head_r) * D;
+                if (NT == 1 && copies > 1) {
+                    // the copies' rows, brought to one maximum and added up through the unit's Q buffer, half
+                    // of the columns at a time: each warp adds up a part of them
+                    const auto meet = [&]() {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(exchange);
+                        return __all_sync(0xffffffffu, mbar_wait(exchange, phases++ & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
+                    };
+                    float4* xo = reinterpret_cast<float4*>(sq + (unit & 1) * S::TILE) + r;    // [copy][D / 8][row]
+                    stats[q4 * 32 + lane] = make_float2(m_use, l);
+                    if (!meet()) { ok = false; break; }
+                    float m_all = m_use, l_all = 0.f;
+                    for (int i = 0; i < copies; ++i) m_all = fmaxf(m_all, stats[i * keys_each + r].x);
+                    for (int i = 0; i < copies; ++i) {
+                        const float2 ml = stats[i * keys_each + r];
+                        l_all = fmaf(ml.y, fast_exp2(ml.x - m_all), l_all);
+                    }
+                    const float mine = fast_exp2(m_use - m_all), inv = l_all == 0.f ? 0.f : 1.f / l_all;
+                    for (int pass = 0; pass < 2; ++pass) {
+                        if (pass && !meet()) { ok = false; break; }
+                        if (warp_live) {
+#pragma unroll
+                            for (int cc = 0; cc < D / 64; ++cc) {
+                                uint32_t o[32];
+                                tmem_ld_32x32b_x32(t_o + pass * (D / 2) + cc * 32, o);
+                                tmem_ld_wait();
+                                if (live) {
+#pragma unroll
+                                    for (int v = 0; v < 8; ++v)
+                                        xo[(cp * (D / 8) + cc * 8 + v) * keys_each] =
+                                            make_float4(__uint_as_float(o[4 * v]) * mine, __uint_as_float(o[4 * v + 1]) * mine,
+                                                        __uint_as_float(o[4 * v + 2]) * mine, __uint_as_float(o[4 * v + 3]) * mine);
+                                }
+                            }
+                        }
+                        if (!meet()) { ok = false; break; }
+                        const int each = D / 8 / copies;
+                        for (int v = cp * each; warp_live && v < (cp + 1) * each; v += 2) {
+                            float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                            for (int i = 0; live && i < copies; ++i) {
+                                const float4 a = xo[(i * (D / 8) + v) * keys_each], b = xo[(i * (D / 8) + v + 1) * keys_each];
+                                o[0] += a.x; o[1] += a.y; o[2] += a.z; o[3] += a.w;
+                                o[4] += b.x; o[5] += b.y; o[6] += b.z; o[7] += b.w;
+                            }
+                            const int col = pass * (D / 2) + v * 4;
+                            float zero = 0.f;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) zero = fmaf(o[e], 0.f, zero);
+                            const bool odd = zero != 0.f && l_all * 0.f == 0.f;       // infinite or NaN scores stay
+                            if (__any_sync(0xffffffffu, odd)) {
+                                const uint32_t kinds = cache_odd_kinds<D>(args, u, node_r, col, odd);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const uint32_t n = kinds >> (3 * e) & 7u;
+                                    if (n) o[e] = __uint_as_float(n & 1u || n == 6u ? 0x7fffffffu : n == 2u ? 0x7f800000u : 0xff800000u);
+                                }
+                            }
+                            if (live && whole)
+                                *reinterpret_cast<uint4*>(orow + col) =
+                                    make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv),
+                                               pack_bf16(o[4] * inv, o[5] * inv), pack_bf16(o[6] * inv, o[7] * inv));
+                            else if (live) {
+                                part[col / 4 * 128] = make_float4(o[0], o[1], o[2], o[3]);
+                                part[(col / 4 + 1) * 128] = make_float4(o[4], o[5], o[6], o[7]);
+                            }
+                        }
+                    }
+                    if (!ok) break;
+                    if (live && !whole && cp == 0) *part_ml = make_float2(m_all, l_all);
+                    fence_proxy_async_smem();                        // Q of the next unit but one comes here
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&q_empty[unit & 1]);
+                } else if (warp_live) {
                     const float inv = l == 0.f ? 0.f : 1.f / l;
-                    float4* part = reinterpret_cast<float4*>(args.ws + (cta * 2l + place) * cache_attn_place_floats<D, NT>()) +
-                                   x * (D / 4) * 128 + r;
-                    __nv_bfloat16* orow = args.out + row * args.ldo + (kvh * args.G + head_r) * D;
 #pragma unroll
                     for (int cc = 0; cc < D / 32; ++cc) {
                         uint32_t o[32];
@@ -887,11 +1026,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                                                                        __uint_as_float(o[4 * v + 2]), __uint_as_float(o[4 * v + 3]));
                         }
                     }
-                    if (live && !whole) {
-                        float2* ml = reinterpret_cast<float2*>(args.ws + (cta * 2l + place) * cache_attn_place_floats<D, NT>() +
-                                                               NT * 128l * D);
-                        ml[x * 128 + r] = make_float2(m_use, l);
-                    }
+                    if (live && !whole) *part_ml = make_float2(m_use, l);
                     tc_fence_before();
                 }
             }
@@ -911,6 +1046,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
 // the first to start inside, if it is. A thread takes 16 columns of a row, three parts in flight; where a
 // long sequence's unit is in many parts, `lanes` neighbouring threads take every lanes-th part each and add
 // theirs up (one sequence of 100000 keys and one K/V head is in 148: 35 us one part after the other).
+__host__ __device__ inline int cache_join_lanes(int parts) { return parts < 6 ? 1 : parts < 24 ? 4 : 16; }
 template <int D, int NT>
 __global__ void __launch_bounds__(128) cache_attention_join(const CacheAttnArgs args) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -919,7 +1055,7 @@ __global__ void __launch_bounds__(128) cache_attention_join(const CacheAttnArgs 
     const int4 cut = args.cuts[2 * c];
     const int rows = cut.x, n = cut.w, items = rows * (D / 16);
     if (items == 0) return;
-    const int lanes = n < 2 * AHEAD ? 1 : n < 8 * AHEAD ? 4 : 16;
+    const int lanes = cache_join_lanes(n);
     const int first_place = args.cuts[2 * (c - 1) + 1].x;            // of the part that the CTA before left last
     const long pf = cache_attn_place_floats<D, NT>();
     const float* part0 = args.ws + ((c - 1) * 2l + first_place) * pf;

@@ -1193,7 +1193,10 @@ static int cache_attn_launch(const CUtensorMap& tq, const CUtensorMap& tk, const
     if (a.ctas < 2) return MICA_OK;
     // the join is launched under the attention kernel's end (it waits for all of it before it reads)
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.ctas - 1, (NT * a.npt * a.G * (D / 16) + 127) / 128);
+    // threads for a unit in as many parts as there are CTAs for each, at least
+    const int parts = a.ctas / std::max(1, static_cast<int>(std::min<long>(static_cast<long>(a.plan.B) * a.KV, a.ctas)));
+    const int items = NT * a.npt * a.G * (D / 16);
+    cfg.gridDim = dim3(a.ctas - 1, (std::max(items, std::min(items * cache_join_lanes(parts), 1024)) + 127) / 128);
     cfg.blockDim = dim3(128);
     cfg.stream = st;
     cudaLaunchAttribute at[1] = {};
@@ -1229,6 +1232,8 @@ int mica_cache_attention(const void* q, long ldq, const void* k_pages, const voi
     int nt = 0;
     cache_attn_rows(max_new, H / KV, &nt, &a.npt);
     if (!workspace || workspace_bytes < cache_attn_bytes(sms, nt, D)) return MICA_ERR_WORKSPACE;
+    const int tile_rows = a.npt * (H / KV);
+    a.copies = nt == 1 && tile_rows <= 64 ? (tile_rows <= 32 ? 4 : 2) : 1;
     a.v_pages = static_cast<const __nv_bfloat16*>(v_pages);
     a.page_stride = page_stride;
     a.mask = reinterpret_cast<const unsigned long long*>(mask); a.ld_mask = ld_mask; a.words = words;

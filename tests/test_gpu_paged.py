@@ -77,6 +77,54 @@ def test_attention_of_one_unit_in_many_parts(heads, new):
         assert torch.equal(o, run_attention(c, max_new=new))
 
 
+@pytest.mark.parametrize('heads,kv,dim,new', [(8, 2, 128, 1), (8, 2, 64, 8), (16, 2, 128, 4), (16, 2, 64, 8), (5, 1, 128, 13),
+                                              (6, 2, 128, 33), (64, 1, 64, 1), (8, 8, 64, 1), (8, 8, 128, 32)])
+def test_attention_of_few_rows(heads, kv, dim, new):
+    """Steps whose rows of a K/V head fill a quarter, a half or more of a row tile, whole units and divided ones,
+    with rows that see nothing, or the keys of one part of a tile only."""
+    for ctx in ([0, 5, 31, 32, 33, 64, 100, 127, 128, 129, 700], [9000], [40] * 70):
+        n = [min(new, 1 + i % new) for i in range(len(ctx) - 1)] + [new]
+        c = Case(ctx, n, heads, kv, dim, 64, seed=len(ctx) + new, mask=tree)
+        o = run_attention(c, max_new=new)
+        check_attention(c, o)
+        assert torch.equal(o, run_attention(c, max_new=new))
+
+
+@pytest.mark.parametrize('heads,new', [(4, 4), (4, 16), (4, 32)])
+def test_few_rows_that_see_nothing_or_one_key(heads, new):
+    made = []
+
+    def blind(rng, t):
+        made.append(torch.zeros(t, t, dtype=torch.bool))
+        if len(made) == 2:
+            made[1][:, t - 1] = True                                    # the second sequence's see its last node
+        return made[-1]
+
+    c = Case([0, 0], [new, new], heads, 1, 128, 32, seed=new, mask=blind)
+    o = run_attention(c, max_new=new)
+    check_attention(c, o)
+    assert torch.equal(o[:new], torch.zeros_like(o[:new]))
+
+
+@pytest.mark.parametrize('new', [1, 8, 16, 33])
+def test_infinities_of_committed_keys(new):
+    """In tiles that every row sees and in the last, alone or two of a kind or of two kinds in a column, whatever
+    part of the tile holds them."""
+    inf = float('inf')
+    c = Case([700, 40000], [new, new], 4, 1, 128, 32, seed=new, mask=tree)
+    for b in range(2):
+        for s, d, bad in ((100, 3, inf), (101, 4, -inf), (130, 5, inf), (190, 5, inf), (131, 6, inf), (250, 6, -inf),
+                          (300, 64, float('nan')), (301, 65, inf), (699, 65, inf), (600, 66, inf), (699, 67, -inf),
+                          (127, 127, -inf)):
+            c.v[c.rows[b][s // 32], 0, s % 32, d] = bad
+            c.keys[b][1][0, s, d] = bad
+    o = run_attention(c, scale=0.01, max_new=new)                        # no weight is so small that it is zero
+    ref = c.attention(0.01)
+    fine = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(o), torch.isnan(ref)) and torch.equal(o.double()[~fine & ~ref.isnan()], ref[~fine & ~ref.isnan()])
+    assert (o.double() - ref)[fine].abs().max() < 0.05                  # 1.1 u (|o| + sum p |v|), |v| < 5.8
+
+
 @pytest.mark.parametrize('bad', [float('nan'), float('inf')])
 def test_odd_values_in_a_causal_extension(bad):
     """Without a mask, rows do not see later rows' K and V: an odd value there changes nothing before its row."""
