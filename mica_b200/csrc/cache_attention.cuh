@@ -612,7 +612,9 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         __syncwarp();
     } else if (warp == 1) {
         // ---------------------------------- MMA issuer --------------------------------
-        if (lane == 0) {
+        // the whole warp, so that the operands' registers are uniform; one thread issues
+        {
+            const bool leader = elect_one();
             constexpr uint32_t idesc_qk = idesc_bf16(128, 128, false);
             constexpr uint32_t idesc_pv = idesc_bf16(128, D, true);
             const uint64_t q_desc0 = smem_desc_sw128(smem_u32(sq), 16, 1024);
@@ -624,42 +626,49 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             int kst = 0, vst = 0, pv = 0;         // ring stages, tiles with P.V issued
             int fills = 0, pv1 = 0;               // NT 2: score tiles issued, P.V of row tile 1
             uint32_t kpar = 0u, vpar = 0u;
+            const auto wait = [&](uint64_t* bar, uint32_t parity) {
+                return __all_sync(0xffffffffu, mma_wait(bar, parity, abort_flag, MICA_DEV_TIMEOUT_MMA));
+            };
             // scores of row tile x with the tile in kst, Q in buffer qb
             const auto scores = [&](int x, int qb) {
                 const int i = NT == 1 ? (t & 1) : x;
                 if (NT == 1) {
-                    if (t >= 2 && !mma_wait(&s_free[i], ((t >> 1) - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+                    if (t >= 2 && !wait(&s_free[i], ((t >> 1) - 1) & 1)) return false;
                 } else {
-                    if (fills > 0 && !mma_wait(&s_free[0], (fills - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+                    if (fills > 0 && !wait(&s_free[0], (fills - 1) & 1)) return false;
                     ++fills;
                 }
                 tc_fence_after();
                 const uint64_t qd = q_desc0 + static_cast<uint64_t>(qb * NT + x) * kStep;
                 const uint64_t kd = k_desc0 + static_cast<uint64_t>(kst) * kStep;
+                if (leader) {
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint64_t off = static_cast<uint64_t>(((kk >> 2) * ATT_HALF_BYTES + (kk & 3) * 32) >> 4);
-                    mma_bf16_ss(tmem + col_s(i), qd + off, kd + off, idesc_qk, kk > 0 ? 1u : 0u);
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint64_t off = static_cast<uint64_t>(((kk >> 2) * ATT_HALF_BYTES + (kk & 3) * 32) >> 4);
+                        mma_bf16_ss(tmem + col_s(i), qd + off, kd + off, idesc_qk, kk > 0 ? 1u : 0u);
+                    }
+                    mma_commit(&s_full[i]);
                 }
-                mma_commit(&s_full[i]);
                 return true;
             };
             const auto values = [&](int x, bool fresh) {
                 const int i = NT == 1 ? (pv & 1) : x;
-                if (!mma_wait(&p_full[i], (NT == 1 ? pv >> 1 : x ? pv1 : pv) & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) return false;
+                if (!wait(&p_full[i], (NT == 1 ? pv >> 1 : x ? pv1 : pv) & 1)) return false;
                 if (NT == 2) pv1 += x;
                 tc_fence_after();
                 const uint64_t vd = v_desc0 + static_cast<uint64_t>(vst) * kStep;
                 const uint32_t o = tmem + col_o(x), p = tmem + col_p(i);
-                mma_bf16_ts(o, p, vd, idesc_pv, fresh ? 0u : 1u);
+                if (leader) {
+                    mma_bf16_ts(o, p, vd, idesc_pv, fresh ? 0u : 1u);
 #pragma unroll
-                for (int kk = 1; kk < 8; ++kk) mma_bf16_ts(o, p + kk * 8, vd + ((kk * 16 * 128) >> 4), idesc_pv, 1u);
-                mma_commit(&pv_done[i]);
+                    for (int kk = 1; kk < 8; ++kk) mma_bf16_ts(o, p + kk * 8, vd + ((kk * 16 * 128) >> 4), idesc_pv, 1u);
+                    mma_commit(&pv_done[i]);
+                }
                 return true;
             };
-            const auto v_ready = [&]() { return mma_wait(&v_full[vst], vpar, abort_flag, MICA_DEV_TIMEOUT_MMA); };
+            const auto v_ready = [&]() { return wait(&v_full[vst], vpar); };
             const auto v_release = [&]() {
-                mma_commit(&v_empty[vst]);
+                if (leader) mma_commit(&v_empty[vst]);
                 if (++vst == S::VST) { vst = 0; vpar ^= 1u; }
                 ++pv;
             };
@@ -667,8 +676,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             // rows are waited for, and the next unit's Q and K may be a while coming.
             for (; !last; ++unit) {
                 const int qb = S::QBUF == 2 ? unit & 1 : 0;
-                if (!mma_wait(&unit_full[unit % CACHE_UNITS], unit / CACHE_UNITS & 1, abort_flag, MICA_DEV_TIMEOUT_MMA) ||
-                    !mma_wait(&q_full[qb], unit / S::QBUF & 1, abort_flag, MICA_DEV_TIMEOUT_MMA)) break;
+                if (!wait(&unit_full[unit % CACHE_UNITS], unit / CACHE_UNITS & 1) ||
+                    !wait(&q_full[qb], unit / S::QBUF & 1)) break;
                 const volatile CacheUnit& u = units[unit % CACHE_UNITS];
                 const int n = u.j1 - u.j0;
                 // the first tile starts the accumulator, except where the softmax has set it
@@ -677,12 +686,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 const auto tiles = [&](auto two) {
                     constexpr bool both = decltype(two)::value;
                     for (int j = 0; j < n; ++j, ++t) {
-                        if (!mma_wait(&k_full[kst], kpar, abort_flag, MICA_DEV_TIMEOUT_MMA) || !scores(0, qb)) return false;
-                        if (!both) mma_commit(&k_empty[kst]);
+                        if (!wait(&k_full[kst], kpar) || !scores(0, qb)) return false;
+                        if (!both && leader) mma_commit(&k_empty[kst]);
                         if (j > 0 && !(v_ready() && values(0, fresh))) return false;
                         if (both) {
                             if (!scores(1, qb)) return false;
-                            mma_commit(&k_empty[kst]);
+                            if (leader) mma_commit(&k_empty[kst]);
                             if (j > 0 && !values(1, fresh)) return false;
                         }
                         if (++kst == S::KST) { kst = 0; kpar ^= 1u; }
@@ -691,7 +700,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                             fresh = false;
                         }
                     }
-                    mma_commit(&q_empty[qb]);
+                    if (leader) mma_commit(&q_empty[qb]);
                     if (!v_ready() || !values(0, fresh) || (both && !values(1, fresh))) return false;
                     v_release();
                     return true;
@@ -700,7 +709,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 else ok = tiles(std::false_type());
                 if (!ok) break;
             }
-            mma_commit(drain);
+            if (leader) mma_commit(drain);
             mbar_wait(drain, 0, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
         }
         __syncwarp();
