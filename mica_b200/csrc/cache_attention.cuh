@@ -400,37 +400,44 @@ __device__ __noinline__ bool cache_safe_v(uint8_t* tile, uint64_t* full, uint32_
 
 // Copies of the rows meet the keys of one another with weights of zero, and 0 * infinity is NaN: a sum that is
 // not finite is set to what the infinities and NaN among the V that its row sees in this CTA's tiles make of it.
-// Three bits for each of 8 columns from `col`: NaN, infinity, -infinity. The whole warp calls it; mend: this
-// thread's row is asked for.
+// Three bits for each of 4 columns from `col`: NaN, infinity, -infinity. The whole warp calls it; mend: this
+// thread's row and columns are asked for.
 template <int D>
 __device__ __noinline__ uint32_t cache_odd_kinds(const CacheAttnArgs& args, const volatile CacheUnit& u, int node_r, int col,
                                                  bool mend) {
     const CachePlan& plan = args.plan;
     const int lane = threadIdx.x & 31, b = u.b, special = u.special;
-    const auto kinds = [&](int key) {
+    const auto kinds = [&](int key, int c0) {
         int page = 0, slot = 0;
         if (!cache_slot(plan, b, key, &page, &slot)) return 0u;
         const uint16_t* v = reinterpret_cast<const uint16_t*>(args.v_pages) + page * args.page_stride +
-                            ((static_cast<long>(u.kvh) << plan.page_log2) + slot) * D + col;
+                            ((static_cast<long>(u.kvh) << plan.page_log2) + slot) * D + c0;
         uint32_t k = 0u;
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 4; ++e) {
             const uint32_t bits = v[e];
             if ((bits & 0x7f80u) == 0x7f80u) k |= (bits & 0x7fu ? 1u : bits & 0x8000u ? 4u : 2u) << (3 * e);
         }
         return k;
     };
-    uint32_t k = 0u;
-    for (int key = u.j0 * 128 + lane; key < min(u.j1, special) * 128; key += 32) k |= kinds(key);    // all rows see these
-    k = __reduce_or_sync(0xffffffffu, k);
+    // the tiles whose keys all rows see, for one set of columns after the other
+    uint32_t mine = 0u;
+    for (uint32_t todo = __ballot_sync(0xffffffffu, mend); todo;) {
+        const int c0 = __shfl_sync(0xffffffffu, col, __ffs(todo) - 1);
+        uint32_t k = 0u;
+        for (int key = u.j0 * 128 + lane; key < min(u.j1, special) * 128; key += 32) k |= kinds(key, c0);
+        k = __reduce_or_sync(0xffffffffu, k);
+        if (col == c0) mine = k;
+        todo &= ~__ballot_sync(0xffffffffu, col == c0);
+    }
     for (int j = max(u.j0, special); mend && j < u.j1; ++j) {
         uint32_t vis[4];
         cache_visible(args, u, 0, node_r, j * 128, vis);
         for (int i = 0; i < 128; ++i) {
             const uint32_t seen = i < 64 ? (i < 32 ? vis[0] : vis[1]) : (i < 96 ? vis[2] : vis[3]);
-            if (seen >> (i & 31) & 1u) k |= kinds(j * 128 + i);
+            if (seen >> (i & 31) & 1u) mine |= kinds(j * 128 + i, col);
         }
     }
-    return mend ? k : 0u;
+    return mend ? mine : 0u;
 }
 
 template <int D, int NT>
@@ -928,9 +935,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 const int tl = t - 1;
                 const int i2 = NT == 1 ? (tl & 1) : x;
                 const int n2 = NT == 1 ? tl >> 1 : tl;
-                bool w = true;
-                if (lane == 0) w = mbar_wait(&pv_done[i2], n2 & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
-                if (!__shfl_sync(0xffffffffu, w, 0)) { ok = false; break; }
+                ok = __all_sync(0xffffffffu, mma_wait(&pv_done[i2], n2 & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
+                if (!ok) break;
                 tc_fence_after();
                 const bool whole = u.flags & 2;
                 const long row = static_cast<long>(u.row0) + x * args.npt + node_r;
@@ -939,74 +945,83 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 float2* part_ml = reinterpret_cast<float2*>(place + NT * 128l * D) + x * 128 + r;
                 __nv_bfloat16* orow = args.out + row * args.ldo + (u.kvh * args.G + head_r) * D;
                 if (NT == 1 && copies > 1) {
-                    // the copies' rows, brought to one maximum and added up through the unit's Q buffer, half
-                    // of the columns at a time: each warp adds up a part of them
+                    // The copies' rows, brought to one maximum and added up through the unit's Q buffer, in two
+                    // halves of the columns where it does not hold all; the four warps share the (row, 4 columns).
                     const auto meet = [&]() {
                         __syncwarp();
                         if (lane == 0) mbar_arrive(exchange);
-                        return __all_sync(0xffffffffu, mbar_wait(exchange, phases++ & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
+                        return __all_sync(0xffffffffu, mma_wait(exchange, phases++ & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
                     };
-                    float4* xo = reinterpret_cast<float4*>(sq + (unit & 1) * S::TILE) + r;    // [copy][D / 8][row]
-                    stats[q4 * 32 + lane] = make_float2(m_use, l);
-                    if (!meet()) { ok = false; break; }
-                    float m_all = m_use, l_all = 0.f;
-                    for (int i = 0; i < copies; ++i) m_all = fmaxf(m_all, stats[i * keys_each + r].x);
-                    for (int i = 0; i < copies; ++i) {
-                        const float2 ml = stats[i * keys_each + r];
-                        l_all = fmaf(ml.y, fast_exp2(ml.x - m_all), l_all);
-                    }
-                    const float mine = fast_exp2(m_use - m_all), inv = l_all == 0.f ? 0.f : 1.f / l_all;
-                    for (int pass = 0; pass < 2; ++pass) {
+                    const int rows = args.npt * args.G, have = min(args.npt, u.nodes) * args.G;   // of a copy; of the unit
+                    const int passes = copies * rows <= 64 ? 1 : 2, quads = D / 4 / passes;
+                    float4* xo = reinterpret_cast<float4*>(sq + (unit & 1) * S::TILE);            // [copy][quads][rows]
+                    if (live) stats[cp * keys_each + r] = make_float2(m_use, l);
+                    for (int pass = 0; pass < passes; ++pass) {
                         if (pass && !meet()) { ok = false; break; }
-                        if (warp_live) {
+                        for (int cc = 0; warp_live && cc < quads / 8; ++cc) {
+                            uint32_t o[32];
+                            tmem_ld_32x32b_x32(t_o + pass * (D / 2) + cc * 32, o);
+                            tmem_ld_wait();
+                            if (live) {
 #pragma unroll
-                            for (int cc = 0; cc < D / 64; ++cc) {
-                                uint32_t o[32];
-                                tmem_ld_32x32b_x32(t_o + pass * (D / 2) + cc * 32, o);
-                                tmem_ld_wait();
-                                if (live) {
-#pragma unroll
-                                    for (int v = 0; v < 8; ++v)
-                                        xo[(cp * (D / 8) + cc * 8 + v) * keys_each] =
-                                            make_float4(__uint_as_float(o[4 * v]) * mine, __uint_as_float(o[4 * v + 1]) * mine,
-                                                        __uint_as_float(o[4 * v + 2]) * mine, __uint_as_float(o[4 * v + 3]) * mine);
-                                }
+                                for (int v = 0; v < 8; ++v)
+                                    xo[(cp * quads + cc * 8 + v) * rows + r] =
+                                        make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]),
+                                                    __uint_as_float(o[4 * v + 2]), __uint_as_float(o[4 * v + 3]));
                             }
                         }
                         if (!meet()) { ok = false; break; }
-                        const int each = D / 8 / copies;
-                        for (int v = cp * each; warp_live && v < (cp + 1) * each; v += 2) {
-                            float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                            for (int i = 0; live && i < copies; ++i) {
-                                const float4 a = xo[(i * (D / 8) + v) * keys_each], b = xo[(i * (D / 8) + v + 1) * keys_each];
-                                o[0] += a.x; o[1] += a.y; o[2] += a.z; o[3] += a.w;
-                                o[4] += b.x; o[5] += b.y; o[6] += b.z; o[7] += b.w;
+                        for (int i0 = q4 * 32; i0 < quads * rows; i0 += 128) {
+                            const int item = i0 + lane, v = min(item / rows, quads - 1), rr = item - v * rows;
+                            const bool mine = rr < have;
+                            float m_all = -1e30f, l_all = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+                            if (mine) {
+                                float2 ml[4];
+                                float4 a[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const int from = k < copies ? k : 0;
+                                    ml[k] = stats[from * keys_each + rr];
+                                    a[k] = xo[(from * quads + v) * rows + rr];
+                                }
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) m_all = fmaxf(m_all, ml[k].x);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    if (k >= copies) continue;
+                                    const float w = fast_exp2(ml[k].x - m_all);
+                                    l_all = fmaf(ml[k].y, w, l_all);
+                                    o[0] = fmaf(a[k].x, w, o[0]);
+                                    o[1] = fmaf(a[k].y, w, o[1]);
+                                    o[2] = fmaf(a[k].z, w, o[2]);
+                                    o[3] = fmaf(a[k].w, w, o[3]);
+                                }
                             }
-                            const int col = pass * (D / 2) + v * 4;
+                            const int quad = pass * quads + v, node = rr / args.G;
                             float zero = 0.f;
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) zero = fmaf(o[e], 0.f, zero);
+                            for (int e = 0; e < 4; ++e) zero = fmaf(o[e], 0.f, zero);
                             const bool odd = zero != 0.f && l_all * 0.f == 0.f;       // infinite or NaN scores stay
                             if (__any_sync(0xffffffffu, odd)) {
-                                const uint32_t kinds = cache_odd_kinds<D>(args, u, node_r, col, odd);
+                                const uint32_t kinds = cache_odd_kinds<D>(args, u, node, quad * 4, odd);
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) {
+                                for (int e = 0; e < 4; ++e) {
                                     const uint32_t n = kinds >> (3 * e) & 7u;
                                     if (n) o[e] = __uint_as_float(n & 1u || n == 6u ? 0x7fffffffu : n == 2u ? 0x7f800000u : 0xff800000u);
                                 }
                             }
-                            if (live && whole)
-                                *reinterpret_cast<uint4*>(orow + col) =
-                                    make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv),
-                                               pack_bf16(o[4] * inv, o[5] * inv), pack_bf16(o[6] * inv, o[7] * inv));
-                            else if (live) {
-                                part[col / 4 * 128] = make_float4(o[0], o[1], o[2], o[3]);
-                                part[(col / 4 + 1) * 128] = make_float4(o[4], o[5], o[6], o[7]);
+                            if (mine && whole) {
+                                const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+                                *reinterpret_cast<uint2*>(args.out + (static_cast<long>(u.row0) + node) * args.ldo +
+                                                          (u.kvh * args.G + rr - node * args.G) * D + quad * 4) =
+                                    make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+                            } else if (mine) {
+                                reinterpret_cast<float4*>(place)[quad * 128 + rr] = make_float4(o[0], o[1], o[2], o[3]);
+                                if (quad == 0) reinterpret_cast<float2*>(place + 128l * D)[rr] = make_float2(m_all, l_all);
                             }
                         }
                     }
                     if (!ok) break;
-                    if (live && !whole && cp == 0) *part_ml = make_float2(m_all, l_all);
                     fence_proxy_async_smem();                        // Q of the next unit but one comes here
                     tc_fence_before();
                     __syncwarp();
