@@ -26,7 +26,11 @@
 // pages of 16 one warp for both was as slow as memory); 1 issues the MMAs (S = Q K^T both from
 // shared memory, O += P V with P in tensor memory); the others softmax, one row a thread, as in
 // attention.cuh. NT = 1: S and P have two buffers each, so scores, softmax and P.V of three
-// consecutive tiles overlap; Q has two, so the next unit's loads run under this one's end. NT = 2:
+// consecutive tiles overlap; Q has two, so the next unit's loads run under this one's end. Up to 16 rows
+// (8 of D = 128) lie in the row tile four times, once in each warp's quarter of tensor memory, and each warp
+// takes 32 keys of a tile for them in place of 128, with its own maximum, sum and accumulator (its weights
+// are zero for the others' keys); a unit's end adds the four up, which costs more than it gains at more
+// rows (64 sequences of 300 to 4000 keys, 32 heads over 8 of 64: 90 -> 78 us with 16 rows, 89 -> 93 with 32). NT = 2:
 // two row tiles share every K and V tile (attention.cuh's schedule).
 // P is rounded to bf16 for the tensor core (V's type): each weight is off by a half step, 2^-8 of it at
 // most, and these errors are independent, so the result is off by about as much as its own rounding to
@@ -61,7 +65,7 @@ struct CacheAttnArgs {
     long ldo;
     int KV, G;                  // K/V heads, query heads of each
     int npt;                    // nodes of a row tile: npt * G <= 128
-    int copies;                 // of the rows in a row tile: 4, 2 or 1 (npt * G <= 128 / copies; NT 1)
+    bool quarters;              // the rows lie in the row tile four times (npt * G <= 16; NT 1)
     int ctas;                   // CTAs of the grid
     float scale_log2;           // scale * log2(e)
     float* ws;                  // partials: [ctas][2] places
@@ -99,7 +103,7 @@ __device__ __forceinline__ int cache_row_blocks(const CacheSeq& s, int R) { retu
 // weight for a tile, 4 with two row tiles and 3 where its nodes fill only one of the two.
 template <int NT>
 struct CacheCost {
-    static constexpr int UNIT = NT == 1 ? 1 : 2;
+    static constexpr int UNIT = 2;
     static constexpr int TILE = NT == 1 ? 1 : 4;
     __device__ __forceinline__ static int weight(const CacheSeq& s, int rb, int R) {
         return NT == 1 ? 1 : s.T - rb * R <= R / 2 ? 3 : 4;
@@ -488,18 +492,18 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     uint64_t* v_fixed = pv_done + 2;           // V of a special tile made safe (all softmax warps)
     uint64_t* unit_full = v_fixed + 1;         // [CACHE_UNITS]
     uint64_t* drain = unit_full + CACHE_UNITS;
-    uint64_t* exchange = drain + 1;            // between the softmax warps at a unit's end (copies)
+    uint64_t* exchange = drain + 1;            // the copies' rows of a unit are all there
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(exchange + 1);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     uint32_t* odd_v = tmem_slot + 2;           // [2][NT][4] keys of a special tile whose V row holds infinities or NaN
     volatile CacheUnit* units = reinterpret_cast<volatile CacheUnit*>(odd_v + 16);
     float2* stats = reinterpret_cast<float2*>(sv + S::VST * S::TILE + S::BARS);
-    const int copies = NT == 1 ? args.copies : 1;
+    const bool quarters = NT == 1 && args.quarters;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 1);
-            mbar_init(&q_empty[i], copies > 1 ? 5 : 1);       // the softmax warps add the copies up in it
+            mbar_init(&q_empty[i], quarters ? 5 : 1);         // the softmax warps add the copies up in it
             mbar_init(&s_full[i], 1);
             mbar_init(&s_free[i], 4);
             mbar_init(&p_full[i], 4);
@@ -552,6 +556,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     w = mbar_wait(&q_empty[qb], static_cast<uint32_t>(unit / S::QBUF & 1) ^ 1u, abort_flag,
                                   MICA_DEV_TIMEOUT_PRODUCER);
                     if (w) {
+                        const int copies = quarters ? 4 : 1;
                         if (wk.s.keys == 0) record_bad_page();
                         const int node0 = wk.rb * R;
                         mbar_arrive_expect_tx(&q_full[qb], NT * copies * S::HALVES * 128u * args.npt * args.G);
@@ -743,10 +748,9 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         const int q4 = warp & 3;                           // tensor-memory lane quarter
         const uint32_t lane_off = static_cast<uint32_t>(q4 * 32) << 16;
         const float c = args.scale_log2;
-        // with copies, copy `cp` of the rows has a part of each tile's keys: this warp's row and its first key
-        const int cp = copies == 4 ? q4 : copies == 2 ? q4 >> 1 : 0, keys_each = 128 / copies;
-        const int r = q4 * 32 + lane - cp * keys_each, key0 = cp * keys_each;
-        if (NT == 1 && copies > 1) {                       // the weights of the other parts stay zero
+        // in quarters each copy of the rows has 32 keys of a tile: this thread's row, its keys' first and number
+        const int r = quarters ? lane : q4 * 32 + lane, key0 = quarters ? q4 * 32 : 0, keys_each = quarters ? 32 : 128;
+        if (quarters) {                                    // the weights of the others' keys stay zero
             uint32_t zero[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) zero[i] = 0u;
@@ -755,7 +759,6 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             tmem_st_wait();
         }
         bool ok = true, last = false;
-        int phases = 0;                                    // of `exchange`
         int t = 0, unit = 0;                               // this row tile's key tiles so far, units
         int skipped = 0;                                   // and those of units it had no rows in
         int fixes = 0;                                     // special tiles so far
@@ -849,8 +852,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     l = l * alpha + (((a0 + a1) + (b0 + b1)) + ((d0 + d1) + (e0 + e1)));
                 };
                 if (warp_live) {
-                    if (NT == 2 || copies == 1) weights(std::integral_constant<int, 4>());
-                    else if (copies == 2) weights(std::integral_constant<int, 2>());
+                    if (!quarters) weights(std::integral_constant<int, 4>());
                     else weights(std::integral_constant<int, 1>());
                 } else {
                     if (lane == 0) mbar_arrive(&s_free[NT == 1 ? i2 : 0]);
@@ -916,12 +918,11 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     }
                 }
                 if (warp_live) {
-                    if (NT == 1 && copies == 4) {
+                    if (quarters) {
                         tmem_st_32x32b_x16(t_p + key0 / 2, *reinterpret_cast<uint32_t (*)[16]>(&pk[0]));
                     } else {
-                        tmem_st_32x32b_x32(t_p + key0 / 2, *reinterpret_cast<uint32_t (*)[32]>(&pk[0]));
-                        if (NT == 2 || copies == 1)
-                            tmem_st_32x32b_x32(t_p + 32, *reinterpret_cast<uint32_t (*)[32]>(&pk[32]));
+                        tmem_st_32x32b_x32(t_p, *reinterpret_cast<uint32_t (*)[32]>(&pk[0]));
+                        tmem_st_32x32b_x32(t_p + 32, *reinterpret_cast<uint32_t (*)[32]>(&pk[32]));
                     }
                     tmem_st_wait();
                 }
@@ -944,84 +945,76 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 float4* part = reinterpret_cast<float4*>(place) + x * (D / 4) * 128 + r;
                 float2* part_ml = reinterpret_cast<float2*>(place + NT * 128l * D) + x * 128 + r;
                 __nv_bfloat16* orow = args.out + row * args.ldo + (u.kvh * args.G + head_r) * D;
-                if (NT == 1 && copies > 1) {
-                    // The copies' rows, brought to one maximum and added up through the unit's Q buffer, in two
-                    // halves of the columns where it does not hold all; the four warps share the (row, 4 columns).
-                    const auto meet = [&]() {
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(exchange);
-                        return __all_sync(0xffffffffu, mma_wait(exchange, phases++ & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
-                    };
+                if (quarters) {
+                    // The copies, brought to one maximum and added up through the unit's Q buffer (their 4 * 16
+                    // rows at most fill it): the four warps share the (row, 4 columns).
                     const int rows = args.npt * args.G, have = min(args.npt, u.nodes) * args.G;   // of a copy; of the unit
-                    const int passes = copies * rows <= 64 ? 1 : 2, quads = D / 4 / passes;
-                    float4* xo = reinterpret_cast<float4*>(sq + (unit & 1) * S::TILE);            // [copy][quads][rows]
-                    if (live) stats[cp * keys_each + r] = make_float2(m_use, l);
-                    for (int pass = 0; pass < passes; ++pass) {
-                        if (pass && !meet()) { ok = false; break; }
-                        for (int cc = 0; warp_live && cc < quads / 8; ++cc) {
-                            uint32_t o[32];
-                            tmem_ld_32x32b_x32(t_o + pass * (D / 2) + cc * 32, o);
-                            tmem_ld_wait();
-                            if (live) {
+                    float4* xo = reinterpret_cast<float4*>(sq + (unit & 1) * S::TILE);            // [copy][D / 4][rows]
+                    if (live) stats[q4 * 32 + r] = make_float2(m_use, l);
 #pragma unroll
-                                for (int v = 0; v < 8; ++v)
-                                    xo[(cp * quads + cc * 8 + v) * rows + r] =
-                                        make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]),
-                                                    __uint_as_float(o[4 * v + 2]), __uint_as_float(o[4 * v + 3]));
-                            }
-                        }
-                        if (!meet()) { ok = false; break; }
-                        for (int i0 = q4 * 32; i0 < quads * rows; i0 += 128) {
-                            const int item = i0 + lane, v = min(item / rows, quads - 1), rr = item - v * rows;
-                            const bool mine = rr < have;
-                            float m_all = -1e30f, l_all = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-                            if (mine) {
-                                float2 ml[4];
-                                float4 a[4];
+                    for (int cc = 0; cc < D / 32; ++cc) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(t_o + cc * 32, o);
+                        tmem_ld_wait();
+                        if (live) {
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    const int from = k < copies ? k : 0;
-                                    ml[k] = stats[from * keys_each + rr];
-                                    a[k] = xo[(from * quads + v) * rows + rr];
-                                }
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) m_all = fmaxf(m_all, ml[k].x);
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    if (k >= copies) continue;
-                                    const float w = fast_exp2(ml[k].x - m_all);
-                                    l_all = fmaf(ml[k].y, w, l_all);
-                                    o[0] = fmaf(a[k].x, w, o[0]);
-                                    o[1] = fmaf(a[k].y, w, o[1]);
-                                    o[2] = fmaf(a[k].z, w, o[2]);
-                                    o[3] = fmaf(a[k].w, w, o[3]);
-                                }
-                            }
-                            const int quad = pass * quads + v, node = rr / args.G;
-                            float zero = 0.f;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) zero = fmaf(o[e], 0.f, zero);
-                            const bool odd = zero != 0.f && l_all * 0.f == 0.f;       // infinite or NaN scores stay
-                            if (__any_sync(0xffffffffu, odd)) {
-                                const uint32_t kinds = cache_odd_kinds<D>(args, u, node, quad * 4, odd);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const uint32_t n = kinds >> (3 * e) & 7u;
-                                    if (n) o[e] = __uint_as_float(n & 1u || n == 6u ? 0x7fffffffu : n == 2u ? 0x7f800000u : 0xff800000u);
-                                }
-                            }
-                            if (mine && whole) {
-                                const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
-                                *reinterpret_cast<uint2*>(args.out + (static_cast<long>(u.row0) + node) * args.ldo +
-                                                          (u.kvh * args.G + rr - node * args.G) * D + quad * 4) =
-                                    make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
-                            } else if (mine) {
-                                reinterpret_cast<float4*>(place)[quad * 128 + rr] = make_float4(o[0], o[1], o[2], o[3]);
-                                if (quad == 0) reinterpret_cast<float2*>(place + 128l * D)[rr] = make_float2(m_all, l_all);
-                            }
+                            for (int v = 0; v < 8; ++v)
+                                xo[(q4 * (D / 4) + cc * 8 + v) * rows + r] =
+                                    make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]),
+                                                __uint_as_float(o[4 * v + 2]), __uint_as_float(o[4 * v + 3]));
                         }
                     }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(exchange);
+                    ok = __all_sync(0xffffffffu, mma_wait(exchange, unit & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
                     if (!ok) break;
+                    for (int i0 = q4 * 32; i0 < D / 4 * rows; i0 += 128) {
+                        const int item = i0 + lane, v = min(item / rows, D / 4 - 1), rr = item - v * rows;
+                        const bool mine = rr < have;
+                        float m_all = -1e30f, l_all = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+                        if (mine) {
+                            float2 ml[4];
+                            float4 a[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                ml[k] = stats[k * 32 + rr];
+                                a[k] = xo[(k * (D / 4) + v) * rows + rr];
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) m_all = fmaxf(m_all, ml[k].x);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float w = fast_exp2(ml[k].x - m_all);
+                                l_all = fmaf(ml[k].y, w, l_all);
+                                o[0] = fmaf(a[k].x, w, o[0]);
+                                o[1] = fmaf(a[k].y, w, o[1]);
+                                o[2] = fmaf(a[k].z, w, o[2]);
+                                o[3] = fmaf(a[k].w, w, o[3]);
+                            }
+                        }
+                        const int node = rr / args.G;
+                        float zero = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) zero = fmaf(o[e], 0.f, zero);
+                        const bool odd = zero != 0.f && l_all * 0.f == 0.f;           // infinite or NaN scores stay
+                        if (__any_sync(0xffffffffu, odd)) {
+                            const uint32_t kinds = cache_odd_kinds<D>(args, u, node, v * 4, odd);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t n = kinds >> (3 * e) & 7u;
+                                if (n) o[e] = __uint_as_float(n & 1u || n == 6u ? 0x7fffffffu : n == 2u ? 0x7f800000u : 0xff800000u);
+                            }
+                        }
+                        if (mine && whole) {
+                            const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+                            *reinterpret_cast<uint2*>(args.out + (static_cast<long>(u.row0) + node) * args.ldo +
+                                                      (u.kvh * args.G + rr - node * args.G) * D + v * 4) =
+                                make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+                        } else if (mine) {
+                            reinterpret_cast<float4*>(place)[v * 128 + rr] = make_float4(o[0], o[1], o[2], o[3]);
+                            if (v == 0) reinterpret_cast<float2*>(place + 128l * D)[rr] = make_float2(m_all, l_all);
+                        }
+                    }
                     fence_proxy_async_smem();                        // Q of the next unit but one comes here
                     tc_fence_before();
                     __syncwarp();

@@ -106,7 +106,7 @@ def test_few_rows_that_see_nothing_or_one_key(heads, new):
     assert torch.equal(o[:new], torch.zeros_like(o[:new]))
 
 
-@pytest.mark.parametrize('new', [1, 8, 16, 33])
+@pytest.mark.parametrize('new', [1, 2, 8, 16, 33])
 def test_infinities_of_committed_keys(new):
     """In tiles that every row sees and in the last, alone or two of a kind or of two kinds in a column, whatever
     part of the tile holds them."""
