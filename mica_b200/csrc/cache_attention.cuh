@@ -374,6 +374,16 @@ __device__ __forceinline__ bool cache_fix_v(uint8_t* tile, int r, int h0, int h1
     return odd;
 }
 
+// Whether the fixes-th special tile has odd values.
+template <int NT>
+__device__ __forceinline__ bool cache_any_odd(const volatile uint32_t* odd_v, int fixes) {
+    const volatile uint32_t* odd = odd_v + (fixes & 1) * 4 * NT;
+    uint32_t some = 0u;
+#pragma unroll
+    for (int i = 0; i < 4 * NT; ++i) some |= odd[i];
+    return some != 0u;
+}
+
 // A tile of V that holds nodes of the step or the end of the keys, made safe by the softmax warps: each waits
 // for it, takes its rows (two row tiles half of the columns each), leaves in `odd` which had odd values, and
 // arrives on v_fixed. (`odd` is one of two sets: all warps pass v_fixed of a special tile before one writes the
@@ -663,15 +673,18 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 }
                 return true;
             };
-            const auto values = [&](int x, bool fresh) {
+            int fixes = 0;                        // special tiles of the units before
+            const auto values = [&](int x, bool fresh, bool special) {
                 const int i = NT == 1 ? (pv & 1) : x;
                 if (!wait(&p_full[i], (NT == 1 ? pv >> 1 : x ? pv1 : pv) & 1)) return false;
                 if (NT == 2) pv1 += x;
                 tc_fence_after();
                 const uint64_t vd = v_desc0 + static_cast<uint64_t>(vst) * kStep;
                 const uint32_t o = tmem + col_o(x), p = tmem + col_p(i);
+                // the unit's first tile starts the accumulator, except where the softmax has put odd values there
+                const bool start = fresh && !(special && cache_any_odd<NT>(odd_v, fixes));
                 if (leader) {
-                    mma_bf16_ts(o, p, vd, idesc_pv, fresh ? 0u : 1u);
+                    mma_bf16_ts(o, p, vd, idesc_pv, start ? 0u : 1u);
 #pragma unroll
                     for (int kk = 1; kk < 8; ++kk) mma_bf16_ts(o, p + kk * 8, vd + ((kk * 16 * 128) >> 4), idesc_pv, 1u);
                     mma_commit(&pv_done[i]);
@@ -692,19 +705,20 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     !wait(&q_full[qb], unit / S::QBUF & 1)) break;
                 const volatile CacheUnit& u = units[unit % CACHE_UNITS];
                 const int n = u.j1 - u.j0;
-                // the first tile starts the accumulator, except where the softmax has set it
-                bool fresh = u.j0 < u.special;
+                bool fresh = true;
+                const bool special = u.j0 >= u.special;                // its first tile is
+                const int specials = max(0, u.j1 - max(u.j0, u.special));
                 last = u.flags & 1;
                 const auto tiles = [&](auto two) {
                     constexpr bool both = decltype(two)::value;
                     for (int j = 0; j < n; ++j, ++t) {
                         if (!wait(&k_full[kst], kpar) || !scores(0, qb)) return false;
                         if (!both && leader) mma_commit(&k_empty[kst]);
-                        if (j > 0 && !(v_ready() && values(0, fresh))) return false;
+                        if (j > 0 && !(v_ready() && values(0, fresh, special))) return false;
                         if (both) {
                             if (!scores(1, qb)) return false;
                             if (leader) mma_commit(&k_empty[kst]);
-                            if (j > 0 && !values(1, fresh)) return false;
+                            if (j > 0 && !values(1, fresh, special)) return false;
                         }
                         if (++kst == S::KST) { kst = 0; kpar ^= 1u; }
                         if (j > 0) {
@@ -713,13 +727,14 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                         }
                     }
                     if (leader) mma_commit(&q_empty[qb]);
-                    if (!v_ready() || !values(0, fresh) || (both && !values(1, fresh))) return false;
+                    if (!v_ready() || !values(0, fresh, special) || (both && !values(1, fresh, special))) return false;
                     v_release();
                     return true;
                 };
                 if (NT == 2 && !(u.flags & 8)) ok = tiles(std::true_type());
                 else ok = tiles(std::false_type());
                 if (!ok) break;
+                fixes += specials;
             }
             if (leader) mma_commit(drain);
             mbar_wait(drain, 0, abort_flag, MICA_DEV_TIMEOUT_DRAIN);
@@ -860,17 +875,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 // this P buffer is free once its last P.V is done; the accumulator once the tile before's is
                 bool any_odd = false;
                 if (special) {
-                    const volatile uint32_t* odd4 = odd_v + (fixes & 1) * 4 * NT;
                     ok = __all_sync(0xffffffffu, mbar_wait(v_fixed, fixes & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
                     if (!ok) break;
-                    uint32_t some = 0u;
-                    for (int i = 0; i < 4 * NT; ++i) some |= odd4[i];
-                    any_odd = some != 0u;
-                    ++fixes;
+                    any_odd = cache_any_odd<NT>(odd_v, fixes++);
                 }
                 const bool fresh = t == t_first;
-                const bool touch = warp_live && (special && fresh || any_odd ||
-                                                 (!fresh && __any_sync(0xffffffffu, moved)));
+                const bool touch = warp_live && (any_odd || (!fresh && __any_sync(0xffffffffu, moved)));
                 // NT 1: the scores were issued after the P.V of the tile two before, and are there
                 if (NT == 2 && n2 > 0)
                     ok = __all_sync(0xffffffffu, mma_wait(&pv_done[i2], (n2 - 1) & 1, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE));
