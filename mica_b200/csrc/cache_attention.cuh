@@ -42,11 +42,11 @@
 // or NaN element of a node's V is replaced by zero and added to the accumulators of the rows that see
 // it, no others.
 //
-// Measured (32 heads over 8, D = 128, cold L2): 13 and 15 tokens over 70761 and 87495 keys 129 us, the key
-// tiles among them at the memory's 6.5 TB/s (1.5 us a tile and SM); 16 trees of up to 64 nodes over up
-// to 9000 keys 93 us, 2.1 us a tile of two row tiles (softmax and the one score buffer, as in
-// attention.cuh); 700 nodes over 20000 keys 220 us, 1.05 PFLOP/s; one token over up to 700 keys 10 us from
-// the first CTA's start to the join's end.
+// Measured (32 heads over 8, D = 128, cold L2): 13 and 15 tokens over 70761 and 87495 keys 130 us (116 warm), the
+// key tiles among them at the memory's 6.5 TB/s (1.5 us a tile and SM); 16 trees of up to 64 nodes over up to
+// 9000 keys 90 us, a tile of two row tiles 1.7 us (softmax: 2100 cycles of it the scores' way through the
+// exponential, 1100 waits, packing and stores); 700 nodes over 20000 keys 207 us, 1.1 PFLOP/s; one token over up
+// to 700 keys 17 us with its launch and the join.
 #pragma once
 
 #include "attention.cuh"
