@@ -271,7 +271,10 @@ struct CacheWalk {
     __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == nk; }
 };
 
-// What a role needs of the unit it is at: the K warp walks the run and leaves it here, four units deep.
+// What a role needs of the unit it is at: the K warp walks the run and leaves it here, four units deep. A
+// place is taken again once every warp that reads it (MMA, V, softmax) has said that it is done with the unit
+// before: row tile 1's warps pass over units that have no rows for them, and nothing else holds the K warp,
+// or the parity of unit_full, to their pace.
 struct CacheUnit {
     int b, kvh, row0, node0, nodes;     // row0: global row of its first node (node0 of its sequence)
     int base, keys, j0, j1;
@@ -292,7 +295,7 @@ struct CacheAttnShape {
     static constexpr int BARS = D == 128 ? 576 : 672;                     // barriers and units
     static constexpr int STATS = NT == 1 ? 128 * 8 : 0;                  // the copies' (max, sum)
     static constexpr int SMEM = 1024 + TILE * (QBUF * NT + KST + VST) + BARS + STATS;
-    static_assert((4 + 2 * KST + 2 * VST + 8 + 1 + CACHE_UNITS + 2) * 8 + 8 + 64 + CACHE_UNITS * sizeof(CacheUnit) <= BARS, "BARS");
+    static_assert((4 + 2 * KST + 2 * VST + 8 + 1 + 2 * CACHE_UNITS + 2) * 8 + 8 + 64 + CACHE_UNITS * sizeof(CacheUnit) <= BARS, "BARS");
 };
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
@@ -501,7 +504,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     uint64_t* pv_done = p_full + 2;            // [2] P.V finished
     uint64_t* v_fixed = pv_done + 2;           // V of a special tile made safe (all softmax warps)
     uint64_t* unit_full = v_fixed + 1;         // [CACHE_UNITS]
-    uint64_t* drain = unit_full + CACHE_UNITS;
+    uint64_t* unit_empty = unit_full + CACHE_UNITS;   // [CACHE_UNITS] read by the MMA, V and softmax warps
+    uint64_t* drain = unit_empty + CACHE_UNITS;
     uint64_t* exchange = drain + 1;            // the copies' rows of a unit are all there
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(exchange + 1);
     volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -522,7 +526,10 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         for (int i = 0; i < S::KST; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
         for (int i = 0; i < S::VST; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
         mbar_init(v_fixed, 4 * NT);
-        for (int i = 0; i < CACHE_UNITS; ++i) mbar_init(&unit_full[i], 1);
+        for (int i = 0; i < CACHE_UNITS; ++i) {
+            mbar_init(&unit_full[i], 1);
+            mbar_init(&unit_empty[i], 2 + 4 * NT);
+        }
         mbar_init(drain, 1);
         mbar_init(exchange, 4);
         *abort_flag = 0u;
@@ -558,12 +565,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         for (; !last && ok; ++unit) {
             const int slot = unit % CACHE_UNITS;
             if (is_k) {
-                // A unit's place is taken again when the one two back (NT 2: one back) has all its scores: those
-                // were issued after the unit before it had its weights, so its rows, and all before, are out.
                 const int qb = S::QBUF == 2 ? unit & 1 : 0;
                 bool w = true;
                 if (lane == 0) {
                     w = mbar_wait(&q_empty[qb], static_cast<uint32_t>(unit / S::QBUF & 1) ^ 1u, abort_flag,
+                                  MICA_DEV_TIMEOUT_PRODUCER) &&
+                        mbar_wait(&unit_empty[slot], static_cast<uint32_t>(unit / CACHE_UNITS & 1) ^ 1u, abort_flag,
                                   MICA_DEV_TIMEOUT_PRODUCER);
                     if (w) {
                         const int copies = quarters ? 4 : 1;
@@ -620,6 +627,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 __syncwarp();
                 if (++st == stages) { st = 0; par ^= 1u; }
             }
+            if (!is_k && lane == 0) mbar_arrive(&unit_empty[slot]);
         }
         // the place of this CTA's last unit, for the join
         if (is_k && lane == 0) args.cuts[2 * cta + 1] = make_int4(unit > 1 ? 1 : 0, 0, 0, 0);
@@ -734,6 +742,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                 if (NT == 2 && !(u.flags & 8)) ok = tiles(std::true_type());
                 else ok = tiles(std::false_type());
                 if (!ok) break;
+                if (leader) mbar_arrive(&unit_empty[unit % CACHE_UNITS]);
                 fixes += specials;
             }
             if (leader) mma_commit(drain);
@@ -788,6 +797,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             if (NT == 2 && x == 1 && (u.flags & 8)) {                 // no rows: row tile 0 goes on alone
                 skipped += t_end - t_first;
                 fixes += max(0, t_end - t_special);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&unit_empty[unit % CACHE_UNITS]);
                 continue;
             }
             const int node_r = r / args.G, head_r = r - node_r * args.G;
@@ -1057,6 +1068,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     tc_fence_before();
                 }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&unit_empty[unit % CACHE_UNITS]);
         }
     }
 

@@ -644,3 +644,16 @@ def test_long_causal_extension_of_many_row_blocks():
     """Thousands of new rows over a context: row blocks of different lengths, cut anywhere in the line."""
     c = Case([100, 900], [1300, 700], 4, 1, 64, 128, seed=31)
     check_attention(c, run_attention(c, max_new=1300))
+
+
+@pytest.mark.parametrize('heads,kv,dim,most', [(4, 4, 128, 130), (32, 4, 128, 40), (16, 4, 64, 70)])
+@pytest.mark.parametrize('mask', [None, tree])
+def test_two_tile_units_before_many_that_fill_one(heads, kv, dim, most, mask):
+    """With two row tiles, units whose nodes fill one are passed over by row tile 1's warps, which may still be
+    writing the rows of a two-tile unit some units back: each CTA has about 20 units, every 19th of two tiles."""
+    new = [most if i % 19 == 0 else 1 + i % 3 for i in range(600)]
+    c = Case([(i * 37) % 120 for i in range(600)], new, heads, kv, dim, 64, seed=heads, mask=mask)
+    o = run_attention(c, max_new=most)
+    check_attention(c, o)
+    for _ in range(20):
+        assert torch.equal(run_attention(c, max_new=most), o)
