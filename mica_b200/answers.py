@@ -41,12 +41,18 @@ class Scores:
     top_id: torch.Tensor           # int64 [top]
 
 
+def _in_vocabulary(name, least, most, vocab):
+    if least < 0 or most >= vocab:
+        raise ValueError(f'{name}: token {least if least < 0 else most} is not in the vocabulary of {vocab}')
+
+
 class _Trie:
     """The answers of one context: its nodes are their distinct proper prefixes, parents first."""
 
-    def __init__(self, answers):
+    def __init__(self, answers, vocab):
         if not answers or any(len(a) == 0 for a in answers):
             raise ValueError('answers: at least one, none of them empty')
+        _in_vocabulary('answers', min(min(a) for a in answers), max(max(a) for a in answers), vocab)
         self.parents, self.tokens, self.depth = [], [], []
         self.children = [{}]           # of the context, then of each node: token -> place among its row's tokens
         seen = {(): -1}
@@ -84,6 +90,7 @@ class AnswerScorer(Prefill):
         self.cache = paged.PagedCache(c.layers, c.kv_heads, c.head_dim, pages, page, model.device)
         self.head = model.lm_head if model.lm_head is not None else model.embed
         self.chunk = chunk
+        self.vocab = min(self.head.shape[0], model.embed.shape[0])
         self._last = {}                # context -> its last row, final norm applied, bf16 [1, hidden]
 
     # ---- one pass ----------------------------------------------------------------------
@@ -133,10 +140,15 @@ class AnswerScorer(Prefill):
 
     @torch.no_grad()
     def extend(self, sids: Sequence[int], ids: Sequence) -> None:
-        """Appends tokens to contexts (1-D tensors or lists, at least one token each), `chunk` rows at a pass."""
+        """Appends tokens to contexts (1-D tensors or lists, at least one token each), `chunk` rows at a pass.
+        Tokens outside the vocabulary are refused where they are on the host; ids on the device are not looked at."""
         if len(set(sids)) != len(sids) or len(sids) != len(ids):
             raise ValueError(f'extend: {len(ids)} token lists for contexts {list(sids)}')
-        rest = [torch.as_tensor(t, dtype=torch.long, device=self.m.device).reshape(-1) for t in ids]
+        rest = [torch.as_tensor(t, dtype=torch.long).reshape(-1) for t in ids]
+        for t in rest:
+            if not t.is_cuda and t.numel():
+                _in_vocabulary('extend', int(t.min()), int(t.max()), self.vocab)
+        rest = [t.to(self.m.device) for t in rest]
         for sid, t in zip(sids, rest):
             if t.numel() == 0 or self.cache.length(sid) + t.numel() > self.max_len:
                 raise ValueError(f'extend: {t.numel()} tokens on {self.cache.length(sid)} (1 .. {self.max_len})')
@@ -180,7 +192,7 @@ class AnswerScorer(Prefill):
     def _run(self, sids, answers, top):
         if len(set(sids)) != len(sids) or len(sids) != len(answers) or not sids:
             raise ValueError(f'answers: {len(answers)} sets for contexts {list(sids)}')
-        tries = [_Trie(a) for a in answers]
+        tries = [_Trie(a, self.vocab) for a in answers]
         base = [self.cache.length(s) for s in sids]
         for b, t in zip(base, tries):
             if b + 1 + max(t.depth, default=-1) > self.max_len:
