@@ -193,6 +193,9 @@ class AnswerScorer(Prefill):
         if len(set(sids)) != len(sids) or len(sids) != len(answers) or not sids:
             raise ValueError(f'answers: {len(answers)} sets for contexts {list(sids)}')
         tries = [_Trie(a, self.vocab) for a in answers]
+        for sid in sids:
+            if self.cache.length(sid) and sid not in self._last:
+                raise ValueError(f'answers: context {sid} has no last row (its last pass failed): extend it')
         base = [self.cache.length(s) for s in sids]
         for b, t in zip(base, tries):
             if b + 1 + max(t.depth, default=-1) > self.max_len:
@@ -240,10 +243,23 @@ class AnswerScorer(Prefill):
     @torch.no_grad()
     def answer(self, sids: Sequence[int], answers: Sequence[Sequence[Sequence[int]]]) -> list:
         """Scores the answers and appends the likeliest one (the first, if several are) to each context.
-        Returns its index per context. Waits for the device."""
+        Returns its index per context. Waits for the device. Where a chosen answer has no room (max_len, or
+        the pages), no context is changed."""
         out, tries, step = self._run(sids, answers, 0)
         best = [int(i) for i in torch.stack([s.logprob.argmax() for s in out]).tolist()]
+        nodes = [t.nodes[i] for t, i in zip(tries, best)]
+        try:
+            for sid, n in zip(sids, nodes):
+                if self.cache.length(sid) + len(n) + 1 > self.max_len:
+                    raise ValueError(f'answer: {len(n) + 1} tokens on {self.cache.length(sid)} (up to {self.max_len})')
+            self.cache.fits_after(sids, [len(n) for n in nodes], [1] * len(sids))
+        except Exception:
+            self.cache.commit(sids, [0] * len(sids))              # the trees' pages go back
+            raise
         if step is not None:
-            self.cache.keep(sids, step, [t.nodes[i] for t, i in zip(tries, best)])
+            for sid, n in zip(sids, nodes):
+                if n:
+                    del self._last[sid]                           # until the answer's last token has been run
+            self.cache.keep(sids, step, nodes)
         self.extend(sids, [[a[i][-1]] for a, i in zip(answers, best)])
         return best

@@ -194,22 +194,36 @@ class PagedCache:
         self._shares[p] = 1
         return p
 
-    def reserve(self, sids: Sequence[int], new: Sequence[int]) -> None:
-        """Room for `new` more tokens of each sequence: pages are added, and a partly filled page that others
-        share is copied (one launch for all). Raises OutOfPages, with nothing changed, when the pool is full."""
-        if len(set(sids)) != len(sids) or len(sids) != len(new) or any(n < 0 for n in new):
-            raise ValueError(f'reserve: {list(new)} tokens of sequences {list(sids)}')
+    def _fits(self, sequences, free: int) -> None:
+        """Raises OutOfPages when room for n more tokens of each (pages, length, n) takes more than `free` pages."""
         need, own = 0, {}
-        for sid, n in zip(sids, new):
-            pages, length = self._seqs[sid]
+        for pages, length, n in sequences:
             need += max(0, -(-(length + n) // self.page) - len(pages))
             if n and length % self.page and len(pages) > length // self.page:
                 p = pages[length // self.page]
                 own[p] = own.get(p, 0) + 1
         # of the sequences that write a shared page, all take a copy unless no other one holds it
         need += sum(k if self._shares[p] > k else k - 1 for p, k in own.items())
-        if need > len(self._free):
-            raise OutOfPages(f'{need} pages needed, {len(self._free)} free')
+        if need > free:
+            raise OutOfPages(f'{need} pages needed, {free} free')
+
+    def fits_after(self, sids: Sequence[int], kept: Sequence[int], new: Sequence[int]) -> None:
+        """Raises OutOfPages when `new` more tokens of each sequence would not fit once kept[b] reserved rows of it
+        are committed, which gives the other rows' pages back. Nothing is changed."""
+        free, after = len(self._free), []
+        for sid, k, n in zip(sids, kept, new):
+            pages, length = self._seqs[sid]
+            held = pages[:-(-(length + k) // self.page)]
+            free += len(pages) - len(held)
+            after.append((held, length + k, n))
+        self._fits(after, free)
+
+    def reserve(self, sids: Sequence[int], new: Sequence[int]) -> None:
+        """Room for `new` more tokens of each sequence: pages are added, and a partly filled page that others
+        share is copied (one launch for all). Raises OutOfPages, with nothing changed, when the pool is full."""
+        if len(set(sids)) != len(sids) or len(sids) != len(new) or any(n < 0 for n in new):
+            raise ValueError(f'reserve: {list(new)} tokens of sequences {list(sids)}')
+        self._fits([(*self._seqs[sid], n) for sid, n in zip(sids, new)], len(self._free))
         src, dst = [], []
         for sid, n in zip(sids, new):
             pages, length = self._seqs[sid]

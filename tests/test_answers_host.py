@@ -32,6 +32,7 @@ def make(monkeypatch):
         return out if rows is None else out[rows]
 
     monkeypatch.setattr(answers.AnswerScorer, '_rows', rows)
+    monkeypatch.setattr(answers.AnswerScorer, 'logits', lambda self, rows: torch.zeros(rows.shape[0], VOCAB))
 
     def build(pages=20, page=16, max_len=100, chunk=1000):
         s = answers.AnswerScorer.__new__(answers.AnswerScorer)
@@ -74,3 +75,68 @@ def test_contexts_with_tokens_outside_the_vocabulary_are_refused(make, bad):
         with pytest.raises(ValueError, match='vocabulary'):
             s.open(ids)
     assert state(s) == was and len(s.passes) == ran
+
+
+def test_an_answer_that_does_not_fit_changes_nothing(make):
+    """The whole chosen answer has to fit, its last token too: in the positions, and in the pages."""
+    s = make(max_len=20)
+    sids = [s.open([9] * 17), s.open([9] * 5)]
+    was = state(s)
+    with pytest.raises(ValueError):
+        s.answer(sids, [[[1, 2, 3, 4]], [[5]]])
+    assert state(s) == was
+    assert s.answer(sids, [[[1, 2, 3, 4], [0, 0, 0]], [[5]]]) == [1, 0]         # one that is not chosen may be longer
+    assert [s.length(x) for x in sids] == [20, 6] and [s._last[x].tolist() for x in sids] == [[[19.0]], [[5.0]]]
+
+    from mica_b200.paged import OutOfPages
+    s = make(pages=2)
+    sids = [s.open([9] * 13), s.open([9] * 3)]
+    was = state(s)
+    with pytest.raises(OutOfPages):
+        s.answer(sids, [[[1, 2, 3, 4]], [[5, 6]]])
+    assert state(s) == was
+    assert s.answer(sids, [[[1, 2, 3]], [[5, 6]]]) == [0, 0] and [s.length(x) for x in sids] == [16, 5]
+
+
+def test_an_answer_takes_the_pages_that_its_tree_gives_back(make):
+    s = make(pages=4)
+    sids = [s.open([9] * 16), s.open([9] * 15)]
+    # the first tree takes two pages and keeps none but one; the second answer's last token needs one
+    assert s.answer(sids, [[[1] * 20, [0, 0]], [[5, 6]]]) == [1, 0]
+    assert [s.length(x) for x in sids] == [18, 17] and s.cache.free_pages == 0
+
+
+def test_an_answer_of_one_token_to_a_fork_without_a_page_for_its_copy(make):
+    from mica_b200.paged import OutOfPages
+    s = make(pages=1)
+    a = s.open([9] * 5)
+    b = s.fork(a)
+    was = state(s)
+    with pytest.raises(OutOfPages):
+        s.answer([b], [[[1]]])
+    assert state(s) == was
+    s.free(a)
+    assert s.answer([b], [[[1]]]) == [0] and s.length(b) == 6
+
+
+def test_a_context_that_lost_its_last_row_is_not_scored(make, monkeypatch):
+    """An error of the last pass (no memory, say) leaves the kept tokens without a row to go on from."""
+    s = make()
+    sid = s.open([9] * 5)
+    rows = type(s)._rows
+
+    def fails(self, ids, step, pos=None, rows_=None, **kw):
+        if len(ids) == 1:
+            raise MemoryError
+        return rows(self, ids, step, pos=pos, **kw)
+
+    monkeypatch.setattr(type(s), '_rows', fails)
+    with pytest.raises(MemoryError):
+        s.answer([sid], [[[1, 2, 3]]])
+    monkeypatch.setattr(type(s), '_rows', rows)
+    assert s.length(sid) == 7
+    for call in (s.score, s.answer):
+        with pytest.raises(ValueError, match='last row'):
+            call([sid], [[[1]]])
+    s.extend([sid], [[3]])
+    assert s.score([sid], [[[1]]])[0].logprob.shape == (1,) and s._last[sid].tolist() == [[7.0]]
