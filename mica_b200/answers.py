@@ -178,7 +178,8 @@ class AnswerScorer(Prefill):
     def fork(self, sid: int) -> int:
         """A context with the same tokens; its pages are shared until one of the two is extended."""
         new = self.cache.fork(sid)
-        self._last[new] = self._last[sid]
+        if sid in self._last:
+            self._last[new] = self._last[sid]
         return new
 
     def free(self, sid: int) -> None:

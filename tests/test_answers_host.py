@@ -140,3 +140,14 @@ def test_a_context_that_lost_its_last_row_is_not_scored(make, monkeypatch):
             call([sid], [[[1]]])
     s.extend([sid], [[3]])
     assert s.score([sid], [[[1]]])[0].logprob.shape == (1,) and s._last[sid].tolist() == [[7.0]]
+
+
+def test_a_fork_needs_no_last_row(make):
+    """A context that has no tokens yet, or lost its last row, forks as it is."""
+    s = make()
+    a = s.cache.open()
+    b = s.fork(a)
+    assert s.length(b) == 0
+    s.extend([b], [[1, 2]])
+    c = s.fork(b)
+    assert s._last[c] is s._last[b] and s.length(a) == 0 and len(s.cache._seqs) == 3
