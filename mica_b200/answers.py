@@ -29,7 +29,7 @@ import torch.nn.functional as F
 from . import int8_kernels as K
 from . import paged
 from ._native import NORM_WEIGHT
-from .logprobs import token_logprobs
+from .logprobs import MAX_TOP, token_logprobs
 from .prefill import Decoder, Prefill
 
 
@@ -153,6 +153,13 @@ class AnswerScorer(Prefill):
             if t.numel() == 0 or self.cache.length(sid) + t.numel() > self.max_len:
                 raise ValueError(f'extend: {t.numel()} tokens on {self.cache.length(sid)} (1 .. {self.max_len})')
         self.cache.reserve(sids, [t.numel() for t in rest])          # all of it, or nothing is changed
+        try:
+            self._extend(sids, rest)
+        except Exception:
+            self.cache.commit(sids, [0] * len(sids))                  # what is still reserved goes back
+            raise
+
+    def _extend(self, sids, rest):
         at = [0] * len(rest)
         while True:
             todo, room = [], self.chunk
@@ -193,6 +200,8 @@ class AnswerScorer(Prefill):
     def _run(self, sids, answers, top):
         if len(set(sids)) != len(sids) or len(sids) != len(answers) or not sids:
             raise ValueError(f'answers: {len(answers)} sets for contexts {list(sids)}')
+        if not 0 <= top <= min(MAX_TOP, self.vocab):
+            raise ValueError(f'answers: top {top} of {self.vocab} tokens (at most {MAX_TOP})')
         tries = [_Trie(a, self.vocab) for a in answers]
         for sid in sids:
             if self.cache.length(sid) and sid not in self._last:
@@ -201,6 +210,13 @@ class AnswerScorer(Prefill):
         for b, t in zip(base, tries):
             if b + 1 + max(t.depth, default=-1) > self.max_len:
                 raise ValueError(f'answers: they pass {self.max_len} positions')
+        try:
+            return self._run_tries(sids, answers, tries, base, top)
+        except Exception:
+            self.cache.commit(sids, [0] * len(sids))                  # the trees' pages go back
+            raise
+
+    def _run_tries(self, sids, answers, tries, base, top):
         new = [len(t.parents) for t in tries]
         step = None
         last = torch.cat([self._last[s] for s in sids])

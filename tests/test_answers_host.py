@@ -151,3 +151,43 @@ def test_a_fork_needs_no_last_row(make):
     s.extend([b], [[1, 2]])
     c = s.fork(b)
     assert s._last[c] is s._last[b] and s.length(a) == 0 and len(s.cache._seqs) == 3
+
+
+@pytest.mark.parametrize('top', [-1, 33, VOCAB + 1])
+def test_top_is_refused_before_anything_runs(make, top):
+    s = make()
+    sid = s.open([9] * 5)
+    was, ran = state(s), len(s.passes)
+    with pytest.raises(ValueError, match='top'):
+        s.score([sid], [[[1, 2]]], top=top)
+    assert state(s) == was and len(s.passes) == ran
+
+
+def test_an_error_in_a_pass_gives_the_reserved_pages_back(make, monkeypatch):
+    from mica_b200 import answers
+    s = make(chunk=20)
+    sids = [s.open([9] * 5), s.open([9] * 30)]
+    was = state(s)
+
+    def fails(*a, **kw):
+        raise MemoryError
+
+    with monkeypatch.context() as m:
+        m.setattr(answers, 'token_logprobs', fails)
+        for call in (s.score, s.answer):
+            with pytest.raises(MemoryError):
+                call(sids, [[[1, 2] * 20], [[3, 4]]])
+            assert state(s) == was
+    rows = type(s)._rows
+    with monkeypatch.context() as m:
+        m.setattr(type(s), '_rows', fails)
+        with pytest.raises(MemoryError):
+            s.extend(sids, [[1] * 40, [2] * 3])
+        assert state(s) == was
+        # the second pass of 20 rows: the first one's tokens stay, with their last row
+        m.setattr(type(s), '_rows', lambda self, ids, *a, **kw: fails() if len(self.passes) > n else rows(self, ids, *a, **kw))
+        n = len(s.passes)
+        with pytest.raises(MemoryError):
+            s.extend(sids, [[1] * 40, [2] * 3])
+    assert s.length(sids[0]) == 25 and s._last[sids[0]].tolist() == [[24.0]] and s.length(sids[1]) == 30
+    assert s.cache.free_pages == was[1] - 1
