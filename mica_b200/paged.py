@@ -260,6 +260,8 @@ class PagedCache:
 
     def commit(self, sids: Sequence[int], new: Sequence[int]) -> None:
         """The first new[b] appended rows of each sequence become committed tokens."""
+        if len(set(sids)) != len(sids) or len(sids) != len(new):
+            raise ValueError(f'commit: {list(new)} tokens of sequences {list(sids)}')
         for sid, n in zip(sids, new):
             pages, length = self._seqs[sid]
             if n < 0 or length + n > len(pages) * self.page:
@@ -270,7 +272,7 @@ class PagedCache:
 
     def keep(self, sids: Sequence[int], step: Step, keep: Sequence[Sequence[int]]) -> None:
         """Commits the rows keep[b] (increasing) of the step's tree: the accepted tokens of each sequence."""
-        if len(sids) != len(keep) or step.rows is None or len(sids) != len(step.rows):
+        if len(set(sids)) != len(sids) or len(sids) != len(keep) or step.rows is None or len(sids) != len(step.rows):
             raise ValueError(f'keep: {len(keep)} lists for {len(sids)} sequences of a step of this cache')
         for sid, rows, n in zip(sids, keep, step.rows):
             pages, length = self._seqs[sid]

@@ -216,3 +216,21 @@ def test_cache_host_state(monkeypatch):
     for bad in (dict(page=24), dict(head_dim=80), dict(pages=0)):
         with pytest.raises(ValueError):
             paged.PagedCache(**{**dict(layers=1, kv_heads=1, head_dim=64, pages=2, device='cpu'), **bad})
+
+
+def test_commit_and_keep_name_each_sequence_once(monkeypatch):
+    """A sequence named twice would pass the check of its room twice, and lists of two lengths lose their ends."""
+    from mica_b200 import paged
+    monkeypatch.setattr(torch.Tensor, 'pin_memory', lambda t: t)
+    c = paged.PagedCache(1, 1, 64, 10, page=16, device='cpu')
+    a, b = c.open(), c.open()
+    step = c.step([a, b], [10, 10])
+    for sids, new in (([a, a], [10, 10]), ([a, b], [1]), ([a], [1, 1]), ([], [1])):
+        with pytest.raises(ValueError):
+            c.commit(sids, new)
+    for sids, rows in (([a, a], [[0], [0]]), ([a], [[0]]), ([a, b], [[0]])):
+        with pytest.raises(ValueError):
+            c.keep(sids, step, rows)
+    assert c.length(a) == c.length(b) == 0
+    c.commit([a, b], [10, 3])
+    assert c.length(a) == 10 and c.length(b) == 3
