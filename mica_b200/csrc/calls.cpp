@@ -82,17 +82,23 @@ const Tensor* ptr(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 struct Step {
-    const Tensor &table, &base, &cu;
+    Tensor table, base, cu;     // rows of the table any distance apart; copies, made in the call, of what a kernel cannot read
     int B, P;
+    long ld;
     Step(const char* name, const Tensor& t, const Tensor& b, const Tensor& c) : table(t), base(b), cu(c) {
         if (t.dim() != 2 || b.dim() != 1 || c.dim() != 1 || t.size(0) != b.size(0) || c.size(0) != b.size(0) + 1 ||
-            t.size(1) < 1 || t.scalar_type() != at::kInt || b.scalar_type() != at::kInt || c.scalar_type() != at::kInt ||
-            !t.is_contiguous() || !b.is_contiguous() || !c.is_contiguous())
-            value(name, ": table ", t.sizes(), ", base ", b.sizes(), ", cu ", c.sizes(), " (int32, contiguous)");
+            t.size(1) < 1 || t.scalar_type() != at::kInt || b.scalar_type() != at::kInt || c.scalar_type() != at::kInt)
+            value(name, ": table ", t.sizes(), ", base ", b.sizes(), ", cu ", c.sizes(), " (int32)");
         if (t.size(0) > std::numeric_limits<int>::max() || t.size(1) > std::numeric_limits<int>::max())
             value(name, ": table ", t.sizes());
         B = static_cast<int>(t.size(0));
         P = static_cast<int>(t.size(1));
+    }
+    void read() {               // on the call's device and stream
+        if ((P > 1 && table.stride(1) != 1) || (B > 1 && table.stride(0) < P)) table = table.contiguous();
+        base = base.contiguous();
+        cu = cu.contiguous();
+        ld = B > 1 ? table.stride(0) : P;
     }
 };
 
@@ -131,7 +137,7 @@ Tensor append(const Tensor& qkv_, const Tensor& q_w, const Tensor& k_w, const Te
               const OptTensor& pos_, double eps) {
     const char* name = "append";
     const Pages pg(name, k, v);
-    const Step st(name, table, base, cu);
+    Step st(name, table, base, cu);
     if (qkv_.dim() != 2 || heads < 1 || heads > 4096 || qkv_.size(1) != (heads + 2 * pg.kv) * pg.d || qkv_.stride(1) != 1)
         value(name, ": qkv ", qkv_.sizes(), " for ", heads, " + 2 x ", pg.kv, " heads of ", pg.d);
     if (q_w.dim() != 1 || q_w.size(0) != pg.d || k_w.sizes() != q_w.sizes() || cos.dim() != 2 || cos.sizes() != sin.sizes() ||
@@ -147,6 +153,7 @@ Tensor append(const Tensor& qkv_, const Tensor& q_w, const Tensor& k_w, const Te
     cuda(name, qkv_, {&q_w, &k_w, &cos, &sin, &k, &v, &table, &base, &cu, ptr(pos_)});
     no_grad(name, {&qkv_, &q_w, &k_w});
     const c10::cuda::CUDAGuard guard(qkv_.device());
+    st.read();
     if (n == 0 || st.B == 0) return at::zeros({n, heads * pg.d}, qkv_.options());      // padding rows alone
     const Tensor qkv = rows16(qkv_), qw = rows16(q_w.contiguous().unsqueeze(0)), kw = rows16(k_w.contiguous().unsqueeze(0));
     const Tensor pos = pos_ ? pos_->contiguous() : Tensor();
@@ -154,7 +161,7 @@ Tensor append(const Tensor& qkv_, const Tensor& q_w, const Tensor& k_w, const Te
     status("mica_cache_append",
            f_append(qkv.data_ptr(), row_stride(qkv), qw.data_ptr(), kw.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.size(0),
                     pos_ ? pos.data_ptr<int64_t>() : nullptr, q.data_ptr(), heads * pg.d, k.data_ptr(), v.data_ptr(), pg.stride,
-                    pg.pages, pg.page, table.data_ptr<int>(), st.P, st.P, base.data_ptr<int>(), cu.data_ptr<int>(), st.B,
+                    pg.pages, pg.page, st.table.data_ptr<int>(), st.ld, st.P, st.base.data_ptr<int>(), st.cu.data_ptr<int>(), st.B,
                     static_cast<int>(n), static_cast<int>(heads), pg.kv, pg.d, static_cast<float>(eps), stream_of(qkv_)));
     return q;
 }
@@ -164,7 +171,7 @@ Tensor attention(const Tensor& q_, const Tensor& k, const Tensor& v, const Tenso
                  std::optional<int64_t> max_new) {
     const char* name = "attention";
     const Pages pg(name, k, v);
-    const Step st(name, table, base, cu);
+    Step st(name, table, base, cu);
     if (q_.dim() != 2 || heads < 1 || heads > 4096 || heads % pg.kv || heads / pg.kv > 128 || q_.size(1) != heads * pg.d ||
         q_.stride(1) != 1)
         value(name, ": q ", q_.sizes(), " for ", heads, " heads of ", pg.d, " over ", pg.kv, " K/V heads");
@@ -172,13 +179,14 @@ Tensor attention(const Tensor& q_, const Tensor& k, const Tensor& v, const Tenso
     const int64_t n = q_.size(0);
     int_rows(name, q_);
     if (mask && (mask->dim() != 2 || mask->scalar_type() != at::kLong || mask->size(0) != n || mask->size(1) < 1 ||
-                 !mask->is_contiguous() || mask->size(1) > (1 << 26)))
-        value(name, ": mask ", mask->scalar_type(), " ", mask->sizes(), " for ", n, " rows (int64 [rows, words], contiguous)");
+                 mask->size(1) > (1 << 26)))
+        value(name, ": mask ", mask->scalar_type(), " ", mask->sizes(), " for ", n, " rows (int64 [rows, words])");
     const double scale = scale_ ? *scale_ : 1.0 / std::sqrt(static_cast<double>(pg.d));
     if (!(scale > 0.0 && scale <= std::numeric_limits<float>::max())) value(name, ": scale ", scale);
     cuda(name, q_, {&k, &v, &table, &base, &cu, ptr(mask)});
     no_grad(name, {&q_, &k, &v});
     const c10::cuda::CUDAGuard guard(q_.device());
+    st.read();
     if (n == 0 || st.B == 0) return at::zeros({n, heads * pg.d}, q_.options());
     const Tensor q = rows16(q_);
     Tensor out = at::empty({n, heads * pg.d}, q_.options());
@@ -186,10 +194,11 @@ Tensor attention(const Tensor& q_, const Tensor& k, const Tensor& v, const Tenso
     const size_t need = f_attention_bytes(static_cast<int>(n), most, static_cast<int>(heads), pg.kv, pg.d);
     const Tensor ws = at::empty({static_cast<int64_t>(need)}, q_.options().dtype(at::kByte));
     const int words = mask ? static_cast<int>(mask->size(1)) : 0;
+    const Tensor bits = !mask ? Tensor() : (words > 1 && mask->stride(1) != 1) || (n > 1 && mask->stride(0) < words) ? mask->contiguous() : *mask;
     status("mica_cache_attention",
            f_attention(q.data_ptr(), row_stride(q), k.data_ptr(), v.data_ptr(), pg.stride, pg.pages, pg.page,
-                       table.data_ptr<int>(), st.P, st.P, base.data_ptr<int>(), cu.data_ptr<int>(),
-                       mask ? mask->data_ptr<int64_t>() : nullptr, words, words, st.B, static_cast<int>(n), most,
+                       st.table.data_ptr<int>(), st.ld, st.P, st.base.data_ptr<int>(), st.cu.data_ptr<int>(),
+                       mask ? bits.data_ptr<int64_t>() : nullptr, mask && n > 1 ? bits.stride(0) : words, words, st.B, static_cast<int>(n), most,
                        static_cast<int>(heads), pg.kv, pg.d, static_cast<float>(scale), out.data_ptr(), heads * pg.d,
                        ws.data_ptr(), need, stream_of(q_)));
     return out;
@@ -243,22 +252,23 @@ Tensor keep_tokens(const Tensor& pool, const Tensor& table, const Tensor& base, 
         !one_of(pool.size(5), {64, 128}))
         value(name, ": pool ", pool.scalar_type(), " ", pool.sizes());
     const long bytes = page_bytes(name, pool);
-    const Step st(name, table, base, cu);
+    Step st(name, table, base, cu);
     if (keep_.dim() != 2 || keep_.size(0) != st.B || n_keep_.dim() != 1 || n_keep_.size(0) != st.B ||
         keep_.scalar_type() != at::kInt || n_keep_.scalar_type() != at::kInt || keep_.size(1) > std::numeric_limits<int>::max())
         value(name, ": keep ", keep_.scalar_type(), " ", keep_.sizes(), ", n_keep ", n_keep_.scalar_type(), " ", n_keep_.sizes(),
               " for ", st.B, " sequences (int32)");
     cuda(name, pool, {&table, &base, &cu, &keep_, &n_keep_});
     const c10::cuda::CUDAGuard guard(pool.device());
-    if (st.B == 0 || keep_.size(1) == 0) return base.clone();
+    st.read();
+    if (st.B == 0 || keep_.size(1) == 0) return st.base.clone();
     const Tensor keep = keep_.contiguous(), n_keep = n_keep_.contiguous();
-    Tensor out = at::empty_like(base);
+    Tensor out = at::empty_like(st.base);
     const int most = static_cast<int>(keep.size(1));
     const long stride = pool.size(0) > 1 ? pool.stride(0) * 2 : bytes;
     status("mica_cache_keep",
            f_keep(pool.data_ptr(), stride, static_cast<int>(pool.size(1) * 2 * pool.size(3)), static_cast<int>(pool.size(0)),
-                  static_cast<int>(pool.size(4)), static_cast<int>(pool.size(5)), table.data_ptr<int>(), st.P, st.P,
-                  base.data_ptr<int>(), cu.data_ptr<int>(), st.B, keep.data_ptr<int>(), most, n_keep.data_ptr<int>(), most,
+                  static_cast<int>(pool.size(4)), static_cast<int>(pool.size(5)), st.table.data_ptr<int>(), st.ld, st.P,
+                  st.base.data_ptr<int>(), st.cu.data_ptr<int>(), st.B, keep.data_ptr<int>(), most, n_keep.data_ptr<int>(), most,
                   out.data_ptr<int>(), stream_of(pool)));
     return out;
 }

@@ -33,8 +33,8 @@ PAGES = (16, 32, 64, 128)      # tokens a page may hold
 
 
 class Step:
-    """The rows of one pass over the cache, described by device tensors (a captured graph serves new
-    values in them):
+    """The rows of one pass over the cache, described by device tensors, taken as they are, whatever their strides
+    (a captured graph serves new values in them):
 
       table int32 [B, P]   pages of each sequence      base int32 [B]   tokens already committed
       cu    int32 [B + 1]  rows cu[b] .. cu[b+1] belong to sequence b (cu[0] = 0; rows behind cu[B]
@@ -54,15 +54,8 @@ class Step:
             raise ValueError(f'Step: table {tuple(table.shape)}, base {tuple(base.shape)}, cu {tuple(cu.shape)}')
         if not table.dtype == base.dtype == cu.dtype == torch.int32:
             raise ValueError(f'Step: int32 tensors, not {table.dtype}, {base.dtype}, {cu.dtype}')
-        if not table.is_contiguous():
-            table = table.contiguous()
-        if not base.is_contiguous() or not cu.is_contiguous():
-            base, cu = base.contiguous(), cu.contiguous()
-        if mask is not None:
-            if mask.dim() != 2 or mask.dtype != torch.int64 or mask.shape[1] < 1:
-                raise ValueError(f'Step: mask is int64 [rows, words], not {mask.dtype} {tuple(mask.shape)}')
-            if not mask.is_contiguous():
-                mask = mask.contiguous()
+        if mask is not None and (mask.dim() != 2 or mask.dtype != torch.int64 or mask.shape[1] < 1):
+            raise ValueError(f'Step: mask is int64 [rows, words], not {mask.dtype} {tuple(mask.shape)}')
         if max_new is not None and max_new < 0:
             raise ValueError(f'Step: max_new {max_new}')
         self.table, self.base, self.cu, self.mask, self.max_new = table, base, cu, mask, max_new

@@ -657,3 +657,56 @@ def test_two_tile_units_before_many_that_fill_one(heads, kv, dim, most, mask):
     check_attention(c, o)
     for _ in range(20):
         assert torch.equal(run_attention(c, max_new=most), o)
+
+
+def test_strided_steps_and_their_new_values_in_a_graph():
+    """Every second word of wider tables: the same bits, and a replayed graph reads what is written there."""
+    from mica_b200 import paged
+    heads, kv, dim = 8, 2, 64
+    c = Case([100, 37, 5], [9, 1, 4], heads, kv, dim, 16, seed=2, mask=tree)
+    i32 = {'dtype': torch.int32, 'device': 'cuda'}
+
+    def spread(t):
+        w = torch.full([2 * n for n in t.shape], -9, dtype=t.dtype, device='cuda')
+        w[tuple(slice(None, None, 2) for _ in t.shape)] = t
+        return w
+
+    wide = [spread(t) for t in (c.table, c.base, c.cu, c.mask)]
+    table, base, cu, mask = wide[0][::2, ::2], wide[1][::2], wide[2][::2], wide[3][::2, ::2]
+    step = paged.Step(table, base, cu, mask=mask)
+    o = run_attention(c)
+    assert torch.equal(paged.attention(c.q, c.k, c.v, step, heads), o)
+    cos, sin = tables(dim, 300)
+    one = torch.ones(dim, dtype=torch.bfloat16, device='cuda')
+    qkv = torch.randn(c.n, (heads + 2 * kv) * dim, device='cuda').bfloat16()
+    keep, n = torch.tensor([[1, 3], [0, 0], [1, 2]], **i32), torch.tensor([2, 1, 2], **i32)
+
+    def run(step, pool):
+        k, v = pool[:, 0, 0], pool[:, 0, 1]
+        q = paged.append(qkv, one, one, cos, sin, k, v, step, heads)
+        a = paged.attention(q, k, v, step, heads)
+        return a, paged.keep_tokens(pool, step, keep, n)
+
+    pool, again = c.pool.clone(), c.pool.clone()
+    for _ in range(2):
+        ref = run(c.step(), pool)
+        got = run(step, again)
+        assert torch.equal(ref[0], got[0]) and torch.equal(ref[1], got[1])
+        assert torch.equal(pool.view(torch.int16), again.view(torch.int16))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run(step, again)
+    rows = c.table.flip(0).contiguous()                     # other pages, other lengths
+    for t, new in ((c.table, rows), (c.base, torch.tensor([3, 20, 60], **i32)), (c.cu, torch.tensor([0, 4, 6, 14], **i32))):
+        t.copy_(new)
+    table.copy_(c.table)
+    base.copy_(c.base)
+    cu.copy_(c.cu)
+    keep.copy_(torch.tensor([[1, 2], [0, 1], [4, 7]], **i32))
+    c.table[c.table < 0] = 0
+    table.copy_(c.table)
+    pool.copy_(again)
+    g.replay()
+    ref = run(c.step(), pool)
+    assert torch.equal(ref[0], out[0]) and torch.equal(ref[1], out[1])
+    assert torch.equal(pool.view(torch.int16), again.view(torch.int16))

@@ -234,3 +234,15 @@ def test_commit_and_keep_name_each_sequence_once(monkeypatch):
     assert c.length(a) == c.length(b) == 0
     c.commit([a, b], [10, 3])
     assert c.length(a) == 10 and c.length(b) == 3
+
+
+def test_a_step_keeps_the_tensors_it_is_given():
+    """Whatever their strides: a captured graph reads new values where they are written."""
+    from mica_b200 import paged
+    i32 = {'dtype': torch.int32}
+    table, base, cu = torch.zeros(2, 9, **i32), torch.zeros(4, **i32), torch.zeros(6, **i32)
+    mask = torch.zeros(5, 3, dtype=torch.int64)
+    step = paged.Step(table[:, ::3], base[::2], cu[::2], mask=mask.t())
+    for t in (table, base, cu, mask):
+        t += 1
+    assert step.table.sum() == 6 and step.base.sum() == 2 and step.cu.sum() == 3 and step.mask.sum() == 15
