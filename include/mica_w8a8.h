@@ -303,7 +303,8 @@ int mica_attention_prefill(const void* qkv, long ld_qkv, void* out, long ld_out,
  *   cu    [B+1]  int32, increasing, cu[0] = 0  rows cu[b]..cu[b+1] of the N rows are sequence b's
  * Row i of sequence b is cache index base[b] + i: slot index % page of page table[b][index / page].
  * Rows behind cu[B] are padding. A base, page number or position out of range records
- * MICA_DEV_BAD_PAGE; what it names is neither read nor written.                            */
+ * MICA_DEV_BAD_PAGE; what it names is neither read nor written. So does a cu that passes N (the
+ * rows below N are served), starts below zero or runs backwards (the attention is zero then).   */
 
 /* Per-head RMSNorm of q and k, rotary embedding and the write of k and v into their pages, in
  * one pass over the QKV projection's output qkv [N, ld] (q: H*D | k: KV*D | v: KV*D):

@@ -8,7 +8,9 @@
 //
 // Every index read from device memory is checked before it is used: a sequence whose base or rows
 // do not fit its table, or a page number outside the pool, records MICA_DEV_BAD_PAGE in the device
-// error word and touches no memory.
+// error word and touches no memory. A cu that passes the step's rows is recorded too (the rows that are
+// there are served), and one that starts below zero or runs backwards: attention gives zeros then, append
+// serves the rows that lie between both ends of a sequence. Rows that are no sequence's are padding.
 #pragma once
 
 #include "qk_rope.cuh"
@@ -27,6 +29,13 @@ struct CachePlan {
 
 __device__ __forceinline__ void record_bad_page() { atomicExch(&g_dev_error, MICA_DEV_BAD_PAGE); }
 
+// Records a cu that runs backwards, starts below zero or passes the rows; a whole warp calls it.
+__device__ __forceinline__ void cache_check_cu(const CachePlan& p) {
+    bool bad = p.cu[0] < 0 || p.cu[p.B] > p.N;
+    for (int b = threadIdx.x & 31; b < p.B; b += 32) bad = bad || p.cu[b] > p.cu[b + 1];
+    if (bad) record_bad_page();
+}
+
 // Sequence of row `row`: the b with cu[b] <= row < cu[b+1], or -1 for a row behind the last
 // sequence. Whole-warp search: each level splits the range 32 ways, one load per lane, so 1024
 // sequences take two loads in a row.
@@ -42,7 +51,7 @@ __device__ __forceinline__ int cache_sequence_of(const CachePlan& p, int row) {
         lo += taken;
         n = step == 1 ? 0 : min(step - 1, n - taken);
     }
-    return lo < p.B && row >= p.cu[lo] ? lo : -1;
+    return lo < p.B && row >= p.cu[lo] && row < p.cu[lo + 1] ? lo : -1;
 }
 
 // Page number and slot of cache index `index` of sequence b; false when it is not in the table or
@@ -136,6 +145,7 @@ __global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a
                 *reinterpret_cast<uint2*>(q + static_cast<long>(h) * D + D / 2) = make_uint2(0u, 0u);
             }
         }
+        if (w == 0) cache_check_cu(a.plan);
         return;
     }
     const auto pair = [&](const __nv_bfloat16* t, uint2& l, uint2& h) {
@@ -199,6 +209,7 @@ __global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a
             }
         }
     }
+    if (w == 0) cache_check_cu(a.plan);          // one warp of the grid, its row sent
 }
 
 // The same for many rows: a CTA takes every grid-th row through a ring in shared memory. One warp looks
@@ -260,7 +271,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32 + 64, APPEND_CTAS) cache_app
                     if (a.plan.cu[lo + half + 1] <= row) { lo += half + 1; n -= half + 1; }
                     else n = half;
                 }
-                if (lo < a.plan.B && row >= a.plan.cu[lo]) {
+                if (lo < a.plan.B && row >= a.plan.cu[lo] && row < a.plan.cu[lo + 1]) {
                     const int base = a.plan.base[lo];
                     const long index = static_cast<long>(base) + (row - a.plan.cu[lo]);
                     int page = 0, slot = 0;
@@ -297,6 +308,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32 + 64, APPEND_CTAS) cache_app
                 if (++st == stages) { st = 0; par ^= 1u; }
             }
         }
+        if (blockIdx.x == 0) cache_check_cu(a.plan);
         // copies in flight land before shared memory is released
         if (lane == 0)
             for (int i = max(0, rows - stages); i < rows; ++i)

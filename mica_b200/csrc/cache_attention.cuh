@@ -83,10 +83,9 @@ struct CacheSeq {
 };
 __device__ __forceinline__ CacheSeq cache_seq(const CachePlan& p, int b) {
     CacheSeq s;
-    s.row0 = p.cu[b];
-    s.T = p.cu[b + 1] - s.row0;
+    s.row0 = min(max(p.cu[b], 0), p.N);
+    s.T = max(min(p.cu[b + 1], p.N) - s.row0, 0);
     s.base = p.base[b];
-    if (s.row0 < 0 || s.T < 0 || s.row0 > p.N || s.T > p.N - s.row0) s.T = 0;
     const long keys = static_cast<long>(s.base) + s.T;
     s.keys = s.base < 0 || keys > (static_cast<long>(p.P) << p.page_log2) ? 0 : static_cast<int>(keys);
     return s;
@@ -122,8 +121,10 @@ struct CachePlace {             // a place of the line: the off-th of sequence b
     long total;
     long off;
     int b;
+    bool ordered;               // cu starts at zero or above and does not run backwards
 };
-// The line's length and the sequence that holds place `first(total)`; every thread of the block calls it.
+// The line's length and the sequence that holds place `first(total)`; every thread of the block calls it. A step
+// whose cu runs backwards (two sequences may claim a row) or starts below zero has no line (total 0, ordered false).
 template <int NT, typename F>
 __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, int R, bool causal, F first) {
     __shared__ long s_warp[32];
@@ -147,7 +148,10 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
         return v;
     };
     const auto tiles = [&](int b) { return b < p.B ? KV * CacheCost<NT>::seq(cache_seq(p, b), R, causal) : 0l; };
+    const auto backwards = [&](int b) { return b < p.B && (p.cu[b] < 0 || p.cu[b] > p.cu[b + 1]); };
+    const CachePlace none{0, 0, -1, false};
     if (p.B <= 32) {                                 // every warp by itself
+        if (__any_sync(0xffffffffu, backwards(lane))) return none;
         const long n = tiles(lane);
         long end = n;
 #pragma unroll
@@ -158,8 +162,11 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
         const long total = __shfl_sync(0xffffffffu, end, 31), t = first(total);
         const uint32_t here = __ballot_sync(0xffffffffu, t >= end - n && t < end);
         const int b = __ffs(here) - 1;
-        return CachePlace{total, t - __shfl_sync(0xffffffffu, end - n, max(b, 0)), b};
+        return CachePlace{total, t - __shfl_sync(0xffffffffu, end - n, max(b, 0)), b, true};
     }
+    bool back = false;
+    for (int b = threadIdx.x; b < p.B; b += blockDim.x) back = back || backwards(b);
+    if (__syncthreads_or(back)) return none;
     const long mine = tiles(threadIdx.x);
     long total = 0;
     if (threadIdx.x == 0) { s_b = -1; s_off = 0; }
@@ -170,7 +177,7 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
             s_off = t - (end - mine);
         }
         __syncthreads();
-        return CachePlace{total, s_off, s_b};
+        return CachePlace{total, s_off, s_b, true};
     }
     long sum = mine;
     for (int b = threadIdx.x + blockDim.x; b < p.B; b += blockDim.x) sum += tiles(b);
@@ -189,7 +196,7 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
         if (before > t) break;
     }
     __syncthreads();
-    return CachePlace{total, s_off, s_b};
+    return CachePlace{total, s_off, s_b, true};
 }
 
 // The runs of the CTAs: total / used places each, the first total % used one more. Fewer CTAs are used
@@ -320,13 +327,18 @@ __device__ __forceinline__ void mask_bits(const unsigned long long* m, int words
 }
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
-// Rows behind the last sequence become zero; the whole block calls it.
-__device__ __forceinline__ void cache_zero_padding(const CacheAttnArgs& args, int D) {
-    const int end = min(max(args.plan.cu[args.plan.B], 0), args.plan.N);
+// Rows before the first sequence and behind the last become zero, all of them in a step without order; a cu that
+// passes the rows, or runs backwards, is recorded. The whole block calls it.
+__device__ __forceinline__ void cache_zero_padding(const CacheAttnArgs& args, int D, bool ordered) {
+    const int N = args.plan.N, past = args.plan.cu[args.plan.B];
+    if (blockIdx.x == 0 && threadIdx.x == 0 && (!ordered || past > N)) record_bad_page();
+    const int first = ordered ? min(args.plan.cu[0], N) : 0, end = ordered ? min(past, N) : 0;
     const int vecs = args.KV * args.G * D / 8;
-    for (long row = end + static_cast<long>(blockIdx.x); row < args.plan.N; row += gridDim.x)
+    for (long i_row = blockIdx.x; i_row < N - (end - first); i_row += gridDim.x) {
+        const long row = i_row < first ? i_row : i_row - first + end;
         for (int i = threadIdx.x; i < vecs; i += blockDim.x)
             *reinterpret_cast<uint4*>(args.out + row * args.ldo + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+    }
 }
 
 // The keys k0 .. k0 + 127 that node `node` of unit u's sequence sees (row: its row of the step), one bit
@@ -483,7 +495,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     if (cta >= share.used || place.b < 0 ||
         !wk.start(plan, args.KV, R, causal, place.b, place.off, share.at(cta + 1) - share.at(cta))) {
         if (threadIdx.x == 0) args.cuts[2 * cta] = make_int4(0, 0, 0, 0);
-        cache_zero_padding(args, D);
+        cache_zero_padding(args, D, place.ordered);
         return;
     }
 
@@ -1079,7 +1091,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         tc_fence_after();
         tmem_free(tmem, 512);
     }
-    cache_zero_padding(args, D);
+    cache_zero_padding(args, D, true);
 }
 
 // Adds up the parts of each divided unit, always in the same order. Blocks (c, y): the unit that CTA c + 1 is

@@ -17,7 +17,8 @@ rows (mica_b200.answers puts them together). The reference keeps whole-prefix st
 Errors follow fused_kernels: ValueError for arguments that fit no call, RuntimeError for what the
 kernels do not serve (a CPU tensor, another dtype, another GPU). There is no CPU branch. What a
 step's tables hold is on the device: a base, page number or position out of range touches nothing
-and is recorded in the device error word (mica_device_error: bad_page).
+and is recorded in the device error word (mica_device_error: bad_page), as is a cu that passes the
+rows (those that are there are served) or runs backwards (attention is zero).
 """
 from __future__ import annotations
 

@@ -710,3 +710,62 @@ def test_strided_steps_and_their_new_values_in_a_graph():
     ref = run(c.step(), pool)
     assert torch.equal(ref[0], out[0]) and torch.equal(ref[1], out[1])
     assert torch.equal(pool.view(torch.int16), again.view(torch.int16))
+
+
+def _error():
+    import ctypes
+
+    from mica_b200 import _native as N
+    code = ctypes.c_int(0)
+    N.call('mica_device_error', ctypes.byref(code), torch.cuda.current_stream().cuda_stream)
+    return code.value
+
+
+@pytest.mark.parametrize('pad', [0, 3000])            # append: a warp a row, and the ring
+@pytest.mark.parametrize('seqs', [3, 40, 700])        # the three ways to find a place in the line
+def test_row_offsets_out_of_range_are_recorded(seqs, pad):
+    """cu behind the rows: those that are there are served, by append and attention alike. cu that runs backwards
+    or starts below zero: zeros. Every row is written either way."""
+    from mica_b200 import paged
+    heads, kv, dim = 4, 2, 64
+    new = [2 + i % 3 for i in range(seqs - 1)] + [6 + pad]
+    c = Case([(i * 7) % 40 for i in range(seqs)], new, heads, kv, dim, 16, seed=seqs)
+    cos, sin = tables(dim, 5000)
+    one = torch.ones(dim, dtype=torch.bfloat16, device='cuda')
+    qkv = torch.randn(c.n, (heads + 2 * kv) * dim, device='cuda').bfloat16()
+    good, was = c.cu.clone(), c.pool.clone()
+
+    def near(a, b):
+        """The line is cut elsewhere: two results, each within u (|o| + sum p |v|) of the exact one, |v| < 5.6."""
+        return bool((a.float() - b.float()).abs().max() <= 2 * U * 2 * 5.6)
+
+    def run(n):
+        pool = was.clone()
+        k, v = pool[:, 0, 0], pool[:, 0, 1]
+        odd = [torch.full_like(c.q[:n], float('nan')) for _ in range(2)]
+        del odd                                         # what the outputs' memory may hold
+        step = paged.Step(c.table, c.base, c.cu)
+        q = paged.append(qkv[:n], one, one, cos, sin, k, v, step, heads)
+        first = _error()
+        return q, paged.attention(q, k, v, step, heads), first, _error()
+
+    _error()
+    q, o, e1, e2 = run(c.n)
+    assert (e1, e2) == (0, 0) and torch.isfinite(o).all()
+    n = c.n - 4                                         # the last sequence passes the rows
+    c.cu[-1] += 1000
+    qs, os_, e1, e2 = run(n)
+    assert (e1, e2) == (9, 9) and torch.equal(qs, q[:n]) and near(os_, o[:n])
+    c.cu.copy_(good)
+    c.cu[1] = c.cu[2] + 1                               # runs backwards
+    qs, os_, e1, e2 = run(c.n)
+    assert (e1, e2) == (9, 9) and float(os_.float().abs().max()) == 0.0 and torch.isfinite(qs).all()
+    c.cu.copy_(good)
+    c.cu[0] = -1
+    qs, os_, e1, e2 = run(c.n)
+    assert (e1, e2) == (9, 9) and float(os_.float().abs().max()) == 0.0
+    c.cu.copy_(good)
+    c.cu[0] = 1                                         # a row before the first sequence is padding
+    qs, os_, e1, e2 = run(c.n)
+    assert (e1, e2) == (0, 0) and float(qs[0].float().abs().max()) == 0.0 and float(os_[0].float().abs().max()) == 0.0
+    assert near(os_[new[0]:], o[new[0]:])
