@@ -459,7 +459,9 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
             }
             if (my_single >= 0) {
                 top = max_nan(top, single);
-                sums = lp_join(sums, LpSums{max_nan(single, LP_FLOOR) * kLog2e, 1.f, 0.f});
+                // with the rounding of mc in its weight, as every other element's
+                const float z = max_nan(single, LP_FLOOR), mc = z * kLog2e, d = fmaf(z, kLog2e, -mc), x = fast_exp2(d);
+                sums = lp_join(sums, LpSums{mc, x, d * x});
             }
             const int slot = nth & 1;
             if (nth >= 2) mbar_wait(&sh.done[slot], ((nth >> 1) - 1) & 1u, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);

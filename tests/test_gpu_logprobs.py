@@ -148,3 +148,21 @@ def test_same_bits_again_on_other_streams_and_in_graphs():
         torch.cuda.synchronize()
         for o in outs:
             assert all(torch.equal(a, b) for a, b in zip(o, ref))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('big', [1000.0, 30000.0, 100000.0])
+def test_a_dominating_logit_at_either_end(dtype, big):
+    """The elements before and behind a row's 16-byte vectors weigh as they would inside one: log probability and
+    entropy near zero for a logit far above the rest, at every offset within 16 bytes."""
+    if dtype == torch.float16 and big > 65504:
+        return
+    wide = torch.randn(4, 5011, device='cuda').to(dtype)
+    for off in range(17):
+        z = wide[:, off:off + 4001].clone().new_zeros(4, 5011)[:, off:off + 4001]
+        z.copy_(wide[:, off:off + 4001])
+        z[0, 0] = z[1, 4000] = z[2, 1] = z[3, 3998] = big
+        z[0, 4000] = big                              # and shared with the other end
+        ids = torch.tensor([[0, 4000], [4000, 0], [1, 0], [3998, 2]], device='cuda')
+        lp, ent, _, _ = check(z, ids, 2)
+        assert lp[1, 0].abs() < 1e-5 and ent[1] < 1e-5 and abs(float(lp[0, 0]) + 0.6931472) < 1e-5
