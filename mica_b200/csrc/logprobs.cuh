@@ -55,9 +55,11 @@ constexpr int LP_BACK = 768;             // vectors read again at once
 constexpr int LP_CLUSTER = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// Logits are held above this in the sums, so that a weight of zero meets no infinity; a row whose
-// maximum is not well above it (or is beyond its negative) is computed again without the limit.
-constexpr float LP_FLOOR = -1e38f;
+// Logits are held above -2^23 in the sums (2^23 is a bf16 number too), and a row whose maximum is beyond 2^23 or
+// not well above -2^23 is computed again without the limit: the pass's weights are 2^fma(z, log2e, -mc), so all of
+// them, the largest's too, carry mc's rounding as a factor, which cancels but has to be small; up to |mc| = 2^24
+// it is within 2^-0.5 .. 2^0.5. Below the limit a weight is 0 in any row that is not computed again.
+constexpr float LP_FLOOR = -8388608.f;
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
@@ -698,7 +700,7 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
             float m = -INFINITY, logs = 0.f, ent = kLn2 * (log2s - sums.w / sums.s);
             // nothing allowed; or beyond the range of the sums, or NaN
             const bool none = top_all == -INFINITY;
-            const bool odd = !none && !(sums.mc > 0.1f * LP_FLOOR && sums.mc < -LP_FLOOR && sums.s < INFINITY);
+            const bool odd = !none && !(sums.mc > 0.1f * LP_FLOOR && sums.mc < -LP_FLOOR && sums.s > 0.f && sums.s < INFINITY);
             if (none) ent = 0.f;
             if (odd) lp_row_plain(a, r.z, e, g, wk.red, m, logs, ent);
             const auto lp = [&](float f) {

@@ -166,3 +166,35 @@ def test_a_dominating_logit_at_either_end(dtype, big):
         ids = torch.tensor([[0, 4000], [4000, 0], [1, 0], [3998, 2]], device='cuda')
         lp, ent, _, _ = check(z, ids, 2)
         assert lp[1, 0].abs() < 1e-5 and ent[1] < 1e-5 and abs(float(lp[0, 0]) + 0.6931472) < 1e-5
+
+
+def check_wide(z, ids, top):
+    """Logits of any finite size: the exact values are within fp32's range or infinite; each is a difference
+    z - m of two fp32 values, rounded once (2^-24 of it), minus log S, and rounded again."""
+    from mica_b200 import logprobs
+    lp, ent, tl, ti = logprobs.token_logprobs(z, ids, top)
+    rl, re, rt, ri = reference(z, ids, top)
+    for got, ref in ((lp, rl), (ent, re), (tl, rt)):
+        r32 = ref.float()
+        fin = torch.isfinite(r32)
+        assert torch.equal(fin, torch.isfinite(got)) and torch.equal(r32[~fin], got[~fin])
+        err = (got.double() - ref)[fin].abs()
+        assert (err <= 2.0 ** -22 * ref[fin].abs() + 2.0 ** -23 * 60 + 2.0 ** -20 * (1 + ref[fin].abs().clamp(max=60))).all(), float(err.max())
+    assert torch.equal(ti, ri)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('n', [1, 5, 400])            # rows in parts, and one after another
+@pytest.mark.parametrize('big', [1e5, 1e6, 5e6, 9e6, 2e7, 1e8, 5e9, 1e10, 1e12, 1e15, 1e20, 1e30, 3e38])
+def test_rows_of_large_logits(dtype, n, big):
+    """Maxima of any size and sign, alone, in numbers, and as a step of ordinary logits."""
+    g = torch.Generator(device='cuda').manual_seed(n)
+    z = torch.randn(5 * n, 3003, generator=g, device='cuda')
+    z[0::5, 17] = big
+    z[1::5, 100:2900] = big
+    z[2::5] = -big                                    # all alike
+    z[3::5] = -big
+    z[3::5, 3000] = -big / 2
+    z[4::5] *= big / 5                                # spread over the whole size
+    ids = torch.tensor([[17, 3000, 2, 3002]], device='cuda').repeat(5 * n, 1)
+    check_wide(z.to(dtype), ids, 6)
