@@ -706,6 +706,7 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
             const auto lp = [&](float f) {
                 if (none) return -INFINITY;
                 if (odd) return (f - m) - logs;
+                if (f < 8.f * LP_FLOOR) return f - (sums.mc + log2s) * kLn2;       // f * log2e may pass fp32's range
                 return (fmaf(f, kLog2e, -sums.mc) - log2s) * kLn2;
             };
             if (e == 0) a.entropy[row] = ent;

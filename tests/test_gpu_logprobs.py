@@ -198,3 +198,17 @@ def test_rows_of_large_logits(dtype, n, big):
     z[4::5] *= big / 5                                # spread over the whole size
     ids = torch.tensor([[17, 3000, 2, 3002]], device='cuda').repeat(5 * n, 1)
     check_wide(z.to(dtype), ids, 6)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_finite_masks_in_ordinary_rows(dtype):
+    """Tokens banned by the type's lowest value, or by any large one, among ordinary logits: their log
+    probabilities are finite, the others' as without them; few and most of the row."""
+    for mask in (torch.finfo(dtype).min, -2.5e38, -1e30, -1e12, -1e9, -7e7, -6e7, -1e7, -1e4):
+        for n in (1, 5, 400):
+            g = torch.Generator(device='cuda').manual_seed(n)
+            z = torch.randn(2 * n, 3003, generator=g, device='cuda')
+            z[0::2, 5:50] = mask
+            z[1::2, 7:] = mask
+            ids = torch.tensor([[6, 3000, 2, 20]], device='cuda').repeat(2 * n, 1)
+            check_wide(z.to(dtype), ids, 10)
