@@ -696,12 +696,16 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
                         for (int w = 1; w < min(parts, LP_EPI / 32); ++w) best = lp_merge32(best, wk.list[w][lane], lane);
                 }
             }
-            const float log2s = log2f(sums.s);
+            // where the sums are those of the largest logit alone, to the bit, its log probability and the entropy are
+            // zero, not the difference of two roundings
+            const float d_top = fmaf(top_all, kLog2e, -sums.mc), x_top = fast_exp2(d_top);
+            const bool alone = sums.s == x_top && sums.w == d_top * x_top;
+            const float log2s = alone ? d_top : log2f(sums.s);
             float m = -INFINITY, logs = 0.f, ent = kLn2 * (log2s - sums.w / sums.s);
             // nothing allowed; or beyond the range of the sums, or NaN
             const bool none = top_all == -INFINITY;
             const bool odd = !none && !(sums.mc > 0.1f * LP_FLOOR && sums.mc < -LP_FLOOR && sums.s > 0.f && sums.s < INFINITY);
-            if (none) ent = 0.f;
+            if (none || alone) ent = 0.f;
             if (odd) lp_row_plain(a, r.z, e, g, wk.red, m, logs, ent);
             const auto lp = [&](float f) {
                 if (none) return -INFINITY;

@@ -212,3 +212,14 @@ def test_finite_masks_in_ordinary_rows(dtype):
             z[1::2, 7:] = mask
             ids = torch.tensor([[6, 3000, 2, 20]], device='cuda').repeat(2 * n, 1)
             check_wide(z.to(dtype), ids, 10)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+def test_one_allowed_token_anywhere(dtype):
+    """Its log probability and the entropy are zero to the bit, in a vector or before and behind them."""
+    z = torch.full((64, 3001), float('-inf'), dtype=dtype, device='cuda')
+    at = torch.tensor([0, 1, 2, 3, 7, 8, 1500, 1501, 2990, 2997, 2998, 2999, 3000] * 5, device='cuda')[:64]
+    row = torch.arange(64, device='cuda')
+    z[row, at] = torch.linspace(-700, 900, 64, device='cuda').to(dtype)
+    lp, ent, tl, ti = check(z, at, 3)
+    assert (lp == 0).all() and (ent == 0).all() and (tl[:, 0] == 0).all() and torch.equal(ti[:, 0], at)
