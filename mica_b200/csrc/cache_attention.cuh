@@ -69,7 +69,8 @@ struct CacheAttnArgs {
     int ctas;                   // CTAs of the grid
     float scale_log2;           // scale * log2(e)
     float* ws;                  // partials: [ctas][2] places
-    int4* cuts;                 // [ctas][2] the unit a CTA starts inside, for the CTA that is the first to
+    int4* cuts;                 // [ctas][2] the unit a CTA starts inside, for the CTA that is the first to (w -1: cu is
+                                // out of order)
 };
 
 // A place of the workspace: rows of O as [NT][D / 4][128] float4 (a warp's rows side by side), then
@@ -121,10 +122,8 @@ struct CachePlace {             // a place of the line: the off-th of sequence b
     long total;
     long off;
     int b;
-    bool ordered;               // cu starts at zero or above and does not run backwards
 };
-// The line's length and the sequence that holds place `first(total)`; every thread of the block calls it. A step
-// whose cu runs backwards (two sequences may claim a row) or starts below zero has no line (total 0, ordered false).
+// The line's length and the sequence that holds place `first(total)`; every thread of the block calls it.
 template <int NT, typename F>
 __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, int R, bool causal, F first) {
     __shared__ long s_warp[32];
@@ -148,10 +147,7 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
         return v;
     };
     const auto tiles = [&](int b) { return b < p.B ? KV * CacheCost<NT>::seq(cache_seq(p, b), R, causal) : 0l; };
-    const auto backwards = [&](int b) { return b < p.B && (p.cu[b] < 0 || p.cu[b] > p.cu[b + 1]); };
-    const CachePlace none{0, 0, -1, false};
     if (p.B <= 32) {                                 // every warp by itself
-        if (__any_sync(0xffffffffu, backwards(lane))) return none;
         const long n = tiles(lane);
         long end = n;
 #pragma unroll
@@ -162,11 +158,8 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
         const long total = __shfl_sync(0xffffffffu, end, 31), t = first(total);
         const uint32_t here = __ballot_sync(0xffffffffu, t >= end - n && t < end);
         const int b = __ffs(here) - 1;
-        return CachePlace{total, t - __shfl_sync(0xffffffffu, end - n, max(b, 0)), b, true};
+        return CachePlace{total, t - __shfl_sync(0xffffffffu, end - n, max(b, 0)), b};
     }
-    bool back = false;
-    for (int b = threadIdx.x; b < p.B; b += blockDim.x) back = back || backwards(b);
-    if (__syncthreads_or(back)) return none;
     const long mine = tiles(threadIdx.x);
     long total = 0;
     if (threadIdx.x == 0) { s_b = -1; s_off = 0; }
@@ -177,7 +170,7 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
             s_off = t - (end - mine);
         }
         __syncthreads();
-        return CachePlace{total, s_off, s_b, true};
+        return CachePlace{total, s_off, s_b};
     }
     long sum = mine;
     for (int b = threadIdx.x + blockDim.x; b < p.B; b += blockDim.x) sum += tiles(b);
@@ -196,7 +189,7 @@ __device__ __forceinline__ CachePlace cache_locate(const CachePlan& p, int KV, i
         if (before > t) break;
     }
     __syncthreads();
-    return CachePlace{total, s_off, s_b, true};
+    return CachePlace{total, s_off, s_b};
 }
 
 // The runs of the CTAs: total / used places each, the first total % used one more. Fewer CTAs are used
@@ -327,18 +320,29 @@ __device__ __forceinline__ void mask_bits(const unsigned long long* m, int words
 }
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
-// Rows before the first sequence and behind the last become zero, all of them in a step without order; a cu that
-// passes the rows, or runs backwards, is recorded. The whole block calls it.
-__device__ __forceinline__ void cache_zero_padding(const CacheAttnArgs& args, int D, bool ordered) {
-    const int N = args.plan.N, past = args.plan.cu[args.plan.B];
-    if (blockIdx.x == 0 && threadIdx.x == 0 && (!ordered || past > N)) record_bad_page();
-    const int first = ordered ? min(args.plan.cu[0], N) : 0, end = ordered ? min(past, N) : 0;
-    const int vecs = args.KV * args.G * D / 8;
-    for (long i_row = blockIdx.x; i_row < N - (end - first); i_row += gridDim.x) {
+// Rows first .. end - 1 of the output stay as they are, all others become zero: by `threads` of each of the blocks.
+__device__ __forceinline__ void cache_zero_rows(const CacheAttnArgs& args, int D, int first, int end, long block, long blocks,
+                                                int thread, int threads) {
+    const int N = args.plan.N, vecs = args.KV * args.G * D / 8;
+    for (long i_row = block; i_row < N - (end - first); i_row += blocks) {
         const long row = i_row < first ? i_row : i_row - first + end;
-        for (int i = threadIdx.x; i < vecs; i += blockDim.x)
+        for (int i = thread; i < vecs; i += threads)
             *reinterpret_cast<uint4*>(args.out + row * args.ldo + i * 8) = make_uint4(0u, 0u, 0u, 0u);
     }
+}
+// Rows before the first sequence and behind the last become zero.
+__device__ __forceinline__ void cache_zero_padding(const CacheAttnArgs& args, int D, int thread, int threads) {
+    const int N = args.plan.N, first = min(max(args.plan.cu[0], 0), N);
+    cache_zero_rows(args, D, first, max(first, min(args.plan.cu[args.plan.B], N)), blockIdx.x, gridDim.x, thread, threads);
+}
+// Looks the row offsets over, by one warp; false when they run backwards or start below zero: two sequences may
+// claim a row then, and the join makes all rows zero.
+__device__ __noinline__ bool cache_ordered(const CachePlan& p) {
+    bool bad = false;
+    for (int b = threadIdx.x & 31; b < p.B; b += 32) bad = bad || p.cu[b] < 0 || p.cu[b] > p.cu[b + 1];
+    const bool ordered = !__any_sync(0xffffffffu, bad);
+    if (blockIdx.x == 0 && (threadIdx.x & 31) == 0 && (!ordered || p.cu[p.B] > p.N)) record_bad_page();
+    return ordered;
 }
 
 // The keys k0 .. k0 + 127 that node `node` of unit u's sequence sees (row: its row of the step), one bit
@@ -494,8 +498,11 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
     CacheWalk<NT> wk;
     if (cta >= share.used || place.b < 0 ||
         !wk.start(plan, args.KV, R, causal, place.b, place.off, share.at(cta + 1) - share.at(cta))) {
-        if (threadIdx.x == 0) args.cuts[2 * cta] = make_int4(0, 0, 0, 0);
-        cache_zero_padding(args, D, place.ordered);
+        if (warp == 3) {
+            const bool ordered = cache_ordered(plan);
+            if (lane == 0) args.cuts[2 * cta] = make_int4(0, 0, 0, ordered ? 0 : -1);
+        }
+        cache_zero_padding(args, D, threadIdx.x, blockDim.x);
         return;
     }
 
@@ -762,11 +769,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         }
         __syncwarp();
     } else if (warp == 3) {
+        const bool ordered = cache_ordered(plan);
         if (lane == 0) {
             // the unit this CTA starts inside, for the join: its first row, node rows, K/V head, and the CTAs
             // that hold parts of it, the one before and `n` from this one on
-            int4 cut = make_int4(0, 0, 0, 0);
-            if (wk.j0 > 0) {
+            int4 cut = make_int4(0, 0, 0, ordered ? 0 : -1);
+            if (ordered && wk.j0 > 0) {
                 // places of the unit before each CTA's run: up to its first tile, up to its last
                 const long first = static_cast<long>(Cost::UNIT) * wk.w, last = static_cast<long>(wk.nk - 1 + Cost::UNIT) * wk.w;
                 const long unit0 = share.at(cta + 1) - wk.left;
@@ -1091,13 +1099,14 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
         tc_fence_after();
         tmem_free(tmem, 512);
     }
-    cache_zero_padding(args, D, true);
+    cache_zero_padding(args, D, threadIdx.x, blockDim.x);
 }
 
 // Adds up the parts of each divided unit, always in the same order. Blocks (c, y): the unit that CTA c + 1 is
 // the first to start inside, if it is. A thread takes 16 columns of a row, three parts in flight; where a
 // long sequence's unit is in many parts, `lanes` neighbouring threads take every lanes-th part each and add
 // theirs up (one sequence of 100000 keys and one K/V head is in 148: 35 us one part after the other).
+// Where the row offsets were out of order it makes all rows zero.
 __host__ __device__ inline int cache_join_lanes(int parts) { return parts < 6 ? 1 : parts < 24 ? 4 : 16; }
 template <int D, int NT>
 __global__ void __launch_bounds__(128) cache_attention_join(const CacheAttnArgs args) {
@@ -1106,7 +1115,12 @@ __global__ void __launch_bounds__(128) cache_attention_join(const CacheAttnArgs 
     const int c = blockIdx.x + 1;
     const int4 cut = args.cuts[2 * c];
     const int rows = cut.x, n = cut.w, items = rows * (D / 16);
-    if (items == 0) return;
+    if (items == 0) {
+        if (n < 0)
+            cache_zero_rows(args, D, 0, 0, static_cast<long>(blockIdx.y) * gridDim.x + blockIdx.x,
+                            static_cast<long>(gridDim.x) * gridDim.y, threadIdx.x, blockDim.x);
+        return;
+    }
     const int lanes = cache_join_lanes(n);
     const int first_place = args.cuts[2 * (c - 1) + 1].x;            // of the part that the CTA before left last
     const long pf = cache_attn_place_floats<D, NT>();
