@@ -9,6 +9,7 @@ runtime, so it does not depend on which libcudart torch happens to load. _calls.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -74,7 +75,14 @@ def build_calls(force: bool = False) -> Path:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    build_calls(force)
+    """The library, then, where torch is installed, the calls: callers of the C ABI need nvcc alone."""
+    out = build_library(force, verbose)
+    if importlib.util.find_spec('torch') is not None:
+        build_calls(force)
+    return out
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
     if not force and up_to_date():
         return OUT
     tmp = OUT.with_suffix('.so.tmp')

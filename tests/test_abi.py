@@ -3,6 +3,7 @@ compute without a GPU), and the ctypes binding covers every declaration."""
 import ctypes
 import re
 import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -85,3 +86,22 @@ def test_entry_points_reject_bad_arguments_without_touching_a_gpu(lib_path):
     assert na(16, 32, 16, 32, 16, 16, None, None, 16, 32, 16, 32, 16, 65537, 32, 32, 0, None) == 7  # rows > limit
     assert lib.mica_option_logits(16, 0, 64, None, 0, 1e-6, 16, 0, 64, None, None, 16, 16, 1, None) == 2
     assert lib.mica_selftest_wait_timeout(None, 10, None) == 1
+
+
+def test_the_library_is_built_first_and_without_torch(monkeypatch):
+    """A caller of the C ABI needs nvcc alone; the Python calls are built where torch is installed."""
+    code = ("import sys; sys.modules['torch'] = None\n"
+            "import mica_b200.build as b; b.up_to_date = lambda: True\n"
+            "assert b.build() == b.OUT")
+    subprocess.run([sys.executable, '-c', code], cwd=ROOT, check=True, timeout=300)
+    from mica_b200 import build
+    done = []
+    monkeypatch.setattr(build, 'up_to_date', lambda: done.append('library') or True)
+
+    def fails(force=False):
+        raise RuntimeError('no host compiler')
+
+    monkeypatch.setattr(build, 'build_calls', fails)
+    with pytest.raises(RuntimeError, match='no host compiler'):
+        build.build()
+    assert done == ['library']
