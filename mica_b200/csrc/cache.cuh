@@ -455,10 +455,10 @@ struct KeepArgs {
     int row_bytes;              // D * 2
 };
 
-__global__ void __launch_bounds__(256) cache_keep_kernel(const KeepArgs a) {
+__device__ __forceinline__ void cache_keep_sequence(const KeepArgs& a, const int b) {
     __shared__ long s_src[KEEP_LIST], s_dst[KEEP_LIST];
     __shared__ int s_count[8], s_moves;
-    const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int base = a.plan.base[b], n = a.n_keep[b], rows = a.plan.cu[b + 1] - a.plan.cu[b];
     const int* list = a.keep + static_cast<long>(b) * a.ld_keep;
     // the list: increasing, below the row count, in pages of the pool
@@ -515,6 +515,10 @@ __global__ void __launch_bounds__(256) cache_keep_kernel(const KeepArgs a) {
         }
         __syncthreads();
     }
+}
+
+__global__ void __launch_bounds__(256) cache_keep_kernel(const KeepArgs a) {
+    for (int b = blockIdx.y; b < a.plan.B; b += gridDim.y) cache_keep_sequence(a, b);
 }
 
 }  // namespace mica

@@ -1296,7 +1296,7 @@ int mica_cache_keep(void* pool, long page_stride, int slabs, int pages, int page
     KeepArgs a = {};
     int rc = cache_plan(&a.plan, table, ld_table, P, base, cu, B, 0, pages, page);
     if (rc) return rc;
-    if (slabs < 1 || (D != 64 && D != 128) || A < 0 || ld_keep < A || B > 65535 ||
+    if (slabs < 1 || (D != 64 && D != 128) || A < 0 || ld_keep < A ||
         page_stride < static_cast<long>(slabs) * page * D * 2)
         return MICA_ERR_SHAPE;
     if (!aligned16(pool) || page_stride % 16 || !aligned_to(table, 4) || !aligned_to(base, 4) || !aligned_to(cu, 4) ||
@@ -1310,7 +1310,7 @@ int mica_cache_keep(void* pool, long page_stride, int slabs, int pages, int page
     // about eight blocks an SM, each with whole batches of slabs
     const long want = static_cast<long>(slabs) * B / (8L * sms);
     a.per_block = static_cast<int>(std::max<long>(1, std::min<long>((want + KEEP_AHEAD - 1) / KEEP_AHEAD, (slabs + KEEP_AHEAD - 1) / KEEP_AHEAD))) * KEEP_AHEAD;
-    cache_keep_kernel<<<dim3(static_cast<unsigned>((slabs + a.per_block - 1) / a.per_block), static_cast<unsigned>(B)), 256, 0,
+    cache_keep_kernel<<<dim3(static_cast<unsigned>((slabs + a.per_block - 1) / a.per_block), static_cast<unsigned>(std::min(B, 65535))), 256, 0,
                         static_cast<cudaStream_t>(stream)>>>(a);
     return launch_status();
 }

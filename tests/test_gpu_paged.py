@@ -769,3 +769,31 @@ def test_row_offsets_out_of_range_are_recorded(seqs, pad):
     qs, os_, e1, e2 = run(c.n)
     assert (e1, e2) == (0, 0) and float(qs[0].float().abs().max()) == 0.0 and float(os_[0].float().abs().max()) == 0.0
     assert near(os_[new[0]:], o[new[0]:])
+
+
+def test_keep_tokens_of_more_sequences_than_a_grid_has_rows():
+    """65541 sequences of one page each, most of which keep nothing or what they have."""
+    from mica_b200 import paged
+    n = 65541
+    i32 = {'dtype': torch.int32, 'device': 'cuda'}
+    pool = torch.randn(n, 1, 2, 1, 16, 64, device='cuda').bfloat16()
+    table = torch.arange(n - 1, -1, -1, **i32)[:, None]
+    base, cu = torch.full((n,), 3, **i32), 5 * torch.arange(n + 1, **i32)
+    keep = torch.tensor([[0, 2, 4]], **i32).repeat(n, 1)
+    count = torch.zeros(n, **i32)
+    some = torch.tensor([0, 1, 5, 6, 65534, 65535, 65536, 65540], device='cuda')
+    count[some] = 3
+    keep[6] = torch.tensor([0, 1, 2], **i32)
+    keep[65536] = torch.tensor([0, 4, 2], **i32)                    # out of order: left as it was
+    ref = pool.clone()
+    for b in some.tolist():
+        p = n - 1 - b
+        if b != 65536:
+            for j, i in enumerate(keep[b].tolist()):
+                ref[p, ..., 3 + j, :] = pool[p, ..., 3 + i, :]
+    step = paged.Step(table, base, cu)
+    _error()
+    new = paged.keep_tokens(pool, step, keep, count)
+    assert _error() == 9 and torch.equal(pool, ref)
+    count[65536] = 0
+    assert torch.equal(new, base + count)

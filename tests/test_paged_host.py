@@ -246,3 +246,8 @@ def test_a_step_keeps_the_tensors_it_is_given():
     for t in (table, base, cu, mask):
         t += 1
     assert step.table.sum() == 6 and step.base.sum() == 2 and step.cu.sum() == 3 and step.mask.sum() == 15
+
+
+def test_keep_serves_any_number_of_sequences(lib):
+    """What is refused first is the pool's place, not the number of sequences."""
+    assert lib.mica_cache_keep(24, 4096, 2, 4, 16, 64, 16, 2, 2, 16, 16, 70000, 16, 3, 16, 3, 32, None) == 3
