@@ -473,6 +473,14 @@ __device__ __noinline__ uint32_t cache_odd_kinds(const CacheAttnArgs& args, cons
     return mend ? mine : 0u;
 }
 
+// A row's weights are 2^fma(s, c, -m), for scores s as they come from the MMA, c = scale * log2(e) and the running
+// maximum m = fl(max c), whose rounding is a factor of all of them and cancels. Beyond |m| = 2^30 that rounding may
+// take them out of fp32's range, and scores that differ at all differ by 64 or more, so only those equal to the
+// largest count: the power of two above c stands in for c there, with which both products are exact. m stays in
+// order across the limit, so sums with different maxima are brought together by 2^(m - m') either way. Nothing
+// seen yet: CACHE_NOTHING. (Scores have to stay within fp32's range when they are multiplied by that.)
+constexpr float CACHE_FAR = 1073741824.f, CACHE_NOTHING = -3e38f;
+
 template <int D, int NT>
 __global__ void __launch_bounds__(CacheAttnShape<D, NT>::THREADS, 1)
 cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
@@ -824,7 +832,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
             const int node_r = r / args.G, head_r = r - node_r * args.G;
             const bool live = node_r < min(args.npt, u.nodes - x * args.npt);             // this thread has a row
             const uint32_t t_o = tmem + col_o(x) + lane_off;
-            float m_use = -1e30f, l = 0.f;
+            float m_use = CACHE_NOTHING, cr = c, l = 0.f;
             for (; t < t_end; ++t) {
                 const int i2 = NT == 1 ? (t & 1) : x;
                 const int n2 = NT == 1 ? t >> 1 : t;                   // uses of that buffer before
@@ -872,13 +880,19 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                         for (int e = 0; e < 8; ++e)
                             mp[e] = i + 8 + e < 32 * W ? fmax3(mp[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 8 + e]))
                                                        : fmaxf(mp[e], __uint_as_float(sr[i + e]));
-                    const float mx = fmax3(fmax3(mp[0], mp[1], mp[2]), fmax3(mp[3], mp[4], mp[5]), fmaxf(mp[6], mp[7])) * c;
-                    if (mx > m_use + ATT_RESCALE_LOG2) {
-                        alpha = fast_exp2(m_use - mx);
-                        m_use = mx;
+                    const float mx = fmax3(fmax3(mp[0], mp[1], mp[2]), fmax3(mp[3], mp[4], mp[5]), fmaxf(mp[6], mp[7]));
+                    if (fmaf(mx, cr, -m_use) > ATT_RESCALE_LOG2) {
+                        float m_new = mx * c;
+                        cr = c;
+                        if (fabsf(m_new) > CACHE_FAR) {
+                            cr = __uint_as_float((__float_as_uint(c) + 0x007fffffu) & 0x7f800000u);
+                            m_new = mx * cr;
+                        }
+                        alpha = fast_exp2(m_use - m_new);
+                        m_use = m_new;
                         moved = live;                // what a thread without a row reads and adds up is nobody's
                     }
-                    const unsigned long long c2 = f2_pack(c, c), nm2 = f2_pack(-m_use, -m_use);
+                    const unsigned long long c2 = f2_pack(cr, cr), nm2 = f2_pack(-m_use, -m_use);
                     unsigned long long sp[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
                     for (int i = 0; i < 16 * W; ++i) {
@@ -1012,7 +1026,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_
                     for (int i0 = q4 * 32; i0 < D / 4 * rows; i0 += 128) {
                         const int item = i0 + lane, v = min(item / rows, D / 4 - 1), rr = item - v * rows;
                         const bool mine = rr < have;
-                        float m_all = -1e30f, l_all = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+                        float m_all = CACHE_NOTHING, l_all = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
                         if (mine) {
                             float2 ml[4];
                             float4 a[4];

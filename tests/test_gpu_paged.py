@@ -797,3 +797,41 @@ def test_keep_tokens_of_more_sequences_than_a_grid_has_rows():
     assert _error() == 9 and torch.equal(pool, ref)
     count[65536] = 0
     assert torch.equal(new, base + count)
+
+
+@pytest.mark.parametrize('heads,new', [(4, 1), (4, 8), (4, 33), (4, 80)])
+@pytest.mark.parametrize('power', [10, 24, 29, 31, 33, 40, 64, 100, 120])
+@pytest.mark.parametrize('sign', [1, -1])
+def test_attention_of_scores_of_any_size(heads, new, power, sign):
+    """Scores k 2^power / 11.3, exact in fp32: all alike, a few largest ones, growing along the axis, one key of
+    each size, in one tile, several, and parts that several CTAs hold. A step of one score is a factor of 2^90 at
+    the least (power 10), so a row is the mean of the values at its largest score."""
+    c = Case([0, 100, 300, 700, 20000], [new] * 5, heads, 1, 128, 64, seed=new, mask=tree)
+    c.q.zero_()
+    c.q[:, ::128] = sign * 2.0 ** (power // 2)
+    for b, (kk, vv) in enumerate(c.keys):
+        s = torch.arange(kk.shape[1], device='cuda')
+        kk.zero_()
+        kk[:, s, 0] = (torch.full_like(s, 3), 1 + s % 3, 1 + s // 64, 1 + s % 101, 1 + s // 1024)[b].bfloat16() * \
+            2.0 ** (power - power // 2)
+        for i in range(0, kk.shape[1], 64):
+            m = min(64, kk.shape[1] - i)
+            c.k[c.rows[b][i // 64], :, :m] = kk[:, i:i + m]
+    o = run_attention(c, max_new=new)
+    check_attention(c, o)
+    assert torch.equal(o, run_attention(c, max_new=new))
+
+
+@pytest.mark.parametrize('scale', [1e-38, 1e-30, 1e30])
+def test_attention_scales_at_the_ends(scale):
+    c = Case([300, 20000], [5, 40], 4, 1, 128, 64, seed=1, mask=tree)
+    if scale > 1:                                           # powers of two, exact: one largest score
+        c.q.zero_()
+        c.q[:, ::128] = 1
+        for b, (kk, _) in enumerate(c.keys):
+            kk.zero_()
+            kk[:, :, 0] = (torch.arange(kk.shape[1], device='cuda') % 128).bfloat16()
+            for i in range(0, kk.shape[1], 64):
+                m = min(64, kk.shape[1] - i)
+                c.k[c.rows[b][i // 64], :, :m] = kk[:, i:i + m]
+    check_attention(c, run_attention(c, scale=scale), scale)
