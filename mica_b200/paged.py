@@ -47,7 +47,7 @@ class Step:
 
     Row i of sequence b sits at cache index base[b] + i and sees all of the committed tokens."""
 
-    __slots__ = ('table', 'base', 'cu', 'mask', 'max_new', 'rows')
+    __slots__ = ('table', 'base', 'cu', 'mask', 'max_new', 'rows', 'lengths')
 
     def __init__(self, table, base, cu, max_new: Optional[int] = None, mask=None):
         if table.dim() != 2 or base.dim() != 1 or cu.dim() != 1 or not (
@@ -60,7 +60,8 @@ class Step:
         if max_new is not None and max_new < 0:
             raise ValueError(f'Step: max_new {max_new}')
         self.table, self.base, self.cu, self.mask, self.max_new = table, base, cu, mask, max_new
-        self.rows = None               # rows of each sequence, where the host knows them (PagedCache.step)
+        self.rows = None               # rows of each sequence and its committed tokens then, where the host
+        self.lengths = None            # knows them (PagedCache.step)
 
 
 def append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, step: Step, heads: int, pos=None, eps: float = 1e-6):
@@ -249,7 +250,7 @@ class PagedCache:
         meta = meta.pin_memory().to(self.pool.device, non_blocking=True)
         w = b * width
         s = Step(meta[:w].view(b, width), meta[w:w + b], meta[w + b:], max_new=max(new, default=0), mask=mask)
-        s.rows = list(new)
+        s.rows, s.lengths = list(new), [self._seqs[i][1] for i in sids]
         return s
 
     def commit(self, sids: Sequence[int], new: Sequence[int]) -> None:
@@ -268,6 +269,8 @@ class PagedCache:
         """Commits the rows keep[b] (increasing) of the step's tree: the accepted tokens of each sequence."""
         if len(set(sids)) != len(sids) or len(sids) != len(keep) or step.rows is None or len(sids) != len(step.rows):
             raise ValueError(f'keep: {len(keep)} lists for {len(sids)} sequences of a step of this cache')
+        if step.lengths is not None and step.lengths != [self._seqs[sid][1] for sid in sids]:
+            raise ValueError(f'keep: sequences {list(sids)} are not as they were when the step was described')
         for sid, rows, n in zip(sids, keep, step.rows):
             pages, length = self._seqs[sid]
             if any(a >= b for a, b in zip(rows, rows[1:])) or (rows and (rows[0] < 0 or rows[-1] >= n)) or (

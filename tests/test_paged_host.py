@@ -251,3 +251,22 @@ def test_a_step_keeps_the_tensors_it_is_given():
 def test_keep_serves_any_number_of_sequences(lib):
     """What is refused first is the pool's place, not the number of sequences."""
     assert lib.mica_cache_keep(24, 4096, 2, 4, 16, 64, 16, 2, 2, 16, 16, 70000, 16, 3, 16, 3, 32, None) == 3
+
+
+def test_keep_refuses_a_step_whose_sequences_have_moved_on(monkeypatch):
+    """The step's rows stand behind the tokens that were committed when it was described."""
+    from mica_b200 import paged
+    monkeypatch.setattr(torch.Tensor, 'pin_memory', lambda t: t)
+    monkeypatch.setattr(paged, 'keep_tokens', lambda *a: None)
+    c = paged.PagedCache(1, 1, 64, 10, page=16, device='cpu')
+    a, b = c.open(), c.open()
+    c.step([b], [2])
+    c.commit([b], [2])
+    step = c.step([a, b], [5, 5])
+    with pytest.raises(ValueError):
+        c.keep([b, a], step, [[0], [1]])               # the other way round
+    c.keep([a, b], step, [[1, 3], [0]])
+    assert c.length(a) == 2 and c.length(b) == 3
+    with pytest.raises(ValueError):
+        c.keep([a, b], step, [[0], [0]])               # once more
+    assert c.length(a) == 2 and c.length(b) == 3
