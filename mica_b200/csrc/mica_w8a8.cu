@@ -1139,12 +1139,14 @@ int mica_cache_append(const void* qkv, long ld, const void* q_w, const void* k_w
     a.k_pages = static_cast<__nv_bfloat16*>(k_pages); a.v_pages = static_cast<__nv_bfloat16*>(v_pages);
     a.page_stride = page_stride; a.H = H; a.KV = KV; a.eps = eps;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // Many rows go through the ring, three CTAs an SM, five rows and more each: 8000 rows of 48 heads of 128 take
-    // 42 us (one CTA an SM 57, two 46, four 44), a warp a row 55. Few rows take one look-up and one load either way,
-    // which the ring has one behind the other, with its barriers.
+    // Many rows go through the ring, three CTAs an SM, two rows and more each; of few rows it has the look-up, the
+    // load and the store one behind the other, with its barriers. 48 heads of 128, a warp a row against the ring:
+    // 500 rows 11.7 and 12.1 us, 1000 16.4 and 13.3, 2000 24.6 and 16.6, 4000 31.8 and 24.8, 8000 55 and 42 (one CTA
+    // an SM 57, two 46, four 44). 40 heads of 64: 500 8.2 and 10.2, 1000 10.2 and 11.0, 1500 14.3 and 12.3, 6000 24.6
+    // and 22.5.
     const long stage = static_cast<long>(H + 2 * KV) * D * 2 + 4 * D;
     const int stages = static_cast<int>(std::min<long>(APPEND_STAGES, APPEND_SMEM / stage));
-    if (N >= 16L * sms && stages >= 3) {
+    if (N >= 7L * sms && stages >= 3) {
         const auto kernel = D == 128 ? cache_append_ring_kernel<128> : cache_append_ring_kernel<64>;
         if ((rc = append_ring_prepare())) return rc;
         kernel<<<APPEND_CTAS * sms, APPEND_WARPS * 32 + 64, static_cast<size_t>(stages) * stage, st>>>(a, stages);
@@ -1232,8 +1234,9 @@ int mica_cache_attention(const void* q, long ldq, const void* k_pages, const voi
     int nt = 0;
     cache_attn_rows(max_new, H / KV, &nt, &a.npt);
     if (!workspace || workspace_bytes < cache_attn_bytes(sms, nt, D)) return MICA_ERR_WORKSPACE;
-    // The rows four times, by their number times D: 64 sequences of 300 to 4000 keys, 32 heads over 8, warm: 99 us once,
-    // 93 four times for 4 rows of 128; 100 and 108 for 16; 90 and 78 for 16 rows of 64; 89 and 93 for 32.
+    // The rows four times, by their number times D: 64 sequences of 300 to 4000 keys, 8 K/V heads, cold L2, once and four
+    // times: 4 rows of 128 99.3 and 96.9 us, 8 99.5 and 97.7, 16 104.4 and 104.8; 4 rows of 64 84 and 65, 8 84 and 66,
+    // 16 86 and 70, 32 (an earlier form, warm) 89 and 93.
     a.quarters = nt == 1 && a.npt * (H / KV) * D <= 1024;
     a.v_pages = static_cast<const __nv_bfloat16*>(v_pages);
     a.page_stride = page_stride;

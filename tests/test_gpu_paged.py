@@ -835,3 +835,27 @@ def test_attention_scales_at_the_ends(scale):
                 m = min(64, kk.shape[1] - i)
                 c.k[c.rows[b][i // 64], :, :m] = kk[:, i:i + m]
     check_attention(c, run_attention(c, scale=scale), scale)
+
+
+@pytest.mark.parametrize('heads,kv,dim', [(32, 8, 128), (24, 8, 64)])
+@pytest.mark.parametrize('more', [-1, 0, 1])
+def test_append_around_the_ring(heads, kv, dim, more):
+    """Row counts where a warp a row gives way to the ring."""
+    from mica_b200 import paged
+    n = 7 * torch.cuda.get_device_properties(0).multi_processor_count + more
+    c = Case([9, 0], [n - 400, 400], heads, kv, dim, 64, seed=heads)
+    g = torch.Generator(device='cuda').manual_seed(1)
+    qkv = (2 * torch.randn(n, (heads + 2 * kv) * dim, generator=g, device='cuda')).bfloat16()
+    qw, kw = (1 + 0.1 * torch.randn(2, dim, generator=g, device='cuda')).bfloat16()
+    cos, sin = tables(dim)
+    q = paged.append(qkv, qw, kw, cos, sin, c.k, c.v, c.step(), heads)
+    index = torch.cat([torch.arange(9, 9 + n - 400), torch.arange(400)]).cuda()
+    x = qkv.view(n, heads + 2 * kv, dim)
+    ref = torch.cat((norm_rope(x[:, :heads], qw, cos[index], sin[index], 1e-6),
+                     norm_rope(x[:, heads:heads + kv], kw, cos[index], sin[index], 1e-6)), 1)
+    bound = U * ref.abs() + 2.0 ** -20 * 4 * ref.abs().amax(-1, keepdim=True) + 1e-12
+    assert ((q.view(n, heads, dim).double() - ref[:, :heads]).abs() <= bound[:, :heads]).all()
+    b = torch.cat([torch.full((t,), i) for i, t in enumerate(c.new)]).cuda()
+    page_of, slot = c.table.long()[b, index // 64], index % 64
+    assert ((c.k[page_of, :, slot].double() - ref[:, heads:]).abs() <= bound[:, heads:]).all()
+    assert torch.equal(c.v[page_of, :, slot], x[:, heads + kv:])
