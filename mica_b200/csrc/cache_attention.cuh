@@ -42,11 +42,13 @@
 // or NaN element of a node's V is replaced by zero and added to the accumulators of the rows that see
 // it, no others.
 //
-// Measured (32 heads over 8, D = 128, cold L2): 13 and 15 tokens over 70761 and 87495 keys 130 us (116 warm), the
-// key tiles among them at the memory's 6.5 TB/s (1.5 us a tile and SM); 16 trees of up to 64 nodes over up to
-// 9000 keys 90 us, a tile of two row tiles 1.7 us (softmax: 2100 cycles of it the scores' way through the
-// exponential, 1100 waits, packing and stores); 700 nodes over 20000 keys 207 us, 1.1 PFLOP/s; one token over up
-// to 700 keys 17 us with its launch and the join.
+// Measured (32 heads over 8, D = 128, cold L2, in a graph): 13 and 15 tokens over 70761 and 87495 keys 131 us (117
+// warm), the key tiles among them at the memory's 6.5 TB/s (1.5 us a tile and SM); 16 trees of up to 64 nodes over up
+// to 9000 keys 90 us, a tile of two row tiles 1.7 us (softmax: 2100 cycles of it the scores' way through the
+// exponential, 1100 waits, packing and stores); 700 nodes over 20000 keys 212 us, 1.08 PFLOP/s (calls back to back,
+// under the power cap, 241 us, 0.95); 8192 causal rows 530 us, 1.04 PFLOP/s; one token over up to 700 keys 18 us
+// with its launch and the join. D = 64: 8 tokens over eight contexts of 8000, 24 heads over 8, 56 us against 20 for
+// the bytes: one softmax warpgroup takes 1.3 us a tile, whose bytes take half of D = 128's time.
 #pragma once
 
 #include "attention.cuh"
@@ -65,7 +67,7 @@ struct CacheAttnArgs {
     long ldo;
     int KV, G;                  // K/V heads, query heads of each
     int npt;                    // nodes of a row tile: npt * G <= 128
-    bool quarters;              // the rows lie in the row tile four times (npt * G <= 16; NT 1)
+    bool quarters;              // the rows lie in the row tile four times (npt * G * D <= 1024; NT 1)
     int ctas;                   // CTAs of the grid
     float scale_log2;           // scale * log2(e)
     float* ws;                  // partials: [ctas][2] places

@@ -20,9 +20,10 @@
 // alternative (about 25 of 640 for 20 alternatives of random logits), and their vectors are read
 // again, from L2, and elements that reach the bound kept. Warps sort them 32 at a time and merge.
 //
-// Measured (cold L2): 1025 rows of 151936 bf16, top 20, 76 us, 65 of them with warm instruction and data
-// caches (4.8 TB/s; without alternatives 69, fp32 112 us = 5.6 TB/s); 6 rows of 151936 fp32, top 8, 16 us
-// of which 8 are a launch. One CTA a row with a pass for each alternative took 6269 us.
+// Measured (cold L2; in brackets with warm instruction and data caches): 1025 rows of 151936, top 20, bf16 76 us
+// (65, 4.8 TB/s), fp16 78 (72), fp32 129 to 138 (118, 5.3 TB/s); 6 rows of 151936 fp32, top 8, 16 us of which 8 are
+// a launch. In the bf16 pass the exponential's pipe is busy 63 % of the time, issue 55 %, memory 60 % of its peak:
+// none is full, and all three wait at the rows' ends. One CTA a row with a pass for each alternative took 6269 us.
 #pragma once
 
 #include "quant.cuh"
@@ -486,23 +487,23 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
             long id = -1;
             if (rank == 0 && e < a.M) id = a.ids[static_cast<long>(row) * a.ld_ids + e];
             mbar_wait(&sh.passed[slot], turn, abort_flag, MICA_DEV_TIMEOUT_EPILOGUE);
-            // six threads' sums and maxima each; two of these are a group
+            // five threads' sums and maxima each; two of these are a group
             constexpr int kEach = LP_THREADS / LP_EPI;
             LpSums sums;
-            float4 six[kEach];
+            float4 five[kEach];
             float top = -INFINITY, mc = -INFINITY;
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
-                six[i] = sh.mine[slot][e + i * LP_EPI];
-                top = max_nan(top, six[i].w);
-                mc = max_nan(mc, six[i].x);
+                five[i] = sh.mine[slot][e + i * LP_EPI];
+                top = max_nan(top, five[i].w);
+                mc = max_nan(mc, five[i].x);
             }
             sums = LpSums{mc, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
-                const float d = fmaxf(six[i].x - mc, -1000.f), f = fast_exp2(d);
-                sums.s = fmaf(six[i].y, f, sums.s);
-                sums.w = fmaf(f, fmaf(d, six[i].y, six[i].z), sums.w);
+                const float d = fmaxf(five[i].x - mc, -1000.f), f = fast_exp2(d);
+                sums.s = fmaf(five[i].y, f, sums.s);
+                sums.w = fmaf(f, fmaf(d, five[i].y, five[i].z), sums.w);
             }
             sums = lp_join_warp(sums);
             if (lane == 0) wk.sums[ew] = sums;
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(LP_BLOCK, 1) token_logprobs_kernel(const Logpr
                 // (strict: are above it)
 #pragma unroll
                 for (int i = 0; i < kEach; ++i)
-                    if (order_key(six[i].w) >= bkey) wk.who[atomicAdd(&wk.n_who, 1)] = e + i * LP_EPI;
+                    if (order_key(five[i].w) >= bkey) wk.who[atomicAdd(&wk.n_who, 1)] = e + i * LP_EPI;
                 const auto gather = [&](bool strict) {
                     const auto keep = [&](float f, int id) {
                         const uint32_t k = order_key(f);
