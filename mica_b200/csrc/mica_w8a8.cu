@@ -1215,7 +1215,8 @@ int mica_cache_attention(const void* q, long ldq, const void* k_pages, const voi
                          int pages, int page, const int* table, long ld_table, int P, const int* base, const int* cu,
                          const int64_t* mask, long ld_mask, int words, int B, int N, int max_new, int H, int KV, int D,
                          float scale, void* out, long ldo, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!q || !k_pages || !v_pages || !table || !base || !cu || !out || !(scale > 0.f) || !std::isfinite(scale))
+    if (!q || !k_pages || !v_pages || !table || !base || !cu || !out || !(scale > 0.f) ||
+        !std::isfinite(scale * 1.4426950408889634f))
         return MICA_ERR_ARG;
     CacheAttnArgs a = {};
     int rc = cache_plan(&a.plan, table, ld_table, P, base, cu, B, N, pages, page);

@@ -146,3 +146,25 @@ def test_refusals_change_nothing(model):
     with pytest.raises(ValueError):
         scorer(model, max_len=50).open(tokens(60, 1))
     assert s.length(sid) == 60 and torch.equal(s.score([sid], [[[5]]])[0].logprob, before)
+
+
+def test_an_answer_without_room_leaves_its_contexts_as_they_were(model):
+    from mica_b200.paged import OutOfPages
+    for kw, ctx, wrong in ((dict(max_len=64), 61, ValueError), (dict(pages=5), 61, OutOfPages)):
+        s = scorer(model, **kw)
+        sids = [s.open(tokens(ctx, 1)), s.open(tokens(5, 2))]
+        sets = [[[7, 8, 9, 10]], [[4, 5]]]
+        before = [r.logprob.clone() for r in s.score(sids, sets)]
+        with pytest.raises(wrong):
+            s.answer(sids, sets)
+        assert [s.length(x) for x in sids] == [ctx, 5] and s.cache.free_pages == s.cache.pool.shape[0] - 5
+        again = [r.logprob for r in s.score(sids, sets)]
+        assert all(torch.equal(a, b) for a, b in zip(before, again))
+
+
+def test_ids_on_the_device_and_on_the_host_are_the_same_context(model):
+    s = scorer(model)
+    ctx = tokens(50, 3)
+    made = [s.open(ctx), s.open(torch.tensor(ctx)), s.open(torch.tensor(ctx, device='cuda', dtype=torch.int32))]
+    got = [r.logprob for r in s.score(made, [ANSWERS] * 3)]
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])

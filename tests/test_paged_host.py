@@ -270,3 +270,7 @@ def test_keep_refuses_a_step_whose_sequences_have_moved_on(monkeypatch):
     with pytest.raises(ValueError):
         c.keep([a, b], step, [[0], [0]])               # once more
     assert c.length(a) == 2 and c.length(b) == 3
+
+
+def test_a_scale_that_passes_fp32_in_base_two_is_refused(lib):
+    assert attention(lib, scale=3e38) == 1 and attention(lib, scale=2e38, ws=8) == 3
