@@ -73,10 +73,13 @@ void cuda(const char* name, const Tensor& t, std::initializer_list<const Tensor*
     if (g_device[i] < 0) g_device[i] = py::reinterpret_borrow<py::object>(g_served)(i).cast<bool>() ? 1 : 0;
     if (!g_device[i]) runtime(name, ": ", t.device().str(), " is not a B200 (sm_100)");
 }
+// Neither gradients nor forward-mode tangents pass through these calls, and what they write is no leaf of a graph.
 void no_grad(const char* name, std::initializer_list<const Tensor*> ts) {
-    if (!at::GradMode::is_enabled()) return;
-    for (const Tensor* t : ts)
-        if (t->requires_grad()) runtime(name, ": no backward pass (call it under torch.no_grad())");
+    const bool grad = at::GradMode::is_enabled();
+    for (const Tensor* t : ts) {
+        if (grad && t->requires_grad()) runtime(name, ": no backward pass (call it under torch.no_grad())");
+        if (t->_fw_grad(0).defined()) runtime(name, ": no forward-mode derivative");
+    }
 }
 const Tensor* ptr(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
@@ -151,7 +154,7 @@ Tensor append(const Tensor& qkv_, const Tensor& q_w, const Tensor& k_w, const Te
         value(name, ": pos is int64 [", n, "], not ", pos_->scalar_type(), " ", pos_->sizes());
     if (!cos.is_contiguous() || !sin.is_contiguous() || cos.size(0) < 1) value(name, ": cos and sin are contiguous [positions, D]");
     cuda(name, qkv_, {&q_w, &k_w, &cos, &sin, &k, &v, &table, &base, &cu, ptr(pos_)});
-    no_grad(name, {&qkv_, &q_w, &k_w});
+    no_grad(name, {&qkv_, &q_w, &k_w, &k, &v});
     const c10::cuda::CUDAGuard guard(qkv_.device());
     st.read();
     if (n == 0 || st.B == 0) return at::zeros({n, heads * pg.d}, qkv_.options());      // padding rows alone
@@ -237,6 +240,7 @@ void copy_pages(const Tensor& pool, const std::vector<int64_t>& src, const std::
     for (int64_t i : src)
         if (written[i]) value(name, ": page ", i, " is read and written");
     cuda(name, pool, {});
+    no_grad(name, {&pool});
     if (s.empty()) return;
     const c10::cuda::CUDAGuard guard(pool.device());
     const long stride = pages > 1 ? pool.stride(0) * static_cast<long>(pool.element_size()) : bytes;
@@ -258,6 +262,7 @@ Tensor keep_tokens(const Tensor& pool, const Tensor& table, const Tensor& base, 
         value(name, ": keep ", keep_.scalar_type(), " ", keep_.sizes(), ", n_keep ", n_keep_.scalar_type(), " ", n_keep_.sizes(),
               " for ", st.B, " sequences (int32)");
     cuda(name, pool, {&table, &base, &cu, &keep_, &n_keep_});
+    no_grad(name, {&pool});
     const c10::cuda::CUDAGuard guard(pool.device());
     st.read();
     if (st.B == 0 || keep_.size(1) == 0) return st.base.clone();

@@ -859,3 +859,32 @@ def test_append_around_the_ring(heads, kv, dim, more):
     page_of, slot = c.table.long()[b, index // 64], index % 64
     assert ((c.k[page_of, :, slot].double() - ref[:, heads:]).abs() <= bound[:, heads:]).all()
     assert torch.equal(c.v[page_of, :, slot], x[:, heads + kv:])
+
+
+def test_tangents_and_pages_that_need_gradients_are_refused():
+    from torch.autograd import forward_ad as fw
+
+    from mica_b200 import logprobs, paged
+    c = Case([10], [2], 8, 2, 64, 32)
+    i32 = {'dtype': torch.int32, 'device': 'cuda'}
+    qkv = torch.randn(2, 12 * 64, device='cuda').bfloat16()
+    cos, sin = tables(64, 100)
+    one = torch.ones(64, dtype=torch.bfloat16, device='cuda')
+    keep, n = torch.zeros(1, 1, **i32), torch.ones(1, **i32)
+    with fw.dual_level(), torch.no_grad():
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            paged.attention(fw.make_dual(c.q, c.q), c.k, c.v, c.step(), 8)
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            paged.append(fw.make_dual(qkv, qkv), one, one, cos, sin, c.k, c.v, c.step(), 8)
+        z = torch.randn(2, 50, device='cuda')
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            logprobs.token_logprobs(fw.make_dual(z, z), torch.zeros(2, dtype=torch.int64, device='cuda'))
+        paged.attention(c.q, c.k, c.v, c.step(), 8)
+    pool = torch.zeros(4, 1, 2, 2, 32, 64, dtype=torch.bfloat16, device='cuda', requires_grad=True)
+    step = paged.Step(c.table.clamp(0, 3), c.base, c.cu)
+    for call in (lambda: paged.copy_pages(pool, [0], [1]), lambda: paged.keep_tokens(pool, step, keep, n),
+                 lambda: paged.append(qkv, one, one, cos, sin, pool[:, 0, 0], pool[:, 0, 1], step, 8)):
+        with pytest.raises(RuntimeError, match='no backward'):
+            call()
+        with torch.no_grad():
+            call()
